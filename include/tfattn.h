@@ -400,6 +400,47 @@ typedef struct tf_fp8_gemm_args {
 
 TF_API tf_status tf_fp8_block_gemm(const tf_fp8_gemm_args* args, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * The K/V pool held in 8 bits.  No counterpart in the reference, whose pools have the activation
+ * dtype: the same four steps (pool store, prologue, decode, extend) over a pool of half the bytes.
+ *
+ * A K or V row (one slot, one kv head, head_dim values; the pool's page is one token, so this is
+ * the block of a page and a head) is head_dim e4m3 codes and one fp32 scale and stands for
+ * code * scale.  A row x is stored as
+ *   amax = max(max_d |x_d|, 1e-12),  code_d = e4m3_rn(x_d * (448 / amax)),  scale = amax / 448
+ * (each fp32 operation rounded once, codes saturating at 448); a row holding an infinity or a NaN
+ * is stored as codes 0 with scale NaN.  k_buffer and v_buffer of the argument structures below
+ * point at codes (1 byte per element, strides in bytes), `dtype` is that of the activations, and
+ * the scales come as (K scale, V scale) pairs in a tf_kv_scale.  Codes 0x7f and 0xff (NaN) are
+ * never written by the store; what a pool that holds them reads as is unspecified.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct tf_kv_scale {
+  float* data;                 /* [num_slots, Hkv, 2] layer view: K scale, V scale; 8-byte aligned */
+  int64_t stride_slot;         /* floats between consecutive slots, even                  */
+  int64_t stride_head;         /* floats between consecutive kv heads, even               */
+} tf_kv_scale;
+
+/* tf_kv_store with the rows quantized.  Locations must be distinct: of two tokens with the same
+ * one, a mix of both rows may remain. */
+TF_API tf_status tf_kv_store_fp8(const tf_kv_store_args* args, const tf_kv_scale* scale,
+                                 void* stream);
+
+/* tf_attn_prologue with the k and v rows quantized into the pool.  Everything is computed in fp32
+ * and rounded once: q_out to its dtype, the rotated k straight to its codes; the rotation angles
+ * positions * inv_freq are taken in 64 bits. */
+TF_API tf_status tf_attn_prologue_fp8(const tf_attn_prologue_args* args, const tf_kv_scale* scale,
+                                      void* stream);
+
+/* tf_paged_decode_attn and tf_paged_extend_attn over such a pool; the attention output and its gate
+ * are computed in fp32 and rounded once.  A request without tokens gets NaN rows in a decode call.
+ * A scale that is not finite makes the rows that see its token NaN and leaves the others alone. */
+TF_API size_t tf_paged_decode_fp8_workspace_size(const tf_paged_attn_args* args);
+TF_API tf_status tf_paged_decode_fp8(const tf_paged_attn_args* args, const tf_kv_scale* scale,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+TF_API size_t tf_paged_extend_fp8_workspace_size(const tf_paged_attn_args* args);
+TF_API tf_status tf_paged_extend_fp8(const tf_paged_attn_args* args, const tf_kv_scale* scale,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

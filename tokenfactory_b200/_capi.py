@@ -153,6 +153,10 @@ class FP8GemmArgs(ctypes.Structure):
     ]
 
 
+class KVScale(ctypes.Structure):
+    _fields_ = [("data", _vp), ("stride_slot", _i64), ("stride_head", _i64)]
+
+
 # (name, restype, argtypes) of every exported entry point, in header order
 SIGNATURES = [
     ("tf_abi_version", ctypes.c_int, []),
@@ -174,6 +178,15 @@ SIGNATURES = [
     ("tf_sample_tokens", _i32, [ctypes.POINTER(SampleArgs), _vp]),
     ("tf_fp8_quantize", _i32, [ctypes.POINTER(FP8QuantArgs), _vp]),
     ("tf_fp8_block_gemm", _i32, [ctypes.POINTER(FP8GemmArgs), _vp]),
+    ("tf_kv_store_fp8", _i32, [ctypes.POINTER(KVStoreArgs), ctypes.POINTER(KVScale), _vp]),
+    ("tf_attn_prologue_fp8", _i32,
+     [ctypes.POINTER(AttnPrologueArgs), ctypes.POINTER(KVScale), _vp]),
+    ("tf_paged_decode_fp8_workspace_size", ctypes.c_size_t, [ctypes.POINTER(PagedAttnArgs)]),
+    ("tf_paged_decode_fp8", _i32, [ctypes.POINTER(PagedAttnArgs), ctypes.POINTER(KVScale), _vp,
+                                   ctypes.c_size_t, _vp]),
+    ("tf_paged_extend_fp8_workspace_size", ctypes.c_size_t, [ctypes.POINTER(PagedAttnArgs)]),
+    ("tf_paged_extend_fp8", _i32, [ctypes.POINTER(PagedAttnArgs), ctypes.POINTER(KVScale), _vp,
+                                   ctypes.c_size_t, _vp]),
 ]
 
 _lib = None

@@ -200,7 +200,7 @@ tf_status tf_kv_store(const tf_kv_store_args* a, void* stream) {
   return cuda_status(launch_kv_store(*a, s), "tf_kv_store");
 }
 
-tf_status tf_attn_prologue(const tf_attn_prologue_args* a, void* stream) {
+static tf_status check_prologue(const tf_attn_prologue_args* a) {
   if (a == nullptr) return fail(TF_ERR_INVALID_ARG, "args is NULL");
   if (a->num_tokens < 0 || a->num_q_heads < 0 || a->num_kv_heads < 0 || a->head_dim < 0)
     return fail(TF_ERR_INVALID_ARG, "negative sizes");
@@ -221,6 +221,12 @@ tf_status tf_attn_prologue(const tf_attn_prologue_args* a, void* stream) {
     if (m[0] < 0 || m[1] < 0 || m[2] < 0 || m[0] + m[1] + m[2] != a->rotary_dim / 2)
       return fail(TF_ERR_INVALID_ARG, "mrope_section must sum to rotary_dim / 2");
   }
+  return TF_OK;
+}
+
+tf_status tf_attn_prologue(const tf_attn_prologue_args* a, void* stream) {
+  tf_status st = check_prologue(a);
+  if (st != TF_OK || a->num_tokens == 0) return st;
   if (!attn_prologue_supported(*a))
     return fail(TF_ERR_UNSUPPORTED,
                 "prologue: head_dim %d with rotary_dim %d is not built (head_dim 64/128/256; "
@@ -448,6 +454,89 @@ tf_status tf_fp8_block_gemm(const tf_fp8_gemm_args* a, void* stream) {
   DeviceGuard g(s);
   if (!g.ok()) return fail(TF_ERR_CUDA, "cannot select the stream's device");
   return cuda_status(launch_fp8_block_gemm(*a, s), "tf_fp8_block_gemm");
+}
+
+static tf_status check_kv_scale(const tf_kv_scale* sc) {
+  if (sc == nullptr || sc->data == nullptr)
+    return fail(TF_ERR_INVALID_ARG, "the pool's scales are NULL");
+  if ((reinterpret_cast<uintptr_t>(sc->data) & 7) != 0 || (sc->stride_slot & 1) != 0 ||
+      (sc->stride_head & 1) != 0)
+    return fail(TF_ERR_ALIGNMENT, "the scale pairs must be 8-byte aligned with even strides");
+  return TF_OK;
+}
+
+tf_status tf_kv_store_fp8(const tf_kv_store_args* a, const tf_kv_scale* sc, void* stream) {
+  if (a == nullptr) return fail(TF_ERR_INVALID_ARG, "args is NULL");
+  if (a->num_tokens < 0 || a->num_kv_heads < 0 || a->head_dim < 0)
+    return fail(TF_ERR_INVALID_ARG, "negative sizes");
+  if (a->num_tokens == 0 || a->num_kv_heads == 0 || a->head_dim == 0) return TF_OK;
+  if (!a->k_buffer || !a->v_buffer || !a->k || !a->v || !a->out_cache_loc)
+    return fail(TF_ERR_INVALID_ARG, "a required tensor pointer is NULL");
+  if (!dtype_ok(a->dtype)) return fail(TF_ERR_INVALID_ARG, "unknown dtype %d", a->dtype);
+  if (a->num_slots <= 0) return fail(TF_ERR_INVALID_ARG, "empty pool");
+  tf_status st = check_kv_scale(sc);
+  if (st != TF_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  DeviceGuard g(s);
+  if (!g.ok()) return fail(TF_ERR_CUDA, "cannot select the stream's device");
+  return cuda_status(launch_kv_store_fp8(*a, *sc, s), "tf_kv_store_fp8");
+}
+
+tf_status tf_attn_prologue_fp8(const tf_attn_prologue_args* a, const tf_kv_scale* sc,
+                               void* stream) {
+  tf_status st = check_prologue(a);
+  if (st != TF_OK || a->num_tokens == 0) return st;
+  st = check_kv_scale(sc);
+  if (st != TF_OK) return st;
+  if (!attn_prologue_fp8_supported(*a))
+    return fail(TF_ERR_UNSUPPORTED,
+                "fp8 prologue: head_dim %d with rotary_dim %d is not built (head_dim 64/128/256; "
+                "rotary_dim even, at most head_dim)",
+                a->head_dim, a->rotary_dim);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  DeviceGuard g(s);
+  if (!g.ok()) return fail(TF_ERR_CUDA, "cannot select the stream's device");
+  return cuda_status(launch_attn_prologue_fp8(*a, *sc, s), "tf_attn_prologue_fp8");
+}
+
+size_t tf_paged_decode_fp8_workspace_size(const tf_paged_attn_args* a) {
+  (void)a;
+  return 0;
+}
+
+tf_status tf_paged_decode_fp8(const tf_paged_attn_args* a, const tf_kv_scale* sc, void* ws,
+                              size_t ws_bytes, void* stream) {
+  (void)ws;
+  (void)ws_bytes;
+  tf_status st = check_paged(a, true);
+  if (st != TF_OK || a->batch_size == 0) return st;
+  st = check_kv_scale(sc);
+  if (st != TF_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  DeviceGuard g(s);
+  if (!g.ok()) return fail(TF_ERR_CUDA, "cannot select the stream's device");
+  tf_paged_attn_args d = *a;
+  d.extend_lens = nullptr;
+  return cuda_status(launch_paged_fp8_simt(d, *sc, s), "tf_paged_decode_fp8");
+}
+
+size_t tf_paged_extend_fp8_workspace_size(const tf_paged_attn_args* a) {
+  (void)a;
+  return 0;
+}
+
+tf_status tf_paged_extend_fp8(const tf_paged_attn_args* a, const tf_kv_scale* sc, void* ws,
+                              size_t ws_bytes, void* stream) {
+  (void)ws;
+  (void)ws_bytes;
+  tf_status st = check_paged(a, false);
+  if (st != TF_OK || a->batch_size == 0 || a->num_tokens == 0) return st;
+  st = check_kv_scale(sc);
+  if (st != TF_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  DeviceGuard g(s);
+  if (!g.ok()) return fail(TF_ERR_CUDA, "cannot select the stream's device");
+  return cuda_status(launch_paged_fp8_simt(*a, *sc, s), "tf_paged_extend_fp8");
 }
 
 }  // extern "C"

@@ -1,0 +1,147 @@
+// KV-pool store with the rows quantized to e4m3 (formulas in tfattn.h): the 8-bit counterpart of
+// kv_store.cu.  HBM-bound: a row is read once, its largest magnitude found by shuffles among the
+// lanes that hold it, and the codes written from the same registers.
+#include "common.cuh"
+#include "kv_fp8.cuh"
+#include "launch.h"
+
+namespace tf {
+namespace {
+
+constexpr int kThreads = 256;
+
+template <typename T> struct Vec8;  // eight elements of a row, loaded in 16-byte pieces
+template <> struct Vec8<float> {
+  float x[8];
+  __device__ __forceinline__ void load(const float* p) {
+    const float4 a = __ldcs(reinterpret_cast<const float4*>(p));
+    const float4 b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  }
+};
+template <typename T> struct Vec8 {
+  float x[8];
+  __device__ __forceinline__ void load(const T* p) {
+    const uint4 w = __ldcs(reinterpret_cast<const uint4*>(p));
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = unpack_lo<T>(u[i]);
+      x[2 * i + 1] = unpack_hi<T>(u[i]);
+    }
+  }
+};
+
+// LPR = D / 8 lanes hold a row, eight elements each; a group of LPR lanes takes the K and the V
+// row of one (token, kv head), so two rows are in flight per lane and the scale pair is one store.
+template <typename T, int LPR>
+__global__ void __launch_bounds__(kThreads) store_vec_kernel(tf_kv_store_args a, tf_kv_scale sc) {
+  const int64_t r = (blockIdx.x * (int64_t)kThreads + threadIdx.x) / LPR;
+  const int l = threadIdx.x % LPR;
+  const int64_t rows = a.num_tokens * (int64_t)a.num_kv_heads;
+  const bool live = r < rows;
+  const int64_t t = live ? r / a.num_kv_heads : 0;
+  const int h = live ? (int)(r - t * a.num_kv_heads) : 0;
+  Vec8<T> x[2];
+  x[0].load((const T*)a.k + t * a.k_stride_tok + h * a.k_stride_head + 8 * l);
+  x[1].load((const T*)a.v + t * a.v_stride_tok + h * a.v_stride_head + 8 * l);
+  const int64_t loc = a.out_cache_loc[t];
+  kv8::RowScale rs[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, kv8::abs_bits(x[j].x[i]));
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    rs[j] = kv8::row_scale(m);
+  }
+  if (!live) return;
+  const int64_t slot = kv8::store_slot(loc, a.num_slots, l == 0 ? a.err : nullptr);
+  if (slot < 0) return;
+  const int64_t off = slot * a.buf_stride_slot + h * a.buf_stride_head + 8 * l;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    uint2 c = make_uint2(0, 0);
+    if (rs[j].finite) {
+      const float m = rs[j].mul;
+      const float* v = x[j].x;
+      c.x = kv8::code4(v[0] * m, v[1] * m, v[2] * m, v[3] * m);
+      c.y = kv8::code4(v[4] * m, v[5] * m, v[6] * m, v[7] * m);
+    }
+    *reinterpret_cast<uint2*>((char*)(j ? a.v_buffer : a.k_buffer) + off) = c;
+  }
+  if (l == 0)
+    *reinterpret_cast<float2*>(sc.data + slot * sc.stride_slot + h * sc.stride_head) =
+        make_float2(rs[0].scale, rs[1].scale);
+}
+
+// any head_dim, strides and alignment: a warp per (token, kv head), each row read twice
+template <typename T>
+__global__ void __launch_bounds__(kThreads) store_any_kernel(tf_kv_store_args a, tf_kv_scale sc) {
+  const int64_t rows = a.num_tokens * (int64_t)a.num_kv_heads;
+  const int lane = threadIdx.x & 31;
+  const int64_t nwarps = ((int64_t)gridDim.x * kThreads) >> 5;
+  for (int64_t r = (blockIdx.x * (int64_t)kThreads + threadIdx.x) >> 5; r < rows; r += nwarps) {
+    const int64_t t = r / a.num_kv_heads;
+    const int h = (int)(r - t * a.num_kv_heads);
+    const int64_t slot = kv8::store_slot(a.out_cache_loc[t], a.num_slots,
+                                         lane == 0 ? a.err : nullptr);
+    if (slot < 0) continue;
+    float scale[2];
+    for (int j = 0; j < 2; ++j) {
+      const T* src = j ? (const T*)a.v + t * a.v_stride_tok + h * a.v_stride_head
+                       : (const T*)a.k + t * a.k_stride_tok + h * a.k_stride_head;
+      uint8_t* dst = (uint8_t*)(j ? a.v_buffer : a.k_buffer) + slot * a.buf_stride_slot +
+                     h * a.buf_stride_head;
+      uint32_t m = 0;
+      for (int d = lane; d < a.head_dim; d += 32) m = max(m, kv8::abs_bits(to_f(src[d])));
+      m = __reduce_max_sync(0xffffffffu, m);
+      const kv8::RowScale rs = kv8::row_scale(m);
+      for (int d = lane; d < a.head_dim; d += 32)
+        dst[d] = rs.finite ? kv8::code1(to_f(src[d]) * rs.mul) : 0;
+      scale[j] = rs.scale;
+    }
+    if (lane == 0)
+      *reinterpret_cast<float2*>(sc.data + slot * sc.stride_slot + h * sc.stride_head) =
+          make_float2(scale[0], scale[1]);
+  }
+}
+
+template <typename T>
+cudaError_t launch_t(const tf_kv_store_args& a, const tf_kv_scale& sc, cudaStream_t s) {
+  const int eb = (int)sizeof(T), d = a.head_dim;
+  const int64_t rows = a.num_tokens * (int64_t)a.num_kv_heads;
+  auto al = [](const void* p, int n) { return (reinterpret_cast<uintptr_t>(p) % n) == 0; };
+  const bool vec = (d == 64 || d == 128 || d == 256) && al(a.k, 16) && al(a.v, 16) &&
+                   al(a.k_buffer, 8) && al(a.v_buffer, 8) && (a.k_stride_tok * eb) % 16 == 0 &&
+                   (a.k_stride_head * eb) % 16 == 0 && (a.v_stride_tok * eb) % 16 == 0 &&
+                   (a.v_stride_head * eb) % 16 == 0 && a.buf_stride_slot % 8 == 0 &&
+                   a.buf_stride_head % 8 == 0;
+  const int lanes = vec ? d / 8 : 32;
+  const int64_t blocks = (rows * lanes + kThreads - 1) / kThreads;
+  if (vec && blocks <= 0x7fffffff) {
+    const unsigned g = (unsigned)blocks;
+    if (d == 64) store_vec_kernel<T, 8><<<g, kThreads, 0, s>>>(a, sc);
+    else if (d == 128) store_vec_kernel<T, 16><<<g, kThreads, 0, s>>>(a, sc);
+    else store_vec_kernel<T, 32><<<g, kThreads, 0, s>>>(a, sc);
+  } else {
+    const unsigned g = (unsigned)(blocks < 148 * 32 ? blocks : 148 * 32);
+    store_any_kernel<T><<<g, kThreads, 0, s>>>(a, sc);
+  }
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_kv_store_fp8(const tf_kv_store_args& a, const tf_kv_scale& sc, cudaStream_t s) {
+  if (a.num_tokens == 0) return cudaSuccess;
+  switch (a.dtype) {
+    case TF_DTYPE_F32: return launch_t<float>(a, sc, s);
+    case TF_DTYPE_BF16: return launch_t<__nv_bfloat16>(a, sc, s);
+    default: return launch_t<__half>(a, sc, s);
+  }
+}
+
+}  // namespace tf

@@ -56,6 +56,15 @@ cudaError_t launch_sample_tokens(const tf_sample_args& a, cudaStream_t s);
 cudaError_t launch_fp8_quantize(const tf_fp8_quant_args& a, cudaStream_t s);
 cudaError_t launch_fp8_block_gemm(const tf_fp8_gemm_args& a, cudaStream_t s);
 
+// the 8-bit K/V pool: kv_fp8.cu (store), prologue_fp8.cu, paged_fp8_simt.cu (any dtype and head_dim
+// <= 256, decode and extend)
+cudaError_t launch_kv_store_fp8(const tf_kv_store_args& a, const tf_kv_scale& sc, cudaStream_t s);
+bool attn_prologue_fp8_supported(const tf_attn_prologue_args& a);
+cudaError_t launch_attn_prologue_fp8(const tf_attn_prologue_args& a, const tf_kv_scale& sc,
+                                     cudaStream_t s);
+cudaError_t launch_paged_fp8_simt(const tf_paged_attn_args& a, const tf_kv_scale& sc,
+                                  cudaStream_t s);
+
 // capi.cu
 int device_sm_count();
 

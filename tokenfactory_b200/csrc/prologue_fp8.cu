@@ -1,0 +1,257 @@
+// Fused full-attention prologue over the 8-bit K/V pool: q/k RMSNorm, partial (M-)RoPE and the
+// quantizing pool store (formulas in tfattn.h), one read of q/k/v and one write of q_out and the
+// pool rows.  HBM-bound.  Everything is fp32 from the loaded values to the one rounding of q_out
+// (to its dtype) and of the codes: unlike prologue.cu, which rounds where the reference's torch
+// lines do, nothing downstream of an 8-bit row would see those roundings.  The angle is the product
+// of an integer and an fp32 frequency in fp64, reduced by whole turns there: in fp32 its rounding
+// alone would reach 2^-9 of a radian at position 32768.
+//
+// A CTA takes kTPC tokens: their cos/sin and slots first, then its warps walk the tokens' rows,
+// kPF rows in flight per warp.  Lane l of the vector form holds the E = D/32 elements [E l, E l + E)
+// of a row; the rotation partner d +- rotary_dim/2 sits in lane l ^ (rotary_dim/2/E) when that is a
+// power of two, and otherwise comes from a copy of the row in shared memory.
+#include "common.cuh"
+#include "kv_fp8.cuh"
+#include "launch.h"
+
+namespace tf {
+namespace prologue8 {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxD = 256;
+constexpr int kTPC = 4;
+constexpr int kPF = 4;
+
+template <typename T, int E, bool VEC>
+__device__ __forceinline__ void load_row(const T* p, float (&x)[E]) {
+  if constexpr (VEC && sizeof(T) == 2 && E == 8) {
+    const uint4 w = __ldcs(reinterpret_cast<const uint4*>(p));
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[2 * i] = unpack_lo<T>(u[i]); x[2 * i + 1] = unpack_hi<T>(u[i]); }
+  } else if constexpr (VEC && sizeof(T) == 2 && E == 4) {
+    const uint2 w = __ldcs(reinterpret_cast<const uint2*>(p));
+    x[0] = unpack_lo<T>(w.x); x[1] = unpack_hi<T>(w.x);
+    x[2] = unpack_lo<T>(w.y); x[3] = unpack_hi<T>(w.y);
+  } else if constexpr (VEC && sizeof(T) == 2 && E == 2) {
+    const uint32_t w = __ldcs(reinterpret_cast<const unsigned int*>(p));
+    x[0] = unpack_lo<T>(w); x[1] = unpack_hi<T>(w);
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = to_f(p[e]);
+  }
+}
+
+template <typename T, int E, bool VEC>
+__device__ __forceinline__ void store_row(T* p, const float (&x)[E]) {
+  if constexpr (VEC && sizeof(T) == 2) {
+    uint32_t w[E / 2];
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) w[i] = pack2_rn<T>(x[2 * i], x[2 * i + 1]);
+    if constexpr (E == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else if constexpr (E == 4) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(p) = w[0];
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) p[e] = from_f<T>(x[e]);
+  }
+}
+
+// codes of the lane's E elements of a row (all lanes of the warp call it); returns the scale
+template <int E, bool VEC>
+__device__ __forceinline__ float store_codes(uint8_t* p, const float (&x)[E]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) m = max(m, kv8::abs_bits(x[e]));
+  m = __reduce_max_sync(0xffffffffu, m);
+  const kv8::RowScale rs = kv8::row_scale(m);
+  uint32_t c[E / 2];
+#pragma unroll
+  for (int i = 0; i < E / 2; ++i)
+    c[i] = rs.finite ? kv8::code2(x[2 * i] * rs.mul, x[2 * i + 1] * rs.mul) : 0u;
+  if constexpr (VEC && E == 8) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+  } else if constexpr (VEC && E == 4) {
+    *reinterpret_cast<uint32_t*>(p) = c[0] | (c[1] << 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      p[2 * i] = (uint8_t)c[i];
+      p[2 * i + 1] = (uint8_t)(c[i] >> 8);
+    }
+  }
+  return rs.scale;
+}
+
+// VEC: rows aligned to the lane's E elements.  XOR: the partner lane is lane ^ pmask.
+template <typename T, int D, bool VEC, bool XOR>
+__global__ void __launch_bounds__(kThreads) prologue_kernel(tf_attn_prologue_args a,
+                                                            tf_kv_scale sc) {
+  constexpr int E = D / 32;
+  constexpr int kRowStep = kWarps / kTPC;
+  __shared__ float cs[kTPC][kMaxD / 2], sn[kTPC][kMaxD / 2];
+  __shared__ int64_t s_loc[kTPC];
+  __shared__ float s_row[XOR ? 1 : kWarps][XOR ? 1 : D];
+  const int64_t t0 = (int64_t)blockIdx.x * kTPC;
+  const int ntok = a.num_tokens - t0 < kTPC ? (int)(a.num_tokens - t0) : kTPC;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int Hq = a.num_q_heads, Hkv = a.num_kv_heads;
+  const int half = a.rotary_dim / 2;
+  const int d0 = lane * E;
+  // warp w serves token w % kTPC: its q rows, and its (k, v) row pairs as rows [Hq, Hq + Hkv)
+  const int tt = warp % kTPC, r0 = warp / kTPC;
+  const bool live = tt < ntok;
+  const int64_t t = t0 + (live ? tt : 0);
+  const int nrows = Hq + Hkv;
+  auto src_of = [&](int r) -> const T* {
+    return r < Hq ? (const T*)a.q + t * a.q_stride_tok + (int64_t)r * a.q_stride_head + d0
+                  : (const T*)a.k + t * a.k_stride_tok + (int64_t)(r - Hq) * a.k_stride_head + d0;
+  };
+  float ring[kPF][E];
+#pragma unroll
+  for (int u = 0; u < kPF; ++u)
+    if (live && r0 + u * kRowStep < nrows) load_row<T, E, VEC>(src_of(r0 + u * kRowStep), ring[u]);
+
+  for (int j = tid; j < ntok * half; j += kThreads) {
+    const int jt = j / half, jj = j - jt * half;
+    int prow = 0;
+    if (a.pos_rows == 3) {
+      if (a.mrope_interleaved) {
+        const int m = jj % 3;
+        if (m == 1 && jj < 3 * a.mrope_section[1]) prow = 1;
+        else if (m == 2 && jj < 3 * a.mrope_section[2]) prow = 2;
+      } else {
+        prow = jj < a.mrope_section[0] ? 0 : (jj < a.mrope_section[0] + a.mrope_section[1] ? 1 : 2);
+      }
+    }
+    // whole turns are removed in fp64 (2 pi to 53 bits: an error of 2^-53 per radian turned)
+    const double f = (double)a.positions[prow * a.pos_stride + t0 + jt] * (double)a.inv_freq[jj];
+    constexpr double k2Pi = 6.283185307179586;
+    float sf, cf;
+    sincosf((float)(f - rint(f * (1.0 / k2Pi)) * k2Pi), &sf, &cf);
+    cs[jt][jj] = cf;
+    sn[jt][jj] = sf;
+  }
+  if (tid < ntok) s_loc[tid] = kv8::store_slot(a.out_cache_loc[t0 + tid], a.num_slots, a.err);
+  __syncthreads();
+  if (!live) return;
+  float wq[E], wk[E];
+  const bool wf32 = a.norm_weight_dtype == TF_DTYPE_F32;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    wq[e] = wf32 ? reinterpret_cast<const float*>(a.q_norm_weight)[d0 + e]
+                 : to_f(reinterpret_cast<const T*>(a.q_norm_weight)[d0 + e]);
+    wk[e] = wf32 ? reinterpret_cast<const float*>(a.k_norm_weight)[d0 + e]
+                 : to_f(reinterpret_cast<const T*>(a.k_norm_weight)[d0 + e]);
+  }
+  const int64_t loc = s_loc[tt];
+  const int pmask = half / E;
+  for (int m0 = 0; r0 + m0 * kRowStep < nrows; m0 += kPF) {
+#pragma unroll
+    for (int u = 0; u < kPF; ++u) {
+      const int r = r0 + (m0 + u) * kRowStep;
+      if (r >= nrows) break;
+      float y[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[e] = ring[u][e];
+      if (r + kPF * kRowStep < nrows) load_row<T, E, VEC>(src_of(r + kPF * kRowStep), ring[u]);
+      const bool isq = r < Hq;
+      if (!isq && loc < 0) continue;
+      float v[E];
+      if (!isq)
+        load_row<T, E, VEC>((const T*)a.v + t * a.v_stride_tok + (int64_t)(r - Hq) * a.v_stride_head + d0, v);
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) ss = fmaf(y[e], y[e], ss);
+      ss = warp_sum(ss);
+      const float rs = 1.0f / sqrtf(ss / (float)D + a.eps);
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[e] = (isq ? wq[e] : wk[e]) * (y[e] * rs);
+      if constexpr (XOR) {
+        const bool rotates = d0 < 2 * half, lower = d0 < half;
+        const int j0 = lower ? d0 : d0 - half;
+        float p[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) p[e] = __shfl_xor_sync(0xffffffffu, y[e], pmask);
+        if (rotates) {
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            y[e] = y[e] * cs[tt][j0 + e] + (lower ? -p[e] : p[e]) * sn[tt][j0 + e];
+        }
+      } else {
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < E; ++e) s_row[warp][d0 + e] = y[e];
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int d = d0 + e;
+          if (d < half) y[e] = y[e] * cs[tt][d] - s_row[warp][d + half] * sn[tt][d];
+          else if (d < 2 * half)
+            y[e] = y[e] * cs[tt][d - half] + s_row[warp][d - half] * sn[tt][d - half];
+        }
+      }
+      if (isq) {
+        store_row<T, E, VEC>((T*)a.q_out + t * a.q_out_stride_tok + (int64_t)r * a.q_out_stride_head + d0, y);
+        continue;
+      }
+      const int h = r - Hq;
+      const int64_t off = loc * a.buf_stride_slot + (int64_t)h * a.buf_stride_head + d0;
+      const float ks = store_codes<E, VEC>((uint8_t*)a.k_buffer + off, y);
+      const float vs = store_codes<E, VEC>((uint8_t*)a.v_buffer + off, v);
+      if (lane == 0)
+        *reinterpret_cast<float2*>(sc.data + loc * sc.stride_slot + h * sc.stride_head) =
+            make_float2(ks, vs);
+    }
+  }
+}
+
+template <typename T, int D>
+static cudaError_t launch_d(const tf_attn_prologue_args& a, const tf_kv_scale& sc, cudaStream_t s) {
+  constexpr int E = D / 32;
+  const int half = a.rotary_dim / 2;
+  const int vb = E * (int)sizeof(T);
+  auto al = [](const void* p, int n) { return (reinterpret_cast<uintptr_t>(p) % n) == 0; };
+  bool vec = al(a.q, vb) && al(a.k, vb) && al(a.v, vb) && al(a.q_out, vb) && al(a.k_buffer, E) &&
+             al(a.v_buffer, E);
+  for (int64_t x : {a.q_stride_tok, a.q_stride_head, a.k_stride_tok, a.k_stride_head,
+                    a.v_stride_tok, a.v_stride_head, a.q_out_stride_tok, a.q_out_stride_head,
+                    a.buf_stride_slot, a.buf_stride_head})
+    vec = vec && x % E == 0;
+  const int pm = half / E;
+  const bool xr = half % E == 0 && pm < 32 && (pm & (pm - 1)) == 0;
+  const unsigned g = (unsigned)((a.num_tokens + kTPC - 1) / kTPC);
+  if (vec && xr) prologue_kernel<T, D, true, true><<<g, kThreads, 0, s>>>(a, sc);
+  else if (vec) prologue_kernel<T, D, true, false><<<g, kThreads, 0, s>>>(a, sc);
+  else prologue_kernel<T, D, false, false><<<g, kThreads, 0, s>>>(a, sc);
+  return cudaGetLastError();
+}
+
+template <typename T>
+static cudaError_t launch_t(const tf_attn_prologue_args& a, const tf_kv_scale& sc, cudaStream_t s) {
+  switch (a.head_dim) {
+    case 64: return launch_d<T, 64>(a, sc, s);
+    case 128: return launch_d<T, 128>(a, sc, s);
+    default: return launch_d<T, 256>(a, sc, s);
+  }
+}
+
+}  // namespace prologue8
+
+bool attn_prologue_fp8_supported(const tf_attn_prologue_args& a) {
+  if (a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256) return false;
+  return a.rotary_dim >= 2 && a.rotary_dim % 2 == 0 && a.rotary_dim <= a.head_dim;
+}
+
+cudaError_t launch_attn_prologue_fp8(const tf_attn_prologue_args& a, const tf_kv_scale& sc,
+                                     cudaStream_t s) {
+  if (a.num_tokens == 0) return cudaSuccess;
+  switch (a.dtype) {
+    case TF_DTYPE_F32: return prologue8::launch_t<float>(a, sc, s);
+    case TF_DTYPE_BF16: return prologue8::launch_t<__nv_bfloat16>(a, sc, s);
+    default: return prologue8::launch_t<__half>(a, sc, s);
+  }
+}
+
+}  // namespace tf

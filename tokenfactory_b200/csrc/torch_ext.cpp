@@ -108,9 +108,25 @@ void* workspace(const c10::Device& d, size_t nbytes) {
 // ---------------------------------------------------------------------------------------------
 // a1 KV store, f1 prologue
 // ---------------------------------------------------------------------------------------------
-void kv_store(const at::Tensor& k_buffer, const at::Tensor& v_buffer, const at::Tensor& loc_in,
-              const at::Tensor& k, const at::Tensor& v, const OptT& err) {
-  const c10::Device dev = need_cuda({&k_buffer, &v_buffer, &loc_in, &k, &v, opt(err)});
+// the (K scale, V scale) pairs of an 8-bit pool layer [num_slots, Hkv, D]
+tf_kv_scale scale_args(const at::Tensor& kv_scale, const at::Tensor& pool) {
+  if (kv_scale.scalar_type() != at::kFloat)
+    type_error(std::string("kv_scale must be float32 (got ") + c10::toString(kv_scale.scalar_type()) + ")");
+  if (pool.dim() != 3 || kv_scale.dim() != 3 || kv_scale.size(0) != pool.size(0) ||
+      kv_scale.size(1) != pool.size(1) || kv_scale.size(2) != 2 || kv_scale.stride(2) != 1)
+    value_error("kv_scale must be [num_slots, Hkv, 2] with unit stride on the (K, V) pair, got " +
+                shape(kv_scale) + " for a pool " + shape(pool));
+  tf_kv_scale s{};
+  s.data = kv_scale.data_ptr<float>();
+  s.stride_slot = kv_scale.stride(0);
+  s.stride_head = kv_scale.stride(1);
+  return s;
+}
+
+// pool_dtype: the element type the pool must have (k's own, or e4m3 codes)
+tf_kv_store_args store_args(const at::Tensor& k_buffer, const at::Tensor& v_buffer,
+                            const at::Tensor& loc_in, const at::Tensor& k, const at::Tensor& v,
+                            at::ScalarType pool_dtype, const OptT& err, at::Tensor& loc) {
   if (k.dim() != 3 || !k.sizes().equals(v.sizes()) || !k_buffer.sizes().equals(v_buffer.sizes()))
     value_error("kv_store shapes: k " + shape(k) + " v " + shape(v) + " pool " + shape(k_buffer) +
                 " / " + shape(v_buffer));
@@ -118,9 +134,10 @@ void kv_store(const at::Tensor& k_buffer, const at::Tensor& v_buffer, const at::
       k.stride(2) != 1 || v.stride(2) != 1)
     value_error("kv_store needs unit stride on head_dim and equal pool strides");
   if (k_buffer.dim() != 3 || k.size(1) != k_buffer.size(1) || k.size(2) != k_buffer.size(2) ||
-      k.scalar_type() != k_buffer.scalar_type() || v.scalar_type() != k.scalar_type())
+      k_buffer.scalar_type() != pool_dtype || v_buffer.scalar_type() != pool_dtype ||
+      v.scalar_type() != k.scalar_type())
     value_error("kv_store: k/v rows must match the pool's [Hkv, D] and dtype");
-  const at::Tensor loc = i64(loc_in, "out_cache_loc");
+  loc = i64(loc_in, "out_cache_loc");
   if (loc.numel() != k.size(0)) value_error("out_cache_loc must have one entry per token");
   tf_kv_store_args a{};
   a.k_buffer = k_buffer.data_ptr();
@@ -140,20 +157,41 @@ void kv_store(const at::Tensor& k_buffer, const at::Tensor& v_buffer, const at::
   a.head_dim = (int32_t)k.size(2);
   a.dtype = dtype_code(k);
   a.err = errp(err);
+  return a;
+}
+
+void kv_store(const at::Tensor& k_buffer, const at::Tensor& v_buffer, const at::Tensor& loc_in,
+              const at::Tensor& k, const at::Tensor& v, const OptT& err) {
+  const c10::Device dev = need_cuda({&k_buffer, &v_buffer, &loc_in, &k, &v, opt(err)});
+  at::Tensor loc;
+  const tf_kv_store_args a =
+      store_args(k_buffer, v_buffer, loc_in, k, v, k.scalar_type(), err, loc);
   c10::cuda::CUDAGuard g(dev);
   check("tf_kv_store", tf_kv_store(&a, stream_of(dev)));
 }
 
-at::Tensor attn_prologue(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+void kv_store_fp8(const at::Tensor& k_buffer, const at::Tensor& v_buffer,
+                  const at::Tensor& kv_scale, const at::Tensor& loc_in, const at::Tensor& k,
+                  const at::Tensor& v, const OptT& err) {
+  const c10::Device dev = need_cuda({&k_buffer, &v_buffer, &kv_scale, &loc_in, &k, &v, opt(err)});
+  at::Tensor loc;
+  const tf_kv_store_args a =
+      store_args(k_buffer, v_buffer, loc_in, k, v, at::ScalarType::Float8_e4m3fn, err, loc);
+  const tf_kv_scale sc = scale_args(kv_scale, k_buffer);
+  c10::cuda::CUDAGuard g(dev);
+  check("tf_kv_store_fp8", tf_kv_store_fp8(&a, &sc, stream_of(dev)));
+}
+
+at::Tensor prologue(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                          const at::Tensor& q_norm_weight, const at::Tensor& k_norm_weight,
                          const at::Tensor& positions, const at::Tensor& inv_freq,
                          const at::Tensor& k_buffer, const at::Tensor& v_buffer,
-                         const at::Tensor& out_cache_loc, double eps,
+                         const OptT& kv_scale, const at::Tensor& out_cache_loc, double eps,
                          std::vector<int64_t> mrope_section, bool mrope_interleaved, OptT q_out,
                          const OptT& err) {
   const c10::Device dev = need_cuda({&q, &k, &v, &q_norm_weight, &k_norm_weight, &positions,
-                                     &inv_freq, &k_buffer, &v_buffer, &out_cache_loc,
-                                     opt(q_out), opt(err)});
+                                     &inv_freq, &k_buffer, &v_buffer, opt(kv_scale),
+                                     &out_cache_loc, opt(q_out), opt(err)});
   if (q.dim() != 3 || k.dim() != 3 || !k.sizes().equals(v.sizes()) ||
       !k_buffer.sizes().equals(v_buffer.sizes()) || k_buffer.dim() != 3)
     value_error("attn_prologue shapes: q " + shape(q) + " k " + shape(k) + " v " + shape(v) +
@@ -166,9 +204,12 @@ at::Tensor attn_prologue(const at::Tensor& q, const at::Tensor& k, const at::Ten
       !k_buffer.strides().equals(v_buffer.strides()))
     value_error("attn_prologue needs unit stride on head_dim and equal pool strides");
   const auto dt = q.scalar_type();
-  if (k.scalar_type() != dt || v.scalar_type() != dt || k_buffer.scalar_type() != dt ||
-      v_buffer.scalar_type() != dt)
-    type_error("attn_prologue: q, k, v and the pools share a dtype");
+  const auto pool_dt = kv_scale.has_value() ? at::ScalarType::Float8_e4m3fn : dt;
+  if (k.scalar_type() != dt || v.scalar_type() != dt || k_buffer.scalar_type() != pool_dt ||
+      v_buffer.scalar_type() != pool_dt)
+    type_error(kv_scale.has_value()
+                   ? "attn_prologue_fp8: q, k and v share a dtype and the pools are float8_e4m3fn"
+                   : "attn_prologue: q, k, v and the pools share a dtype");
   if (q_norm_weight.scalar_type() != k_norm_weight.scalar_type() ||
       (q_norm_weight.scalar_type() != dt && q_norm_weight.scalar_type() != at::kFloat))
     type_error("attn_prologue: norm weights are float32 or of the activation dtype");
@@ -190,6 +231,9 @@ at::Tensor attn_prologue(const at::Tensor& q, const at::Tensor& k, const at::Ten
   const at::Tensor loc = i64(out_cache_loc, "out_cache_loc");
   if (loc.numel() != t) value_error("out_cache_loc must have one entry per token");
   if (mrope_section.size() != 3) value_error("mrope_section must have three entries");
+  if (kv_scale.has_value() && q_out.has_value() &&
+      (!q_out->sizes().equals(q.sizes()) || q_out->stride(2) != 1 || q_out->scalar_type() != dt))
+    value_error("q_out must be [T, Hq, D] of q's dtype with unit stride on head_dim");
   at::Tensor qo = q_out.has_value() ? *q_out : at::empty({t, hq, d}, q.options());
   const at::Tensor qw = q_norm_weight.contiguous(), kw = k_norm_weight.contiguous();
   tf_attn_prologue_args a{};
@@ -229,8 +273,37 @@ at::Tensor attn_prologue(const at::Tensor& q, const at::Tensor& k, const at::Ten
   a.norm_weight_dtype = dtype_code(qw);
   a.err = errp(err);
   c10::cuda::CUDAGuard g(dev);
-  check("tf_attn_prologue", tf_attn_prologue(&a, stream_of(dev)));
+  if (kv_scale.has_value()) {
+    const tf_kv_scale sc = scale_args(*kv_scale, k_buffer);
+    check("tf_attn_prologue_fp8", tf_attn_prologue_fp8(&a, &sc, stream_of(dev)));
+  } else {
+    check("tf_attn_prologue", tf_attn_prologue(&a, stream_of(dev)));
+  }
   return qo;
+}
+
+at::Tensor attn_prologue(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                         const at::Tensor& q_norm_weight, const at::Tensor& k_norm_weight,
+                         const at::Tensor& positions, const at::Tensor& inv_freq,
+                         const at::Tensor& k_buffer, const at::Tensor& v_buffer,
+                         const at::Tensor& out_cache_loc, double eps,
+                         std::vector<int64_t> mrope_section, bool mrope_interleaved, OptT q_out,
+                         const OptT& err) {
+  return prologue(q, k, v, q_norm_weight, k_norm_weight, positions, inv_freq, k_buffer, v_buffer,
+                  c10::nullopt, out_cache_loc, eps, std::move(mrope_section), mrope_interleaved,
+                  std::move(q_out), err);
+}
+
+at::Tensor attn_prologue_fp8(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                             const at::Tensor& q_norm_weight, const at::Tensor& k_norm_weight,
+                             const at::Tensor& positions, const at::Tensor& inv_freq,
+                             const at::Tensor& k_buffer, const at::Tensor& v_buffer,
+                             const at::Tensor& kv_scale, const at::Tensor& out_cache_loc,
+                             double eps, std::vector<int64_t> mrope_section,
+                             bool mrope_interleaved, OptT q_out, const OptT& err) {
+  return prologue(q, k, v, q_norm_weight, k_norm_weight, positions, inv_freq, k_buffer, v_buffer,
+                  kv_scale, out_cache_loc, eps, std::move(mrope_section), mrope_interleaved,
+                  std::move(q_out), err);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -246,7 +319,7 @@ tf_paged_attn_args paged_args(const at::Tensor& q, const at::Tensor& k_buffer,
                               const OptT& extend_lens, double scale, const OptT& gate,
                               int64_t gate_mode, const at::Tensor& out, int64_t max_seq_len,
                               int64_t max_extend_len, int64_t slot_mode, const OptT& err,
-                              PagedKeep& keep) {
+                              at::ScalarType pool_dtype, PagedKeep& keep) {
   if (q.dim() != 3 || k_buffer.dim() != 3 || !k_buffer.sizes().equals(v_buffer.sizes()))
     value_error("paged attention shapes: q " + shape(q) + ", pool " + shape(k_buffer));
   const int64_t t = q.size(0), hq = q.size(1), d = q.size(2);
@@ -255,9 +328,11 @@ tf_paged_attn_args paged_args(const at::Tensor& q, const at::Tensor& k_buffer,
   if (out.dim() != 3 || q.stride(2) != 1 || k_buffer.stride(2) != 1 || out.stride(2) != 1 ||
       !k_buffer.strides().equals(v_buffer.strides()))
     value_error("paged attention needs unit stride on head_dim");
-  if (q.scalar_type() != k_buffer.scalar_type() || v_buffer.scalar_type() != q.scalar_type() ||
+  if (k_buffer.scalar_type() != pool_dtype || v_buffer.scalar_type() != pool_dtype ||
       out.scalar_type() != q.scalar_type())
-    type_error("q, pools and out must share a dtype");
+    type_error(pool_dtype == q.scalar_type()
+                   ? "q, pools and out must share a dtype"
+                   : "q and out must share a dtype and the pools must be float8_e4m3fn");
   if (gate.has_value()) {
     if (!gate->sizes().equals(q.sizes()) || gate->stride(2) != 1 ||
         gate->scalar_type() != q.scalar_type())
@@ -316,7 +391,7 @@ at::Tensor paged_decode(const at::Tensor& q, const at::Tensor& k_buffer, const a
   PagedKeep keep;
   tf_paged_attn_args a = paged_args(q, k_buffer, v_buffer, req_to_token, req_pool_indices,
                                     seq_lens, c10::nullopt, scale, gate, gate_mode, o, max_seq_len,
-                                    1, slot_mode, err, keep);
+                                    1, slot_mode, err, q.scalar_type(), keep);
   c10::cuda::CUDAGuard g(dev);
   const size_t nbytes = tf_paged_decode_workspace_size(&a);
   void* ws = nbytes ? workspace(dev, nbytes) : nullptr;
@@ -335,11 +410,77 @@ at::Tensor paged_extend(const at::Tensor& q, const at::Tensor& k_buffer, const a
   PagedKeep keep;
   tf_paged_attn_args a = paged_args(q, k_buffer, v_buffer, req_to_token, req_pool_indices,
                                     seq_lens, extend_lens, scale, gate, gate_mode, o, max_seq_len,
-                                    max_extend_len, slot_mode, err, keep);
+                                    max_extend_len, slot_mode, err, q.scalar_type(), keep);
   c10::cuda::CUDAGuard g(dev);
   const size_t nbytes = tf_paged_extend_workspace_size(&a);
   void* ws = nbytes ? workspace(dev, nbytes) : nullptr;
   check("tf_paged_extend_attn", tf_paged_extend_attn(&a, ws, nbytes, stream_of(dev)));
+  return o;
+}
+
+// Scratch of the calls on an 8-bit pool comes from the caching allocator for each call: stream
+// ordered, and inside a capture part of that graph's own memory, so that neither two captured
+// graphs nor a graph and eager calls share it.
+at::Tensor call_scratch(const c10::Device& d, size_t nbytes) {
+  if (nbytes == 0) return at::Tensor();
+  return at::empty({(int64_t)nbytes}, at::TensorOptions().dtype(at::kByte).device(d));
+}
+
+// out of the shape the paged 8-bit calls write
+at::Tensor attn_out(const at::Tensor& q, const OptT& out) {
+  if (!out.has_value()) return at::empty(q.sizes(), q.options());
+  if (!out->sizes().equals(q.sizes())) value_error("out must have q's shape " + shape(q));
+  return *out;
+}
+
+at::Tensor paged_decode_fp8(const at::Tensor& q, const at::Tensor& k_buffer,
+                            const at::Tensor& v_buffer, const at::Tensor& kv_scale,
+                            const at::Tensor& req_to_token, const at::Tensor& req_pool_indices,
+                            const at::Tensor& seq_lens, double scale, int64_t max_seq_len,
+                            const OptT& gate, int64_t gate_mode, const OptT& out,
+                            int64_t slot_mode, const OptT& err) {
+  const c10::Device dev = need_cuda({&q, &k_buffer, &v_buffer, &kv_scale, &req_to_token,
+                                     &req_pool_indices, &seq_lens, opt(gate), opt(out), opt(err)});
+  c10::cuda::CUDAGuard g(dev);
+  at::Tensor o = attn_out(q, out);
+  PagedKeep keep;
+  const tf_paged_attn_args a =
+      paged_args(q, k_buffer, v_buffer, req_to_token, req_pool_indices, seq_lens, c10::nullopt,
+                 scale, gate, gate_mode, o, max_seq_len, 1, slot_mode, err,
+                 at::ScalarType::Float8_e4m3fn, keep);
+  if (keep.sl.numel() != keep.rpi.numel()) value_error("seq_lens must have one entry per request");
+  const tf_kv_scale sc = scale_args(kv_scale, k_buffer);
+  const size_t nbytes = tf_paged_decode_fp8_workspace_size(&a);
+  const at::Tensor ws = call_scratch(dev, nbytes);
+  check("tf_paged_decode_fp8",
+        tf_paged_decode_fp8(&a, &sc, nbytes ? ws.data_ptr() : nullptr, nbytes, stream_of(dev)));
+  return o;
+}
+
+at::Tensor paged_extend_fp8(const at::Tensor& q, const at::Tensor& k_buffer,
+                            const at::Tensor& v_buffer, const at::Tensor& kv_scale,
+                            const at::Tensor& req_to_token, const at::Tensor& req_pool_indices,
+                            const at::Tensor& seq_lens, const at::Tensor& extend_lens,
+                            double scale, int64_t max_seq_len, int64_t max_extend_len,
+                            const OptT& gate, int64_t gate_mode, const OptT& out,
+                            int64_t slot_mode, const OptT& err) {
+  const c10::Device dev =
+      need_cuda({&q, &k_buffer, &v_buffer, &kv_scale, &req_to_token, &req_pool_indices, &seq_lens,
+                 &extend_lens, opt(gate), opt(out), opt(err)});
+  c10::cuda::CUDAGuard g(dev);
+  at::Tensor o = attn_out(q, out);
+  PagedKeep keep;
+  const tf_paged_attn_args a =
+      paged_args(q, k_buffer, v_buffer, req_to_token, req_pool_indices, seq_lens, extend_lens,
+                 scale, gate, gate_mode, o, max_seq_len, max_extend_len, slot_mode, err,
+                 at::ScalarType::Float8_e4m3fn, keep);
+  if (keep.sl.numel() != keep.rpi.numel() || keep.el.numel() != keep.rpi.numel())
+    value_error("seq_lens and extend_lens must have one entry per request");
+  const tf_kv_scale sc = scale_args(kv_scale, k_buffer);
+  const size_t nbytes = tf_paged_extend_fp8_workspace_size(&a);
+  const at::Tensor ws = call_scratch(dev, nbytes);
+  check("tf_paged_extend_fp8",
+        tf_paged_extend_fp8(&a, &sc, nbytes ? ws.data_ptr() : nullptr, nbytes, stream_of(dev)));
   return o;
 }
 
@@ -703,4 +844,8 @@ PYBIND11_MODULE(_C, m) {
   m.def("sample_tokens", &sample_tokens);
   m.def("fp8_quantize", &fp8_quantize);
   m.def("fp8_block_gemm", &fp8_block_gemm);
+  m.def("kv_store_fp8", &kv_store_fp8);
+  m.def("attn_prologue_fp8", &attn_prologue_fp8);
+  m.def("paged_decode_fp8", &paged_decode_fp8);
+  m.def("paged_extend_fp8", &paged_extend_fp8);
 }

@@ -295,3 +295,69 @@ def block_fp8_linear(x: torch.Tensor, weight: torch.Tensor,
     q, scale = fp8_quantize(x2d)
     out = fp8_block_gemm(q, scale, weight, weight_scale_inv, bias, x.dtype, block_h, block_w)
     return out.reshape(*x.shape[:-1], N)
+
+
+# ---------------------------------------------------------------------------------------------
+# the K/V pool held in 8 bits
+# ---------------------------------------------------------------------------------------------
+# k_buffer / v_buffer are float8_e4m3fn layer views [num_slots, Hkv, D] of equal strides (unit on D)
+# and kv_scale a float32 layer view [num_slots, Hkv, 2] of (K scale, V scale) pairs: a row stands for
+# codes * scale.  hybrid_model.HybridCachePool allocates them with a head's K and V rows adjacent.
+def kv_store_fp8(k_buffer: torch.Tensor, v_buffer: torch.Tensor, kv_scale: torch.Tensor,
+                 out_cache_loc: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                 err: Optional[torch.Tensor] = None) -> None:
+    """kv_store into an 8-bit pool: with amax = max(max |x|, 1e-12) of a k or v row, its slot gets
+    codes e4m3(x * (448 / amax)) and scale amax / 448 (each operation in fp32; a row with an infinity
+    or a NaN gets codes 0 and scale NaN).
+
+    k, v: [T, Hkv, D] float32 / bfloat16 / float16; out_cache_loc [T] int64, distinct (of two tokens
+    with one location a mix may remain); negative locations wrap, others outside the pool are
+    recorded in ``err`` and skipped."""
+    _C.kv_store_fp8(k_buffer, v_buffer, kv_scale, out_cache_loc, k, v, err)
+
+
+def attn_prologue_fp8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                      q_norm_weight: torch.Tensor, k_norm_weight: torch.Tensor,
+                      positions: torch.Tensor, inv_freq: torch.Tensor, k_buffer: torch.Tensor,
+                      v_buffer: torch.Tensor, kv_scale: torch.Tensor, out_cache_loc: torch.Tensor,
+                      eps: float = 1e-6, mrope_section=(11, 11, 10),
+                      mrope_interleaved: bool = True, q_out: Optional[torch.Tensor] = None,
+                      err: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """attn_prologue (q/k RMSNorm + partial (M-)RoPE + pool store) into an 8-bit pool: the rotated k
+    and v rows are stored as kv_store_fp8 does.  Everything is fp32 and rounded once, the angles
+    positions * inv_freq are taken in 64 bits; head_dim 64, 128 or 256, any even rotary_dim.
+    Returns the rotated q [T, Hq, D]."""
+    if positions.dim() == 2 and positions.stride(-1) != 1:
+        positions = positions.contiguous()
+    return _C.attn_prologue_fp8(q, k, v, q_norm_weight, k_norm_weight, positions, inv_freq,
+                                k_buffer, v_buffer, kv_scale, out_cache_loc, float(eps),
+                                list(mrope_section), bool(mrope_interleaved), q_out, err)
+
+
+def paged_decode_fp8(q: torch.Tensor, k_buffer: torch.Tensor, v_buffer: torch.Tensor,
+                     kv_scale: torch.Tensor, req_to_token: torch.Tensor,
+                     req_pool_indices: torch.Tensor, seq_lens: torch.Tensor, scale: float,
+                     max_seq_len: int, gate: Optional[torch.Tensor] = None,
+                     gate_mode: str = "none", out: Optional[torch.Tensor] = None,
+                     slot_mode: str = "clamp", err: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """paged_decode over an 8-bit pool: softmax(q K^T scale) V, times act(gate), in fp32 and rounded
+    once to q's dtype.  A request of length 0 gets NaN rows.  Returns out [B, Hq, D]."""
+    return _C.paged_decode_fp8(q, k_buffer, v_buffer, kv_scale, req_to_token, req_pool_indices,
+                               seq_lens, float(scale), int(max_seq_len), gate,
+                               GATE_MODES[gate_mode], out, SLOT_MODES[slot_mode], err)
+
+
+def paged_extend_fp8(q: torch.Tensor, k_buffer: torch.Tensor, v_buffer: torch.Tensor,
+                     kv_scale: torch.Tensor, req_to_token: torch.Tensor,
+                     req_pool_indices: torch.Tensor, seq_lens: torch.Tensor,
+                     extend_lens: torch.Tensor, scale: float, max_seq_len: int,
+                     max_extend_len: int, gate: Optional[torch.Tensor] = None,
+                     gate_mode: str = "none", out: Optional[torch.Tensor] = None,
+                     slot_mode: str = "clamp", err: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """paged_extend over an 8-bit pool (the new tokens' rows already stored): query i of request b
+    sees positions <= seq_len_b - extend_len_b + i; rows of q behind the last request are left as
+    they were in ``out``.  Returns out [T, Hq, D]."""
+    return _C.paged_extend_fp8(q, k_buffer, v_buffer, kv_scale, req_to_token, req_pool_indices,
+                               seq_lens, extend_lens, float(scale), int(max_seq_len),
+                               int(max_extend_len), gate, GATE_MODES[gate_mode], out,
+                               SLOT_MODES[slot_mode], err)

@@ -53,14 +53,16 @@ def norm_rotate(x, w, positions, inv_freq, eps, mrope_section=(11, 11, 10), inte
 
 
 def attention(q, k_rows, v_rows, req_to_token, req_pool_indices, seq_lens, extend_lens, scale,
-              gate=None, gate_mode="none", slot_mode="clamp"):
-    """(out, magnitude, score magnitude) [T, Hq, D] float64 of paged attention over dequantized pool
-    rows k_rows / v_rows [slots, Hkv, D].  magnitude is the same sum with |v| and |act(gate)|: what a
-    relative error of the weights is multiplied by; score magnitude is the row's largest
-    scale * sum_d |q_d k_d|: what a relative error of the products adds to a score.  Requests without
-    keys give NaN."""
+              gate=None, gate_mode="none", slot_mode="clamp", v_scale=None):
+    """(out, magnitude, score magnitude, step magnitude) [T, Hq, D] float64 of paged attention over
+    dequantized pool rows k_rows / v_rows [slots, Hkv, D].  magnitude is the same sum with |v| and
+    |act(gate)|: what a relative error of the weights is multiplied by; score magnitude is the row's
+    largest scale * sum_d |q_d k_d|: what a relative error of the products adds to a score; step
+    magnitude, with v_scale [slots, Hkv] given, is max_j p_j * max_j v_scale_j * sum_j |v code_j|
+    |act(gate)|: what an error of each weight * scale relative to the largest possible one is
+    multiplied by.  Requests without keys give NaN."""
     q = np.asarray(q, np.float64)
-    smag = np.zeros(q.shape)
+    smag, step = np.zeros(q.shape), np.zeros(q.shape)
     hkv = k_rows.shape[1]
     g = q.shape[1] // hkv
     out, mag = np.full(q.shape, np.nan), np.full(q.shape, np.nan)
@@ -79,9 +81,14 @@ def attention(q, k_rows, v_rows, req_to_token, req_pool_indices, seq_lens, exten
                     x = np.exp(x - x.max(-1, keepdims=True))
                     x /= x.sum(-1, keepdims=True)
                     out[t, hs], mag[t, hs] = x @ v[:, h], x @ np.abs(v[:, h])
+                    if v_scale is not None:
+                        vs = np.abs(v_scale[s[:m], h])
+                        ok = np.isfinite(vs) & (vs > 0)
+                        codes = (np.abs(v[ok, h]) / vs[ok, None]).sum(0)
+                        step[t, hs] = x.max(-1)[:, None] * vs[ok].max(initial=0) * codes
             t += 1
     if gate_mode != "none":
         x = np.asarray(gate, np.float64)
         act = 1 / (1 + np.exp(-x)) * (x if gate_mode == "silu" else 1)
-        out, mag = out * act, mag * np.abs(act)
-    return out, mag, smag
+        out, mag, step = out * act, mag * np.abs(act), step * np.abs(act)
+    return out, mag, smag, step

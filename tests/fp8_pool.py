@@ -79,19 +79,27 @@ class Case:
         rows = self.codes.float().double().numpy() * self.scale.double().numpy()[..., None]
         return O.attention(self.q.double().numpy(), rows[:, :, 0], rows[:, :, 1], self.r2t.numpy(),
                            self.rows.tolist(), self.seq, self.ext, self.d ** -0.5,
-                           self.gate.double().numpy(), self.gate_mode, slot_mode)
+                           self.gate.double().numpy(), self.gate_mode, slot_mode,
+                           self.scale[..., 1].double().numpy())
 
 
 def check(got, ref, dtype, d, what=""):
-    """got against (out, magnitude, score magnitude): one rounding of the output, the weights'
-    error, and the fp32 sums (d products a score and as many weighted rows: each addition is off by
-    at most 2^-24 of the running magnitude; the activation's exponential by 2^-20)."""
-    out, mag, smag = ref
+    """got against (out, magnitude, score magnitude, step magnitude): one rounding of the output, the
+    weights' error, and the fp32 sums (d products a score and as many weighted rows: each addition
+    is off by at most 2^-24 of the running magnitude; the activation's exponential by 2^-20).
+
+    The step: a sum of e4m3 terms has an absolute error too, half the subnormal step, 2^-10.  The
+    weights w_j = 2^7 p_j vs_j / P are scaled by P = max_j p_j 2^ev_j <= max_j p_j max_j vs_j (2^ev_j the
+    power of two below the largest vs of token j's tile), so p_j vs_j is off by at most
+    2^-17 max p max vs, and a sum over the V codes by that times sum_j |code_j|."""
+    out, mag, smag, step = ref
     got = got.detach().double().cpu().numpy()
     assert got.shape == out.shape, (got.shape, out.shape)
     assert np.array_equal(np.isnan(got), np.isnan(out)), f"{what}: NaNs in other places"
     tol = (torch.finfo(DTYPES[dtype]).eps / 2 * np.abs(out)
            + mag * (WEIGHT_ERR[dtype] + 2 * d * 2.0 ** -24 * (1 + smag) + 2.0 ** -20) + 1e-30)
+    if dtype != "f32":
+        tol = tol + 2.0 ** -17 * step
     if dtype == "f16":
         tol = tol + 2.0 ** -25  # half a step of a subnormal output
     bad = np.abs(got - out) > tol

@@ -38,7 +38,7 @@ def test_oracle_rows():
 def test_oracle_attention_of_one_key_is_its_value():
     q = np.ones((1, 2, 4))
     k = v = np.arange(8.0).reshape(2, 1, 4)
-    out, mag, _ = O.attention(q, k, v, np.array([[1]]), [0], [1], [1], 0.5)
+    out, mag, _, _ = O.attention(q, k, v, np.array([[1]]), [0], [1], [1], 0.5)
     assert (out == v[1, 0]).all() and (mag == np.abs(v[1, 0])).all()
 
 

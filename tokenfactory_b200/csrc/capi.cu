@@ -499,44 +499,58 @@ tf_status tf_attn_prologue_fp8(const tf_attn_prologue_args* a, const tf_kv_scale
   return cuda_status(launch_attn_prologue_fp8(*a, *sc, s), "tf_attn_prologue_fp8");
 }
 
-size_t tf_paged_decode_fp8_workspace_size(const tf_paged_attn_args* a) {
-  (void)a;
-  return 0;
+// Which kernel a call over an 8-bit pool takes: the few-rows kernel while a request has at most
+// kFewRows query rows per kv head, the CUDA-core kernel otherwise.
+enum class Fp8Path { kRows, kSimt };
+constexpr int64_t kFewRows = 32;
+
+static Fp8Path fp8_path(const tf_paged_attn_args& a, bool decode) {
+  const int64_t rows = (int64_t)(a.num_q_heads / a.num_kv_heads) * (decode ? 1 : a.max_extend_len);
+  return (decode || rows <= kFewRows) && paged_fp8_rows_supported(a) ? Fp8Path::kRows : Fp8Path::kSimt;
 }
 
-tf_status tf_paged_decode_fp8(const tf_paged_attn_args* a, const tf_kv_scale* sc, void* ws,
-                              size_t ws_bytes, void* stream) {
-  (void)ws;
-  (void)ws_bytes;
-  tf_status st = check_paged(a, true);
-  if (st != TF_OK || a->batch_size == 0) return st;
-  st = check_kv_scale(sc);
-  if (st != TF_OK) return st;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  DeviceGuard g(s);
-  if (!g.ok()) return fail(TF_ERR_CUDA, "cannot select the stream's device");
-  tf_paged_attn_args d = *a;
-  d.extend_lens = nullptr;
-  return cuda_status(launch_paged_fp8_simt(d, *sc, s), "tf_paged_decode_fp8");
+static size_t fp8_workspace(const tf_paged_attn_args* a, bool decode) {
+  if (a == nullptr || a->batch_size <= 0 || check_paged(a, decode) != TF_OK) return 0;
+  return fp8_path(*a, decode) == Fp8Path::kRows ? paged_fp8_rows_workspace(*a, device_sm_count()) : 0;
 }
 
-size_t tf_paged_extend_fp8_workspace_size(const tf_paged_attn_args* a) {
-  (void)a;
-  return 0;
-}
-
-tf_status tf_paged_extend_fp8(const tf_paged_attn_args* a, const tf_kv_scale* sc, void* ws,
-                              size_t ws_bytes, void* stream) {
-  (void)ws;
-  (void)ws_bytes;
-  tf_status st = check_paged(a, false);
+static tf_status paged_fp8(const tf_paged_attn_args* a, const tf_kv_scale* sc, void* ws,
+                           size_t ws_bytes, void* stream, bool decode, const char* what) {
+  tf_status st = check_paged(a, decode);
   if (st != TF_OK || a->batch_size == 0 || a->num_tokens == 0) return st;
   st = check_kv_scale(sc);
   if (st != TF_OK) return st;
+  tf_paged_attn_args d = *a;
+  if (decode) d.extend_lens = nullptr;
+  const Fp8Path path = fp8_path(d, decode);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   DeviceGuard g(s);
   if (!g.ok()) return fail(TF_ERR_CUDA, "cannot select the stream's device");
-  return cuda_status(launch_paged_fp8_simt(*a, *sc, s), "tf_paged_extend_fp8");
+  const int nsm = device_sm_count();
+  const size_t need = path == Fp8Path::kRows ? paged_fp8_rows_workspace(d, nsm) : 0;
+  if (need != 0) {
+    if (ws == nullptr || ws_bytes < need)
+      return fail(TF_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, need, ws_bytes);
+    if ((reinterpret_cast<uintptr_t>(ws) & 255) != 0)
+      return fail(TF_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
+  }
+  if (path == Fp8Path::kRows) return cuda_status(launch_paged_fp8_rows(d, *sc, ws, nsm, s), what);
+  return cuda_status(launch_paged_fp8_simt(d, *sc, s), what);
+}
+
+size_t tf_paged_decode_fp8_workspace_size(const tf_paged_attn_args* a) {
+  return fp8_workspace(a, true);
+}
+tf_status tf_paged_decode_fp8(const tf_paged_attn_args* a, const tf_kv_scale* sc, void* ws,
+                              size_t ws_bytes, void* stream) {
+  return paged_fp8(a, sc, ws, ws_bytes, stream, true, "tf_paged_decode_fp8");
+}
+size_t tf_paged_extend_fp8_workspace_size(const tf_paged_attn_args* a) {
+  return fp8_workspace(a, false);
+}
+tf_status tf_paged_extend_fp8(const tf_paged_attn_args* a, const tf_kv_scale* sc, void* ws,
+                              size_t ws_bytes, void* stream) {
+  return paged_fp8(a, sc, ws, ws_bytes, stream, false, "tf_paged_extend_fp8");
 }
 
 }  // extern "C"

@@ -64,6 +64,11 @@ cudaError_t launch_attn_prologue_fp8(const tf_attn_prologue_args& a, const tf_kv
                                      cudaStream_t s);
 cudaError_t launch_paged_fp8_simt(const tf_paged_attn_args& a, const tf_kv_scale& sc,
                                   cudaStream_t s);
+// paged_fp8_rows.cu: bf16 / fp16, few query rows per kv head (decode, extends of a few tokens)
+bool paged_fp8_rows_supported(const tf_paged_attn_args& a);
+size_t paged_fp8_rows_workspace(const tf_paged_attn_args& a, int num_sms);
+cudaError_t launch_paged_fp8_rows(const tf_paged_attn_args& a, const tf_kv_scale& sc, void* ws,
+                                  int num_sms, cudaStream_t s);
 
 // capi.cu
 int device_sm_count();

@@ -1,0 +1,995 @@
+// Paged GQA attention over the 8-bit K/V pool for few query rows per kv head: decode, and extends of
+// a few tokens per request (drafted tokens).  HBM-bound: every K/V row is read once, and the e4m3
+// codes go into the tensor cores as they are.
+//
+// Mathematics.  A token j has codes K8_j, V8_j and scales ks_j, vs_j; a query row has logits
+//   s_j = (q . K8_j) ks_j scale log2(e)      out = sum_j 2^(s_j) vs_j V8_j / sum_j 2^(s_j).
+// Both products run as mma.m16n8k32 e4m3 x e4m3 with fp32 sums (exact products; measured on
+// 2048-long sums: relative error 1e-7).  The operands that are not codes are sums of e4m3 terms:
+//   q, scaled by a power of two per row:  hi + lo (bfloat16: all 8 bits), + a third for float16;
+//   the weight w_j = 2^(s_j + ev - M) vs_j 2^(7 - ev): as many terms, i.e. to 8 or 12 bits, below
+//   2^-17 of the largest to that absolute step.  ev is the exponent of the largest vs of a tile and
+//   M the running maximum of s_j + ev, so that w stays under 448 whatever the scales are; the sum
+//   of weights l = sum 2^(s_j - M) is fp32 and unsplit.
+// Measured alternatives: converting codes to f16 costs two conversions per four codes, and
+// mma.m16n8k16 f16 issues at half the rate of the e4m3 form at half its depth.
+//
+// Fragments.  S^T = K8.Q^T: A = 16 tokens x 32 dims.  A thread's 16-byte read of a token's row is its
+// A fragment of two k-steps for the dim order 64 j + 16 t + {0..3 | 4..7}, {8..11 | 12..15}
+// (t = lane % 4), and Q^T is held in the same order.  O^T = V8^T.W^T: A = 16 dims x 32 tokens, from
+// ldmatrix.trans on pairs of codes and byte permutes: row r of the fragment is dim 2 r, row r + 8 dim
+// 2 r + 1, and the tokens of a thread come in the order 2t, 2t+8, 2t+1, 2t+9, which movmatrix gives
+// the weights as well (two tokens' codes per 16-bit element).
+//
+// Work.  A CTA has four warps.  TEAM of them (1, 2 or 4) share a ring of 32-token stages and take
+// eight query rows each; HG kv heads of a group run side by side, so that a token's rows of all
+// heads, its scales and its slot id are read at about the same time; the WH = 4 / (TEAM HG) teams of
+// a head take its tiles in turn and merge in shared memory.  The sequence of (request, head group)
+// units, each of ceil(len / 32) tiles, is cut into one range per CTA, balanced by tiles plus a fixed
+// cost per unit; every CTA finds its own range from the lengths (a scan of the batch in shared
+// memory: no plan launch).  Units cut by a boundary leave (M, l, O) partials for a combine kernel.
+// Rows are fetched by bulk copies, a stage's copies completing on its mbarrier, and the ring runs on
+// across units.
+#include <type_traits>
+
+#include "common.cuh"
+#include "kv_fp8.cuh"
+#include "launch.h"
+
+namespace tf {
+namespace rows8 {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kTok = 32;  // tokens of a tile
+constexpr int kRows = 8;  // query rows of a warp (n of the mma tiles)
+constexpr int kCache = 96;  // requests whose metadata a CTA keeps in shared memory
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMaxCtas = 256;
+constexpr int kMaxBatch = 32768;  // the batch scan lives in the ring's shared memory
+
+struct ReqMeta {
+  int32_t len, ext, row, start;  // tokens, new tokens, req_to_token row, first query token
+};
+
+template <int D>
+struct Cfg {
+  // row strides in shared memory: 64 mod 128 bytes for the 16-byte fragment reads of K (two rows a
+  // phase), an odd multiple of 16 for the 8-row matrices of V
+  static constexpr int kKS = D % 128 == 0 ? D + 64 : D;
+  static constexpr int kVS = D + 16;
+  static constexpr int kOffV = kTok * kKS;
+  static constexpr int kOffScale = kOffV + kTok * kVS;
+  static constexpr int kStage = kOffScale + kTok * 8;
+  static constexpr int kStages = D == 256 ? 12 : (D == 128 ? 20 : 40);  // without a merge buffer
+  static constexpr int kMergeStride = D + 4;  // floats per row
+  static constexpr int kMerge = kWarps * kRows * (kMergeStride + 2) * 4;
+  static constexpr int kFixed = kCache * (int)sizeof(ReqMeta) + 64;
+  static_assert(kStage % 16 == 0 && kKS % 16 == 0 && kVS % 16 == 0, "bulk copy alignment");
+};
+
+// What a launch is divided by; computed on the host.
+struct Shape {
+  int team, hg, wh;   // warps sharing a ring, kv heads side by side, teams taking a head's tiles in turn
+  int groups;         // units per request
+  int passes;         // row passes of a kv head (more than 8 * team query rows)
+  int stages;         // ring stages per kv head of a group
+  int nctas;
+  int min_tiles;      // tiles worth a CTA of their own
+  int piece_cost;     // fixed cost of a unit in tiles
+  int smem, ring;     // bytes
+};
+
+// The unit that a CTA's range starts in, for the combine kernel.
+struct CutInfo {
+  int b, u, start, ext, nt, t0;
+};
+
+struct Ws {
+  int64_t* cta_g;  // [nctas + 1] first tile of each CTA's range
+  CutInfo* cut;    // [nctas]
+  float* ml;       // [2 nctas][4 warps][8 rows][2]
+  float* o;        // [2 nctas][4 warps][8 rows][D]
+};
+
+__host__ __device__ inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+__host__ __device__ inline Ws carve(void* base, int nctas, int D) {
+  char* p = (char*)base;
+  Ws w;
+  w.cta_g = (int64_t*)p;
+  p += align256((size_t)(nctas + 1) * 8);
+  w.cut = (CutInfo*)p;
+  p += align256((size_t)nctas * sizeof(CutInfo));
+  w.ml = (float*)p;
+  p += align256((size_t)2 * nctas * kWarps * kRows * 2 * 4);
+  w.o = (float*)p;
+  return w;
+}
+inline size_t ws_bytes(int nctas, int D) {
+  return align256((size_t)(nctas + 1) * 8) + align256((size_t)nctas * sizeof(CutInfo)) +
+         align256((size_t)2 * nctas * kWarps * kRows * 2 * 4) +
+         (size_t)2 * nctas * kWarps * kRows * D * 4;
+}
+
+__device__ __forceinline__ void mma8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                     uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ float2 lds_f2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a));
+}
+__device__ __forceinline__ uint32_t movmatrix_t(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// the two values of a code pair
+__device__ __forceinline__ float2 value2(uint32_t c) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)c, __NV_E4M3);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+// next e4m3 terms of the pair (a, b); a and b become what is left
+__device__ __forceinline__ uint32_t term2(float& a, float& b) {
+  const uint32_t c = kv8::code2(a, b);
+  const float2 v = value2(c);
+  a -= v.x;
+  b -= v.y;
+  return c;
+}
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126..127
+
+// tiles of a request: none when it has no query rows or a length its table cannot hold
+__device__ __forceinline__ int64_t checked_len(const tf_paged_attn_args& a, int b, int64_t& ext,
+                                               bool& bad) {
+  int64_t L = a.seq_lens[b];
+  ext = a.extend_lens ? a.extend_lens[b] : 1;
+  if (ext < 0) ext = 0;
+  bad = false;
+  if (L < 0) L = 0;
+  if (a.extend_lens == nullptr) {
+    if (L > a.r2t_cols) { bad = true; L = a.r2t_cols; }
+  } else if (ext > 0 && (L > a.r2t_cols || L < ext)) {
+    bad = true;
+    ext = 0;
+  }
+  return L;
+}
+__device__ __forceinline__ int tiles_of(int64_t L, int64_t ext) {
+  return ext > 0 ? (int)((L + kTok - 1) / kTok) : 0;
+}
+
+// The units of a CTA's range in order.  Metadata of the first kCache requests of the range sits in
+// shared memory, further ones are read from global memory as the walk reaches them.
+struct Walker {
+  const tf_paged_attn_args* a;
+  const ReqMeta* cache;
+  int cache_b0, cache_n;
+  int groups;
+  int64_t g, g1;     // next tile, end of the range
+  int b, u;          // its request and group
+  int64_t unit_g;    // first tile of unit (b, u)
+  ReqMeta m;
+  int nt;
+  __device__ __forceinline__ void load(int prev_end) {
+    const int i = b - cache_b0;
+    if (i < cache_n) {
+      m = cache[i];
+    } else {
+      int64_t ext;
+      bool bad;
+      const int64_t L = checked_len(*a, b, ext, bad);
+      m.len = (int32_t)L;
+      m.ext = (int32_t)ext;
+      const int64_t r = a->req_pool_indices[b];
+      if (r < 0 || r >= a->r2t_rows) record_err(a->err, TF_KERR_REQ_RANGE);
+      m.row = r < 0 || r >= a->r2t_rows ? 0 : (int32_t)r;
+      m.start = prev_end;
+    }
+    nt = tiles_of(m.len, m.ext);
+  }
+  // piece [g, g + n) of unit (b, u); false at the end of the range
+  __device__ __forceinline__ bool next(int& t0, int& n) {
+    if (g >= g1) return false;
+    while (g >= unit_g + nt) {
+      unit_g += nt;
+      if (++u == groups) {
+        u = 0;
+        ++b;
+        const int raw = a->extend_lens ? max((int)a->extend_lens[b - 1], 0) : 1;
+        load(m.start + raw);
+      }
+    }
+    t0 = (int)(g - unit_g);
+    const int64_t e = unit_g + nt < g1 ? unit_g + nt : g1;
+    n = (int)(e - g);
+    g = e;
+    return true;
+  }
+};
+
+// N pairs of output values x[i] at dims d0 + 16 i (times the gate's activation) of one query row; the
+// gate is requested as a whole before the first store
+template <typename T, int N>
+__device__ __forceinline__ void put_row(const tf_paged_attn_args& a, int64_t tok, int hq, int d0,
+                                        const float (&x0)[N], const float (&x1)[N], bool wide_o,
+                                        bool wide_g) {
+  float f0[N], f1[N];
+  if (a.gate_mode != TF_GATE_NONE) {
+    const T* gp = (const T*)a.gate + tok * a.gate_stride_tok + (int64_t)hq * a.gate_stride_head + d0;
+    uint32_t w[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (wide_g) {
+        w[i] = *reinterpret_cast<const uint32_t*>(gp + 16 * i);
+      } else {
+        const unsigned short* u = reinterpret_cast<const unsigned short*>(gp + 16 * i);
+        w[i] = u[0] | ((uint32_t)u[1] << 16);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float g0 = unpack_lo<T>(w[i]), g1 = unpack_hi<T>(w[i]);
+      f0[i] = x0[i] * (a.gate_mode == TF_GATE_SILU ? silu_f(g0) : sigmoid_f(g0));
+      f1[i] = x1[i] * (a.gate_mode == TF_GATE_SILU ? silu_f(g1) : sigmoid_f(g1));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) { f0[i] = x0[i]; f1[i] = x1[i]; }
+  }
+  T* op = (T*)a.out + tok * a.out_stride_tok + (int64_t)hq * a.out_stride_head + d0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (wide_o) {
+      *reinterpret_cast<uint32_t*>(op + 16 * i) = pack2_rn<T>(f0[i], f1[i]);
+    } else {
+      op[16 * i] = from_f<T>(f0[i]);
+      op[16 * i + 1] = from_f<T>(f1[i]);
+    }
+  }
+}
+__device__ __forceinline__ bool pairs_ok(const void* p, int64_t s0, int64_t s1) {
+  return ((reinterpret_cast<uintptr_t>(p) & 3) | ((s0 | s1) & 1)) == 0;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    rows_kernel(const tf_paged_attn_args a, const tf_kv_scale sc, const Shape sh, Ws ws) {
+  using C = Cfg<D>;
+  constexpr int kTerms = sizeof(T) == 2 && std::is_same<T, __half>::value ? 3 : 2;
+  constexpr int NJ = D / 64;   // 16-byte reads of a K row per thread
+  constexpr int NM = D / 16;   // dim tiles of O
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int gq = lane >> 2, tq = lane & 3;
+  const int B = a.batch_size;
+  const int G = a.num_q_heads / a.num_kv_heads;
+  const int c = blockIdx.x;
+
+  ReqMeta* cache = reinterpret_cast<ReqMeta*>(smem + sh.ring);
+  int* sh_i = reinterpret_cast<int*>(cache + kCache);  // [16] words
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + sh.ring + C::kFixed);
+
+  // the combine kernel's CTAs may take their places now; they wait for this grid
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // ---- this CTA's range: ts[b] = first tile of request b (all groups of a request are adjacent)
+  int* ts = reinterpret_cast<int*>(smem);  // in the ring's space, before its first copy
+  {
+    const int per = (B + kThreads - 1) / kThreads;
+    const int lo = min(tid * per, B), hi = min(lo + per, B);
+    int sum = 0;
+    for (int b = lo; b < hi; ++b) {
+      int64_t ext;
+      bool bad;
+      const int64_t L = checked_len(a, b, ext, bad);
+      if (bad && c == 0) record_err(a.err, TF_KERR_SLOT_RANGE);
+      ts[b] = sum;
+      sum += tiles_of(L, ext);
+    }
+    int incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) sh_i[warp] = incl;
+    __syncthreads();
+    int base = incl - sum;
+    for (int w = 0; w < warp; ++w) base += sh_i[w];
+    for (int b = lo; b < hi; ++b) ts[b] += base;
+    if (tid == kThreads - 1) ts[B] = base + sum;
+  }
+  __syncthreads();
+  const int NG = sh.groups;
+  const int64_t total = (int64_t)ts[B] * NG;
+  const int64_t want = (total + sh.min_tiles - 1) / sh.min_tiles;
+  const int nctas = want < gridDim.x ? (int)want : (int)gridDim.x;
+  const int64_t beta = sh.piece_cost;
+  // first tile at cost position x = cc (total + beta units) / nctas; a unit's first beta is fixed cost
+  auto boundary = [&](int cc) -> int64_t {
+    if (cc >= nctas) return total;
+    const int64_t U = (int64_t)B * NG;
+    const int64_t x = (int64_t)cc * (total + beta * U) / nctas;
+    int lo = 0, hi = B - 1;  // last request whose cost start ts[b] NG + beta b NG is at most x
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (((int64_t)ts[mid] + beta * mid) * NG <= x) lo = mid; else hi = mid - 1;
+    }
+    const int64_t nt = ts[lo + 1] - ts[lo];
+    const int64_t rem = x - ((int64_t)ts[lo] + beta * lo) * NG;
+    int64_t u = rem / (nt + beta);
+    if (u > NG - 1) u = NG - 1;
+    int64_t off = rem - u * (nt + beta) - beta;
+    off = off < 0 ? 0 : (off > nt ? nt : off);
+    return (int64_t)ts[lo] * NG + u * nt + off;
+  };
+  const int64_t g0 = boundary(c), g1 = boundary(c + 1);
+  if (tid == 0) {
+    ws.cta_g[c] = g0;
+    if (c == gridDim.x - 1) ws.cta_g[c + 1] = total;
+  }
+  // requests without keys: softmax over nothing is NaN
+  if (a.extend_lens == nullptr) {
+    const bool wide = pairs_ok(a.out, a.out_stride_tok, a.out_stride_head);
+    for (int b = c; b < B; b += gridDim.x) {
+      if (ts[b + 1] != ts[b]) continue;
+      for (int e = tid; e < a.num_q_heads * (D / 2); e += kThreads) {
+        T* op = (T*)a.out + (int64_t)b * a.out_stride_tok +
+                (int64_t)(e / (D / 2)) * a.out_stride_head + 2 * (e % (D / 2));
+        if (wide) {
+          *reinterpret_cast<uint32_t*>(op) = pack2_rn<T>(NAN, NAN);
+        } else {
+          op[0] = op[1] = from_f<T>(NAN);
+        }
+      }
+    }
+  }
+  if (g0 >= g1) return;
+  int bf = 0;  // the range's first request: ts[bf] NG <= g0 < ts[bf + 1] NG
+  {
+    int lo = 0, hi = B - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if ((int64_t)ts[mid + 1] * NG > g0) hi = mid; else lo = mid + 1;
+    }
+    bf = lo;
+  }
+  const int cn = min(kCache, B - bf);
+  const int64_t bf_g = (int64_t)ts[bf] * NG;
+  const int bf_nt = ts[bf + 1] - ts[bf];
+  int q_before = bf;  // query tokens before request bf
+  if (a.extend_lens != nullptr) {
+    int s = 0;
+    for (int b = tid; b < bf; b += kThreads) s += max((int)a.extend_lens[b], 0);
+    s = __reduce_add_sync(0xffffffffu, s);
+    __syncthreads();
+    if (lane == 0) sh_i[warp] = s;
+    __syncthreads();
+    q_before = sh_i[0] + sh_i[1] + sh_i[2] + sh_i[3];
+  }
+  for (int i = tid; i < cn; i += kThreads) {
+    const int b = bf + i;
+    int64_t ext;
+    bool bad;
+    ReqMeta m;
+    m.len = (int32_t)checked_len(a, b, ext, bad);
+    m.ext = (int32_t)ext;
+    const int64_t r = a.req_pool_indices[b];
+    if (r < 0 || r >= a.r2t_rows) record_err(a.err, TF_KERR_REQ_RANGE);
+    m.row = r < 0 || r >= a.r2t_rows ? 0 : (int32_t)r;
+    m.start = b;
+    cache[i] = m;
+  }
+  const int nstages = sh.stages * sh.hg;
+  if (tid == 0) {
+    for (int i = 0; i < nstages; ++i) {
+      mbar_init(&bars[2 * i], sh.team * 33);   // full: a transaction arrive and 32 copy arrives a warp
+      mbar_init(&bars[2 * i + 1], sh.team);    // empty
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  // ts is dead from here on: its (generic) accesses come before the first bulk copy over it
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncthreads();
+  if (a.extend_lens != nullptr && tid == 0) {
+    int s = q_before;
+    for (int i = 0; i < cn; ++i) {
+      cache[i].start = s;
+      s += max((int)a.extend_lens[bf + i], 0);
+    }
+  }
+  __syncthreads();
+
+  // ---- this warp's place
+  const int member = warp % sh.team;
+  const int hsel = (warp / sh.team) % sh.hg;
+  const int wsel = warp / (sh.team * sh.hg);
+  const uint32_t ring = smem_u32(smem) + (uint32_t)(hsel * sh.stages * C::kStage);
+  uint64_t* full = bars + 2 * hsel * sh.stages;
+  const int share = kTok / sh.team;  // tokens of a stage that this warp fetches
+
+  Walker prod;
+  prod.a = &a;
+  prod.cache = cache;
+  prod.cache_b0 = bf;
+  prod.cache_n = cn;
+  prod.groups = NG;
+  prod.g = g0;
+  prod.g1 = g1;
+  prod.b = bf;
+  prod.u = bf_nt ? (int)((g0 - bf_g) / bf_nt) : 0;
+  prod.unit_g = bf_g + (int64_t)prod.u * bf_nt;
+  prod.load(0);
+  Walker cons = prod;
+
+  // ---- producer: tiles of this team in sequence, one slot id ahead
+  const int ntiles = (int)(g1 - g0);
+  int pq = wsel;                   // next tile of the range to fetch
+  int p_end = 0, p_first = 0, p_t0 = 0;  // its piece: tiles [p_first, p_end) of the range, from t0
+  int64_t next_raw = 0;
+  auto raw_of = [&](int q) -> int64_t {  // req_to_token entry of this lane's token of tile q
+    while (q >= p_end) {
+      int n;
+      p_first = p_end;
+      if (!prod.next(p_t0, n)) return 0;
+      p_end = p_first + n;
+    }
+    int pos = (p_t0 + q - p_first) * kTok + member * share + lane;
+    if (pos >= prod.m.len) pos = prod.m.len - 1;
+    return a.req_to_token[(int64_t)prod.m.row * a.r2t_stride + pos];
+  };
+  int f_head = 0;  // kv head of the tile whose id is in next_raw
+  auto fetch_id = [&](int q) {
+    if (q < ntiles) next_raw = raw_of(q);
+    f_head = (prod.u / sh.passes) * sh.hg + hsel;
+  };
+  bool ok = true;
+  auto issue = [&]() {
+    if (pq >= ntiles) return;
+    const int st = pq % sh.stages, round = pq / sh.stages;
+    if (round > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait(&full[2 * st + 1], (round - 1) & 1));
+    if (!ok) return;
+    const uint32_t sp = ring + (uint32_t)(st * C::kStage);
+    if (lane == 0) mbar_arrive_expect_tx(&full[2 * st], (uint32_t)(share * 2 * D));
+    __syncwarp();
+    if (lane < share) {
+      const int64_t s = resolve_slot(next_raw, a.num_slots, a.slot_mode, a.err);
+      const int i = member * share + lane;
+      const int64_t off = s * a.kv_stride_slot + (int64_t)f_head * a.kv_stride_head;
+      bulk_g2s(sp + i * C::kKS, (const char*)a.k_buffer + off, D, &full[2 * st]);
+      bulk_g2s(sp + C::kOffV + i * C::kVS, (const char*)a.v_buffer + off, D, &full[2 * st]);
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(sp + C::kOffScale + i * 8),
+                   "l"(sc.data + s * sc.stride_slot + (int64_t)f_head * sc.stride_head)
+                   : "memory");
+    }
+    cp_async_arrive_noinc(&full[2 * st]);
+    pq += sh.wh;
+    fetch_id(pq);
+  };
+  fetch_id(pq);
+  // the ring minus one stage is filled ahead; a stage is refilled one tile after its last use
+  for (int i = 0; i < (sh.stages + sh.wh - 1) / sh.wh; ++i)
+    if (pq < sh.stages) issue();
+
+  const bool wide_o = pairs_ok(a.out, a.out_stride_tok, a.out_stride_head);
+  const bool wide_g = pairs_ok(a.gate, a.gate_stride_tok, a.gate_stride_head);
+  float* merge = reinterpret_cast<float*>(smem + sh.ring + C::kFixed + 16 * nstages);
+  int cfirst = 0;  // tiles of the range before the current piece
+  int t0, n;
+  while (cons.next(t0, n)) {
+    if (cfirst == 0 && tid == 0)
+      ws.cut[c] = CutInfo{cons.b, cons.u, cons.m.start, cons.m.ext, cons.nt, t0};
+    const int b = cons.b, u = cons.u, L = cons.m.len, E = cons.m.ext;
+    const int kvh = (u / sh.passes) * sh.hg + hsel;
+    const int row0 = ((u % sh.passes) * sh.team + member) * kRows;  // first of this warp's rows
+    const int nrows = E * G - row0;                                 // valid ones (may be <= 0)
+    const int64_t qtok0 = a.extend_lens ? cons.m.start : b;
+
+    // ---- Q: row gq of this warp, dims 64 j + 16 tq + [0, 16), as sums of e4m3 terms
+    uint4 qf[kTerms][NJ];
+    float c2[2];
+    {
+      float x[NJ][16];
+      uint32_t am = 0;
+      const int r = row0 + gq;
+      const bool valid = gq < nrows && qtok0 + r / G < a.num_tokens;
+      const T* qp = (const T*)a.q + (qtok0 + r / G) * a.q_stride_tok +
+                    (int64_t)(kvh * G + r % G) * a.q_stride_head + 16 * tq;
+      const bool vec = ((reinterpret_cast<uintptr_t>(a.q) & 15) |
+                        ((a.q_stride_tok | a.q_stride_head) & 7)) == 0;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        if (valid && vec) {
+#pragma unroll
+          for (int hlf = 0; hlf < 2; ++hlf) {
+            const uint4 w = *reinterpret_cast<const uint4*>(qp + 64 * j + 8 * hlf);
+            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              x[j][8 * hlf + 2 * i] = unpack_lo<T>(ww[i]);
+              x[j][8 * hlf + 2 * i + 1] = unpack_hi<T>(ww[i]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[j][i] = valid ? to_f(qp[64 * j + i]) : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) am = max(am, kv8::abs_bits(x[j][i]));
+      }
+      am = max(am, __shfl_xor_sync(0xffffffffu, am, 1));
+      am = max(am, __shfl_xor_sync(0xffffffffu, am, 2));
+      const int ex = max((int)(am >> 23) - 127, -100);  // row maximum in [2^ex, 2^(ex+1))
+      const float mul = pow2i(7 - ex);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[j][i] *= mul;
+#pragma unroll
+        for (int k = 0; k < kTerms; ++k) {
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t lo = term2(x[j][4 * i], x[j][4 * i + 1]);
+            w[i] = lo | (term2(x[j][4 * i + 2], x[j][4 * i + 3]) << 16);
+          }
+          qf[k][j] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      // logit factor of row gq; a row that is not finite gives NaN logits
+      const float cr = am < 0x7f800000u ? a.scale * kLog2e * pow2i(max(ex - 7, -126)) : NAN;
+      c2[0] = __shfl_sync(0xffffffffu, cr, (2 * tq) * 4);
+      c2[1] = __shfl_sync(0xffffffffu, cr, (2 * tq + 1) * 4);
+    }
+    int lim[2];  // tokens visible to rows 2 tq and 2 tq + 1
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int i = (row0 + 2 * tq + k) / G;
+      lim[k] = i < E ? L - E + i + 1 : L;
+    }
+    const int lim_min = L - E + row0 / G + 1;  // tokens visible to every row of the warp
+
+    float acc[NM][4];
+#pragma unroll
+    for (int m = 0; m < NM; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
+    float M[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    // this team's tiles of the piece: range positions q with q % wh == wsel
+    int q = cfirst + (wsel - cfirst % sh.wh + sh.wh) % sh.wh;
+    for (; q < cfirst + n && ok; q += sh.wh) {
+      const int st = q % sh.stages, round = q / sh.stages;
+      ok = __all_sync(0xffffffffu, mbar_wait(&full[2 * st], round & 1));
+      if (!ok) break;
+      const uint32_t sp = ring + (uint32_t)(st * C::kStage);
+      const int tok0 = (t0 + q - cfirst) * kTok;
+      if (nrows > 0) {
+        // ---- S^T = K8.Q^T: tokens 16 mt + gq (+8), rows 2 tq, 2 tq + 1; two chains per tile
+        float s[2][2][4];
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int h2 = 0; h2 < 2; ++h2) s[mt][h2][0] = s[mt][h2][1] = s[mt][h2][2] = s[mt][h2][3] = 0.f;
+        const uint32_t kp = sp + gq * C::kKS + 16 * tq;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) {
+            const uint4 k0 = lds128(kp + (16 * mt) * C::kKS + 64 * j);
+            const uint4 k1 = lds128(kp + (16 * mt + 8) * C::kKS + 64 * j);
+#pragma unroll
+            for (int k = 0; k < kTerms; ++k) {
+              mma8(s[mt][0], k0.x, k1.x, k0.y, k1.y, qf[k][j].x, qf[k][j].y);
+              mma8(s[mt][1], k0.z, k1.z, k0.w, k1.w, qf[k][j].z, qf[k][j].w);
+            }
+          }
+        }
+        // ---- scales of tokens gq + 8 i.  One that is not finite: NaN logits for the rows that see
+        // the token, weight 0 for the others
+        float ksc[4], vsc[4], vmax = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 p = lds_f2(sp + C::kOffScale + (gq + 8 * i) * 8);
+          const bool fin = kv8::abs_bits(p.x) < 0x7f800000u && kv8::abs_bits(p.y) < 0x7f800000u;
+          ksc[i] = fin ? p.x : NAN;
+          vsc[i] = fin ? p.y : 0.f;
+          vmax = fmaxf(vmax, fabsf(vsc[i]));
+        }
+        float sv[4][2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int e = 2 * (i & 1) + k;
+            sv[i][k] = (s[i >> 1][0][e] + s[i >> 1][1][e]) * ksc[i] * c2[k];
+          }
+        if (tok0 + kTok > lim_min) {  // some token is hidden from some row
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              if (tok0 + gq + 8 * i >= lim[k]) sv[i][k] = -INFINITY;
+        }
+        float mx[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          mx[k] = fmaxf(fmaxf(sv[0][k], sv[1][k]), fmaxf(sv[2][k], sv[3][k]));
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+          mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], o));
+          mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], o));
+          vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+        }
+        const int ev = min(max((int)(__float_as_uint(vmax) >> 23) - 127, -100), 126);
+        const float vmul = pow2i(max(7 - ev, -126)), lmul = pow2i(max(-ev, -126));
+        float al[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          // a tile hidden from the row as a whole keeps M (and -inf - -inf out of the exponent)
+          const float mn = fmaxf(M[k], mx[k] + (float)ev);
+          al[k] = M[k] == mn ? 1.f : ex2(M[k] - mn);
+          M[k] = mn;
+          const float sub = mn == -INFINITY && tok0 >= lim[k] ? 0.f : (float)ev - mn;
+          float ls = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            sv[i][k] = ex2(sv[i][k] + sub);
+            ls += sv[i][k];
+          }
+          l[k] = fmaf(ls, lmul, l[k] * al[k]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sv[i][k] *= vsc[i] * vmul;
+        }
+        if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {
+#pragma unroll
+          for (int m = 0; m < NM; ++m) {
+            acc[m][0] *= al[0];
+            acc[m][1] *= al[1];
+            acc[m][2] *= al[0];
+            acc[m][3] *= al[1];
+          }
+        }
+        // ---- W^T as B fragments: 16-bit elements (token gq, token gq + 8) of rows 2 tq, 2 tq + 1,
+        // transposed to row gq, tokens 2 tq, 2 tq + 8, 2 tq + 1, 2 tq + 9
+        uint32_t wb[kTerms][2];
+#pragma unroll
+        for (int k = 0; k < kTerms; ++k) {
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            const uint32_t lo = term2(sv[2 * hf][0], sv[2 * hf + 1][0]);
+            const uint32_t hi = term2(sv[2 * hf][1], sv[2 * hf + 1][1]);
+            wb[k][hf] = movmatrix_t(lo | (hi << 16));
+          }
+        }
+        // ---- O^T += V8^T.W^T
+        const uint32_t vp = sp + C::kOffV + lane * C::kVS;
+#pragma unroll
+        for (int m = 0; m < NM; ++m) {
+          uint32_t r[4];
+          ldsm4_t(vp + 16 * m, r);
+          const uint32_t a0 = __byte_perm(r[0], r[1], 0x6240), a1 = __byte_perm(r[0], r[1], 0x7351);
+          const uint32_t a2 = __byte_perm(r[2], r[3], 0x6240), a3 = __byte_perm(r[2], r[3], 0x7351);
+#pragma unroll
+          for (int k = 0; k < kTerms; ++k) mma8(acc[m], a0, a1, a2, a3, wb[k][0], wb[k][1]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[2 * st + 1]);
+      issue();
+    }
+    cfirst += n;
+
+    // ---- the piece is done: O / l, or partials when the unit goes on in another CTA
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+      l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
+      l[1] += __shfl_xor_sync(0xffffffffu, l[1], o);
+    }
+    if (sh.wh > 1) {  // merge the teams of a head: the first one ends up with all of it
+      float* mr = merge + warp * kRows * (C::kMergeStride + 2);
+      float* mlr = mr + kRows * C::kMergeStride;
+      if (wsel > 0) {
+        if (gq == 0) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            mlr[2 * (2 * tq + k)] = M[k];
+            mlr[2 * (2 * tq + k) + 1] = l[k];
+          }
+        }
+#pragma unroll
+        for (int m = 0; m < NM; ++m) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            *reinterpret_cast<float2*>(mr + (2 * tq + k) * C::kMergeStride + 16 * m + 2 * gq) =
+                make_float2(acc[m][k], acc[m][2 + k]);
+        }
+      }
+      __syncthreads();
+      if (wsel == 0) {
+        for (int w = 1; w < sh.wh; ++w) {
+          const float* om = merge + (warp + w * sh.team * sh.hg) * kRows * (C::kMergeStride + 2);
+          const float* oml = om + kRows * C::kMergeStride;
+          float f[2], fo[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float mo = oml[2 * (2 * tq + k)], lo = oml[2 * (2 * tq + k) + 1];
+            const float mn = fmaxf(M[k], mo);
+            f[k] = M[k] == mn ? 1.f : ex2(M[k] - mn);
+            fo[k] = mo == mn ? 1.f : ex2(mo - mn);
+            M[k] = mn;
+            l[k] = l[k] * f[k] + lo * fo[k];
+          }
+#pragma unroll
+          for (int m = 0; m < NM; ++m) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float2 v =
+                  *reinterpret_cast<const float2*>(om + (2 * tq + k) * C::kMergeStride + 16 * m + 2 * gq);
+              acc[m][k] = acc[m][k] * f[k] + v.x * fo[k];
+              acc[m][2 + k] = acc[m][2 + k] * f[k] + v.y * fo[k];
+            }
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (wsel > 0 || nrows <= 0) continue;
+    const int nt = cons.nt;
+    if (t0 == 0 && n == nt) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int r = row0 + 2 * tq + k;
+        const int64_t tok = qtok0 + r / G;
+        if (r >= E * G || tok >= a.num_tokens) continue;
+        const float inv = (1.f / 128.f) / l[k];
+        float x0[NM], x1[NM];
+#pragma unroll
+        for (int m = 0; m < NM; ++m) {
+          x0[m] = acc[m][k] * inv;
+          x1[m] = acc[m][2 + k] * inv;
+        }
+        put_row<T, NM>(a, tok, kvh * G + r % G, 2 * gq, x0, x1, wide_o, wide_g);
+      }
+    } else {
+      const int ps = ((2 * c + (cfirst == n ? 0 : 1)) * kWarps + hsel * sh.team + member) * kRows;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int r = 2 * tq + k;
+        if (gq == 0) *reinterpret_cast<float2*>(ws.ml + (ps + r) * 2) = make_float2(M[k], l[k]);
+#pragma unroll
+        for (int m = 0; m < NM; ++m)
+          *reinterpret_cast<float2*>(ws.o + (int64_t)(ps + r) * D + 16 * m + 2 * gq) =
+              make_float2(acc[m][k], acc[m][2 + k]);
+      }
+    }
+  }
+  if (!ok) {  // a wait gave up: report it, and leave no copy of this warp in flight
+    if (lane == 0) record_err(a.err, TF_KERR_TIMEOUT);
+    for (int i = 0; i < sh.stages; ++i) {
+      const int q = pq - sh.wh - i;
+      if (q >= 0) mbar_wait(&full[2 * (q % sh.stages)], (q / sh.stages) & 1);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// combine: CTA (c, w) merges warp place w of the unit that the boundary of range c cuts, when it is
+// the first boundary inside that unit.  PG groups of 256 threads take the pieces in turn; a thread
+// holds 4 values of one row.
+// ---------------------------------------------------------------------------------------------
+template <typename T, int D, int PG>
+__global__ void __launch_bounds__(256 * PG)
+    combine_kernel(const tf_paged_attn_args a, const Shape sh, Ws ws) {
+  constexpr int kVec = D / 4;  // 4-value vectors of a row
+  constexpr int kSteps = (kRows * kVec + 255) / 256;
+  __shared__ float red[PG > 1 ? PG : 1][PG > 1 ? 256 : 1][PG > 1 ? 5 : 1];
+  __shared__ float s_M[kRows];
+  __shared__ int64_t s_g[kMaxCtas + 1];
+  __shared__ int s_slot[kMaxCtas];
+  __shared__ int s_np;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int c = blockIdx.x + 1, w = blockIdx.y;
+  const int n = gridDim.x + 1;  // decode CTAs
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const CutInfo ci = ws.cut[c];
+  for (int i = tid; i <= n; i += 256 * PG) s_g[i] = ws.cta_g[i];
+  __syncthreads();
+  const int64_t g = s_g[c];
+  if (g >= s_g[n] || s_g[c + 1] == g || ci.t0 == 0) return;  // empty range, or nothing cut here
+  const int64_t su = g - ci.t0, eu = su + ci.nt;
+  int c0 = c - 1;
+  while (s_g[c0] == g) --c0;   // empty ranges before this one
+  if (s_g[c0] > su) return;    // not the first boundary inside the unit
+  const int G = a.num_q_heads / a.num_kv_heads;
+  const int hsel = w / sh.team, member = w % sh.team;
+  const int row0 = ((ci.u % sh.passes) * sh.team + member) * kRows;
+  if (row0 >= ci.ext * G) return;
+  // partial rows of the unit's pieces, one per range that is not empty: its first piece when the
+  // range starts inside the unit (or with it), else its last
+  if (tid < 32) {
+    int np = 0;
+    for (int c1 = c0; c1 < n && s_g[c1] < eu; c1 += 32) {
+      const int cc = c1 + lane;
+      const bool has = cc < n && s_g[cc] < eu && s_g[cc + 1] > s_g[cc];
+      const unsigned m = __ballot_sync(0xffffffffu, has);
+      if (has) s_slot[np + __popc(m & ((1u << lane) - 1))] =
+          ((2 * cc + (s_g[cc] >= su ? 0 : 1)) * kWarps + w) * kRows;
+      np += __popc(m);
+    }
+    if (lane == 0) s_np = np;
+  }
+  __syncthreads();
+  const int np = s_np;
+  {  // the rows' maxima over all pieces: eight threads a piece in the first warp
+    float m = -INFINITY;
+    if (tid < 32) {
+      const int r = lane & 7;
+      for (int i = lane >> 3; i < np; i += 4) m = fmaxf(m, ws.ml[(s_slot[i] + r) * 2]);
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+      if (lane < 8) s_M[lane] = m;
+    }
+  }
+  __syncthreads();
+  const int grp = tid / 256, t = tid % 256;
+#pragma unroll 1
+  for (int step = 0; step < kSteps; ++step) {
+    const int e = step * 256 + t;
+    const int r = e / kVec, v = e % kVec;
+    float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+    if (r < kRows) {
+      const float M = s_M[r];
+#pragma unroll 8
+      for (int i = grp; i < np; i += PG) {
+        const int s = s_slot[i] + r;
+        const float2 ml = *reinterpret_cast<const float2*>(ws.ml + s * 2);
+        const float4 x = *reinterpret_cast<const float4*>(ws.o + (int64_t)s * D + 4 * v);
+        const float f = ml.x == M ? 1.f : ex2(ml.x - M);
+        o[0] = fmaf(f, x.x, o[0]);
+        o[1] = fmaf(f, x.y, o[1]);
+        o[2] = fmaf(f, x.z, o[2]);
+        o[3] = fmaf(f, x.w, o[3]);
+        l = fmaf(f, ml.y, l);
+      }
+    }
+    if constexpr (PG > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) red[grp][t][i] = o[i];
+      red[grp][t][4] = l;
+      __syncthreads();
+      if (grp == 0) {
+#pragma unroll
+        for (int p = 1; p < PG; ++p) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] += red[p][t][i];
+          l += red[p][t][4];
+        }
+      }
+    }
+    const int rr = row0 + r;
+    const int64_t tok = ci.start + rr / G;
+    if (grp == 0 && r < kRows && rr < ci.ext * G && tok < a.num_tokens) {
+      const int hq = ((ci.u / sh.passes) * sh.hg + hsel) * G + rr % G;
+      const float inv = (1.f / 128.f) / l;
+      const bool wo = pairs_ok(a.out, a.out_stride_tok, a.out_stride_head);
+      const bool wg = pairs_ok(a.gate, a.gate_stride_tok, a.gate_stride_head);
+#pragma unroll
+      for (int h2 = 0; h2 < 2; ++h2) {
+        const float x0[1] = {o[2 * h2] * inv}, x1[1] = {o[2 * h2 + 1] * inv};
+        put_row<T, 1>(a, tok, hq, 4 * v + 2 * h2, x0, x1, wo, wg);
+      }
+    }
+  }
+}
+
+inline int gcd(int a, int b) { return b == 0 ? a : gcd(b, a % b); }
+
+// how a call is divided (max_rows: query rows of one kv head of the longest request)
+template <int D>
+static Shape shape_of(const tf_paged_attn_args& a, int num_sms) {
+  using C = Cfg<D>;
+  const int G = a.num_q_heads / a.num_kv_heads;
+  const int64_t rows = (int64_t)G * (a.extend_lens ? a.max_extend_len : 1);
+  const int need = rows > kRows ? (int)((rows + kRows - 1) / kRows) : 1;
+  Shape s;
+  s.team = need <= 1 ? 1 : (need <= 2 ? 2 : 4);
+  s.passes = (need + s.team - 1) / s.team;
+  s.hg = gcd(a.num_kv_heads, kWarps / s.team);
+  s.wh = kWarps / (s.team * s.hg);
+  s.groups = a.num_kv_heads / s.hg * s.passes;
+  int stages = C::kStages;
+  auto bytes = [&](int n) {
+    return n * C::kStage + C::kFixed + 16 * n + (s.wh > 1 ? C::kMerge : 0);
+  };
+  while (bytes(stages / s.hg * s.hg) > 232448) --stages;
+  s.stages = stages / s.hg;
+  s.ring = s.stages * s.hg * C::kStage;
+  s.smem = bytes(s.stages * s.hg);
+  s.nctas = num_sms;
+  s.min_tiles = 2 * s.wh;
+  s.piece_cost = 8;
+  return s;
+}
+
+template <typename T, int D>
+static cudaError_t launch_td(const tf_paged_attn_args& a, const tf_kv_scale& sc, void* wsp,
+                             int num_sms, cudaStream_t s) {
+  if (num_sms > kMaxCtas) num_sms = kMaxCtas;
+  const Shape sh = shape_of<D>(a, num_sms);
+  if ((int64_t)(a.batch_size + 1) * 4 > sh.ring) return cudaErrorInvalidValue;
+  const Ws ws = carve(wsp, num_sms, D);
+  cudaError_t e = cudaFuncSetAttribute(rows_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       sh.smem);
+  if (e != cudaSuccess) return e;
+  rows_kernel<T, D><<<num_sms, kThreads, sh.smem, s>>>(a, sc, sh, ws);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || num_sms == 1) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(num_sms - 1), (unsigned)(sh.hg * sh.team));
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  // few units, so many pieces each: four groups of threads share them
+  const bool deep = (int64_t)a.batch_size * sh.groups * 8 < num_sms;
+  cfg.blockDim = dim3(deep ? 1024 : 256);
+  return deep ? cudaLaunchKernelEx(&cfg, combine_kernel<T, D, 4>, a, sh, ws)
+              : cudaLaunchKernelEx(&cfg, combine_kernel<T, D, 1>, a, sh, ws);
+}
+
+template <typename T>
+static cudaError_t launch_t(const tf_paged_attn_args& a, const tf_kv_scale& sc, void* ws,
+                            int num_sms, cudaStream_t s) {
+  switch (a.head_dim) {
+    case 64: return launch_td<T, 64>(a, sc, ws, num_sms, s);
+    case 128: return launch_td<T, 128>(a, sc, ws, num_sms, s);
+    default: return launch_td<T, 256>(a, sc, ws, num_sms, s);
+  }
+}
+
+}  // namespace rows8
+
+bool paged_fp8_rows_supported(const tf_paged_attn_args& a) {
+  if (a.dtype != TF_DTYPE_BF16 && a.dtype != TF_DTYPE_F16) return false;
+  if (a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256) return false;
+  if (a.batch_size > rows8::kMaxBatch || a.r2t_rows > 0x7fffffff || a.r2t_cols > 0x7fffffff)
+    return false;
+  auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  return al(a.k_buffer) && al(a.v_buffer) && a.kv_stride_slot % 16 == 0 && a.kv_stride_head % 16 == 0;
+}
+
+size_t paged_fp8_rows_workspace(const tf_paged_attn_args& a, int num_sms) {
+  return rows8::ws_bytes(num_sms < rows8::kMaxCtas ? num_sms : rows8::kMaxCtas, a.head_dim);
+}
+
+cudaError_t launch_paged_fp8_rows(const tf_paged_attn_args& a, const tf_kv_scale& sc, void* ws,
+                                  int num_sms, cudaStream_t s) {
+  if (a.batch_size == 0) return cudaSuccess;
+  return a.dtype == TF_DTYPE_BF16 ? rows8::launch_t<__nv_bfloat16>(a, sc, ws, num_sms, s)
+                                  : rows8::launch_t<__half>(a, sc, ws, num_sms, s);
+}
+
+}  // namespace tf

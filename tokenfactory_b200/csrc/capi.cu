@@ -502,7 +502,7 @@ tf_status tf_attn_prologue_fp8(const tf_attn_prologue_args* a, const tf_kv_scale
 // Which kernel a call over an 8-bit pool takes: the few-rows kernel while a request has at most
 // kFewRows query rows per kv head, the CUDA-core kernel otherwise.
 enum class Fp8Path { kRows, kSimt };
-constexpr int64_t kFewRows = 32;
+constexpr int64_t kFewRows = 64;
 
 static Fp8Path fp8_path(const tf_paged_attn_args& a, bool decode) {
   const int64_t rows = (int64_t)(a.num_q_heads / a.num_kv_heads) * (decode ? 1 : a.max_extend_len);

@@ -1,35 +1,32 @@
 // Paged GQA attention over the 8-bit K/V pool for few query rows per kv head: decode, and extends of
-// a few tokens per request (drafted tokens).  HBM-bound: every K/V row is read once, and the e4m3
-// codes go into the tensor cores as they are.
+// a few tokens per request (drafted tokens).  HBM-bound: every K/V row is read once.
 //
 // Mathematics.  A token j has codes K8_j, V8_j and scales ks_j, vs_j; a query row has logits
 //   s_j = (q . K8_j) ks_j scale log2(e)      out = sum_j 2^(s_j) vs_j V8_j / sum_j 2^(s_j).
-// Both products run as mma.m16n8k32 e4m3 x e4m3 with fp32 sums (exact products; measured on
-// 2048-long sums: relative error 1e-7).  The operands that are not codes are sums of e4m3 terms:
-//   q, scaled by a power of two per row:  hi + lo (bfloat16: all 8 bits), + a third for float16;
-//   the weight w_j = 2^(s_j + ev - M) vs_j 2^(7 - ev): as many terms, i.e. to 8 or 12 bits, below
-//   2^-17 of the largest to that absolute step.  ev is the exponent of the largest vs of a tile and
-//   M the running maximum of s_j + ev, so that w stays under 448 whatever the scales are; the sum
-//   of weights l = sum 2^(s_j - M) is fp32 and unsplit.
-// Measured alternatives: converting codes to f16 costs two conversions per four codes, and
-// mma.m16n8k16 f16 issues at half the rate of the e4m3 form at half its depth.
+// Both products run as mma.m16n8k16 f16 with fp32 sums.  e4m3 codes are exact in f16; q is scaled by
+// a power of two per row into f16's range (exact for bfloat16 too); the only rounding before the
+// output is that of the weights w_j = 2^(s_j + ev - M) vs_j 2^(7 - ev) to f16 (11 bits).  ev is the
+// exponent of the largest vs of a tile and M the running maximum of s_j + ev, so that w stays in
+// f16's range whatever the scales are; the sum of weights l = sum 2^(s_j - M) is fp32.
+// mma.m16n8k32 on the codes themselves was measured at 36 clocks a warp instruction, against 8 for
+// the f16 form with half its depth plus its conversions.
 //
-// Fragments.  S^T = K8.Q^T: A = 16 tokens x 32 dims.  A thread's 16-byte read of a token's row is its
-// A fragment of two k-steps for the dim order 64 j + 16 t + {0..3 | 4..7}, {8..11 | 12..15}
-// (t = lane % 4), and Q^T is held in the same order.  O^T = V8^T.W^T: A = 16 dims x 32 tokens, from
-// ldmatrix.trans on pairs of codes and byte permutes: row r of the fragment is dim 2 r, row r + 8 dim
-// 2 r + 1, and the tokens of a thread come in the order 2t, 2t+8, 2t+1, 2t+9, which movmatrix gives
-// the weights as well (two tokens' codes per 16-bit element).
+// Fragments.  S^T = K8.Q^T: A = 16 tokens x 16 dims.  A thread's 16-byte read of a token's row is its A
+// fragment of four k-steps for the dim order 64 j + 16 t + 4 i + {0,1 | 2,3} (t = lane % 4), and Q^T is
+// held in the same order.  O^T = V8^T.W^T: A = 16 dims x 16 tokens, from ldmatrix.trans on pairs of
+// codes and a byte permute; row r of the fragment is dim 2 r, row r + 8 dim 2 r + 1.  W^T comes from
+// the logits' layout through movmatrix.
 //
-// Work.  A CTA has four warps.  TEAM of them (1, 2 or 4) share a ring of 32-token stages and take
-// eight query rows each; HG kv heads of a group run side by side, so that a token's rows of all
-// heads, its scales and its slot id are read at about the same time; the WH = 4 / (TEAM HG) teams of
-// a head take its tiles in turn and merge in shared memory.  The sequence of (request, head group)
-// units, each of ceil(len / 32) tiles, is cut into one range per CTA, balanced by tiles plus a fixed
-// cost per unit; every CTA finds its own range from the lengths (a scan of the batch in shared
-// memory: no plan launch).  Units cut by a boundary leave (M, l, O) partials for a combine kernel.
-// Rows are fetched by bulk copies, a stage's copies completing on its mbarrier, and the ring runs on
-// across units.
+// Work.  A CTA has eight warps.  TEAM of them (a power of two) share stages of 32 tokens of one kv
+// head and take eight query rows each; HG kv heads of a group run side by side, so that a token's
+// rows of all heads, its scales and its slot id are read at about the same time; the
+// WH = 8 / (TEAM HG) teams of a head take its tiles in turn and merge in shared memory.  The sequence
+// of (request, head group) units, each of ceil(len / 32) tiles, is cut into one range per CTA,
+// balanced by tiles plus a fixed cost per unit; every CTA finds its own range from the lengths (a scan
+// of the batch in shared memory: no plan launch).  Units cut by a boundary leave (M, l, O) partials
+// for a combine kernel.  Rows are fetched by 16-byte cp.async (a bulk copy per row was measured at
+// 528 us against 349 us for 128 requests: copies of 256 bytes), a stage's copies completing on its
+// mbarrier, and the ring of stages runs on across units.
 #include <type_traits>
 
 #include "common.cuh"
@@ -39,7 +36,7 @@
 namespace tf {
 namespace rows8 {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kTok = 32;  // tokens of a tile
 constexpr int kRows = 8;  // query rows of a warp (n of the mma tiles)
@@ -61,9 +58,10 @@ struct Cfg {
   static constexpr int kOffV = kTok * kKS;
   static constexpr int kOffScale = kOffV + kTok * kVS;
   static constexpr int kStage = kOffScale + kTok * 8;
-  static constexpr int kStages = D == 256 ? 12 : (D == 128 ? 20 : 40);  // without a merge buffer
-  static constexpr int kMergeStride = D + 4;  // floats per row
-  static constexpr int kMerge = kWarps * kRows * (kMergeStride + 2) * 4;
+  static constexpr int kStages = D == 256 ? 12 : (D == 128 ? 20 : 40);  // at most
+  // merge of a head's teams: 64 dims of a row at a time, then its (M, l)
+  static constexpr int kMergeStride = 64 + 4;
+  static constexpr int kMergeRows = kRows * (kMergeStride + 2);  // floats per warp
   static constexpr int kFixed = kCache * (int)sizeof(ReqMeta) + 64;
   static_assert(kStage % 16 == 0 && kKS % 16 == 0 && kVS % 16 == 0, "bulk copy alignment");
 };
@@ -73,7 +71,7 @@ struct Shape {
   int team, hg, wh;   // warps sharing a ring, kv heads side by side, teams taking a head's tiles in turn
   int groups;         // units per request
   int passes;         // row passes of a kv head (more than 8 * team query rows)
-  int stages;         // ring stages per kv head of a group
+  int stages;         // ring stages
   int nctas;
   int min_tiles;      // tiles worth a CTA of their own
   int piece_cost;     // fixed cost of a unit in tiles
@@ -88,8 +86,8 @@ struct CutInfo {
 struct Ws {
   int64_t* cta_g;  // [nctas + 1] first tile of each CTA's range
   CutInfo* cut;    // [nctas]
-  float* ml;       // [2 nctas][4 warps][8 rows][2]
-  float* o;        // [2 nctas][4 warps][8 rows][D]
+  float* ml;       // [2 nctas][8 warps][8 rows][2]
+  float* o;        // [2 nctas][8 warps][8 rows][D]
 };
 
 __host__ __device__ inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -111,23 +109,23 @@ inline size_t ws_bytes(int nctas, int D) {
          (size_t)2 * nctas * kWarps * kRows * D * 4;
 }
 
-__device__ __forceinline__ void mma8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                     uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-      "{%8,%9}, {%0,%1,%2,%3};"
+__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                      uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
+// the low and the high two codes of a word as f16 pairs
+__device__ __forceinline__ uint32_t cvt_lo(uint32_t w) {
+  uint32_t r;
+  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %1;\n cvt.rn.f16x2.e4m3x2 %0, a;\n}" : "=r"(r) : "r"(w));
+  return r;
 }
-__device__ __forceinline__ float2 lds_f2(uint32_t a) {
-  float2 v;
-  asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a));
-  return v;
+__device__ __forceinline__ uint32_t cvt_hi(uint32_t w) {
+  uint32_t r;
+  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %1;\n cvt.rn.f16x2.e4m3x2 %0, b;\n}" : "=r"(r) : "r"(w));
+  return r;
 }
 __device__ __forceinline__ void ldsm4_t(uint32_t a, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -144,18 +142,24 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// the two values of a code pair
-__device__ __forceinline__ float2 value2(uint32_t c) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)c, __NV_E4M3);
-  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+// Stage use counters.  A stage passes from team to team, and one team can be more than a ring ahead of
+// another, so "consumed in round r" is a count that only grows: an mbarrier's parity cannot tell a
+// round from the one before the last.
+__device__ __forceinline__ void count_use(uint32_t* c) {
+  asm volatile("red.release.cta.shared::cta.add.u32 [%0], 1;" ::"r"(smem_u32(c)) : "memory");
 }
-// next e4m3 terms of the pair (a, b); a and b become what is left
-__device__ __forceinline__ uint32_t term2(float& a, float& b) {
-  const uint32_t c = kv8::code2(a, b);
-  const float2 v = value2(c);
-  a -= v.x;
-  b -= v.y;
-  return c;
+__device__ __forceinline__ uint32_t uses(const uint32_t* c) {
+  uint32_t v;
+  asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(smem_u32(c)) : "memory");
+  return v;
+}
+__device__ __forceinline__ bool wait_uses(const uint32_t* c, uint32_t n) {  // bounded
+  if (uses(c) >= n) return true;
+  const uint64_t t0 = global_ns();
+  for (uint32_t it = 0;; ++it) {
+    if (uses(c) >= n) return true;
+    if ((it & 63u) == 63u && global_ns() - t0 > kSpinLimitNs) return false;
+  }
 }
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126..127
 
@@ -276,7 +280,6 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
     rows_kernel(const tf_paged_attn_args a, const tf_kv_scale sc, const Shape sh, Ws ws) {
   using C = Cfg<D>;
-  constexpr int kTerms = sizeof(T) == 2 && std::is_same<T, __half>::value ? 3 : 2;
   constexpr int NJ = D / 64;   // 16-byte reads of a K row per thread
   constexpr int NM = D / 16;   // dim tiles of O
   extern __shared__ __align__(128) unsigned char smem[];
@@ -289,6 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   ReqMeta* cache = reinterpret_cast<ReqMeta*>(smem + sh.ring);
   int* sh_i = reinterpret_cast<int*>(cache + kCache);  // [16] words
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + sh.ring + C::kFixed);
+  uint32_t* used = reinterpret_cast<uint32_t*>(bars + sh.stages);  // warps done with a stage, in all
 
   // the combine kernel's CTAs may take their places now; they wait for this grid
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -386,7 +390,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     if (lane == 0) sh_i[warp] = s;
     __syncthreads();
-    q_before = sh_i[0] + sh_i[1] + sh_i[2] + sh_i[3];
+    q_before = 0;
+    for (int w = 0; w < kWarps; ++w) q_before += sh_i[w];
   }
   for (int i = tid; i < cn; i += kThreads) {
     const int b = bf + i;
@@ -401,11 +406,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     m.start = b;
     cache[i] = m;
   }
-  const int nstages = sh.stages * sh.hg;
+  const int nstages = sh.stages;
   if (tid == 0) {
     for (int i = 0; i < nstages; ++i) {
-      mbar_init(&bars[2 * i], sh.team * 33);   // full: a transaction arrive and 32 copy arrives a warp
-      mbar_init(&bars[2 * i + 1], sh.team);    // empty
+      mbar_init(&bars[i], sh.team * 32);  // every lane's copies have landed
+      used[i] = 0;
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -425,8 +430,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int member = warp % sh.team;
   const int hsel = (warp / sh.team) % sh.hg;
   const int wsel = warp / (sh.team * sh.hg);
-  const uint32_t ring = smem_u32(smem) + (uint32_t)(hsel * sh.stages * C::kStage);
-  uint64_t* full = bars + 2 * hsel * sh.stages;
+  const uint32_t ring = smem_u32(smem);
+  uint64_t* full = bars;
+  // tile q of head hsel of the group is number q hg + hsel of the ring
+  const int step = sh.wh * sh.hg, first = wsel * sh.hg + hsel;
   const int share = kTok / sh.team;  // tokens of a stage that this warp fetches
 
   Walker prod;
@@ -465,37 +472,68 @@ __global__ void __launch_bounds__(kThreads, 1)
     f_head = (prod.u / sh.passes) * sh.hg + hsel;
   };
   bool ok = true;
+  int p_st = first, p_round = 0;  // stage and round of tile pq
   auto issue = [&]() {
     if (pq >= ntiles) return;
-    const int st = pq % sh.stages, round = pq / sh.stages;
-    if (round > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait(&full[2 * st + 1], (round - 1) & 1));
+    if (p_round > 0)
+      ok = __all_sync(0xffffffffu, ok && wait_uses(&used[p_st], (uint32_t)(p_round * sh.team)));
     if (!ok) return;
-    const uint32_t sp = ring + (uint32_t)(st * C::kStage);
-    if (lane == 0) mbar_arrive_expect_tx(&full[2 * st], (uint32_t)(share * 2 * D));
-    __syncwarp();
-    if (lane < share) {
-      const int64_t s = resolve_slot(next_raw, a.num_slots, a.slot_mode, a.err);
-      const int i = member * share + lane;
-      const int64_t off = s * a.kv_stride_slot + (int64_t)f_head * a.kv_stride_head;
-      bulk_g2s(sp + i * C::kKS, (const char*)a.k_buffer + off, D, &full[2 * st]);
-      bulk_g2s(sp + C::kOffV + i * C::kVS, (const char*)a.v_buffer + off, D, &full[2 * st]);
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(sp + C::kOffScale + i * 8),
-                   "l"(sc.data + s * sc.stride_slot + (int64_t)f_head * sc.stride_head)
-                   : "memory");
+    const uint32_t sp = ring + (uint32_t)(p_st * C::kStage);
+    const int64_t sl = resolve_slot(next_raw, a.num_slots, a.slot_mode, lane < share ? a.err : nullptr);
+    // row offset of this lane's token in 16-byte pieces (32 bits: the host checks)
+    const uint32_t off =
+        (uint32_t)((sl * a.kv_stride_slot + (int64_t)f_head * a.kv_stride_head) >> 4);
+    constexpr int CPR = D / 16;    // 16-byte pieces of a row
+    constexpr int RPI = 32 / CPR;  // rows a warp instruction copies
+    const int sub = lane / CPR, ch = lane % CPR;
+    const char* kg = (const char*)a.k_buffer + 16 * ch;
+    const char* vg = (const char*)a.v_buffer + 16 * ch;
+    const uint32_t kd = sp + (member * share + sub) * C::kKS + 16 * ch;
+    const uint32_t vd = sp + C::kOffV + (member * share + sub) * C::kVS + 16 * ch;
+    auto rows = [&](int i0, auto n) {
+      constexpr int N = decltype(n)::value;
+      uint32_t o[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] = __shfl_sync(0xffffffffu, off, i0 + i * RPI + sub);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        cp_async16(kd + (i0 + i * RPI) * C::kKS, kg + (uint64_t)o[i] * 16);
+        cp_async16(vd + (i0 + i * RPI) * C::kVS, vg + (uint64_t)o[i] * 16);
+      }
+    };
+    if (sh.team == 1) {
+#pragma unroll
+      for (int i0 = 0; i0 < kTok; i0 += 4 * RPI) rows(i0, std::integral_constant<int, 4>());
+    } else {
+      for (int i0 = 0; i0 < share; i0 += RPI) rows(i0, std::integral_constant<int, 1>());
     }
-    cp_async_arrive_noinc(&full[2 * st]);
+    if (lane < share)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(
+                       sp + C::kOffScale + (member * share + lane) * 8),
+                   "l"(sc.data + sl * sc.stride_slot + (int64_t)f_head * sc.stride_head)
+                   : "memory");
+    cp_async_arrive_noinc(&full[p_st]);
     pq += sh.wh;
+    p_st += step;
+    if (p_st >= sh.stages) {
+      p_st -= sh.stages;
+      ++p_round;
+    }
     fetch_id(pq);
   };
   fetch_id(pq);
-  // the ring minus one stage is filled ahead; a stage is refilled one tile after its last use
-  for (int i = 0; i < (sh.stages + sh.wh - 1) / sh.wh; ++i)
-    if (pq < sh.stages) issue();
+  // Tile x of the ring may be fetched once x - stages has been consumed.  A team waits for that only
+  // when x - stages is not behind its own current tile in the sequence: whoever has to consume it
+  // is then not held up by this team (nor by the barriers at the end of a piece), and as a team's
+  // own tiles are at most a ring apart (step <= stages) its next tile is always on its way.
+  while (pq < ntiles && pq * sh.hg + hsel < sh.stages) issue();
 
   const bool wide_o = pairs_ok(a.out, a.out_stride_tok, a.out_stride_head);
   const bool wide_g = pairs_ok(a.gate, a.gate_stride_tok, a.gate_stride_head);
   float* merge = reinterpret_cast<float*>(smem + sh.ring + C::kFixed + 16 * nstages);
   int cfirst = 0;  // tiles of the range before the current piece
+  int cq = wsel, st = first;  // this team's next tile of the range and its stage
+  uint32_t c_phase = 0;
   int t0, n;
   while (cons.next(t0, n)) {
     if (cfirst == 0 && tid == 0)
@@ -506,12 +544,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int nrows = E * G - row0;                                 // valid ones (may be <= 0)
     const int64_t qtok0 = a.extend_lens ? cons.m.start : b;
 
-    // ---- Q: row gq of this warp, dims 64 j + 16 tq + [0, 16), as sums of e4m3 terms
-    uint4 qf[kTerms][NJ];
+    // ---- Q: row gq of this warp, dims 64 j + 16 tq + [0, 16), scaled into f16's range
+    uint32_t qf[NJ][8];
     float c2[2];
     {
-      float x[NJ][16];
-      uint32_t am = 0;
       const int r = row0 + gq;
       const bool valid = gq < nrows && qtok0 + r / G < a.num_tokens;
       const T* qp = (const T*)a.q + (qtok0 + r / G) * a.q_stride_tok +
@@ -519,46 +555,40 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool vec = ((reinterpret_cast<uintptr_t>(a.q) & 15) |
                         ((a.q_stride_tok | a.q_stride_head) & 7)) == 0;
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
+      for (int j = 0; j < NJ; ++j) {  // pairs of T
         if (valid && vec) {
 #pragma unroll
           for (int hlf = 0; hlf < 2; ++hlf) {
             const uint4 w = *reinterpret_cast<const uint4*>(qp + 64 * j + 8 * hlf);
-            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              x[j][8 * hlf + 2 * i] = unpack_lo<T>(ww[i]);
-              x[j][8 * hlf + 2 * i + 1] = unpack_hi<T>(ww[i]);
-            }
+            qf[j][4 * hlf] = w.x;
+            qf[j][4 * hlf + 1] = w.y;
+            qf[j][4 * hlf + 2] = w.z;
+            qf[j][4 * hlf + 3] = w.w;
           }
         } else {
+          const unsigned short* u = reinterpret_cast<const unsigned short*>(qp + 64 * j);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) x[j][i] = valid ? to_f(qp[64 * j + i]) : 0.f;
+          for (int i = 0; i < 8; ++i)
+            qf[j][i] = valid ? u[2 * i] | ((uint32_t)u[2 * i + 1] << 16) : 0u;
         }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) am = max(am, kv8::abs_bits(x[j][i]));
       }
+      uint32_t am = 0;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          am = max(am, max(kv8::abs_bits(unpack_lo<T>(qf[j][i])), kv8::abs_bits(unpack_hi<T>(qf[j][i]))));
       am = max(am, __shfl_xor_sync(0xffffffffu, am, 1));
       am = max(am, __shfl_xor_sync(0xffffffffu, am, 2));
       const int ex = max((int)(am >> 23) - 127, -100);  // row maximum in [2^ex, 2^(ex+1))
-      const float mul = pow2i(7 - ex);
+      const float mul = pow2i(14 - ex);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
+      for (int j = 0; j < NJ; ++j)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[j][i] *= mul;
-#pragma unroll
-        for (int k = 0; k < kTerms; ++k) {
-          uint32_t w[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t lo = term2(x[j][4 * i], x[j][4 * i + 1]);
-            w[i] = lo | (term2(x[j][4 * i + 2], x[j][4 * i + 3]) << 16);
-          }
-          qf[k][j] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      }
+        for (int i = 0; i < 8; ++i)
+          qf[j][i] = pack2_rn<__half>(unpack_lo<T>(qf[j][i]) * mul, unpack_hi<T>(qf[j][i]) * mul);
       // logit factor of row gq; a row that is not finite gives NaN logits
-      const float cr = am < 0x7f800000u ? a.scale * kLog2e * pow2i(max(ex - 7, -126)) : NAN;
+      const float cr = am < 0x7f800000u ? a.scale * kLog2e * pow2i(max(ex - 14, -126)) : NAN;
       c2[0] = __shfl_sync(0xffffffffu, cr, (2 * tq) * 4);
       c2[1] = __shfl_sync(0xffffffffu, cr, (2 * tq + 1) * 4);
     }
@@ -576,32 +606,33 @@ __global__ void __launch_bounds__(kThreads, 1)
     float M[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
     // this team's tiles of the piece: range positions q with q % wh == wsel
-    int q = cfirst + (wsel - cfirst % sh.wh + sh.wh) % sh.wh;
-    for (; q < cfirst + n && ok; q += sh.wh) {
-      const int st = q % sh.stages, round = q / sh.stages;
-      ok = __all_sync(0xffffffffu, mbar_wait(&full[2 * st], round & 1));
+    for (; cq < cfirst + n && ok; cq += sh.wh) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&full[st], c_phase));
       if (!ok) break;
       const uint32_t sp = ring + (uint32_t)(st * C::kStage);
-      const int tok0 = (t0 + q - cfirst) * kTok;
+      const unsigned char* stage = smem + st * C::kStage;
+      const int tok0 = (t0 + cq - cfirst) * kTok;
       if (nrows > 0) {
-        // ---- S^T = K8.Q^T: tokens 16 mt + gq (+8), rows 2 tq, 2 tq + 1; two chains per tile
+        // ---- S^T = K8.Q^T: tokens 16 mt + gq (+8), rows 2 tq, 2 tq + 1; two chains per token tile
         float s[2][2][4];
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-          for (int h2 = 0; h2 < 2; ++h2) s[mt][h2][0] = s[mt][h2][1] = s[mt][h2][2] = s[mt][h2][3] = 0.f;
-        const uint32_t kp = sp + gq * C::kKS + 16 * tq;
+          for (int k = 0; k < 2; ++k) s[mt][k][0] = s[mt][k][1] = s[mt][k][2] = s[mt][k][3] = 0.f;
+        const unsigned char* kp = stage + gq * C::kKS + 16 * tq;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
+          uint4 kf[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            kf[i] = *reinterpret_cast<const uint4*>(kp + 8 * i * C::kKS + 64 * j);
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt) {
-            const uint4 k0 = lds128(kp + (16 * mt) * C::kKS + 64 * j);
-            const uint4 k1 = lds128(kp + (16 * mt + 8) * C::kKS + 64 * j);
-#pragma unroll
-            for (int k = 0; k < kTerms; ++k) {
-              mma8(s[mt][0], k0.x, k1.x, k0.y, k1.y, qf[k][j].x, qf[k][j].y);
-              mma8(s[mt][1], k0.z, k1.z, k0.w, k1.w, qf[k][j].z, qf[k][j].w);
-            }
+            const uint4 k0 = kf[2 * mt], k1 = kf[2 * mt + 1];
+            mma16(s[mt][0], cvt_lo(k0.x), cvt_lo(k1.x), cvt_hi(k0.x), cvt_hi(k1.x), qf[j][0], qf[j][1]);
+            mma16(s[mt][1], cvt_lo(k0.y), cvt_lo(k1.y), cvt_hi(k0.y), cvt_hi(k1.y), qf[j][2], qf[j][3]);
+            mma16(s[mt][0], cvt_lo(k0.z), cvt_lo(k1.z), cvt_hi(k0.z), cvt_hi(k1.z), qf[j][4], qf[j][5]);
+            mma16(s[mt][1], cvt_lo(k0.w), cvt_lo(k1.w), cvt_hi(k0.w), cvt_hi(k1.w), qf[j][6], qf[j][7]);
           }
         }
         // ---- scales of tokens gq + 8 i.  One that is not finite: NaN logits for the rows that see
@@ -609,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float ksc[4], vsc[4], vmax = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float2 p = lds_f2(sp + C::kOffScale + (gq + 8 * i) * 8);
+          const float2 p = *reinterpret_cast<const float2*>(stage + C::kOffScale + (gq + 8 * i) * 8);
           const bool fin = kv8::abs_bits(p.x) < 0x7f800000u && kv8::abs_bits(p.y) < 0x7f800000u;
           ksc[i] = fin ? p.x : NAN;
           vsc[i] = fin ? p.y : 0.f;
@@ -669,33 +700,36 @@ __global__ void __launch_bounds__(kThreads, 1)
             acc[m][3] *= al[1];
           }
         }
-        // ---- W^T as B fragments: 16-bit elements (token gq, token gq + 8) of rows 2 tq, 2 tq + 1,
-        // transposed to row gq, tokens 2 tq, 2 tq + 8, 2 tq + 1, 2 tq + 9
-        uint32_t wb[kTerms][2];
+        // ---- W^T as B fragments: (token gq + 8 i; rows 2 tq, 2 tq + 1) transposed to (row gq; tokens
+        // 8 i + 2 tq, + 1)
+        uint32_t wb[4];
 #pragma unroll
-        for (int k = 0; k < kTerms; ++k) {
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            const uint32_t lo = term2(sv[2 * hf][0], sv[2 * hf + 1][0]);
-            const uint32_t hi = term2(sv[2 * hf][1], sv[2 * hf + 1][1]);
-            wb[k][hf] = movmatrix_t(lo | (hi << 16));
-          }
-        }
+        for (int i = 0; i < 4; ++i) wb[i] = movmatrix_t(pack2_rn<__half>(sv[i][0], sv[i][1]));
         // ---- O^T += V8^T.W^T
         const uint32_t vp = sp + C::kOffV + lane * C::kVS;
 #pragma unroll
-        for (int m = 0; m < NM; ++m) {
-          uint32_t r[4];
-          ldsm4_t(vp + 16 * m, r);
-          const uint32_t a0 = __byte_perm(r[0], r[1], 0x6240), a1 = __byte_perm(r[0], r[1], 0x7351);
-          const uint32_t a2 = __byte_perm(r[2], r[3], 0x6240), a3 = __byte_perm(r[2], r[3], 0x7351);
+        for (int m0 = 0; m0 < NM; m0 += 4) {
+          uint32_t r[4][4];
 #pragma unroll
-          for (int k = 0; k < kTerms; ++k) mma8(acc[m], a0, a1, a2, a3, wb[k][0], wb[k][1]);
+          for (int i = 0; i < 4; ++i) ldsm4_t(vp + 16 * (m0 + i), r[i]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            // codes (2 g, 2 g + 1) of tokens 2 t, 2 t + 1 -> dim 2 g of both, dim 2 g + 1 of both
+#pragma unroll
+            for (int k = 0; k < 4; ++k) r[i][k] = __byte_perm(r[i][k], 0, 0x3120);
+            mma16(acc[m0 + i], cvt_lo(r[i][0]), cvt_hi(r[i][0]), cvt_lo(r[i][1]), cvt_hi(r[i][1]), wb[0], wb[1]);
+            mma16(acc[m0 + i], cvt_lo(r[i][2]), cvt_hi(r[i][2]), cvt_lo(r[i][3]), cvt_hi(r[i][3]), wb[2], wb[3]);
+          }
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&full[2 * st + 1]);
-      issue();
+      if (lane == 0) count_use(&used[st]);
+      for (const int cx = cq * sh.hg + hsel + sh.stages; ok && pq < ntiles && pq * sh.hg + hsel <= cx;) issue();
+      st += step;
+      if (st >= sh.stages) {
+        st -= sh.stages;
+        c_phase ^= 1u;
+      }
     }
     cfirst += n;
 
@@ -705,53 +739,76 @@ __global__ void __launch_bounds__(kThreads, 1)
       l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
       l[1] += __shfl_xor_sync(0xffffffffu, l[1], o);
     }
-    if (sh.wh > 1) {  // merge the teams of a head: the first one ends up with all of it
-      float* mr = merge + warp * kRows * (C::kMergeStride + 2);
-      float* mlr = mr + kRows * C::kMergeStride;
-      if (wsel > 0) {
-        if (gq == 0) {
+    if (sh.wh > 1) {  // merge the teams of a head into the first one, 64 dims at a time
+      const int place = hsel * sh.team + member, per = sh.hg * sh.team;
+      float* mine = merge + ((wsel - 1) * per + place) * C::kMergeRows;
+      float f[2][kWarps], mn[2] = {M[0], M[1]};
+      if (wsel > 0 && gq == 0) {
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            mlr[2 * (2 * tq + k)] = M[k];
-            mlr[2 * (2 * tq + k) + 1] = l[k];
-          }
-        }
-#pragma unroll
-        for (int m = 0; m < NM; ++m) {
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-            *reinterpret_cast<float2*>(mr + (2 * tq + k) * C::kMergeStride + 16 * m + 2 * gq) =
-                make_float2(acc[m][k], acc[m][2 + k]);
-        }
+        for (int k = 0; k < 2; ++k)
+          *reinterpret_cast<float2*>(mine + kRows * C::kMergeStride + 2 * (2 * tq + k)) =
+              make_float2(M[k], l[k]);
       }
-      __syncthreads();
-      if (wsel == 0) {
-        for (int w = 1; w < sh.wh; ++w) {
-          const float* om = merge + (warp + w * sh.team * sh.hg) * kRows * (C::kMergeStride + 2);
-          const float* oml = om + kRows * C::kMergeStride;
-          float f[2], fo[2];
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float mo = oml[2 * (2 * tq + k)], lo = oml[2 * (2 * tq + k) + 1];
-            const float mn = fmaxf(M[k], mo);
-            f[k] = M[k] == mn ? 1.f : ex2(M[k] - mn);
-            fo[k] = mo == mn ? 1.f : ex2(mo - mn);
-            M[k] = mn;
-            l[k] = l[k] * f[k] + lo * fo[k];
-          }
+      for (int m0 = 0; m0 < NM; m0 += 4) {
+        if (wsel > 0) {
 #pragma unroll
-          for (int m = 0; m < NM; ++m) {
+          for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              *reinterpret_cast<float2*>(mine + (2 * tq + k) * C::kMergeStride + 16 * m + 2 * gq) =
+                  make_float2(acc[m0 + m][k], acc[m0 + m][2 + k]);
+        }
+        __syncthreads();
+        if (wsel == 0) {
+          if (m0 == 0) {  // factors of all teams
+            float2 o[2][kWarps];
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) {
+              if (w >= sh.wh) break;
+              const float* om = merge + ((w - 1) * per + place) * C::kMergeRows + kRows * C::kMergeStride;
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                o[k][w] = *reinterpret_cast<const float2*>(om + 2 * (2 * tq + k));
+                mn[k] = fmaxf(mn[k], o[k][w].x);
+              }
+            }
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              const float2 v =
-                  *reinterpret_cast<const float2*>(om + (2 * tq + k) * C::kMergeStride + 16 * m + 2 * gq);
-              acc[m][k] = acc[m][k] * f[k] + v.x * fo[k];
-              acc[m][2 + k] = acc[m][2 + k] * f[k] + v.y * fo[k];
+              f[k][0] = M[k] == mn[k] ? 1.f : ex2(M[k] - mn[k]);
+              l[k] *= f[k][0];
+#pragma unroll
+              for (int w = 1; w < kWarps; ++w) {
+                if (w >= sh.wh) break;
+                f[k][w] = o[k][w].x == mn[k] ? 1.f : ex2(o[k][w].x - mn[k]);
+                l[k] = fmaf(o[k][w].y, f[k][w], l[k]);
+              }
+              M[k] = mn[k];
             }
           }
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              acc[m0 + m][k] *= f[k][0];
+              acc[m0 + m][2 + k] *= f[k][0];
+            }
+#pragma unroll
+          for (int w = 1; w < kWarps; ++w) {
+            if (w >= sh.wh) break;
+            const float* om = merge + ((w - 1) * per + place) * C::kMergeRows;
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const float2 v = *reinterpret_cast<const float2*>(om + (2 * tq + k) * C::kMergeStride + 16 * m + 2 * gq);
+                acc[m0 + m][k] = fmaf(v.x, f[k][w], acc[m0 + m][k]);
+                acc[m0 + m][2 + k] = fmaf(v.y, f[k][w], acc[m0 + m][2 + k]);
+              }
+          }
         }
+        __syncthreads();
       }
-      __syncthreads();
     }
     if (wsel > 0 || nrows <= 0) continue;
     const int nt = cons.nt;
@@ -783,13 +840,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   }
-  if (!ok) {  // a wait gave up: report it, and leave no copy of this warp in flight
-    if (lane == 0) record_err(a.err, TF_KERR_TIMEOUT);
-    for (int i = 0; i < sh.stages; ++i) {
-      const int q = pq - sh.wh - i;
-      if (q >= 0) mbar_wait(&full[2 * (q % sh.stages)], (q / sh.stages) & 1);
-    }
-  }
+  if (!ok && lane == 0) record_err(a.err, TF_KERR_TIMEOUT);  // a wait gave up
+  cp_async_wait_all();
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -913,19 +965,17 @@ static Shape shape_of(const tf_paged_attn_args& a, int num_sms) {
   const int64_t rows = (int64_t)G * (a.extend_lens ? a.max_extend_len : 1);
   const int need = rows > kRows ? (int)((rows + kRows - 1) / kRows) : 1;
   Shape s;
-  s.team = need <= 1 ? 1 : (need <= 2 ? 2 : 4);
+  s.team = need <= 1 ? 1 : (need <= 2 ? 2 : (need <= 4 ? 4 : 8));
   s.passes = (need + s.team - 1) / s.team;
   s.hg = gcd(a.num_kv_heads, kWarps / s.team);
   s.wh = kWarps / (s.team * s.hg);
   s.groups = a.num_kv_heads / s.hg * s.passes;
-  int stages = C::kStages;
-  auto bytes = [&](int n) {
-    return n * C::kStage + C::kFixed + 16 * n + (s.wh > 1 ? C::kMerge : 0);
-  };
-  while (bytes(stages / s.hg * s.hg) > 232448) --stages;
-  s.stages = stages / s.hg;
-  s.ring = s.stages * s.hg * C::kStage;
-  s.smem = bytes(s.stages * s.hg);
+  const int merge = (s.wh - 1) * s.hg * s.team * C::kMergeRows * 4;
+  s.stages = C::kStages;
+  auto bytes = [&](int n) { return n * C::kStage + C::kFixed + 16 * n + merge; };
+  while (bytes(s.stages) > 232448) --s.stages;
+  s.ring = s.stages * C::kStage;
+  s.smem = bytes(s.stages);
   s.nctas = num_sms;
   s.min_tiles = 2 * s.wh;
   s.piece_cost = 8;
@@ -978,6 +1028,8 @@ bool paged_fp8_rows_supported(const tf_paged_attn_args& a) {
   if (a.batch_size > rows8::kMaxBatch || a.r2t_rows > 0x7fffffff || a.r2t_cols > 0x7fffffff)
     return false;
   auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  // row offsets are kept in 32 bits of 16-byte pieces: pools of up to 64 GiB a layer
+  if (a.num_slots * a.kv_stride_slot + a.num_kv_heads * a.kv_stride_head >= (int64_t)1 << 36) return false;
   return al(a.k_buffer) && al(a.v_buffer) && a.kv_stride_slot % 16 == 0 && a.kv_stride_head % 16 == 0;
 }
 

@@ -59,9 +59,9 @@ struct Cfg {
   static constexpr int kOffScale = kOffV + kTok * kVS;
   static constexpr int kStage = kOffScale + kTok * 8;
   static constexpr int kStages = D == 256 ? 12 : (D == 128 ? 20 : 40);  // at most
-  // merge of a head's teams: 64 dims of a row at a time, then its (M, l)
-  static constexpr int kMergeStride = 64 + 4;
-  static constexpr int kMergeRows = kRows * (kMergeStride + 2);  // floats per warp
+  // epilogue: 64 dims of every warp's rows, then their (M, l) and what each is multiplied by
+  static constexpr int kEpiStride = 64 + 4;  // floats per row
+  static constexpr int kEpi = kWarps * kRows * (kEpiStride + 3) * 4;
   static constexpr int kFixed = kCache * (int)sizeof(ReqMeta) + 64;
   static_assert(kStage % 16 == 0 && kKS % 16 == 0 && kVS % 16 == 0, "bulk copy alignment");
 };
@@ -232,53 +232,102 @@ struct Walker {
   }
 };
 
-// N pairs of output values x[i] at dims d0 + 16 i (times the gate's activation) of one query row; the
-// gate is requested as a whole before the first store
-template <typename T, int N>
-__device__ __forceinline__ void put_row(const tf_paged_attn_args& a, int64_t tok, int hq, int d0,
-                                        const float (&x0)[N], const float (&x1)[N], bool wide_o,
-                                        bool wide_g) {
-  float f0[N], f1[N];
+// 4 output values of a query row at dims d.. (times the gate's activation); v8: rows can be moved in
+// 8-byte pieces
+template <typename T>
+__device__ __forceinline__ void put4(const tf_paged_attn_args& a, int64_t tok, int hq, int d, float4 x,
+                                     bool v8) {
+  float o[4] = {x.x, x.y, x.z, x.w};
   if (a.gate_mode != TF_GATE_NONE) {
-    const T* gp = (const T*)a.gate + tok * a.gate_stride_tok + (int64_t)hq * a.gate_stride_head + d0;
-    uint32_t w[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (wide_g) {
-        w[i] = *reinterpret_cast<const uint32_t*>(gp + 16 * i);
-      } else {
-        const unsigned short* u = reinterpret_cast<const unsigned short*>(gp + 16 * i);
-        w[i] = u[0] | ((uint32_t)u[1] << 16);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float g0 = unpack_lo<T>(w[i]), g1 = unpack_hi<T>(w[i]);
-      f0[i] = x0[i] * (a.gate_mode == TF_GATE_SILU ? silu_f(g0) : sigmoid_f(g0));
-      f1[i] = x1[i] * (a.gate_mode == TF_GATE_SILU ? silu_f(g1) : sigmoid_f(g1));
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) { f0[i] = x0[i]; f1[i] = x1[i]; }
-  }
-  T* op = (T*)a.out + tok * a.out_stride_tok + (int64_t)hq * a.out_stride_head + d0;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    if (wide_o) {
-      *reinterpret_cast<uint32_t*>(op + 16 * i) = pack2_rn<T>(f0[i], f1[i]);
+    const T* gp = (const T*)a.gate + tok * a.gate_stride_tok + (int64_t)hq * a.gate_stride_head + d;
+    uint32_t w[2];
+    if (v8) {
+      const uint2 u = *reinterpret_cast<const uint2*>(gp);
+      w[0] = u.x;
+      w[1] = u.y;
     } else {
-      op[16 * i] = from_f<T>(f0[i]);
-      op[16 * i + 1] = from_f<T>(f1[i]);
+      const unsigned short* u = reinterpret_cast<const unsigned short*>(gp);
+      w[0] = u[0] | ((uint32_t)u[1] << 16);
+      w[1] = u[2] | ((uint32_t)u[3] << 16);
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float g = i & 1 ? unpack_hi<T>(w[i >> 1]) : unpack_lo<T>(w[i >> 1]);
+      const float sg = sigmoid_f(g);
+      o[i] *= a.gate_mode == TF_GATE_SILU ? g * sg : sg;
+    }
+  }
+  T* op = (T*)a.out + tok * a.out_stride_tok + (int64_t)hq * a.out_stride_head + d;
+  const uint32_t p0 = pack2_rn<T>(o[0], o[1]), p1 = pack2_rn<T>(o[2], o[3]);
+  if (v8) {
+    *reinterpret_cast<uint2*>(op) = make_uint2(p0, p1);
+  } else {
+    unsigned short* u = reinterpret_cast<unsigned short*>(op);
+    u[0] = (unsigned short)p0;
+    u[1] = (unsigned short)(p0 >> 16);
+    u[2] = (unsigned short)p1;
+    u[3] = (unsigned short)(p1 >> 16);
   }
 }
-__device__ __forceinline__ bool pairs_ok(const void* p, int64_t s0, int64_t s1) {
-  return ((reinterpret_cast<uintptr_t>(p) & 3) | ((s0 | s1) & 1)) == 0;
+__device__ __forceinline__ bool rows_v8(const tf_paged_attn_args& a) {
+  return ((reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.gate)) & 7) == 0 &&
+         ((a.out_stride_tok | a.out_stride_head | a.gate_stride_tok | a.gate_stride_head) & 3) == 0;
+}
+
+// A finished piece, for the whole CTA.
+struct Piece {
+  int b, u, ext, nt, t0, n, slot;  // slot: partial place of this CTA (2 c or 2 c + 1)
+  int64_t qtok0;
+};
+
+// 64 dims (d0..) of every row of a piece from the epilogue buffer: the teams of a head are summed, and
+// the result is normalised and put out, or left as partials.  One copy of this code serves all
+// pieces and dims: unrolled into the kernel it ran once a piece from a cold instruction cache
+// (15-35 us a piece were measured).
+template <typename T, int D>
+__device__ __noinline__ void finish64(const tf_paged_attn_args& a, const Shape& sh, const Ws& ws,
+                                      const float* epi, const Piece& p, int d0) {
+  constexpr int kS = Cfg<D>::kEpiStride;
+  const float* fac = epi + kWarps * kRows * kS;         // [warp][row] what the warp's row counts
+  const float* ml = fac + kWarps * kRows;               // [warp][row][2]; the first team's: merged
+  const int per = sh.hg * sh.team;
+  const int G = a.num_q_heads / a.num_kv_heads;
+  const bool v8 = rows_v8(a), whole = p.t0 == 0 && p.n == p.nt;
+#pragma unroll 1
+  for (int e = threadIdx.x; e < per * kRows * 16; e += kThreads) {
+    const int v = e & 15, r = (e >> 4) & (kRows - 1), place = e >> 7;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int w = place; w < kWarps; w += per) {
+      const float f = fac[w * kRows + r];
+      const float4 x = *reinterpret_cast<const float4*>(epi + (w * kRows + r) * kS + 4 * v);
+      o.x = fmaf(f, x.x, o.x);
+      o.y = fmaf(f, x.y, o.y);
+      o.z = fmaf(f, x.z, o.z);
+      o.w = fmaf(f, x.w, o.w);
+    }
+    if (whole) {
+      const int hsel = place / sh.team, member = place - hsel * sh.team;
+      const int row = ((p.u % sh.passes) * sh.team + member) * kRows + r;
+      const int64_t tok = p.qtok0 + row / G;
+      if (row >= p.ext * G || tok >= a.num_tokens) continue;
+      const int hq = ((p.u / sh.passes) * sh.hg + hsel) * G + row % G;
+      const float inv = (1.f / 128.f) / ml[(place * kRows + r) * 2 + 1];
+      put4<T>(a, tok, hq, d0 + 4 * v, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), v8);
+    } else {
+      const int64_t ps = (int64_t)(p.slot * kWarps + place) * kRows + r;
+      *reinterpret_cast<float4*>(ws.o + ps * D + d0 + 4 * v) = o;
+      if (d0 == 0 && v == 0)
+        *reinterpret_cast<float2*>(ws.ml + ps * 2) =
+            make_float2(ml[(place * kRows + r) * 2], ml[(place * kRows + r) * 2 + 1]);
+    }
+  }
 }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
-    rows_kernel(const tf_paged_attn_args a, const tf_kv_scale sc, const Shape sh, Ws ws) {
+    rows_kernel(const __grid_constant__ tf_paged_attn_args a, const __grid_constant__ tf_kv_scale sc,
+                const __grid_constant__ Shape sh, const __grid_constant__ Ws ws) {
   using C = Cfg<D>;
   constexpr int NJ = D / 64;   // 16-byte reads of a K row per thread
   constexpr int NM = D / 16;   // dim tiles of O
@@ -290,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int c = blockIdx.x;
 
   ReqMeta* cache = reinterpret_cast<ReqMeta*>(smem + sh.ring);
-  int* sh_i = reinterpret_cast<int*>(cache + kCache);  // [16] words
+  int* sh_i = reinterpret_cast<int*>(cache + kCache);  // [16] words, 8-byte aligned
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + sh.ring + C::kFixed);
   uint32_t* used = reinterpret_cast<uint32_t*>(bars + sh.stages);  // warps done with a stage, in all
 
@@ -299,9 +348,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // ---- this CTA's range: ts[b] = first tile of request b (all groups of a request are adjacent)
   int* ts = reinterpret_cast<int*>(smem);  // in the ring's space, before its first copy
+  const int plan_per = (B + kThreads - 1) / kThreads;
+  const int plan_lo = min(tid * plan_per, B), plan_hi = min(plan_lo + plan_per, B);
   {
-    const int per = (B + kThreads - 1) / kThreads;
-    const int lo = min(tid * per, B), hi = min(lo + per, B);
+    const int lo = plan_lo, hi = plan_hi;
     int sum = 0;
     for (int b = lo; b < hi; ++b) {
       int64_t ext;
@@ -330,55 +380,47 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int64_t want = (total + sh.min_tiles - 1) / sh.min_tiles;
   const int nctas = want < gridDim.x ? (int)want : (int)gridDim.x;
   const int64_t beta = sh.piece_cost;
-  // first tile at cost position x = cc (total + beta units) / nctas; a unit's first beta is fixed cost
-  auto boundary = [&](int cc) -> int64_t {
-    if (cc >= nctas) return total;
-    const int64_t U = (int64_t)B * NG;
-    const int64_t x = (int64_t)cc * (total + beta * U) / nctas;
-    int lo = 0, hi = B - 1;  // last request whose cost start ts[b] NG + beta b NG is at most x
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (((int64_t)ts[mid] + beta * mid) * NG <= x) lo = mid; else hi = mid - 1;
+  // A range begins at cost position x = cc (total + beta units) / nctas: a unit's first beta of cost is
+  // fixed.  The request holding x lies with one thread; the range's first request with another.
+  const int64_t U = (int64_t)B * NG;
+  int64_t* sh_g = reinterpret_cast<int64_t*>(sh_i + 8);  // g0, g1
+  int* sh_b = sh_i + 12;
+  if (tid == 0) { sh_g[0] = sh_g[1] = total; }
+  __syncthreads();
+#pragma unroll 1
+  for (int k = 0; k < 2; ++k) {
+    if (c + k >= nctas) continue;
+    const int64_t x = (int64_t)(c + k) * (total + beta * U) / nctas;
+#pragma unroll 1
+    for (int b = plan_lo; b < plan_hi; ++b) {
+      const int64_t nt = ts[b + 1] - ts[b], rem = x - ((int64_t)ts[b] + beta * b) * NG;
+      if (rem < 0 || rem >= (nt + beta) * NG) continue;
+      const int64_t u = rem / (nt + beta);
+      int64_t off = rem - u * (nt + beta) - beta;
+      sh_g[k] = (int64_t)ts[b] * NG + u * nt + (off < 0 ? 0 : off);
     }
-    const int64_t nt = ts[lo + 1] - ts[lo];
-    const int64_t rem = x - ((int64_t)ts[lo] + beta * lo) * NG;
-    int64_t u = rem / (nt + beta);
-    if (u > NG - 1) u = NG - 1;
-    int64_t off = rem - u * (nt + beta) - beta;
-    off = off < 0 ? 0 : (off > nt ? nt : off);
-    return (int64_t)ts[lo] * NG + u * nt + off;
-  };
-  const int64_t g0 = boundary(c), g1 = boundary(c + 1);
+  }
+  __syncthreads();
+  const int64_t g0 = sh_g[0], g1 = sh_g[1];
   if (tid == 0) {
     ws.cta_g[c] = g0;
     if (c == gridDim.x - 1) ws.cta_g[c + 1] = total;
   }
   // requests without keys: softmax over nothing is NaN
   if (a.extend_lens == nullptr) {
-    const bool wide = pairs_ok(a.out, a.out_stride_tok, a.out_stride_head);
     for (int b = c; b < B; b += gridDim.x) {
       if (ts[b + 1] != ts[b]) continue;
-      for (int e = tid; e < a.num_q_heads * (D / 2); e += kThreads) {
-        T* op = (T*)a.out + (int64_t)b * a.out_stride_tok +
-                (int64_t)(e / (D / 2)) * a.out_stride_head + 2 * (e % (D / 2));
-        if (wide) {
-          *reinterpret_cast<uint32_t*>(op) = pack2_rn<T>(NAN, NAN);
-        } else {
-          op[0] = op[1] = from_f<T>(NAN);
-        }
-      }
+      for (int e = tid; e < a.num_q_heads * D; e += kThreads)
+        ((T*)a.out)[(int64_t)b * a.out_stride_tok + (int64_t)(e / D) * a.out_stride_head + e % D] =
+            from_f<T>(NAN);
     }
   }
   if (g0 >= g1) return;
-  int bf = 0;  // the range's first request: ts[bf] NG <= g0 < ts[bf + 1] NG
-  {
-    int lo = 0, hi = B - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if ((int64_t)ts[mid + 1] * NG > g0) hi = mid; else lo = mid + 1;
-    }
-    bf = lo;
-  }
+#pragma unroll 1
+  for (int b = plan_lo; b < plan_hi; ++b)  // the range's first request: ts[b] NG <= g0 < ts[b + 1] NG
+    if ((int64_t)ts[b] * NG <= g0 && g0 < (int64_t)ts[b + 1] * NG) *sh_b = b;
+  __syncthreads();
+  const int bf = *sh_b;
   const int cn = min(kCache, B - bf);
   const int64_t bf_g = (int64_t)ts[bf] * NG;
   const int bf_nt = ts[bf + 1] - ts[bf];
@@ -406,9 +448,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     m.start = b;
     cache[i] = m;
   }
-  const int nstages = sh.stages;
   if (tid == 0) {
-    for (int i = 0; i < nstages; ++i) {
+    for (int i = 0; i < sh.stages; ++i) {
       mbar_init(&bars[i], sh.team * 32);  // every lane's copies have landed
       used[i] = 0;
     }
@@ -528,9 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // own tiles are at most a ring apart (step <= stages) its next tile is always on its way.
   while (pq < ntiles && pq * sh.hg + hsel < sh.stages) issue();
 
-  const bool wide_o = pairs_ok(a.out, a.out_stride_tok, a.out_stride_head);
-  const bool wide_g = pairs_ok(a.gate, a.gate_stride_tok, a.gate_stride_head);
-  float* merge = reinterpret_cast<float*>(smem + sh.ring + C::kFixed + 16 * nstages);
+  float* epi = reinterpret_cast<float*>(smem + sh.ring + C::kFixed + 16 * sh.stages);
   int cfirst = 0;  // tiles of the range before the current piece
   int cq = wsel, st = first;  // this team's next tile of the range and its stage
   uint32_t c_phase = 0;
@@ -739,104 +778,42 @@ __global__ void __launch_bounds__(kThreads, 1)
       l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
       l[1] += __shfl_xor_sync(0xffffffffu, l[1], o);
     }
-    if (sh.wh > 1) {  // merge the teams of a head into the first one, 64 dims at a time
-      const int place = hsel * sh.team + member, per = sh.hg * sh.team;
-      float* mine = merge + ((wsel - 1) * per + place) * C::kMergeRows;
-      float f[2][kWarps], mn[2] = {M[0], M[1]};
-      if (wsel > 0 && gq == 0) {
+    {
+      float* fac = epi + kWarps * kRows * C::kEpiStride;
+      float* ml = fac + kWarps * kRows;
+      if (gq == 0) {
 #pragma unroll
         for (int k = 0; k < 2; ++k)
-          *reinterpret_cast<float2*>(mine + kRows * C::kMergeStride + 2 * (2 * tq + k)) =
-              make_float2(M[k], l[k]);
+          *reinterpret_cast<float2*>(ml + (warp * kRows + 2 * tq + k) * 2) = make_float2(M[k], l[k]);
       }
+      float* mine = epi + warp * kRows * C::kEpiStride;
+      const Piece pc = {b, u, E, cons.nt, t0, n, 2 * c + (cfirst == n ? 0 : 1), qtok0};
 #pragma unroll
       for (int m0 = 0; m0 < NM; m0 += 4) {
-        if (wsel > 0) {
 #pragma unroll
-          for (int m = 0; m < 4; ++m)
+        for (int m = 0; m < 4; ++m)
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
-              *reinterpret_cast<float2*>(mine + (2 * tq + k) * C::kMergeStride + 16 * m + 2 * gq) =
-                  make_float2(acc[m0 + m][k], acc[m0 + m][2 + k]);
-        }
+          for (int k = 0; k < 2; ++k)
+            *reinterpret_cast<float2*>(mine + (2 * tq + k) * C::kEpiStride + 16 * m + 2 * gq) =
+                make_float2(acc[m0 + m][k], acc[m0 + m][2 + k]);
         __syncthreads();
-        if (wsel == 0) {
-          if (m0 == 0) {  // factors of all teams
-            float2 o[2][kWarps];
-#pragma unroll
-            for (int w = 1; w < kWarps; ++w) {
-              if (w >= sh.wh) break;
-              const float* om = merge + ((w - 1) * per + place) * C::kMergeRows + kRows * C::kMergeStride;
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                o[k][w] = *reinterpret_cast<const float2*>(om + 2 * (2 * tq + k));
-                mn[k] = fmaxf(mn[k], o[k][w].x);
-              }
+        if (m0 == 0) {  // factors of the teams of a head, and its (M, l) in the first team's place
+          const int per = sh.hg * sh.team;
+          if (tid < per * kRows) {
+            float mx = -INFINITY, ls = 0.f;
+            for (int w = tid; w < kWarps * kRows; w += per * kRows) mx = fmaxf(mx, ml[2 * w]);
+            for (int w = tid; w < kWarps * kRows; w += per * kRows) {
+              const float mw = ml[2 * w], f = mw == mx ? 1.f : ex2(mw - mx);
+              fac[w] = f;
+              ls = fmaf(f, ml[2 * w + 1], ls);
             }
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              f[k][0] = M[k] == mn[k] ? 1.f : ex2(M[k] - mn[k]);
-              l[k] *= f[k][0];
-#pragma unroll
-              for (int w = 1; w < kWarps; ++w) {
-                if (w >= sh.wh) break;
-                f[k][w] = o[k][w].x == mn[k] ? 1.f : ex2(o[k][w].x - mn[k]);
-                l[k] = fmaf(o[k][w].y, f[k][w], l[k]);
-              }
-              M[k] = mn[k];
-            }
+            ml[2 * tid] = mx;
+            ml[2 * tid + 1] = ls;
           }
-#pragma unroll
-          for (int m = 0; m < 4; ++m)
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              acc[m0 + m][k] *= f[k][0];
-              acc[m0 + m][2 + k] *= f[k][0];
-            }
-#pragma unroll
-          for (int w = 1; w < kWarps; ++w) {
-            if (w >= sh.wh) break;
-            const float* om = merge + ((w - 1) * per + place) * C::kMergeRows;
-#pragma unroll
-            for (int m = 0; m < 4; ++m)
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                const float2 v = *reinterpret_cast<const float2*>(om + (2 * tq + k) * C::kMergeStride + 16 * m + 2 * gq);
-                acc[m0 + m][k] = fmaf(v.x, f[k][w], acc[m0 + m][k]);
-                acc[m0 + m][2 + k] = fmaf(v.y, f[k][w], acc[m0 + m][2 + k]);
-              }
-          }
+          __syncthreads();
         }
+        finish64<T, D>(a, sh, ws, epi, pc, 16 * m0);
         __syncthreads();
-      }
-    }
-    if (wsel > 0 || nrows <= 0) continue;
-    const int nt = cons.nt;
-    if (t0 == 0 && n == nt) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int r = row0 + 2 * tq + k;
-        const int64_t tok = qtok0 + r / G;
-        if (r >= E * G || tok >= a.num_tokens) continue;
-        const float inv = (1.f / 128.f) / l[k];
-        float x0[NM], x1[NM];
-#pragma unroll
-        for (int m = 0; m < NM; ++m) {
-          x0[m] = acc[m][k] * inv;
-          x1[m] = acc[m][2 + k] * inv;
-        }
-        put_row<T, NM>(a, tok, kvh * G + r % G, 2 * gq, x0, x1, wide_o, wide_g);
-      }
-    } else {
-      const int ps = ((2 * c + (cfirst == n ? 0 : 1)) * kWarps + hsel * sh.team + member) * kRows;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int r = 2 * tq + k;
-        if (gq == 0) *reinterpret_cast<float2*>(ws.ml + (ps + r) * 2) = make_float2(M[k], l[k]);
-#pragma unroll
-        for (int m = 0; m < NM; ++m)
-          *reinterpret_cast<float2*>(ws.o + (int64_t)(ps + r) * D + 16 * m + 2 * gq) =
-              make_float2(acc[m][k], acc[m][2 + k]);
       }
     }
   }
@@ -851,7 +828,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ---------------------------------------------------------------------------------------------
 template <typename T, int D, int PG>
 __global__ void __launch_bounds__(256 * PG)
-    combine_kernel(const tf_paged_attn_args a, const Shape sh, Ws ws) {
+    combine_kernel(const __grid_constant__ tf_paged_attn_args a, const __grid_constant__ Shape sh,
+                   const __grid_constant__ Ws ws) {
   constexpr int kVec = D / 4;  // 4-value vectors of a row
   constexpr int kSteps = (kRows * kVec + 255) / 256;
   __shared__ float red[PG > 1 ? PG : 1][PG > 1 ? 256 : 1][PG > 1 ? 5 : 1];
@@ -944,13 +922,7 @@ __global__ void __launch_bounds__(256 * PG)
     if (grp == 0 && r < kRows && rr < ci.ext * G && tok < a.num_tokens) {
       const int hq = ((ci.u / sh.passes) * sh.hg + hsel) * G + rr % G;
       const float inv = (1.f / 128.f) / l;
-      const bool wo = pairs_ok(a.out, a.out_stride_tok, a.out_stride_head);
-      const bool wg = pairs_ok(a.gate, a.gate_stride_tok, a.gate_stride_head);
-#pragma unroll
-      for (int h2 = 0; h2 < 2; ++h2) {
-        const float x0[1] = {o[2 * h2] * inv}, x1[1] = {o[2 * h2 + 1] * inv};
-        put_row<T, 1>(a, tok, hq, 4 * v + 2 * h2, x0, x1, wo, wg);
-      }
+      put4<T>(a, tok, hq, 4 * v, make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv), rows_v8(a));
     }
   }
 }
@@ -970,9 +942,8 @@ static Shape shape_of(const tf_paged_attn_args& a, int num_sms) {
   s.hg = gcd(a.num_kv_heads, kWarps / s.team);
   s.wh = kWarps / (s.team * s.hg);
   s.groups = a.num_kv_heads / s.hg * s.passes;
-  const int merge = (s.wh - 1) * s.hg * s.team * C::kMergeRows * 4;
   s.stages = C::kStages;
-  auto bytes = [&](int n) { return n * C::kStage + C::kFixed + 16 * n + merge; };
+  auto bytes = [&](int n) { return n * C::kStage + C::kFixed + 16 * n + C::kEpi; };
   while (bytes(s.stages) > 232448) --s.stages;
   s.ring = s.stages * C::kStage;
   s.smem = bytes(s.stages);

@@ -183,52 +183,44 @@ __device__ __forceinline__ int tiles_of(int64_t L, int64_t ext) {
   return ext > 0 ? (int)((L + kTok - 1) / kTok) : 0;
 }
 
-// The units of a CTA's range in order.  Metadata of the first kCache requests of the range sits in
-// shared memory, further ones are read from global memory as the walk reaches them.
-struct Walker {
-  const tf_paged_attn_args* a;
+// The requests a walk can be at: the first kCache of the range from shared memory, further ones from
+// global memory as the walk reaches them.
+struct Requests {
+  const tf_paged_attn_args& a;
   const ReqMeta* cache;
-  int cache_b0, cache_n;
-  int groups;
-  int64_t g, g1;     // next tile, end of the range
-  int b, u;          // its request and group
-  int64_t unit_g;    // first tile of unit (b, u)
-  ReqMeta m;
-  int nt;
-  __device__ __forceinline__ void load(int prev_end) {
-    const int i = b - cache_b0;
-    if (i < cache_n) {
-      m = cache[i];
-    } else {
-      int64_t ext;
-      bool bad;
-      const int64_t L = checked_len(*a, b, ext, bad);
-      m.len = (int32_t)L;
-      m.ext = (int32_t)ext;
-      const int64_t r = a->req_pool_indices[b];
-      if (r < 0 || r >= a->r2t_rows) record_err(a->err, TF_KERR_REQ_RANGE);
-      m.row = r < 0 || r >= a->r2t_rows ? 0 : (int32_t)r;
-      m.start = prev_end;
-    }
-    nt = tiles_of(m.len, m.ext);
+  int b0, n, groups;
+  __device__ __forceinline__ ReqMeta at(int b, int start) const {
+    if (b - b0 < n) return cache[b - b0];
+    int64_t ext;
+    bool bad;
+    ReqMeta m;
+    m.len = (int32_t)checked_len(a, b, ext, bad);
+    m.ext = (int32_t)ext;
+    const int64_t r = a.req_pool_indices[b];
+    if (r < 0 || r >= a.r2t_rows) record_err(a.err, TF_KERR_REQ_RANGE);
+    m.row = r < 0 || r >= a.r2t_rows ? 0 : (int32_t)r;
+    m.start = start;
+    return m;
   }
-  // piece [g, g + n) of unit (b, u); false at the end of the range
-  __device__ __forceinline__ bool next(int& t0, int& n) {
-    if (g >= g1) return false;
-    while (g >= unit_g + nt) {
-      unit_g += nt;
-      if (++u == groups) {
+};
+
+// The units of a CTA's range in order; tiles are counted from the range's first.
+struct Walker {
+  int b, u;     // request and group
+  int unit_g;   // first tile of unit (b, u)
+  ReqMeta m;
+  __device__ __forceinline__ int nt() const { return tiles_of(m.len, m.ext); }
+  // the unit that holds tile q (of the current unit or a later one)
+  __device__ __forceinline__ void seek(const Requests& rq, int q) {
+    while (q >= unit_g + nt()) {
+      unit_g += nt();
+      if (++u == rq.groups) {
         u = 0;
+        const int before = rq.a.extend_lens && b + 1 - rq.b0 >= rq.n ? max((int)rq.a.extend_lens[b], 0) : 1;
         ++b;
-        const int raw = a->extend_lens ? max((int)a->extend_lens[b - 1], 0) : 1;
-        load(m.start + raw);
+        m = rq.at(b, m.start + before);
       }
     }
-    t0 = (int)(g - unit_g);
-    const int64_t e = unit_g + nt < g1 ? unit_g + nt : g1;
-    n = (int)(e - g);
-    g = e;
-    return true;
   }
 };
 
@@ -242,7 +234,7 @@ __device__ __forceinline__ void put4(const tf_paged_attn_args& a, int64_t tok, i
     const T* gp = (const T*)a.gate + tok * a.gate_stride_tok + (int64_t)hq * a.gate_stride_head + d;
     uint32_t w[2];
     if (v8) {
-      const uint2 u = *reinterpret_cast<const uint2*>(gp);
+      const uint2 u = __ldg(reinterpret_cast<const uint2*>(gp));
       w[0] = u.x;
       w[1] = u.y;
     } else {
@@ -276,8 +268,8 @@ __device__ __forceinline__ bool rows_v8(const tf_paged_attn_args& a) {
 
 // A finished piece, for the whole CTA.
 struct Piece {
-  int b, u, ext, nt, t0, n, slot;  // slot: partial place of this CTA (2 c or 2 c + 1)
-  int64_t qtok0;
+  int u, ext, start, slot;  // slot: partial place of this CTA (2 c or 2 c + 1)
+  bool whole;
 };
 
 // 64 dims (d0..) of every row of a piece from the epilogue buffer: the teams of a head are summed, and
@@ -292,7 +284,7 @@ __device__ __noinline__ void finish64(const tf_paged_attn_args& a, const Shape& 
   const float* ml = fac + kWarps * kRows;               // [warp][row][2]; the first team's: merged
   const int per = sh.hg * sh.team;
   const int G = a.num_q_heads / a.num_kv_heads;
-  const bool v8 = rows_v8(a), whole = p.t0 == 0 && p.n == p.nt;
+  const bool v8 = rows_v8(a);
 #pragma unroll 1
   for (int e = threadIdx.x; e < per * kRows * 16; e += kThreads) {
     const int v = e & 15, r = (e >> 4) & (kRows - 1), place = e >> 7;
@@ -306,10 +298,10 @@ __device__ __noinline__ void finish64(const tf_paged_attn_args& a, const Shape& 
       o.z = fmaf(f, x.z, o.z);
       o.w = fmaf(f, x.w, o.w);
     }
-    if (whole) {
+    if (p.whole) {
       const int hsel = place / sh.team, member = place - hsel * sh.team;
       const int row = ((p.u % sh.passes) * sh.team + member) * kRows + r;
-      const int64_t tok = p.qtok0 + row / G;
+      const int64_t tok = p.start + row / G;
       if (row >= p.ext * G || tok >= a.num_tokens) continue;
       const int hq = ((p.u / sh.passes) * sh.hg + hsel) * G + row % G;
       const float inv = (1.f / 128.f) / ml[(place * kRows + r) * 2 + 1];
@@ -350,6 +342,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   int* ts = reinterpret_cast<int*>(smem);  // in the ring's space, before its first copy
   const int plan_per = (B + kThreads - 1) / kThreads;
   const int plan_lo = min(tid * plan_per, B), plan_hi = min(plan_lo + plan_per, B);
+  ReqMeta mine_m = {0, 0, 0, 0};  // of request plan_lo when every thread has at most one
+  if (plan_per == 1 && plan_lo < B) {
+    const int64_t r = a.req_pool_indices[plan_lo];
+    mine_m.row = r < 0 || r >= a.r2t_rows ? -1 : (int32_t)r;
+  }
   {
     const int lo = plan_lo, hi = plan_hi;
     int sum = 0;
@@ -358,6 +355,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool bad;
       const int64_t L = checked_len(a, b, ext, bad);
       if (bad && c == 0) record_err(a.err, TF_KERR_SLOT_RANGE);
+      mine_m.len = (int32_t)L;
+      mine_m.ext = (int32_t)ext;
       ts[b] = sum;
       sum += tiles_of(L, ext);
     }
@@ -435,7 +434,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     q_before = 0;
     for (int w = 0; w < kWarps; ++w) q_before += sh_i[w];
   }
-  for (int i = tid; i < cn; i += kThreads) {
+  if (plan_per == 1) {
+    if (plan_lo >= bf && plan_lo < bf + cn && plan_hi > plan_lo) {
+      if (mine_m.row < 0) {
+        record_err(a.err, TF_KERR_REQ_RANGE);
+        mine_m.row = 0;
+      }
+      mine_m.start = plan_lo;
+      cache[plan_lo - bf] = mine_m;
+    }
+  } else for (int i = tid; i < cn; i += kThreads) {
     const int b = bf + i;
     int64_t ext;
     bool bad;
@@ -455,9 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  // ts is dead from here on: its (generic) accesses come before the first bulk copy over it
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  __syncthreads();
+  __syncthreads();  // ts is dead from here on
   if (a.extend_lens != nullptr && tid == 0) {
     int s = q_before;
     for (int i = 0; i < cn; ++i) {
@@ -477,112 +483,119 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int step = sh.wh * sh.hg, first = wsel * sh.hg + hsel;
   const int share = kTok / sh.team;  // tokens of a stage that this warp fetches
 
+  const Requests rq{a, cache, bf, cn, NG};
   Walker prod;
-  prod.a = &a;
-  prod.cache = cache;
-  prod.cache_b0 = bf;
-  prod.cache_n = cn;
-  prod.groups = NG;
-  prod.g = g0;
-  prod.g1 = g1;
   prod.b = bf;
-  prod.u = bf_nt ? (int)((g0 - bf_g) / bf_nt) : 0;
-  prod.unit_g = bf_g + (int64_t)prod.u * bf_nt;
-  prod.load(0);
+  prod.u = (int)((g0 - bf_g) / bf_nt);
+  prod.unit_g = (int)(bf_g + (int64_t)prod.u * bf_nt - g0);
+  prod.m = rq.at(bf, 0);
   Walker cons = prod;
 
-  // ---- producer: tiles of this team in sequence, one slot id ahead
+  // ---- producer: this team's tiles in sequence, their req_to_token entries kAhead tiles ahead
   const int ntiles = (int)(g1 - g0);
-  int pq = wsel;                   // next tile of the range to fetch
-  int p_end = 0, p_first = 0, p_t0 = 0;  // its piece: tiles [p_first, p_end) of the range, from t0
-  int64_t next_raw = 0;
-  auto raw_of = [&](int q) -> int64_t {  // req_to_token entry of this lane's token of tile q
-    while (q >= p_end) {
-      int n;
-      p_first = p_end;
-      if (!prod.next(p_t0, n)) return 0;
-      p_end = p_first + n;
-    }
-    int pos = (p_t0 + q - p_first) * kTok + member * share + lane;
-    if (pos >= prod.m.len) pos = prod.m.len - 1;
-    return a.req_to_token[(int64_t)prod.m.row * a.r2t_stride + pos];
-  };
-  int f_head = 0;  // kv head of the tile whose id is in next_raw
-  auto fetch_id = [&](int q) {
-    if (q < ntiles) next_raw = raw_of(q);
-    f_head = (prod.u / sh.passes) * sh.hg + hsel;
-  };
+  constexpr int kAhead = 2;
+  int64_t raw[kAhead];
+  int head[kAhead];           // their kv heads
+  int pq = wsel - kAhead * sh.wh;  // next tile to fetch (below 0: the entries' own head start)
+  int p_st = first, p_round = 0;   // its stage and round
   bool ok = true;
-  int p_st = first, p_round = 0;  // stage and round of tile pq
   auto issue = [&]() {
-    if (pq >= ntiles) return;
-    if (p_round > 0)
-      ok = __all_sync(0xffffffffu, ok && wait_uses(&used[p_st], (uint32_t)(p_round * sh.team)));
-    if (!ok) return;
-    const uint32_t sp = ring + (uint32_t)(p_st * C::kStage);
-    const int64_t sl = resolve_slot(next_raw, a.num_slots, a.slot_mode, lane < share ? a.err : nullptr);
-    // row offset of this lane's token in 16-byte pieces (32 bits: the host checks)
-    const uint32_t off =
-        (uint32_t)((sl * a.kv_stride_slot + (int64_t)f_head * a.kv_stride_head) >> 4);
-    constexpr int CPR = D / 16;    // 16-byte pieces of a row
-    constexpr int RPI = 32 / CPR;  // rows a warp instruction copies
-    const int sub = lane / CPR, ch = lane % CPR;
-    const char* kg = (const char*)a.k_buffer + 16 * ch;
-    const char* vg = (const char*)a.v_buffer + 16 * ch;
-    const uint32_t kd = sp + (member * share + sub) * C::kKS + 16 * ch;
-    const uint32_t vd = sp + C::kOffV + (member * share + sub) * C::kVS + 16 * ch;
-    auto rows = [&](int i0, auto n) {
-      constexpr int N = decltype(n)::value;
-      uint32_t o[N];
+    if (pq >= 0) {
+      if (p_round > 0)
+        ok = __all_sync(0xffffffffu, ok && wait_uses(&used[p_st], (uint32_t)(p_round * sh.team)));
+      if (!ok) return;
+      const uint32_t sp = ring + (uint32_t)(p_st * C::kStage);
+      const int64_t sl = resolve_slot(raw[0], a.num_slots, a.slot_mode, lane < share ? a.err : nullptr);
+      // row offset of this lane's token in 16-byte pieces (32 bits: the host checks)
+      const uint32_t off =
+          (uint32_t)((sl * a.kv_stride_slot + (int64_t)head[0] * a.kv_stride_head) >> 4);
+      constexpr int CPR = D / 16;    // 16-byte pieces of a row
+      constexpr int RPI = 32 / CPR;  // rows a warp instruction copies
+      const int sub = lane / CPR, ch = lane % CPR;
+      const char* kg = (const char*)a.k_buffer + 16 * ch;
+      const char* vg = (const char*)a.v_buffer + 16 * ch;
+      const uint32_t kd = sp + (member * share + sub) * C::kKS + 16 * ch;
+      const uint32_t vd = sp + C::kOffV + (member * share + sub) * C::kVS + 16 * ch;
+      auto rows = [&](int i0, auto n) {
+        constexpr int N = decltype(n)::value;
+        uint32_t o[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) o[i] = __shfl_sync(0xffffffffu, off, i0 + i * RPI + sub);
+        for (int i = 0; i < N; ++i) o[i] = __shfl_sync(0xffffffffu, off, i0 + i * RPI + sub);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        cp_async16(kd + (i0 + i * RPI) * C::kKS, kg + (uint64_t)o[i] * 16);
-        cp_async16(vd + (i0 + i * RPI) * C::kVS, vg + (uint64_t)o[i] * 16);
+        for (int i = 0; i < N; ++i) {
+          cp_async16(kd + (i0 + i * RPI) * C::kKS, kg + (uint64_t)o[i] * 16);
+          cp_async16(vd + (i0 + i * RPI) * C::kVS, vg + (uint64_t)o[i] * 16);
+        }
+      };
+      if (sh.team == 1) {
+#pragma unroll
+        for (int i0 = 0; i0 < kTok; i0 += 4 * RPI) rows(i0, std::integral_constant<int, 4>());
+      } else {
+#pragma unroll 1
+        for (int i0 = 0; i0 < share; i0 += RPI) rows(i0, std::integral_constant<int, 1>());
       }
-    };
-    if (sh.team == 1) {
+      if (lane < share)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(
+                         sp + C::kOffScale + (member * share + lane) * 8),
+                     "l"(sc.data + sl * sc.stride_slot + (int64_t)head[0] * sc.stride_head)
+                     : "memory");
+      cp_async_arrive_noinc(&full[p_st]);
+      p_st += step;
+      if (p_st >= sh.stages) {
+        p_st -= sh.stages;
+        ++p_round;
+      }
+    }
 #pragma unroll
-      for (int i0 = 0; i0 < kTok; i0 += 4 * RPI) rows(i0, std::integral_constant<int, 4>());
-    } else {
-      for (int i0 = 0; i0 < share; i0 += RPI) rows(i0, std::integral_constant<int, 1>());
+    for (int i = 0; i + 1 < kAhead; ++i) {
+      raw[i] = raw[i + 1];
+      head[i] = head[i + 1];
     }
-    if (lane < share)
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(
-                       sp + C::kOffScale + (member * share + lane) * 8),
-                   "l"(sc.data + sl * sc.stride_slot + (int64_t)f_head * sc.stride_head)
-                   : "memory");
-    cp_async_arrive_noinc(&full[p_st]);
+    const int fq = pq + kAhead * sh.wh;
+    if (fq < ntiles) {
+      prod.seek(rq, fq);
+      const int pos = min((fq - prod.unit_g) * kTok + member * share + lane, prod.m.len - 1);
+      raw[kAhead - 1] = a.req_to_token[(int64_t)prod.m.row * a.r2t_stride + pos];
+      head[kAhead - 1] = (prod.u / sh.passes) * sh.hg + hsel;
+    }
     pq += sh.wh;
-    p_st += step;
-    if (p_st >= sh.stages) {
-      p_st -= sh.stages;
-      ++p_round;
-    }
-    fetch_id(pq);
   };
-  fetch_id(pq);
+
   // Tile x of the ring may be fetched once x - stages has been consumed.  A team waits for that only
   // when x - stages is not behind its own current tile in the sequence: whoever has to consume it
   // is then not held up by this team (nor by the barriers at the end of a piece), and as a team's
   // own tiles are at most a ring apart (step <= stages) its next tile is always on its way.
-  while (pq < ntiles && pq * sh.hg + hsel < sh.stages) issue();
-
+  int x_lim = sh.stages - 1;  // the last tile that may be fetched now
   float* epi = reinterpret_cast<float*>(smem + sh.ring + C::kFixed + 16 * sh.stages);
-  int cfirst = 0;  // tiles of the range before the current piece
   int cq = wsel, st = first;  // this team's next tile of the range and its stage
   uint32_t c_phase = 0;
-  int t0, n;
-  while (cons.next(t0, n)) {
-    if (cfirst == 0 && tid == 0)
-      ws.cut[c] = CutInfo{cons.b, cons.u, cons.m.start, cons.m.ext, cons.nt, t0};
-    const int b = cons.b, u = cons.u, L = cons.m.len, E = cons.m.ext;
+  for (int p0 = 0, p1; p0 < ntiles; p0 = p1) {  // pieces: tiles [p0, p1) of the range
+    cons.seek(rq, p0);
+    p1 = min(cons.unit_g + cons.nt(), ntiles);
+    if (p0 == 0 && tid == 0)
+      ws.cut[c] = CutInfo{cons.b, cons.u, cons.m.start, cons.m.ext, cons.nt(), -cons.unit_g};
+    const int u = cons.u, L = cons.m.len, E = cons.m.ext;
     const int kvh = (u / sh.passes) * sh.hg + hsel;
     const int row0 = ((u % sh.passes) * sh.team + member) * kRows;  // first of this warp's rows
     const int nrows = E * G - row0;                                 // valid ones (may be <= 0)
-    const int64_t qtok0 = a.extend_lens ? cons.m.start : b;
+    const int64_t qtok0 = cons.m.start;
 
+    // the gate rows of the piece are wanted at its end: into L2 now, 128 bytes a thread (a load under
+    // a saturated memory takes microseconds)
+    if (a.gate_mode != TF_GATE_NONE && p1 == cons.unit_g + cons.nt()) {
+      constexpr int kLines = D * 2 / 128 > 0 ? D * 2 / 128 : 1;
+      const int per = sh.hg * sh.team;
+      for (int e = tid; e < per * kRows * kLines; e += kThreads) {
+        const int r = (e / kLines) % kRows, place = e / kLines / kRows;
+        const int row = ((u % sh.passes) * sh.team + place % sh.team) * kRows + r;
+        const int64_t tok = qtok0 + row / G;
+        if (row < E * G && tok < a.num_tokens)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(
+              (const T*)a.gate + tok * a.gate_stride_tok +
+              (int64_t)(((u / sh.passes) * sh.hg + place / sh.team) * G + row % G) * a.gate_stride_head +
+              (e % kLines) * 64));
+      }
+    }
     // ---- Q: row gq of this warp, dims 64 j + 16 tq + [0, 16), scaled into f16's range
     uint32_t qf[NJ][8];
     float c2[2];
@@ -644,13 +657,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int m = 0; m < NM; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
     float M[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-    // this team's tiles of the piece: range positions q with q % wh == wsel
-    for (; cq < cfirst + n && ok; cq += sh.wh) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&full[st], c_phase));
+    // this team's tiles of the piece: those with cq % wh == wsel
+#pragma unroll 1
+    for (;;) {
+      while (pq < ntiles && pq * sh.hg + hsel <= x_lim && ok) issue();
+      if (cq >= p1) break;
+      ok = __all_sync(0xffffffffu, ok && mbar_wait(&full[st], c_phase));
       if (!ok) break;
       const uint32_t sp = ring + (uint32_t)(st * C::kStage);
       const unsigned char* stage = smem + st * C::kStage;
-      const int tok0 = (t0 + cq - cfirst) * kTok;
+      const int tok0 = (cq - cons.unit_g) * kTok;
       if (nrows > 0) {
         // ---- S^T = K8.Q^T: tokens 16 mt + gq (+8), rows 2 tq, 2 tq + 1; two chains per token tile
         float s[2][2][4];
@@ -763,14 +779,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
       if (lane == 0) count_use(&used[st]);
-      for (const int cx = cq * sh.hg + hsel + sh.stages; ok && pq < ntiles && pq * sh.hg + hsel <= cx;) issue();
+      x_lim = cq * sh.hg + hsel + sh.stages;
+      cq += sh.wh;
       st += step;
       if (st >= sh.stages) {
         st -= sh.stages;
         c_phase ^= 1u;
       }
     }
-    cfirst += n;
 
     // ---- the piece is done: O / l, or partials when the unit goes on in another CTA
 #pragma unroll
@@ -787,7 +803,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           *reinterpret_cast<float2*>(ml + (warp * kRows + 2 * tq + k) * 2) = make_float2(M[k], l[k]);
       }
       float* mine = epi + warp * kRows * C::kEpiStride;
-      const Piece pc = {b, u, E, cons.nt, t0, n, 2 * c + (cfirst == n ? 0 : 1), qtok0};
+      const Piece pc = {u, E, cons.m.start, 2 * c + (p0 == 0 ? 0 : 1),
+                        p0 == cons.unit_g && p1 == cons.unit_g + cons.nt()};
 #pragma unroll
       for (int m0 = 0; m0 < NM; m0 += 4) {
 #pragma unroll
@@ -822,18 +839,19 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ---------------------------------------------------------------------------------------------
-// combine: CTA (c, w) merges warp place w of the unit that the boundary of range c cuts, when it is
-// the first boundary inside that unit.  PG groups of 256 threads take the pieces in turn; a thread
-// holds 4 values of one row.
+// combine: CTA (c, place, rows) merges RZ rows of one warp place of the unit that the boundary of range
+// c cuts, when it is the first boundary inside that unit.  A thread holds 4 values of one row; the
+// PG = 256 / (RZ D / 4) groups of threads take the pieces in turn (one row a CTA and many groups when
+// few units have many pieces each).
 // ---------------------------------------------------------------------------------------------
-template <typename T, int D, int PG>
-__global__ void __launch_bounds__(256 * PG)
+template <typename T, int D, int RZ>
+__global__ void __launch_bounds__(256)
     combine_kernel(const __grid_constant__ tf_paged_attn_args a, const __grid_constant__ Shape sh,
                    const __grid_constant__ Ws ws) {
   constexpr int kVec = D / 4;  // 4-value vectors of a row
-  constexpr int kSteps = (kRows * kVec + 255) / 256;
-  __shared__ float red[PG > 1 ? PG : 1][PG > 1 ? 256 : 1][PG > 1 ? 5 : 1];
-  __shared__ float s_M[kRows];
+  constexpr int PG = 256 / (RZ * kVec);
+  static_assert(PG >= 1 && PG * RZ * kVec == 256, "threads of a CTA");
+  __shared__ float red[PG > 1 ? 256 : 1][PG > 1 ? 5 : 1];
   __shared__ int64_t s_g[kMaxCtas + 1];
   __shared__ int s_slot[kMaxCtas];
   __shared__ int s_np;
@@ -842,7 +860,7 @@ __global__ void __launch_bounds__(256 * PG)
   const int n = gridDim.x + 1;  // decode CTAs
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const CutInfo ci = ws.cut[c];
-  for (int i = tid; i <= n; i += 256 * PG) s_g[i] = ws.cta_g[i];
+  for (int i = tid; i <= n; i += 256) s_g[i] = ws.cta_g[i];
   __syncthreads();
   const int64_t g = s_g[c];
   if (g >= s_g[n] || s_g[c + 1] == g || ci.t0 == 0) return;  // empty range, or nothing cut here
@@ -870,60 +888,75 @@ __global__ void __launch_bounds__(256 * PG)
   }
   __syncthreads();
   const int np = s_np;
-  {  // the rows' maxima over all pieces: eight threads a piece in the first warp
-    float m = -INFINITY;
-    if (tid < 32) {
-      const int r = lane & 7;
-      for (int i = lane >> 3; i < np; i += 4) m = fmaxf(m, ws.ml[(s_slot[i] + r) * 2]);
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-      if (lane < 8) s_M[lane] = m;
+  const int r = blockIdx.z * RZ + (tid / kVec) % RZ, v = tid % kVec, grp = tid / (kVec * RZ);
+  // running merge of this group's pieces; a batch of pieces is requested before it is added
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float M = -INFINITY, l = 0.f;
+  constexpr int kBatch = 4;
+  for (int i0 = grp; i0 < np; i0 += kBatch * PG) {
+    float2 ml[kBatch];
+    float4 x[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int i = i0 + j * PG;
+      if (i < np) {
+        const int64_t s = s_slot[i] + r;
+        ml[j] = *reinterpret_cast<const float2*>(ws.ml + s * 2);
+        x[j] = *reinterpret_cast<const float4*>(ws.o + s * D + 4 * v);
+      } else {
+        ml[j] = make_float2(-INFINITY, 0.f);
+        x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+    float mn = M;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) mn = fmaxf(mn, ml[j].x);
+    const float f0 = M == mn ? 1.f : ex2(M - mn);
+    o.x *= f0;
+    o.y *= f0;
+    o.z *= f0;
+    o.w *= f0;
+    l *= f0;
+    M = mn;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const float f = ml[j].x == mn ? 1.f : ex2(ml[j].x - mn);
+      o.x = fmaf(f, x[j].x, o.x);
+      o.y = fmaf(f, x[j].y, o.y);
+      o.z = fmaf(f, x[j].z, o.z);
+      o.w = fmaf(f, x[j].w, o.w);
+      l = fmaf(f, ml[j].y, l);
     }
   }
-  __syncthreads();
-  const int grp = tid / 256, t = tid % 256;
-#pragma unroll 1
-  for (int step = 0; step < kSteps; ++step) {
-    const int e = step * 256 + t;
-    const int r = e / kVec, v = e % kVec;
-    float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
-    if (r < kRows) {
-      const float M = s_M[r];
-#pragma unroll 8
-      for (int i = grp; i < np; i += PG) {
-        const int s = s_slot[i] + r;
-        const float2 ml = *reinterpret_cast<const float2*>(ws.ml + s * 2);
-        const float4 x = *reinterpret_cast<const float4*>(ws.o + (int64_t)s * D + 4 * v);
-        const float f = ml.x == M ? 1.f : ex2(ml.x - M);
-        o[0] = fmaf(f, x.x, o[0]);
-        o[1] = fmaf(f, x.y, o[1]);
-        o[2] = fmaf(f, x.z, o[2]);
-        o[3] = fmaf(f, x.w, o[3]);
-        l = fmaf(f, ml.y, l);
-      }
-    }
-    if constexpr (PG > 1) {
-      __syncthreads();
+  if constexpr (PG > 1) {  // the groups meet: the maximum first
+    __shared__ float s_m[256];
+    s_m[tid] = M;
+    __syncthreads();
+    float mn = M;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) red[grp][t][i] = o[i];
-      red[grp][t][4] = l;
-      __syncthreads();
-      if (grp == 0) {
+    for (int p = 0; p < PG; ++p) mn = fmaxf(mn, s_m[p * RZ * kVec + tid % (RZ * kVec)]);
+    const float f = M == mn ? 1.f : ex2(M - mn);
+    red[tid][0] = o.x * f;
+    red[tid][1] = o.y * f;
+    red[tid][2] = o.z * f;
+    red[tid][3] = o.w * f;
+    red[tid][4] = l * f;
+    __syncthreads();
+    if (grp > 0) return;
+    float t[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int p = 1; p < PG; ++p) {
+    for (int p = 0; p < PG; ++p)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] += red[p][t][i];
-          l += red[p][t][4];
-        }
-      }
-    }
-    const int rr = row0 + r;
-    const int64_t tok = ci.start + rr / G;
-    if (grp == 0 && r < kRows && rr < ci.ext * G && tok < a.num_tokens) {
-      const int hq = ((ci.u / sh.passes) * sh.hg + hsel) * G + rr % G;
-      const float inv = (1.f / 128.f) / l;
-      put4<T>(a, tok, hq, 4 * v, make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv), rows_v8(a));
-    }
+      for (int i = 0; i < 5; ++i) t[i] += red[p * RZ * kVec + tid][i];
+    o = make_float4(t[0], t[1], t[2], t[3]);
+    l = t[4];
+  }
+  const int rr = row0 + r;
+  const int64_t tok = ci.start + rr / G;
+  if (rr < ci.ext * G && tok < a.num_tokens) {
+    const int hq = ((ci.u / sh.passes) * sh.hg + hsel) * G + rr % G;
+    const float inv = (1.f / 128.f) / l;
+    put4<T>(a, tok, hq, 4 * v, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), rows_v8(a));
   }
 }
 
@@ -966,19 +999,20 @@ static cudaError_t launch_td(const tf_paged_attn_args& a, const tf_kv_scale& sc,
   rows_kernel<T, D><<<num_sms, kThreads, sh.smem, s>>>(a, sc, sh, ws);
   e = cudaGetLastError();
   if (e != cudaSuccess || num_sms == 1) return e;
+  // few units have many pieces each: a CTA per row, its groups of threads sharing the pieces
+  constexpr int kWide = 256 / (D / 4) < kRows ? 256 / (D / 4) : kRows;
+  const bool deep = (int64_t)a.batch_size * sh.groups * 8 < num_sms;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(num_sms - 1), (unsigned)(sh.hg * sh.team));
+  cfg.gridDim = dim3((unsigned)(num_sms - 1), (unsigned)(sh.hg * sh.team), (unsigned)(deep ? kRows : kRows / kWide));
+  cfg.blockDim = dim3(256);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  // few units, so many pieces each: four groups of threads share them
-  const bool deep = (int64_t)a.batch_size * sh.groups * 8 < num_sms;
-  cfg.blockDim = dim3(deep ? 1024 : 256);
-  return deep ? cudaLaunchKernelEx(&cfg, combine_kernel<T, D, 4>, a, sh, ws)
-              : cudaLaunchKernelEx(&cfg, combine_kernel<T, D, 1>, a, sh, ws);
+  return deep ? cudaLaunchKernelEx(&cfg, combine_kernel<T, D, 1>, a, sh, ws)
+              : cudaLaunchKernelEx(&cfg, combine_kernel<T, D, kWide>, a, sh, ws);
 }
 
 template <typename T>

@@ -500,18 +500,28 @@ tf_status tf_attn_prologue_fp8(const tf_attn_prologue_args* a, const tf_kv_scale
 }
 
 // Which kernel a call over an 8-bit pool takes: the few-rows kernel while a request has at most
-// kFewRows query rows per kv head, the CUDA-core kernel otherwise.
-enum class Fp8Path { kRows, kSimt };
+// kFewRows query rows per kv head, the tcgen05 kernel beyond, the CUDA-core kernel for the dtypes,
+// head dims and layouts that neither is built for.
+enum class Fp8Path { kRows, kTile, kSimt };
 constexpr int64_t kFewRows = 64;
 
 static Fp8Path fp8_path(const tf_paged_attn_args& a, bool decode) {
   const int64_t rows = (int64_t)(a.num_q_heads / a.num_kv_heads) * (decode ? 1 : a.max_extend_len);
-  return (decode || rows <= kFewRows) && paged_fp8_rows_supported(a) ? Fp8Path::kRows : Fp8Path::kSimt;
+  if ((decode || rows <= kFewRows) && paged_fp8_rows_supported(a)) return Fp8Path::kRows;
+  return !decode && paged_fp8_extend_supported(a) ? Fp8Path::kTile : Fp8Path::kSimt;
+}
+
+static size_t fp8_path_workspace(const tf_paged_attn_args& a, Fp8Path path) {
+  switch (path) {
+    case Fp8Path::kRows: return paged_fp8_rows_workspace(a, device_sm_count());
+    case Fp8Path::kTile: return paged_fp8_extend_workspace(a, device_sm_count());
+    default: return 0;
+  }
 }
 
 static size_t fp8_workspace(const tf_paged_attn_args* a, bool decode) {
-  if (a == nullptr || a->batch_size <= 0 || check_paged(a, decode) != TF_OK) return 0;
-  return fp8_path(*a, decode) == Fp8Path::kRows ? paged_fp8_rows_workspace(*a, device_sm_count()) : 0;
+  if (check_paged(a, decode) != TF_OK || a->batch_size == 0 || a->num_tokens == 0) return 0;
+  return fp8_path_workspace(*a, fp8_path(*a, decode));
 }
 
 static tf_status paged_fp8(const tf_paged_attn_args* a, const tf_kv_scale* sc, void* ws,
@@ -527,7 +537,7 @@ static tf_status paged_fp8(const tf_paged_attn_args* a, const tf_kv_scale* sc, v
   DeviceGuard g(s);
   if (!g.ok()) return fail(TF_ERR_CUDA, "cannot select the stream's device");
   const int nsm = device_sm_count();
-  const size_t need = path == Fp8Path::kRows ? paged_fp8_rows_workspace(d, nsm) : 0;
+  const size_t need = fp8_path_workspace(d, path);
   if (need != 0) {
     if (ws == nullptr || ws_bytes < need)
       return fail(TF_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, need, ws_bytes);
@@ -535,6 +545,7 @@ static tf_status paged_fp8(const tf_paged_attn_args* a, const tf_kv_scale* sc, v
       return fail(TF_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
   }
   if (path == Fp8Path::kRows) return cuda_status(launch_paged_fp8_rows(d, *sc, ws, nsm, s), what);
+  if (path == Fp8Path::kTile) return cuda_status(launch_paged_fp8_extend(d, *sc, ws, nsm, s), what);
   return cuda_status(launch_paged_fp8_simt(d, *sc, s), what);
 }
 

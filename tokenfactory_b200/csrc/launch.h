@@ -70,6 +70,12 @@ size_t paged_fp8_rows_workspace(const tf_paged_attn_args& a, int num_sms);
 cudaError_t launch_paged_fp8_rows(const tf_paged_attn_args& a, const tf_kv_scale& sc, void* ws,
                                   int num_sms, cudaStream_t s);
 
+// paged_fp8_extend.cu: bf16 / fp16 extend on tcgen05 / TMEM
+bool paged_fp8_extend_supported(const tf_paged_attn_args& a);
+size_t paged_fp8_extend_workspace(const tf_paged_attn_args& a, int num_sms);
+cudaError_t launch_paged_fp8_extend(const tf_paged_attn_args& a, const tf_kv_scale& sc, void* ws,
+                                    int num_sms, cudaStream_t s);
+
 // capi.cu
 int device_sm_count();
 

@@ -1,0 +1,926 @@
+// Paged GQA extend over the 8-bit K/V pool on the 5th-generation tensor cores, for bf16 / fp16
+// activations at head_dim 128 and 256.  A dense contraction: 4 D flops per visible (query row, key).
+//
+// Two CTAs of a cluster on an SM pair run one M=256 tile (128/G query tokens x G heads a CTA) with
+// tcgen05.mma.cta_group::2, as paged_extend_tc.cu does over 16-bit pools: CTA r holds query rows
+// [128 r, 128 r + 128) and of every 128-key tile keys [64 r, 64 r + 64) of K and dims [r D/2, (r+1) D/2)
+// of V; softmax warps own their CTA's rows, producer warps gather its halves, one thread of rank 0
+// issues the products.  What the 8-bit pool changes:
+//   producers   load 16 codes a lane, convert them to f16 (exact) and store them into the swizzled
+//               tile; a slot's loads are in flight while the one before it is converted
+//   scales      are not multiplied into the tiles (a second rounding of every element): a key's logit
+//               is its product times ks_j in fp32, and its weight p_j = 2^(s_j - M) enters P as
+//               f16(p_j vs_j).  M follows s_j + ev_j, ev_j the exponent of the largest vs of the tile,
+//               so that P stays in f16's range whatever the scales are; l = sum p_j is fp32.
+//   Q           is scaled by a power of two per row into f16's range (bfloat16 stays exact)
+// A scale that is not finite gives its key NaN logits and a V row of zeros, so that only the rows that
+// see it are NaN.  Every wait is bounded; one that gives up raises an abort flag in both CTAs and
+// TF_KERR_TIMEOUT.
+//
+// Few query tiles over a long prefix leave SM pairs idle: the key tiles are then split over
+// grid.z clusters, which leave (M, l, O) partials for a combine kernel.
+#include "common.cuh"
+#include "kv_fp8.cuh"
+#include "launch.h"
+#include "tcgen05.cuh"
+
+namespace tf {
+namespace ext8 {
+
+constexpr int kRows = 128;       // query rows of a CTA
+constexpr int kKeys = 128;       // keys of a tile
+constexpr int kSmWarps = 8;      // softmax: two warps per 32-row group, 64 keys each
+constexpr int kPrWarps = 4;      // producers
+constexpr int kPrWarp0 = kSmWarps;
+constexpr int kIssueWarp = kSmWarps + kPrWarps;  // MMA issue (rank 0) / slot relay (rank 1)
+constexpr int kFwdWarp = kIssueWarp + 1;         // rank 1: forwards "P written" to rank 0
+constexpr int kThreads = (kFwdWarp + 1) * 32;
+constexpr int kPrThreads = kPrWarps * 32;
+constexpr int kScaleTiles = 4;   // ring of the tiles' scales
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRescaleLog2 = 8.f;
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max_of_64(const float (&s)[2][32]) {
+  float t[22];
+#pragma unroll
+  for (int i = 0; i < 21; ++i) {
+    const int k = 3 * i;
+    t[i] = max3(s[k >> 5][k & 31], s[(k + 1) >> 5][(k + 1) & 31], s[(k + 2) >> 5][(k + 2) & 31]);
+  }
+  t[21] = s[1][31];
+  float u[8];
+#pragma unroll
+  for (int i = 0; i < 7; ++i) u[i] = max3(t[3 * i], t[3 * i + 1], t[3 * i + 2]);
+  u[7] = t[21];
+  return fmaxf(max3(u[0], u[1], u[2]), max3(u[3], u[4], max3(u[5], u[6], u[7])));
+}
+__device__ __forceinline__ float ex2_ftz(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126..127
+
+// ---- cluster pair helpers
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t peer_addr(uint32_t local, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local), "r"(rank));
+  return r;
+}
+// CTA-scope release: what the waiter reads next is complete behind the tcgen05 / proxy fences that
+// precede every call
+__device__ __forceinline__ void remote_arrive(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ void remote_store(uint32_t cluster_addr, int v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ bool try_wait_cluster(uint32_t addr, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(addr), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Bounded waits; a timeout raises the abort flag of both CTAs.  CLUSTER: acquire at cluster scope.
+template <bool CLUSTER>
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort,
+                                         uint32_t peer_abort, unsigned backoff_ns = 0) {
+  const uint32_t addr = smem_u32(bar);
+  auto done = [&] { return CLUSTER ? try_wait_cluster(addr, parity) : mbar_try_wait(addr, parity); };
+  if (done()) return true;
+  const uint64_t t0 = global_ns();
+  for (uint32_t it = 1;; ++it) {
+    if (backoff_ns) __nanosleep(backoff_ns);
+    if (done()) return true;
+    if ((it & 63u) == 0) {
+      if (*abort) return false;
+      if (global_ns() - t0 > kSpinLimitNs) {
+        *abort = 1;
+        remote_store(peer_abort, 1);
+        return false;
+      }
+    }
+  }
+}
+// Bounded, but not ended by the abort flag: the pair's products are drained before TMEM is released.
+__device__ __forceinline__ bool drain(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = smem_u32(bar);
+  const uint64_t t0 = global_ns();
+  for (uint32_t it = 0;; ++it) {
+    if (try_wait_cluster(addr, parity)) return true;
+    if ((it & 63u) == 63u && global_ns() - t0 > kSpinLimitNs) return false;
+  }
+}
+__device__ __forceinline__ void mma2_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc ? 1u : 0u)
+      : "memory");
+}
+__device__ __forceinline__ void mma2_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc ? 1u : 0u)
+      : "memory");
+}
+__device__ __forceinline__ void commit_both(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+      " [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3)
+      : "memory");
+}
+// instruction descriptor, kind::f16 with f16 inputs and fp32 accumulation
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool b_mn_major) {
+  return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+__device__ __forceinline__ uint32_t cvt_lo(uint32_t w) {
+  uint32_t r;
+  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %1;\n cvt.rn.f16x2.e4m3x2 %0, a;\n}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t cvt_hi(uint32_t w) {
+  uint32_t r;
+  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %1;\n cvt.rn.f16x2.e4m3x2 %0, b;\n}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ uint4 ldg_nc(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+template <int D>
+struct Cfg {
+  static constexpr int kKB = D / 64;              // 64-dim blocks of a row
+  static constexpr int kQBlock = kRows * 128;     // one block of this CTA's Q rows
+  static constexpr int kQBytes = kKB * kQBlock;
+  static constexpr int kKBlk = (kKeys / 2) * 128; // K half: 64 keys x 128 B per block
+  static constexpr int kVBlk = kKeys * 128;       // V half: 128 keys x 128 B per block
+  static constexpr int kSlotBytes = kKB * kKBlk;  // == (kKB / 2) * kVBlk
+  static constexpr int kSlots = D == 256 ? 4 : 8;
+  static constexpr int kOffRing = kQBytes;
+  static constexpr int kOffBars = kOffRing + kSlots * kSlotBytes;
+  // full, empty [kSlots]; s_full[2], p_full[2], o_done, q_full, fin, q_dead, sc_full[kScaleTiles]
+  static constexpr int kNumBars = 2 * kSlots + 8 + kScaleTiles;
+  static constexpr int kOffWords = kOffBars + 8 * kNumBars;      // tmem holder, abort, q0
+  static constexpr int kOffIds = (kOffWords + 16 + 15) & ~15;    // int64 [2][kPrWarps][32]
+  static constexpr int kOffPmax = kOffIds + 2 * kPrWarps * 32 * 8;  // float [2][2][kRows]
+  static constexpr int kOffRow = kOffPmax + 2 * 2 * kRows * 4;   // float [kRows]: logit factor of a row
+  static constexpr int kOffKs = kOffRow + kRows * 4;             // float [kScaleTiles][kKeys]
+  static constexpr int kOffVs = kOffKs + kScaleTiles * kKeys * 4;
+  static constexpr int kOffEv = kOffVs + kScaleTiles * kKeys * 4;   // float [kScaleTiles][kPrWarps]
+  static constexpr int kSmem = kOffEv + kScaleTiles * kPrWarps * 4 + 1024;
+  static constexpr int kColS = 0;                 // two S buffers of kKeys columns; P_j over S_j
+  static constexpr int kColO = 2 * kKeys;
+  static constexpr int kTmemCols = 512;
+  static_assert(kSlotBytes == (kKB / 2) * kVBlk, "K and V halves share the slot size");
+  static_assert(kSmem <= 232448, "shared memory per CTA");
+  static_assert(kColO + D <= kTmemCols, "TMEM columns");
+  static_assert(2 * kRows * 4 <= kSlotBytes && kRows * D * 2 <= kQBytes, "epilogue staging");
+};
+
+struct Split {
+  int n;        // clusters that share the keys of a query tile
+  float* ml;    // [n][T][Hq][2]
+  float* o;     // [n][T][Hq][D]
+};
+
+// 16-byte pieces of the gate and output rows can be moved whole
+__device__ __forceinline__ bool rows_v16(const tf_paged_attn_args& a) {
+  return ((reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.gate)) & 15) == 0 &&
+         ((a.out_stride_tok | a.out_stride_head | a.gate_stride_tok | a.gate_stride_head) & 7) == 0;
+}
+__device__ __forceinline__ float act(float x, int mode) {
+  const float s = sigmoid_f(x);
+  return mode == TF_GATE_SILU ? x * s : s;
+}
+
+template <typename T, int D>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    extend_kernel(const __grid_constant__ tf_paged_attn_args a, const __grid_constant__ tf_kv_scale sc,
+                  int pairs_per_req, const __grid_constant__ Split sp) {
+  using C = Cfg<D>;
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t raw_base = smem_u32(smem_raw);
+  const uint32_t base = (raw_base + 1023) & ~1023u;
+  unsigned char* sbase = smem_raw + (base - raw_base);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sbase + C::kOffBars);
+  uint64_t* empty = full + C::kSlots;
+  uint64_t* s_full = empty + C::kSlots;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_done = p_full + 2;
+  uint64_t* q_full = o_done + 1;
+  uint64_t* fin = q_full + 1;
+  uint64_t* q_dead = fin + 1;    // the last S product has completed: Q's shared memory is free
+  uint64_t* sc_full = q_dead + 1;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(sbase + C::kOffWords);
+  volatile int* abort = reinterpret_cast<volatile int*>(sbase + C::kOffWords + 4);
+  int64_t* s_q0 = reinterpret_cast<int64_t*>(sbase + C::kOffWords + 8);
+  int64_t* ids_all = reinterpret_cast<int64_t*>(sbase + C::kOffIds);
+  float* pmax = reinterpret_cast<float*>(sbase + C::kOffPmax);
+  float* rowf = reinterpret_cast<float*>(sbase + C::kOffRow);
+  float* ks_s = reinterpret_cast<float*>(sbase + C::kOffKs);
+  float* vs_s = reinterpret_cast<float*>(sbase + C::kOffVs);
+  float* ev_s = reinterpret_cast<float*>(sbase + C::kOffEv);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = cluster_rank();
+  const uint32_t peer = rank ^ 1u;
+  const uint32_t peer_abort = peer_addr(smem_u32((const void*)abort), peer);
+  const int Hkv = a.num_kv_heads, G = a.num_q_heads / Hkv;
+  const int TQ = kRows / G;  // query tokens per CTA
+  const int pidx = blockIdx.x >> 1;
+  const int b = pidx / pairs_per_req;
+  const int qp = pairs_per_req - 1 - (pidx - b * pairs_per_req);  // longest tiles first
+  const int h = blockIdx.y, z = blockIdx.z;
+  const int64_t E = a.extend_lens ? a.extend_lens[b] : 1;
+  const int64_t pair_start = (int64_t)qp * 2 * TQ;
+  if (pair_start >= E) return;  // both CTAs of the pair leave here, before any cluster barrier
+  const int64_t L = a.seq_lens[b];
+  if (L > a.r2t_cols || L < E) {
+    if (tid == 0 && rank == 0) record_err(a.err, TF_KERR_SLOT_RANGE);
+    return;
+  }
+  const int64_t P = L - E;
+  const int64_t cta_start = pair_start + (int64_t)rank * TQ;  // first token of this CTA's rows
+  const int64_t pair_end = E - pair_start < 2 * TQ ? E : pair_start + 2 * TQ;
+  const int64_t kv_end = P + pair_end;  // keys [0, kv_end) are visible to some row of the pair
+  const int all_tiles = (int)((kv_end + kKeys - 1) / kKeys);
+  // this cluster's key tiles [jb, jb + ntiles)
+  const int per = (all_tiles + sp.n - 1) / sp.n;
+  const int jb = z * per;
+  const int ntiles = all_tiles - jb < per ? all_tiles - jb : per;
+
+  if (warp == 0) {
+    int64_t acc = 0;
+    for (int i = lane; i < b; i += 32) {
+      const int64_t e = a.extend_lens ? a.extend_lens[i] : 1;
+      acc += e > 0 ? e : 0;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+    if (lane == 0) *s_q0 = acc;
+  }
+  if (ntiles <= 0) {  // nothing left for this cluster: an empty partial (both CTAs come here)
+    __syncthreads();
+    const int64_t q0 = *s_q0 + cta_start;
+    const int ri = tid / G;
+    if (tid < kRows && ri < TQ && cta_start + ri < E && q0 + ri < a.num_tokens) {
+      const int64_t row = ((int64_t)z * a.num_tokens + q0 + ri) * a.num_q_heads + h * G + tid % G;
+      *reinterpret_cast<float2*>(sp.ml + 2 * row) = make_float2(-INFINITY, 0.f);
+    }
+    return;
+  }
+  if (tid == 0) {
+    const uint32_t in_count = rank == 0 ? kPrThreads + 1 : kPrThreads;
+    for (int i = 0; i < C::kSlots; ++i) {
+      mbar_init(&full[i], in_count);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], rank == 0 ? kSmWarps + 1 : kSmWarps);
+    }
+    mbar_init(o_done, 1);
+    mbar_init(q_full, in_count);
+    mbar_init(fin, 1);
+    mbar_init(q_dead, 1);
+    for (int i = 0; i < kScaleTiles; ++i) mbar_init(&sc_full[i], kPrThreads);
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  // producers: the slot-id chain of the first key tiles is requested before the set-up barrier.  Lane
+  // l < 16 takes key 64 rank + 16 pw + l (this CTA's K rows and V rows), lane l >= 16 key
+  // 64 (1 - rank) + 16 pw + l - 16 (V rows only): a warp's V rows include its K rows
+  constexpr int kPrefetch = 4;
+  int64_t raw_q[kPrefetch] = {0, 0, 0, 0};
+  const int64_t* r2t = a.req_to_token;
+  int my_key = 0;
+  const int pw = warp - kPrWarp0;
+  auto raw_of = [&](int tile) -> int64_t {  // tile counts from jb
+    int64_t key = (int64_t)(jb + tile) * kKeys + my_key;
+    if (key >= kv_end) key = (int64_t)(jb + tile) * kKeys;  // past the window: the tile's first key
+    return r2t[key];
+  };
+  if (warp >= kPrWarp0 && warp < kIssueWarp) {
+    int64_t row = a.req_pool_indices[b];
+    if (row < 0 || row >= a.r2t_rows) {
+      if (tid == kPrWarp0 * 32 && rank == 0) record_err(a.err, TF_KERR_REQ_RANGE);
+      row = 0;
+    }
+    r2t = a.req_to_token + row * a.r2t_stride;
+    my_key = lane < 16 ? 64 * (int)rank + 16 * pw + lane : 64 * (1 - (int)rank) + 16 * pw + lane - 16;
+#pragma unroll
+    for (int i = 0; i < kPrefetch; ++i)
+      if (i < ntiles) raw_q[i] = raw_of(i);
+  }
+  if (warp == kIssueWarp) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_holder)), "r"(C::kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc::fence_before_sync();
+  cluster_sync();  // barriers of both CTAs initialised, TMEM allocated in both
+  tc::fence_after_sync();
+  const uint32_t tmem = *tmem_holder;
+  const int64_t q0 = *s_q0 + cta_start;
+  int64_t left = E - cta_start < TQ ? E - cta_start : TQ;
+  if (left > a.num_tokens - q0) left = a.num_tokens - q0;
+  const int n_tok = left > 0 ? (int)left : 0;  // query tokens of this CTA
+
+  if (warp >= kPrWarp0 && warp < kIssueWarp) {
+    // ======================= producers: this CTA's halves =======================
+    {  // Q: this CTA's 128 rows, scaled into f16's range; a row sits with D / 8 lanes
+      constexpr int CPR = D / 8, RPI = 32 / CPR;
+      const int sub = lane / CPR, ch = lane - (lane / CPR) * CPR;
+      const T* q = reinterpret_cast<const T*>(a.q);
+      const bool vec = ((reinterpret_cast<uintptr_t>(a.q) & 15) |
+                        ((a.q_stride_tok | a.q_stride_head) & 7)) == 0;
+#pragma unroll 4
+      for (int i = 0; i < 32; i += RPI) {
+        const int r = pw * 32 + i + sub;
+        const int ti = r / G, g = r - (r / G) * G;
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (ti < n_tok) {
+          const T* src = q + (q0 + ti) * a.q_stride_tok + (int64_t)(h * G + g) * a.q_stride_head + ch * 8;
+          if (vec) {
+            const uint4 v = *reinterpret_cast<const uint4*>(src);
+            w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+          } else {
+            const unsigned short* u = reinterpret_cast<const unsigned short*>(src);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = u[2 * k] | ((uint32_t)u[2 * k + 1] << 16);
+          }
+        }
+        uint32_t am = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          am = max(am, max(kv8::abs_bits(unpack_lo<T>(w[k])), kv8::abs_bits(unpack_hi<T>(w[k]))));
+#pragma unroll
+        for (int o = CPR / 2; o > 0; o >>= 1) am = max(am, __shfl_xor_sync(0xffffffffu, am, o));
+        const int ex = max((int)(am >> 23) - 127, -100);  // row maximum in [2^ex, 2^(ex+1))
+        const float mul = pow2i(14 - ex);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = pack2_rn<__half>(unpack_lo<T>(w[k]) * mul, unpack_hi<T>(w[k]) * mul);
+        sts128(base + (ch >> 3) * C::kQBlock + r * 128 + (((ch & 7) ^ (r & 7)) << 4), w[0], w[1], w[2], w[3]);
+        // a row that is not finite gives NaN logits
+        if (ch == 0) rowf[r] = am < 0x7f800000u ? a.scale * kLog2e * pow2i(max(ex - 14, -126)) : NAN;
+      }
+      tc::fence_proxy_async_smem();
+      mbar_arrive(q_full);
+    }
+    const char* kbuf = (const char*)a.k_buffer + (int64_t)h * a.kv_stride_head;
+    const char* vbuf = (const char*)a.v_buffer + (int64_t)h * a.kv_stride_head + rank * (D / 2);
+    const float* scp = sc.data + (int64_t)h * sc.stride_head;
+    constexpr int kLoads = D / 32;  // 16-byte loads of a lane per slot, K (16 rows a warp) and V (32) alike
+    float2 scl = make_float2(0.f, 0.f);  // of the K tile loaded last
+    // loads of a slot into registers
+    auto load = [&](int tile, bool isv, uint4 (&w)[kLoads]) {
+      int64_t* ids = ids_all + ((tile & 1) * kPrWarps + pw) * 32;
+      if (!isv) {  // this tile's slot ids (used by K now and by V later) and scales
+        const int64_t raw = raw_q[0];
+#pragma unroll
+        for (int i = 0; i + 1 < kPrefetch; ++i) raw_q[i] = raw_q[i + 1];
+        raw_q[kPrefetch - 1] = tile + kPrefetch < ntiles ? raw_of(tile + kPrefetch) : 0;
+        const int64_t sl = resolve_slot(raw, a.num_slots, a.slot_mode, a.err);
+        scl = __ldg(reinterpret_cast<const float2*>(scp + sl * sc.stride_slot));
+        __syncwarp();
+        ids[lane] = sl * a.kv_stride_slot;
+        __syncwarp();
+        constexpr int CPR = D / 16, RPI = 32 / CPR;
+        const int sub = lane / CPR, ch = lane - (lane / CPR) * CPR;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) w[i] = ldg_nc(kbuf + ids[i * RPI + sub] + ch * 16);
+      } else {
+        constexpr int CPR = D / 32, RPI = 32 / CPR;
+        const int sub = lane / CPR, ch = lane - (lane / CPR) * CPR;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) w[i] = ldg_nc(vbuf + ids[i * RPI + sub] + ch * 16);
+      }
+    };
+    int slot = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    // registers -> slot; 16 codes are two 16-byte chunks of f16, and lanes of odd 64-dim blocks
+    // store theirs in the other order (both orders together are free of bank conflicts)
+    auto put = [&](int tile, bool isv, const uint4 (&w)[kLoads], float2 s2) {
+      ok = __all_sync(0xffffffffu, wait_bar<false>(&empty[slot], phase ^ 1u, abort, peer_abort, 64));
+      if (!ok) return;
+      const uint32_t sb = base + C::kOffRing + slot * C::kSlotBytes;
+      const bool fin2 = kv8::abs_bits(s2.x) < 0x7f800000u && kv8::abs_bits(s2.y) < 0x7f800000u;
+      if (!isv) {
+        const int si = (tile & (kScaleTiles - 1)) * kKeys + my_key;
+        ks_s[si] = fin2 ? s2.x : NAN;
+        vs_s[si] = fin2 ? s2.y : 0.f;
+        const float vm = warp_max(fin2 ? fabsf(s2.y) : 0.f);
+        if (lane == 0)
+          ev_s[(tile & (kScaleTiles - 1)) * kPrWarps + pw] =
+              (float)min(max((int)(__float_as_uint(vm) >> 23) - 127, -100), 126);
+        mbar_arrive(&sc_full[tile & (kScaleTiles - 1)]);
+      }
+      const unsigned finm = __ballot_sync(0xffffffffu, fin2);
+      const int CPR = isv ? D / 32 : D / 16, RPI = 32 / CPR;
+      const int sub = lane / CPR, ch = lane - sub * CPR;
+      const int blk = ch >> 2, c0 = 2 * (ch & 3), odd = blk & 1;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int idx = i * RPI + sub;  // row of this warp
+        int row;
+        uint32_t dst;
+        if (!isv) {
+          row = 16 * pw + idx;
+          dst = sb + blk * C::kKBlk + row * 128;
+        } else {
+          row = idx < 16 ? 64 * (int)rank + 16 * pw + idx : 64 * (1 - (int)rank) + 16 * pw + idx - 16;
+          dst = sb + blk * C::kVBlk + row * 128;
+        }
+        uint4 v = w[i];
+        if (isv && !((finm >> idx) & 1u)) v = make_uint4(0, 0, 0, 0);
+        uint32_t f[8] = {cvt_lo(v.x), cvt_hi(v.x), cvt_lo(v.y), cvt_hi(v.y),
+                         cvt_lo(v.z), cvt_hi(v.z), cvt_lo(v.w), cvt_hi(v.w)};
+        const uint32_t d0 = dst + ((c0 ^ (row & 7)) << 4), d1 = dst + (((c0 + 1) ^ (row & 7)) << 4);
+        sts128(odd ? d1 : d0, odd ? f[4] : f[0], odd ? f[5] : f[1], odd ? f[6] : f[2], odd ? f[7] : f[3]);
+        sts128(odd ? d0 : d1, odd ? f[0] : f[4], odd ? f[1] : f[5], odd ? f[2] : f[6], odd ? f[3] : f[7]);
+      }
+      tc::fence_proxy_async_smem();
+      mbar_arrive(&full[slot]);
+      if (++slot == C::kSlots) { slot = 0; phase ^= 1u; }
+    };
+    // Slots in the order the products take them, K0 K1 V0 K2 V1 K3 ..., each loading while the one before
+    // it is converted.  K_{j+2} takes the id buffer of tile j, which V_j's loads have read.
+    uint4 wk[kLoads], wv[kLoads];
+    load(0, false, wk);
+    float2 s0 = scl, s1 = scl;  // scales of tiles j and j + 1
+    put(0, false, wk, s0);
+    if (ok && ntiles > 1) {
+      load(1, false, wk);
+      s1 = scl;
+    }
+    for (int j = 0; ok && j < ntiles; ++j) {
+      load(j, true, wv);
+      if (j + 1 < ntiles) {
+        put(j + 1, false, wk, s1);
+        if (!ok) break;
+      }
+      if (j + 2 < ntiles) load(j + 2, false, wk);
+      put(j, true, wv, s0);
+      s0 = s1;
+      s1 = scl;
+    }
+    // Output gate: once the last S product has completed (q_dead) the Q region is free; each producer
+    // warp copies 32 gate rows of this CTA into it while the last tiles still run (16-byte chunks
+    // XOR-swizzled by the row).  Every producer thread reaches the closing barrier.
+    const T* gate = reinterpret_cast<const T*>(a.gate);
+    const bool staged = a.gate_mode != TF_GATE_NONE && sp.n == 1 && rows_v16(a);
+    constexpr int kChunks = D / 8, kRowsPerInstr = 32 / kChunks;
+    const int gsub = lane / kChunks, gch = lane - (lane / kChunks) * kChunks;
+    bool okg = ok && wait_bar<false>(q_dead, 0, abort, peer_abort);
+    okg = __all_sync(0xffffffffu, okg);
+    if (okg && staged) {
+#pragma unroll 1
+      for (int i = 0; i < 32; i += kRowsPerInstr) {
+        const int row = pw * 32 + i + gsub;
+        const int ti = row / G, g = row - (row / G) * G;
+        if (ti < n_tok)
+          cp_async16(base + row * (D * 2) + ((gch ^ (row & (kChunks - 1))) << 4),
+                     gate + (q0 + ti) * a.gate_stride_tok + (int64_t)(h * G + g) * a.gate_stride_head + gch * 8);
+      }
+    }
+    cp_async_wait_all();
+    named_barrier(6, (kSmWarps + kPrWarps) * 32);  // gate rows staged for the softmax warps
+  } else if (warp == kIssueWarp && rank == 1) {
+    // ======================= relay: this CTA's halves landed -> rank 0 =======================
+    if (lane == 0) {
+      bool ok = wait_bar<false>(q_full, 0, abort, peer_abort);
+      if (ok) {
+        tc::fence_proxy_async_smem();
+        remote_arrive(peer_addr(smem_u32(q_full), 0));
+      }
+      int slot = 0;
+      uint32_t phase = 0;
+      for (int it = 0; ok && it < 2 * ntiles; ++it) {
+        ok = wait_bar<false>(&full[slot], phase, abort, peer_abort);
+        if (!ok) break;
+        tc::fence_proxy_async_smem();
+        remote_arrive(peer_addr(smem_u32(&full[slot]), 0));
+        if (++slot == C::kSlots) { slot = 0; phase ^= 1u; }
+      }
+      // rank 0's products done with this CTA's TMEM and smem; waited for also after an abort (bounded)
+      mbar_wait(fin, 0);
+    }
+    __syncwarp();
+  } else if (warp == kFwdWarp) {
+    // =========== rank 1: "this CTA's P_j is in TMEM" -> rank 0's p_full, one arrive per tile ===========
+    if (rank == 1 && lane == 0) {
+      const uint32_t pf0 = peer_addr(smem_u32(&p_full[0]), 0), pf1 = peer_addr(smem_u32(&p_full[1]), 0);
+      for (int j = 0; j < ntiles; ++j) {
+        if (!wait_bar<false>(&p_full[j & 1], (j >> 1) & 1, abort, peer_abort)) break;
+        tc::fence_after_sync();
+        tc::fence_before_sync();
+        remote_arrive((j & 1) ? pf1 : pf0);
+      }
+    }
+    __syncwarp();
+  } else if (warp == kIssueWarp) {
+    // ======================= MMA issue for the pair (rank 0, one thread) =======================
+    if (lane == 0) {
+      constexpr uint32_t kIdS = idesc_f16(2 * kRows, kKeys, false);
+      constexpr uint32_t kIdO = idesc_f16(2 * kRows, D, true);
+      bool ok = wait_bar<true>(q_full, 0, abort, peer_abort);
+      tc::fence_proxy_async_smem();
+      int slot = 0;
+      uint32_t phase = 0;
+      auto take = [&]() -> uint32_t {
+        ok = ok && wait_bar<true>(&full[slot], phase, abort, peer_abort);
+        tc::fence_proxy_async_smem();
+        return base + C::kOffRing + slot * C::kSlotBytes;
+      };
+      auto release = [&]() {
+        commit_both(&empty[slot]);
+        if (++slot == C::kSlots) { slot = 0; phase ^= 1u; }
+      };
+      auto issue_s = [&](int t) {
+        const uint32_t kb = take();
+        if (!ok) return;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint64_t ad = tc::sw128_desc(base + (kk >> 2) * C::kQBlock + (kk & 3) * 32, 16, 1024);
+          const uint64_t bd = tc::sw128_desc(kb + (kk >> 2) * C::kKBlk + (kk & 3) * 32, 16, 1024);
+          mma2_ss(tmem + C::kColS + (t & 1) * kKeys, ad, bd, kIdS, kk > 0);
+        }
+        commit_both(&s_full[t & 1]);
+        if (t == ntiles - 1) commit_both(q_dead);
+        release();
+      };
+      auto issue_pv = [&](int t) {
+        ok = ok && wait_bar<true>(&p_full[t & 1], (t >> 1) & 1, abort, peer_abort);
+        tc::fence_after_sync();
+        const uint32_t vb = take();
+        if (!ok) return;
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 16; ++kk) {
+          // P_j: keys [64 hf, 64 hf + 64) packed in columns [64 hf, 64 hf + 32) of S buffer j & 1
+          const uint64_t bd = tc::sw128_desc(vb + kk * 2048, C::kVBlk, 1024);
+          mma2_ts(tmem + C::kColO, tmem + C::kColS + (t & 1) * kKeys + 64 * (kk >> 2) + (kk & 3) * 8, bd,
+                  kIdO, t > 0 || kk > 0);
+        }
+        commit_both(o_done);
+        release();
+      };
+      if (ok) issue_s(0);
+      if (ok && ntiles > 1) issue_s(1);
+      for (int j = 0; ok && j < ntiles; ++j) {
+        issue_pv(j);
+        if (ok && j + 2 < ntiles) issue_s(j + 2);
+      }
+      if (!ok) commit_both(q_dead);  // aborted before the last S: release the waiters anyway
+      commit_both(fin);  // completes once every product issued above has completed
+      drain(fin, 0);     // also after an abort (bounded): none may be in flight when TMEM is released
+    }
+    __syncwarp();
+  } else if (warp < kSmWarps) {
+    // ============ softmax + epilogue: thread (half, r) = keys [64 half, +64) of row r ============
+    const int r = tid & (kRows - 1);
+    const int half = tid >> 7;
+    const int ri = r / G;
+    const bool row_valid = ri < n_tok;
+    const int64_t klim = P + cta_start + ri + 1;  // keys [0, klim) are visible to this row
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    constexpr int kOHalf = D / 2;  // O columns rescaled and stored by this thread
+    float m_used = -INFINITY, l_sum = 0.f, c2 = 0.f;
+    bool ok = true;
+    // No early exit from this loop: the two warps of a row group meet at a barrier every tile, so
+    // a failed wait only turns the remaining iterations into barrier-only ones.
+    for (int j = 0; j < ntiles; ++j) {
+      const int bi = j & 1, si = j & (kScaleTiles - 1);
+      // rows' factors and keys' scales come straight from the producers' barriers
+      if (ok && j == 0) ok = __all_sync(0xffffffffu, wait_bar<false>(q_full, 0, abort, peer_abort));
+      if (ok) ok = __all_sync(0xffffffffu, wait_bar<false>(&sc_full[si], (j / kScaleTiles) & 1, abort, peer_abort));
+      if (ok) ok = __all_sync(0xffffffffu, wait_bar<false>(&s_full[bi], (j >> 1) & 1, abort, peer_abort));
+      float s[2][32];
+      float pm = -INFINITY, ev = 0.f;
+      if (ok) {
+        tc::fence_after_sync();
+        if (j == 0) c2 = rowf[r];
+        const uint32_t sa = tmem + lane_base + C::kColS + bi * kKeys + 64 * half;
+        tc::ld32(sa, s[0]);
+        tc::ld32(sa + 32, s[1]);
+        const float4 e4 = *reinterpret_cast<const float4*>(ev_s + si * kPrWarps);
+        ev = fmaxf(fmaxf(e4.x, e4.y), fmaxf(e4.z, e4.w));
+        const float4* kp = reinterpret_cast<const float4*>(ks_s + si * kKeys + 64 * half);
+        tc::wait_ld();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const float4 v = kp[k];
+          float* x = &s[k >> 3][4 * (k & 7)];
+          x[0] *= v.x;
+          x[1] *= v.y;
+          x[2] *= v.z;
+          x[3] *= v.w;
+        }
+        // keys [0, vis) of this thread's 64 are visible to the row (0 for rows past the request end)
+        const int64_t rem = row_valid ? klim - (int64_t)(jb + j) * kKeys - 64 * half : 0;
+        const int vis = rem <= 0 ? 0 : (rem >= 64 ? 64 : (int)rem);
+        if (vis < 64) {
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (hh * 32 + k >= vis) s[hh][k] = -INFINITY;
+        }
+        pm = max_of_64(s);
+      }
+      // the row max over both halves (c2 > 0)
+      pmax[(bi * 2 + half) * kRows + r] = pm;
+      named_barrier(1 + (warp & 3), 64);
+      const float pm_other = pmax[(bi * 2 + (half ^ 1)) * kRows + r];
+      if (!ok) continue;
+      const float tmax = fmaf(fmaxf(pm, pm_other), c2, ev);
+      const bool need = tmax > m_used + kRescaleLog2 || (m_used == -INFINITY && tmax > -INFINITY);
+      const float m_new = need ? tmax : m_used;
+      const float alpha = need ? (m_used == -INFINITY ? 0.f : exp2f(m_used - m_new)) : 1.f;
+      m_used = m_new;
+      l_sum *= alpha;
+      if (j > 0 && __any_sync(0xffffffffu, need)) {  // rescale this thread's half of its O row
+        ok = __all_sync(0xffffffffu, wait_bar<false>(o_done, (j - 1) & 1, abort, peer_abort));
+        if (!ok) continue;
+        tc::fence_after_sync();
+#pragma unroll 1
+        for (int cc = 0; cc < kOHalf / 32; ++cc) {
+          const uint32_t ta = tmem + lane_base + C::kColO + half * kOHalf + cc * 32;
+          float o[32];
+          tc::ld32(ta, o);
+          tc::wait_ld();
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] *= alpha;
+          tc::st32(ta, o);
+        }
+      }
+      const float nmu = m_used == -INFINITY ? 0.f : -m_used;
+      float pk[32], ls[4] = {0.f, 0.f, 0.f, 0.f};
+      const float4* vp = reinterpret_cast<const float4*>(vs_s + si * kKeys + 64 * half);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const float4 v = vp[k];
+        const float* x = &s[k >> 3][4 * (k & 7)];
+        const float p0 = ex2_ftz(fmaf(x[0], c2, nmu)), p1 = ex2_ftz(fmaf(x[1], c2, nmu));
+        const float p2 = ex2_ftz(fmaf(x[2], c2, nmu)), p3 = ex2_ftz(fmaf(x[3], c2, nmu));
+        ls[k & 3] += (p0 + p1) + (p2 + p3);
+        pk[2 * k] = __uint_as_float(pack2_rn<__half>(p0 * v.x, p1 * v.y));
+        pk[2 * k + 1] = __uint_as_float(pack2_rn<__half>(p2 * v.z, p3 * v.w));
+      }
+      l_sum += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+      // P over the first 32 of this thread's 64 S columns: only this thread read them
+      tc::st32(tmem + lane_base + C::kColS + bi * kKeys + 64 * half, pk);
+      tc::wait_st();
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[bi]);  // rank 1's forward warp passes it on to rank 0
+    }
+    const bool gated = a.gate_mode != TF_GATE_NONE;
+    const bool vec = rows_v16(a);
+    if (ok) ok = __all_sync(0xffffffffu, wait_bar<false>(fin, 0, abort, peer_abort));
+    // ---- epilogue.  Once fin completed, no product reads Q or the ring any more: the two halves' row
+    // sums meet in the ring
+    float* l_part = reinterpret_cast<float*>(sbase + C::kOffRing);
+    if (ok) l_part[half * kRows + r] = l_sum;
+    named_barrier(5, kSmWarps * 32);
+    const float l_tot = ok ? l_part[r] + l_part[kRows + r] : 0.f;
+    named_barrier(6, (kSmWarps + kPrWarps) * 32);  // gate rows are staged
+    if (ok) {
+      tc::fence_after_sync();
+      const int hq = h * G + (r - ri * G);
+      const int64_t t = q0 + ri;
+      const float inv = 1.f / l_tot;
+      float* po = nullptr;
+      if (sp.n > 1 && row_valid) {
+        const int64_t row = ((int64_t)z * a.num_tokens + t) * a.num_q_heads + hq;
+        po = sp.o + row * D + half * kOHalf;
+        if (half == 0) *reinterpret_cast<float2*>(sp.ml + 2 * row) = make_float2(m_used, l_tot);
+      }
+      T* orow = (T*)a.out + t * a.out_stride_tok + (int64_t)hq * a.out_stride_head + half * kOHalf;
+      const T* grow = (const T*)a.gate + t * a.gate_stride_tok + (int64_t)hq * a.gate_stride_head + half * kOHalf;
+      constexpr int kChunks = D / 8;
+#pragma unroll 1
+      for (int cc = 0; cc < kOHalf / 32; ++cc) {
+        float o[32];
+        tc::ld32(tmem + lane_base + C::kColO + half * kOHalf + cc * 32, o);
+        tc::wait_ld();
+        if (!row_valid) continue;
+        if (sp.n > 1) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            *reinterpret_cast<float4*>(po + cc * 32 + 4 * k) = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+        } else if (vec) {
+#pragma unroll
+          for (int c8 = 0; c8 < 4; ++c8) {
+            uint32_t gw[4] = {0, 0, 0, 0}, ow[4];
+            if (gated) {
+              const int chunk = (half * kOHalf + cc * 32) / 8 + c8;
+              asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                           : "=r"(gw[0]), "=r"(gw[1]), "=r"(gw[2]), "=r"(gw[3])
+                           : "r"(base + r * (D * 2) + ((chunk ^ (r & (kChunks - 1))) << 4)));
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              float x0 = o[c8 * 8 + 2 * k] * inv, x1 = o[c8 * 8 + 2 * k + 1] * inv;
+              if (gated) {
+                x0 *= act(unpack_lo<T>(gw[k]), a.gate_mode);
+                x1 *= act(unpack_hi<T>(gw[k]), a.gate_mode);
+              }
+              ow[k] = pack2_rn<T>(x0, x1);
+            }
+            *reinterpret_cast<uint4*>(orow + cc * 32 + c8 * 8) = make_uint4(ow[0], ow[1], ow[2], ow[3]);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            float x = o[k] * inv;
+            if (gated) x *= act(to_f(grow[cc * 32 + k]), a.gate_mode);
+            orow[cc * 32 + k] = from_f<T>(x);
+          }
+        }
+      }
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  // rank 0's products read this CTA's shared memory and TMEM, and remote arrivals target rank 0's
+  // barriers: neither CTA releases TMEM or exits before both are done
+  cluster_sync();
+  if (tid == 0 && *abort) record_err(a.err, TF_KERR_TIMEOUT);
+  tc::fence_after_sync();
+  if (warp == kIssueWarp)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemCols)
+                 : "memory");
+}
+
+// one warp per (token, head): the clusters' partials of a row
+template <typename T, int D>
+__global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ tf_paged_attn_args a,
+                                                    const __grid_constant__ Split sp, int64_t rows) {
+  const int64_t row = (blockIdx.x * 256ll + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  // only rows of a request have partials
+  int64_t total = 0;
+  for (int i = lane; i < a.batch_size; i += 32) {
+    const int64_t e = a.extend_lens ? a.extend_lens[i] : 1;
+    total += e > 0 ? e : 0;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if (row >= rows || row >= total * a.num_q_heads) return;
+  const int64_t t = row / a.num_q_heads;
+  const int hq = (int)(row - t * a.num_q_heads);
+  // a request whose lengths were refused has no partials either
+  {
+    int64_t base = 0;
+    bool bad = false;
+    for (int i0 = 0; i0 < a.batch_size; i0 += 32) {
+      int64_t e = i0 + lane < a.batch_size ? (a.extend_lens ? a.extend_lens[i0 + lane] : 1) : 0;
+      if (e < 0) e = 0;
+      int64_t incl = e;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+      }
+      const bool mine = t >= base + incl - e && t < base + incl;
+      const int64_t L = mine ? a.seq_lens[i0 + lane] : 0;
+      bad = bad || __any_sync(0xffffffffu, mine && (L > a.r2t_cols || L < e));
+      base += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (bad) return;
+  }
+  const float* mlp = sp.ml + 2 * row;
+  const float* op = sp.o + row * D;
+  const int64_t step = a.num_tokens * (int64_t)a.num_q_heads;
+  float M = -INFINITY;
+  for (int z = 0; z < sp.n; ++z) M = fmaxf(M, mlp[2 * z * step]);
+  constexpr int V = D / 128;  // 16-byte pieces of a lane
+  float4 o[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+  for (int z = 0; z < sp.n; ++z) {
+    const float2 ml = *reinterpret_cast<const float2*>(mlp + 2 * z * step);
+    if (ml.x == -INFINITY && ml.y == 0.f) continue;  // no keys there, and no O written
+    const float f = ml.x == M ? 1.f : exp2f(ml.x - M);
+    l = fmaf(f, ml.y, l);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float4 x = *reinterpret_cast<const float4*>(op + z * step * D + 128 * i + 4 * lane);
+      o[i].x = fmaf(f, x.x, o[i].x);
+      o[i].y = fmaf(f, x.y, o[i].y);
+      o[i].z = fmaf(f, x.z, o[i].z);
+      o[i].w = fmaf(f, x.w, o[i].w);
+    }
+  }
+  const float inv = 1.f / l;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const float x[4] = {o[i].x * inv, o[i].y * inv, o[i].z * inv, o[i].w * inv};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int d = 128 * i + 4 * lane + k;
+      float y = x[k];
+      if (a.gate_mode != TF_GATE_NONE)
+        y *= act(to_f(((const T*)a.gate)[t * a.gate_stride_tok + (int64_t)hq * a.gate_stride_head + d]), a.gate_mode);
+      ((T*)a.out)[t * a.out_stride_tok + (int64_t)hq * a.out_stride_head + d] = from_f<T>(y);
+    }
+  }
+}
+
+// Clusters that share a query tile's keys: enough to give every SM pair one, while each keeps at
+// least eight key tiles (a cluster's fixed cost, about 17 us, is that of eleven tiles).
+static int splits_of(const tf_paged_attn_args& a, int num_sms) {
+  const int G = a.num_q_heads / a.num_kv_heads;
+  const int64_t pairs = ((int64_t)a.max_extend_len * G + 2 * kRows - 1) / (2 * kRows);
+  const int64_t clusters = a.batch_size * pairs * a.num_kv_heads;
+  const int64_t slots = num_sms / 2;
+  int64_t n = clusters > 0 ? slots / clusters : 1;
+  const int64_t most = a.max_seq_len / (8 * kKeys);
+  n = n < most ? n : most;
+  return n < 1 ? 1 : (n > 32 ? 32 : (int)n);
+}
+
+template <typename T, int D>
+static cudaError_t launch_td(const tf_paged_attn_args& a, const tf_kv_scale& sc, void* ws, int num_sms,
+                             cudaStream_t s) {
+  const int G = a.num_q_heads / a.num_kv_heads;
+  const int TQ = kRows / G;
+  const int pairs = (a.max_extend_len + 2 * TQ - 1) / (2 * TQ);
+  Split sp{splits_of(a, num_sms), nullptr, nullptr};
+  const int64_t rows = (int64_t)a.num_tokens * a.num_q_heads;
+  if (sp.n > 1) {
+    sp.ml = (float*)ws;
+    sp.o = sp.ml + ((2 * sp.n * rows + 63) & ~(int64_t)63);
+  }
+  cudaError_t e = cudaFuncSetAttribute(extend_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       Cfg<D>::kSmem);
+  if (e != cudaSuccess) return e;
+  dim3 grid((unsigned)(2 * a.batch_size * pairs), (unsigned)a.num_kv_heads, (unsigned)sp.n);
+  extend_kernel<T, D><<<grid, kThreads, Cfg<D>::kSmem, s>>>(a, sc, pairs, sp);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || sp.n == 1) return e;
+  merge_kernel<T, D><<<(unsigned)((rows + 7) / 8), 256, 0, s>>>(a, sp, rows);
+  return cudaGetLastError();
+}
+
+}  // namespace ext8
+
+bool paged_fp8_extend_supported(const tf_paged_attn_args& a) {
+  if (a.dtype != TF_DTYPE_BF16 && a.dtype != TF_DTYPE_F16) return false;
+  if (a.head_dim != 128 && a.head_dim != 256) return false;
+  const int G = a.num_q_heads / a.num_kv_heads;
+  if (G < 1 || G > 16) return false;
+  if (a.max_extend_len <= 0 || a.num_kv_heads > 65535) return false;
+  if (!(a.scale > 0.f)) return false;  // the softmax takes its max before the scale
+  auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  return al(a.k_buffer) && al(a.v_buffer) && a.kv_stride_slot % 16 == 0 && a.kv_stride_head % 16 == 0;
+}
+
+size_t paged_fp8_extend_workspace(const tf_paged_attn_args& a, int num_sms) {
+  const int n = ext8::splits_of(a, num_sms);
+  if (n == 1) return 0;
+  const int64_t rows = (int64_t)a.num_tokens * a.num_q_heads;
+  return (((2 * n * rows + 63) & ~(int64_t)63) + n * rows * a.head_dim) * 4;
+}
+
+cudaError_t launch_paged_fp8_extend(const tf_paged_attn_args& a, const tf_kv_scale& sc, void* ws,
+                                    int num_sms, cudaStream_t s) {
+  const bool bf = a.dtype == TF_DTYPE_BF16;
+  if (a.head_dim == 128)
+    return bf ? ext8::launch_td<__nv_bfloat16, 128>(a, sc, ws, num_sms, s)
+              : ext8::launch_td<__half, 128>(a, sc, ws, num_sms, s);
+  return bf ? ext8::launch_td<__nv_bfloat16, 256>(a, sc, ws, num_sms, s)
+            : ext8::launch_td<__half, 256>(a, sc, ws, num_sms, s);
+}
+
+}  // namespace tf

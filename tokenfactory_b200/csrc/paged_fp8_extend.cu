@@ -7,7 +7,9 @@
 // of V; softmax warps own their CTA's rows, producer warps gather its halves, one thread of rank 0
 // issues the products.  What the 8-bit pool changes:
 //   producers   load 16 codes a lane, convert them to f16 (exact) and store them into the swizzled
-//               tile; a slot's loads are in flight while the one before it is converted
+//               tile.  Four warps make the K slots and four the V slots, each with the next slot of its
+//               kind on its way into registers while one is converted: a tile's slots are free too
+//               late for a load and a conversion in turn
 //   scales      are not multiplied into the tiles (a second rounding of every element): a key's logit
 //               is its product times ks_j in fp32, and its weight p_j = 2^(s_j - M) enters P as
 //               f16(p_j vs_j).  M follows s_j + ev_j, ev_j the exponent of the largest vs of the tile,
@@ -19,6 +21,8 @@
 //
 // Few query tiles over a long prefix leave SM pairs idle: the key tiles are then split over
 // grid.z clusters, which leave (M, l, O) partials for a combine kernel.
+#include <type_traits>
+
 #include "common.cuh"
 #include "kv_fp8.cuh"
 #include "launch.h"
@@ -29,14 +33,12 @@ namespace ext8 {
 
 constexpr int kRows = 128;       // query rows of a CTA
 constexpr int kKeys = 128;       // keys of a tile
-constexpr int kSmWarps = 8;      // softmax: two warps per 32-row group, 64 keys each
-constexpr int kPrWarps = 4;      // producers
+constexpr int kSmWarps = 8;      // softmax: warps 0-3 take the even tiles, 4-7 the odd ones
+constexpr int kPrWarps = 8;      // producers: four of K (16 rows of a tile each), four of V (32 rows)
 constexpr int kPrWarp0 = kSmWarps;
 constexpr int kIssueWarp = kSmWarps + kPrWarps;  // MMA issue (rank 0) / slot relay (rank 1)
 constexpr int kFwdWarp = kIssueWarp + 1;         // rank 1: forwards "P written" to rank 0
 constexpr int kThreads = (kFwdWarp + 1) * 32;
-constexpr int kPrThreads = kPrWarps * 32;
-constexpr int kScaleTiles = 4;   // ring of the tiles' scales
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleLog2 = 8.f;
 
@@ -65,6 +67,52 @@ __device__ __forceinline__ float ex2_ftz(float x) {
   return y;
 }
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126..127
+
+// two fp32 operations in one instruction (each rounded as its scalar form)
+__device__ __forceinline__ uint64_t pk2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void up2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// 64 raw products times their keys' scales; the ones from `vis` on are hidden
+__device__ __forceinline__ void scale_mask(float (&s)[2][32], const float* ks, int vis) {
+  const ulonglong2* kp = reinterpret_cast<const ulonglong2*>(ks);
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const ulonglong2 v = kp[k];
+    float* x = &s[k >> 3][4 * (k & 7)];
+    up2(mul2(pk2(x[0], x[1]), v.x), x[0], x[1]);
+    up2(mul2(pk2(x[2], x[3]), v.y), x[2], x[3]);
+  }
+  if (vis < 64) {
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int k = 0; k < 32; ++k)
+        if (hh * 32 + k >= vis) s[hh][k] = -INFINITY;
+  }
+}
+__device__ __forceinline__ void bar_arrive(int id, int nthreads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
+}
 
 // ---- cluster pair helpers
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -183,25 +231,29 @@ struct Cfg {
   static constexpr int kVBlk = kKeys * 128;       // V half: 128 keys x 128 B per block
   static constexpr int kSlotBytes = kKB * kKBlk;  // == (kKB / 2) * kVBlk
   static constexpr int kSlots = D == 256 ? 4 : 8;
+  // Ring of the tiles' scales.  Those of tile t are written once V_{t-1} has been stored, for which
+  // PV_{t-1-kSlots/2} had completed: the softmax of that tile is done with its scales, a later one's
+  // may not be.
+  static constexpr int kScaleTiles = D == 256 ? 4 : 8;
+  static_assert(kScaleTiles >= kSlots / 2 + 1, "scales in use are not overwritten");
   static constexpr int kOffRing = kQBytes;
   static constexpr int kOffBars = kOffRing + kSlots * kSlotBytes;
   // full, empty [kSlots]; s_full[2], p_full[2], o_done, q_full, fin, q_dead, sc_full[kScaleTiles]
   static constexpr int kNumBars = 2 * kSlots + 8 + kScaleTiles;
   static constexpr int kOffWords = kOffBars + 8 * kNumBars;      // tmem holder, abort, q0
-  static constexpr int kOffIds = (kOffWords + 16 + 15) & ~15;    // int64 [2][kPrWarps][32]
-  static constexpr int kOffPmax = kOffIds + 2 * kPrWarps * 32 * 8;  // float [2][2][kRows]
-  static constexpr int kOffRow = kOffPmax + 2 * 2 * kRows * 4;   // float [kRows]: logit factor of a row
+  static constexpr int kOffM = (kOffWords + 16 + 15) & ~15;      // float [2][kRows]: running maxima
+  static constexpr int kOffRow = kOffM + 2 * kRows * 4;          // float [kRows]: logit factor of a row
   static constexpr int kOffKs = kOffRow + kRows * 4;             // float [kScaleTiles][kKeys]
   static constexpr int kOffVs = kOffKs + kScaleTiles * kKeys * 4;
-  static constexpr int kOffEv = kOffVs + kScaleTiles * kKeys * 4;   // float [kScaleTiles][kPrWarps]
-  static constexpr int kSmem = kOffEv + kScaleTiles * kPrWarps * 4 + 1024;
+  static constexpr int kOffEv = kOffVs + kScaleTiles * kKeys * 4;   // float [kScaleTiles][4]
+  static constexpr int kSmem = kOffEv + kScaleTiles * 4 * 4 + 1024;
   static constexpr int kColS = 0;                 // two S buffers of kKeys columns; P_j over S_j
   static constexpr int kColO = 2 * kKeys;
   static constexpr int kTmemCols = 512;
   static_assert(kSlotBytes == (kKB / 2) * kVBlk, "K and V halves share the slot size");
   static_assert(kSmem <= 232448, "shared memory per CTA");
   static_assert(kColO + D <= kTmemCols, "TMEM columns");
-  static_assert(2 * kRows * 4 <= kSlotBytes && kRows * D * 2 <= kQBytes, "epilogue staging");
+  static_assert(4 * kRows * 4 <= kSlotBytes && kRows * D * 2 <= kQBytes, "epilogue staging");
 };
 
 struct Split {
@@ -241,8 +293,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(sbase + C::kOffWords);
   volatile int* abort = reinterpret_cast<volatile int*>(sbase + C::kOffWords + 4);
   int64_t* s_q0 = reinterpret_cast<int64_t*>(sbase + C::kOffWords + 8);
-  int64_t* ids_all = reinterpret_cast<int64_t*>(sbase + C::kOffIds);
-  float* pmax = reinterpret_cast<float*>(sbase + C::kOffPmax);
+  float* m_s = reinterpret_cast<float*>(sbase + C::kOffM);
   float* rowf = reinterpret_cast<float*>(sbase + C::kOffRow);
   float* ks_s = reinterpret_cast<float*>(sbase + C::kOffKs);
   float* vs_s = reinterpret_cast<float*>(sbase + C::kOffVs);
@@ -297,26 +348,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     return;
   }
   if (tid == 0) {
-    const uint32_t in_count = rank == 0 ? kPrThreads + 1 : kPrThreads;
+    const uint32_t in_count = rank == 0 ? kPrWarps + 1 : kPrWarps;  // one arrive a warp
     for (int i = 0; i < C::kSlots; ++i) {
-      mbar_init(&full[i], in_count);
+      mbar_init(&full[i], rank == 0 ? kPrWarps / 2 + 1 : kPrWarps / 2);
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], rank == 0 ? kSmWarps + 1 : kSmWarps);
+      mbar_init(&p_full[i], rank == 0 ? kSmWarps / 2 + 1 : kSmWarps / 2);
     }
     mbar_init(o_done, 1);
     mbar_init(q_full, in_count);
     mbar_init(fin, 1);
     mbar_init(q_dead, 1);
-    for (int i = 0; i < kScaleTiles; ++i) mbar_init(&sc_full[i], kPrThreads);
+    for (int i = 0; i < C::kScaleTiles; ++i) mbar_init(&sc_full[i], kPrWarps / 2);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   // producers: the slot-id chain of the first key tiles is requested before the set-up barrier.  Lane
-  // l < 16 takes key 64 rank + 16 pw + l (this CTA's K rows and V rows), lane l >= 16 key
-  // 64 (1 - rank) + 16 pw + l - 16 (V rows only): a warp's V rows include its K rows
+  // l of K warp w takes key 64 rank + 16 w + l % 16 of a tile, lane l of V warp w key 32 w + l
   constexpr int kPrefetch = 4;
   int64_t raw_q[kPrefetch] = {0, 0, 0, 0};
   const int64_t* r2t = a.req_to_token;
@@ -334,7 +384,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       row = 0;
     }
     r2t = a.req_to_token + row * a.r2t_stride;
-    my_key = lane < 16 ? 64 * (int)rank + 16 * pw + lane : 64 * (1 - (int)rank) + 16 * pw + lane - 16;
+    my_key = pw < 4 ? 64 * (int)rank + 16 * pw + (lane & 15) : 32 * (pw - 4) + lane;
 #pragma unroll
     for (int i = 0; i < kPrefetch; ++i)
       if (i < ntiles) raw_q[i] = raw_of(i);
@@ -363,8 +413,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const bool vec = ((reinterpret_cast<uintptr_t>(a.q) & 15) |
                         ((a.q_stride_tok | a.q_stride_head) & 7)) == 0;
 #pragma unroll 4
-      for (int i = 0; i < 32; i += RPI) {
-        const int r = pw * 32 + i + sub;
+      for (int i = 0; i < kRows / kPrWarps; i += RPI) {
+        const int r = pw * (kRows / kPrWarps) + i + sub;
         const int ti = r / G, g = r - (r / G) * G;
         uint32_t w[4] = {0, 0, 0, 0};
         if (ti < n_tok) {
@@ -393,108 +443,94 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (ch == 0) rowf[r] = am < 0x7f800000u ? a.scale * kLog2e * pow2i(max(ex - 14, -126)) : NAN;
       }
       tc::fence_proxy_async_smem();
-      mbar_arrive(q_full);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
     }
-    const char* kbuf = (const char*)a.k_buffer + (int64_t)h * a.kv_stride_head;
-    const char* vbuf = (const char*)a.v_buffer + (int64_t)h * a.kv_stride_head + rank * (D / 2);
     const float* scp = sc.data + (int64_t)h * sc.stride_head;
-    constexpr int kLoads = D / 32;  // 16-byte loads of a lane per slot, K (16 rows a warp) and V (32) alike
-    float2 scl = make_float2(0.f, 0.f);  // of the K tile loaded last
-    // loads of a slot into registers
-    auto load = [&](int tile, bool isv, uint4 (&w)[kLoads]) {
-      int64_t* ids = ids_all + ((tile & 1) * kPrWarps + pw) * 32;
-      if (!isv) {  // this tile's slot ids (used by K now and by V later) and scales
+    bool ok = true;
+    // the slots of one kind
+    auto produce = [&](auto kind) {
+      constexpr bool kV = decltype(kind)::value;
+      constexpr int kRowsW = kV ? 32 : 16;             // rows of a tile that a warp makes
+      constexpr int CPR = kV ? D / 32 : D / 16;        // 16-byte pieces of a row of codes
+      constexpr int RPI = 32 / CPR, kLoads = kRowsW / RPI;
+      constexpr int kBlkBytes = kV ? C::kVBlk : C::kKBlk;
+      const int sub = lane / CPR, ch = lane - (lane / CPR) * CPR;
+      const char* src = kV ? (const char*)a.v_buffer + (int64_t)h * a.kv_stride_head + rank * (D / 2) + ch * 16
+                           : (const char*)a.k_buffer + (int64_t)h * a.kv_stride_head + ch * 16;
+      const int row0 = (kV ? 32 * (pw - 4) : 16 * pw) + sub;
+      // 16 codes are two 16-byte chunks of f16; lanes of odd 64-dim blocks store theirs in the other
+      // order (a bank conflict otherwise)
+      const int blk = ch >> 2;
+      const bool odd = blk & 1;
+      const int ca = 2 * (ch & 3) + (odd ? 1 : 0), cb = 2 * (ch & 3) + (odd ? 0 : 1);
+      auto load = [&](int tile, uint4 (&w)[kLoads], float2& s2) {
         const int64_t raw = raw_q[0];
 #pragma unroll
-        for (int i = 0; i + 1 < kPrefetch; ++i) raw_q[i] = raw_q[i + 1];
+        for (int k = 0; k + 1 < kPrefetch; ++k) raw_q[k] = raw_q[k + 1];
         raw_q[kPrefetch - 1] = tile + kPrefetch < ntiles ? raw_of(tile + kPrefetch) : 0;
         const int64_t sl = resolve_slot(raw, a.num_slots, a.slot_mode, a.err);
-        scl = __ldg(reinterpret_cast<const float2*>(scp + sl * sc.stride_slot));
-        __syncwarp();
-        ids[lane] = sl * a.kv_stride_slot;
-        __syncwarp();
-        constexpr int CPR = D / 16, RPI = 32 / CPR;
-        const int sub = lane / CPR, ch = lane - (lane / CPR) * CPR;
+        const uint32_t off = (uint32_t)((sl * a.kv_stride_slot) >> 4);  // 16-byte pieces (the host checks)
+        uint32_t o[kLoads];
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) w[i] = ldg_nc(kbuf + ids[i * RPI + sub] + ch * 16);
-      } else {
-        constexpr int CPR = D / 32, RPI = 32 / CPR;
-        const int sub = lane / CPR, ch = lane - (lane / CPR) * CPR;
+        for (int k = 0; k < kLoads; ++k) o[k] = __shfl_sync(0xffffffffu, off, k * RPI + sub);
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) w[i] = ldg_nc(vbuf + ids[i * RPI + sub] + ch * 16);
-      }
-    };
-    int slot = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    // registers -> slot; 16 codes are two 16-byte chunks of f16, and lanes of odd 64-dim blocks
-    // store theirs in the other order (both orders together are free of bank conflicts)
-    auto put = [&](int tile, bool isv, const uint4 (&w)[kLoads], float2 s2) {
-      ok = __all_sync(0xffffffffu, wait_bar<false>(&empty[slot], phase ^ 1u, abort, peer_abort, 64));
-      if (!ok) return;
-      const uint32_t sb = base + C::kOffRing + slot * C::kSlotBytes;
-      const bool fin2 = kv8::abs_bits(s2.x) < 0x7f800000u && kv8::abs_bits(s2.y) < 0x7f800000u;
-      if (!isv) {
-        const int si = (tile & (kScaleTiles - 1)) * kKeys + my_key;
-        ks_s[si] = fin2 ? s2.x : NAN;
-        vs_s[si] = fin2 ? s2.y : 0.f;
-        const float vm = warp_max(fin2 ? fabsf(s2.y) : 0.f);
-        if (lane == 0)
-          ev_s[(tile & (kScaleTiles - 1)) * kPrWarps + pw] =
-              (float)min(max((int)(__float_as_uint(vm) >> 23) - 127, -100), 126);
-        mbar_arrive(&sc_full[tile & (kScaleTiles - 1)]);
-      }
-      const unsigned finm = __ballot_sync(0xffffffffu, fin2);
-      const int CPR = isv ? D / 32 : D / 16, RPI = 32 / CPR;
-      const int sub = lane / CPR, ch = lane - sub * CPR;
-      const int blk = ch >> 2, c0 = 2 * (ch & 3), odd = blk & 1;
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int idx = i * RPI + sub;  // row of this warp
-        int row;
-        uint32_t dst;
-        if (!isv) {
-          row = 16 * pw + idx;
-          dst = sb + blk * C::kKBlk + row * 128;
-        } else {
-          row = idx < 16 ? 64 * (int)rank + 16 * pw + idx : 64 * (1 - (int)rank) + 16 * pw + idx - 16;
-          dst = sb + blk * C::kVBlk + row * 128;
+        for (int k = 0; k < kLoads; ++k) w[k] = ldg_nc(src + (uint64_t)o[k] * 16);
+        if (kV) s2 = __ldg(reinterpret_cast<const float2*>(scp + sl * sc.stride_slot));
+      };
+      int slot = kV ? 2 : 0;   // ring place: K0 K1 V0 K2 V1 K3 ... V_{n-2} V_{n-1}
+      uint32_t phase = 0;
+      auto put = [&](int tile, uint4 (&w)[kLoads], float2 s2) {
+        unsigned keep = 0xffffffffu;  // rows that are not zeroed
+        if (kV) {
+          // scales of the tile.  One that is not finite: NaN logits, and a V row of zeros
+          const bool fin = kv8::abs_bits(s2.x) < 0x7f800000u && kv8::abs_bits(s2.y) < 0x7f800000u;
+          const int st = tile & (C::kScaleTiles - 1);
+          ks_s[st * kKeys + my_key] = fin ? s2.x : NAN;
+          vs_s[st * kKeys + my_key] = fin ? s2.y : 0.f;
+          const float vm = warp_max(fin ? fabsf(s2.y) : 0.f);
+          if (lane == 0)
+            ev_s[st * 4 + pw - 4] = (float)min(max((int)(__float_as_uint(vm) >> 23) - 127, -100), 126);
+          keep = __ballot_sync(0xffffffffu, fin);
+          if (lane == 0) mbar_arrive(&sc_full[st]);
         }
-        uint4 v = w[i];
-        if (isv && !((finm >> idx) & 1u)) v = make_uint4(0, 0, 0, 0);
-        uint32_t f[8] = {cvt_lo(v.x), cvt_hi(v.x), cvt_lo(v.y), cvt_hi(v.y),
-                         cvt_lo(v.z), cvt_hi(v.z), cvt_lo(v.w), cvt_hi(v.w)};
-        const uint32_t d0 = dst + ((c0 ^ (row & 7)) << 4), d1 = dst + (((c0 + 1) ^ (row & 7)) << 4);
-        sts128(odd ? d1 : d0, odd ? f[4] : f[0], odd ? f[5] : f[1], odd ? f[6] : f[2], odd ? f[7] : f[3]);
-        sts128(odd ? d0 : d1, odd ? f[0] : f[4], odd ? f[1] : f[5], odd ? f[2] : f[6], odd ? f[3] : f[7]);
+        // the slot's place and round: position i = 2 tile - 1 (K), 2 tile + 2 (V), shifted at the ends
+        const int i = kV ? (tile == ntiles - 1 ? 2 * ntiles - 1 : 2 * tile + 2) : (tile == 0 ? 0 : 2 * tile - 1);
+        slot = i % C::kSlots;
+        phase = (uint32_t)(i / C::kSlots) & 1u;
+        ok = __all_sync(0xffffffffu, wait_bar<false>(&empty[slot], phase ^ 1u, abort, peer_abort, 32));
+        if (!ok) return;
+        const uint32_t sb = base + C::kOffRing + slot * C::kSlotBytes + blk * kBlkBytes;
+#pragma unroll
+        for (int k = 0; k < kLoads; ++k) {
+          const int row = row0 + k * RPI;
+          uint4 v = w[k];
+          if (kV && !((keep >> (k * RPI + sub)) & 1u)) v = make_uint4(0, 0, 0, 0);
+          if (odd) v = make_uint4(v.z, v.w, v.x, v.y);
+          const uint32_t dst = sb + row * 128;
+          sts128(dst + ((ca ^ (row & 7)) << 4), cvt_lo(v.x), cvt_hi(v.x), cvt_lo(v.y), cvt_hi(v.y));
+          sts128(dst + ((cb ^ (row & 7)) << 4), cvt_lo(v.z), cvt_hi(v.z), cvt_lo(v.w), cvt_hi(v.w));
+        }
+        tc::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[slot]);
+      };
+      uint4 wa[kLoads], wb[kLoads];
+      float2 sa = make_float2(0.f, 0.f), sb2 = sa;
+      load(0, wa, sa);
+#pragma unroll 1
+      for (int j = 0; ok && j < ntiles; j += 2) {
+        if (j + 1 < ntiles) load(j + 1, wb, sb2);
+        put(j, wa, sa);
+        if (!ok || j + 1 >= ntiles) break;
+        if (j + 2 < ntiles) load(j + 2, wa, sa);
+        put(j + 1, wb, sb2);
       }
-      tc::fence_proxy_async_smem();
-      mbar_arrive(&full[slot]);
-      if (++slot == C::kSlots) { slot = 0; phase ^= 1u; }
     };
-    // Slots in the order the products take them, K0 K1 V0 K2 V1 K3 ..., each loading while the one before
-    // it is converted.  K_{j+2} takes the id buffer of tile j, which V_j's loads have read.
-    uint4 wk[kLoads], wv[kLoads];
-    load(0, false, wk);
-    float2 s0 = scl, s1 = scl;  // scales of tiles j and j + 1
-    put(0, false, wk, s0);
-    if (ok && ntiles > 1) {
-      load(1, false, wk);
-      s1 = scl;
-    }
-    for (int j = 0; ok && j < ntiles; ++j) {
-      load(j, true, wv);
-      if (j + 1 < ntiles) {
-        put(j + 1, false, wk, s1);
-        if (!ok) break;
-      }
-      if (j + 2 < ntiles) load(j + 2, false, wk);
-      put(j, true, wv, s0);
-      s0 = s1;
-      s1 = scl;
-    }
+    if (pw < 4) produce(std::false_type());
+    else produce(std::true_type());
     // Output gate: once the last S product has completed (q_dead) the Q region is free; each producer
-    // warp copies 32 gate rows of this CTA into it while the last tiles still run (16-byte chunks
+    // warp copies its share of the gate rows of this CTA into it while the last tiles still run (16-byte chunks
     // XOR-swizzled by the row).  Every producer thread reaches the closing barrier.
     const T* gate = reinterpret_cast<const T*>(a.gate);
     const bool staged = a.gate_mode != TF_GATE_NONE && sp.n == 1 && rows_v16(a);
@@ -504,8 +540,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     okg = __all_sync(0xffffffffu, okg);
     if (okg && staged) {
 #pragma unroll 1
-      for (int i = 0; i < 32; i += kRowsPerInstr) {
-        const int row = pw * 32 + i + gsub;
+      for (int i = 0; i < kRows / kPrWarps; i += kRowsPerInstr) {
+        const int row = pw * (kRows / kPrWarps) + i + gsub;
         const int ti = row / G, g = row - (row / G) * G;
         if (ti < n_tok)
           cp_async16(base + row * (D * 2) + ((gch ^ (row & (kChunks - 1))) << 4),
@@ -513,7 +549,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
     }
     cp_async_wait_all();
-    named_barrier(6, (kSmWarps + kPrWarps) * 32);  // gate rows staged for the softmax warps
+    named_barrier(10, (kSmWarps + kPrWarps) * 32);  // gate rows staged for the softmax warps
   } else if (warp == kIssueWarp && rank == 1) {
     // ======================= relay: this CTA's halves landed -> rank 0 =======================
     if (lane == 0) {
@@ -605,114 +641,137 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else if (warp < kSmWarps) {
-    // ============ softmax + epilogue: thread (half, r) = keys [64 half, +64) of row r ============
+    // ============ softmax + epilogue: thread (wg, r) = row r of the tiles j with j % 2 == wg ============
+    // The two warpgroups work on neighbouring tiles at once, one's exponentials beside the other's
+    // scaling and maxima.  A row's running maximum passes from tile to tile through shared memory
+    // (named barriers 1-8, one per warp pair and direction); each warpgroup keeps its own sum.
     const int r = tid & (kRows - 1);
-    const int half = tid >> 7;
+    const int wg = tid >> 7;
     const int ri = r / G;
     const bool row_valid = ri < n_tok;
     const int64_t klim = P + cta_start + ri + 1;  // keys [0, klim) are visible to this row
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    constexpr int kOHalf = D / 2;  // O columns rescaled and stored by this thread
-    float m_used = -INFINITY, l_sum = 0.f, c2 = 0.f;
-    bool ok = true;
-    // No early exit from this loop: the two warps of a row group meet at a barrier every tile, so
-    // a failed wait only turns the remaining iterations into barrier-only ones.
-    for (int j = 0; j < ntiles; ++j) {
-      const int bi = j & 1, si = j & (kScaleTiles - 1);
-      // rows' factors and keys' scales come straight from the producers' barriers
-      if (ok && j == 0) ok = __all_sync(0xffffffffu, wait_bar<false>(q_full, 0, abort, peer_abort));
-      if (ok) ok = __all_sync(0xffffffffu, wait_bar<false>(&sc_full[si], (j / kScaleTiles) & 1, abort, peer_abort));
-      if (ok) ok = __all_sync(0xffffffffu, wait_bar<false>(&s_full[bi], (j >> 1) & 1, abort, peer_abort));
+    constexpr int kOHalf = D / 2;  // O columns stored by this thread
+    const int bar_in = 1 + 2 * (warp & 3) + wg, bar_out = 1 + 2 * (warp & 3) + (wg ^ 1);
+    float m_used = -INFINITY, l_sum = 0.f;
+    bool ok = __all_sync(0xffffffffu, wait_bar<false>(q_full, 0, abort, peer_abort));
+    const float c2 = rowf[r];
+    // No early exit from this loop: the warps of a pair meet at a barrier every tile, so a failed
+    // wait only turns the remaining iterations into barrier-only ones.
+    for (int j = wg; j < ntiles; j += 2) {
+      const int si = j & (C::kScaleTiles - 1);
+      const uint32_t sa = tmem + lane_base + C::kColS + wg * kKeys;
+      const float* ks = ks_s + si * kKeys;
+      const float* vs = vs_s + si * kKeys;
+      // keys [0, vis) of the tile are visible to the row (0 for rows past the request end)
+      const int64_t rem = row_valid ? klim - (int64_t)(jb + j) * kKeys : 0;
+      const int vis = rem <= 0 ? 0 : (rem >= kKeys ? kKeys : (int)rem);
+      if (ok) ok = __all_sync(0xffffffffu, wait_bar<false>(&sc_full[si], (j / C::kScaleTiles) & 1, abort, peer_abort));
+      if (ok) ok = __all_sync(0xffffffffu, wait_bar<false>(&s_full[wg], (j >> 1) & 1, abort, peer_abort));
       float s[2][32];
-      float pm = -INFINITY, ev = 0.f;
+      float tmax = -INFINITY;
       if (ok) {
         tc::fence_after_sync();
-        if (j == 0) c2 = rowf[r];
-        const uint32_t sa = tmem + lane_base + C::kColS + bi * kKeys + 64 * half;
-        tc::ld32(sa, s[0]);
-        tc::ld32(sa + 32, s[1]);
-        const float4 e4 = *reinterpret_cast<const float4*>(ev_s + si * kPrWarps);
-        ev = fmaxf(fmaxf(e4.x, e4.y), fmaxf(e4.z, e4.w));
-        const float4* kp = reinterpret_cast<const float4*>(ks_s + si * kKeys + 64 * half);
-        tc::wait_ld();
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const float4 v = kp[k];
-          float* x = &s[k >> 3][4 * (k & 7)];
-          x[0] *= v.x;
-          x[1] *= v.y;
-          x[2] *= v.z;
-          x[3] *= v.w;
+#pragma unroll 1
+        for (int hf = 0; hf < 2; ++hf) {
+          tc::ld32(sa + 64 * hf, s[0]);
+          tc::ld32(sa + 64 * hf + 32, s[1]);
+          tc::wait_ld();
+          scale_mask(s, ks + 64 * hf, vis - 64 * hf);
+          tc::st32(sa + 64 * hf, s[0]);  // scaled, for the second pass
+          tc::st32(sa + 64 * hf + 32, s[1]);
+          tmax = fmaxf(tmax, max_of_64(s));
         }
-        // keys [0, vis) of this thread's 64 are visible to the row (0 for rows past the request end)
-        const int64_t rem = row_valid ? klim - (int64_t)(jb + j) * kKeys - 64 * half : 0;
-        const int vis = rem <= 0 ? 0 : (rem >= 64 ? 64 : (int)rem);
-        if (vis < 64) {
-#pragma unroll
-          for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (hh * 32 + k >= vis) s[hh][k] = -INFINITY;
-        }
-        pm = max_of_64(s);
+        tc::wait_st();
+        const float4 e0 = *reinterpret_cast<const float4*>(ev_s + si * 4);
+        const float ev = fmaxf(max3(e0.x, e0.y, e0.z), e0.w);
+        tmax = fmaf(tmax, c2, ev);  // c2 > 0
       }
-      // the row max over both halves (c2 > 0)
-      pmax[(bi * 2 + half) * kRows + r] = pm;
-      named_barrier(1 + (warp & 3), 64);
-      const float pm_other = pmax[(bi * 2 + (half ^ 1)) * kRows + r];
+      float m_prev = -INFINITY;
+      if (j > 0) {
+        named_barrier(bar_in, 64);
+        m_prev = m_s[(wg ^ 1) * kRows + r];
+      }
+      const bool need = ok && (tmax > m_prev + kRescaleLog2 || (m_prev == -INFINITY && tmax > -INFINITY));
+      const float m_new = need ? tmax : m_prev;
+      if (j + 1 < ntiles) {
+        m_s[wg * kRows + r] = m_new;
+        __syncwarp();
+        bar_arrive(bar_out, 64);
+      }
       if (!ok) continue;
-      const float tmax = fmaf(fmaxf(pm, pm_other), c2, ev);
-      const bool need = tmax > m_used + kRescaleLog2 || (m_used == -INFINITY && tmax > -INFINITY);
-      const float m_new = need ? tmax : m_used;
-      const float alpha = need ? (m_used == -INFINITY ? 0.f : exp2f(m_used - m_new)) : 1.f;
+      l_sum *= m_used == m_new ? 1.f : ex2_ftz(m_used - m_new);  // from this warpgroup's last tile
       m_used = m_new;
-      l_sum *= alpha;
-      if (j > 0 && __any_sync(0xffffffffu, need)) {  // rescale this thread's half of its O row
+      if (j > 0 && __any_sync(0xffffffffu, need)) {  // rescale the O rows (after PV_{j-1})
+        const float alpha = m_prev == m_new ? 1.f : ex2_ftz(m_prev - m_new);
         ok = __all_sync(0xffffffffu, wait_bar<false>(o_done, (j - 1) & 1, abort, peer_abort));
         if (!ok) continue;
         tc::fence_after_sync();
 #pragma unroll 1
-        for (int cc = 0; cc < kOHalf / 32; ++cc) {
-          const uint32_t ta = tmem + lane_base + C::kColO + half * kOHalf + cc * 32;
-          float o[32];
-          tc::ld32(ta, o);
+        for (int cc = 0; cc < D / 32; ++cc) {
+          const uint32_t ta = tmem + lane_base + C::kColO + cc * 32;
+          tc::ld32(ta, s[0]);
           tc::wait_ld();
 #pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] *= alpha;
-          tc::st32(ta, o);
+          for (int k = 0; k < 32; ++k) s[0][k] *= alpha;
+          tc::st32(ta, s[0]);
         }
       }
-      const float nmu = m_used == -INFINITY ? 0.f : -m_used;
-      float pk[32], ls[4] = {0.f, 0.f, 0.f, 0.f};
-      const float4* vp = reinterpret_cast<const float4*>(vs_s + si * kKeys + 64 * half);
+      const float nmu = m_new == -INFINITY ? 0.f : -m_new;
+      const uint64_t c22 = pk2(c2, c2), nmu2 = pk2(nmu, nmu);
+      uint64_t ls2[2] = {0, 0};
+#pragma unroll 1
+      for (int hf = 0; hf < 2; ++hf) {
+        tc::ld32(sa + 64 * hf, s[0]);
+        tc::ld32(sa + 64 * hf + 32, s[1]);
+        tc::wait_ld();
+        const ulonglong2* vp = reinterpret_cast<const ulonglong2*>(vs + 64 * hf);
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        const float4 v = vp[k];
-        const float* x = &s[k >> 3][4 * (k & 7)];
-        const float p0 = ex2_ftz(fmaf(x[0], c2, nmu)), p1 = ex2_ftz(fmaf(x[1], c2, nmu));
-        const float p2 = ex2_ftz(fmaf(x[2], c2, nmu)), p3 = ex2_ftz(fmaf(x[3], c2, nmu));
-        ls[k & 3] += (p0 + p1) + (p2 + p3);
-        pk[2 * k] = __uint_as_float(pack2_rn<__half>(p0 * v.x, p1 * v.y));
-        pk[2 * k + 1] = __uint_as_float(pack2_rn<__half>(p2 * v.z, p3 * v.w));
+        for (int q = 0; q < 2; ++q) {
+          float pk[16];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const ulonglong2 v = vp[8 * q + k];
+            const float* x = &s[q][4 * k];
+            float e0, e1, e2, e3;
+            up2(fma2(pk2(x[0], x[1]), c22, nmu2), e0, e1);
+            up2(fma2(pk2(x[2], x[3]), c22, nmu2), e2, e3);
+            const uint64_t p01 = pk2(ex2_ftz(e0), ex2_ftz(e1)), p23 = pk2(ex2_ftz(e2), ex2_ftz(e3));
+            ls2[0] = add2(ls2[0], p01);
+            ls2[1] = add2(ls2[1], p23);
+            up2(mul2(p01, v.x), e0, e1);
+            up2(mul2(p23, v.y), e2, e3);
+            pk[2 * k] = __uint_as_float(pack2_rn<__half>(e0, e1));
+            pk[2 * k + 1] = __uint_as_float(pack2_rn<__half>(e2, e3));
+          }
+          // P over the first 32 of these 64 S columns, which only this thread uses and has read
+          tc::st16(sa + 64 * hf + 16 * q, pk);
+        }
       }
-      l_sum += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-      // P over the first 32 of this thread's 64 S columns: only this thread read them
-      tc::st32(tmem + lane_base + C::kColS + bi * kKeys + 64 * half, pk);
+      float q0s, q1s;
+      up2(add2(ls2[0], ls2[1]), q0s, q1s);
+      l_sum += q0s + q1s;
       tc::wait_st();
       tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[bi]);  // rank 1's forward warp passes it on to rank 0
+      if (lane == 0) mbar_arrive(&p_full[wg]);  // rank 1's forward warp passes it on to rank 0
     }
     const bool gated = a.gate_mode != TF_GATE_NONE;
     const bool vec = rows_v16(a);
     if (ok) ok = __all_sync(0xffffffffu, wait_bar<false>(fin, 0, abort, peer_abort));
     // ---- epilogue.  Once fin completed, no product reads Q or the ring any more: the two halves' row
     // sums meet in the ring
-    float* l_part = reinterpret_cast<float*>(sbase + C::kOffRing);
-    if (ok) l_part[half * kRows + r] = l_sum;
-    named_barrier(5, kSmWarps * 32);
-    const float l_tot = ok ? l_part[r] + l_part[kRows + r] : 0.f;
-    named_barrier(6, (kSmWarps + kPrWarps) * 32);  // gate rows are staged
+    float2* l_part = reinterpret_cast<float2*>(sbase + C::kOffRing);  // [2][kRows] (m, l)
+    if (ok) l_part[wg * kRows + r] = make_float2(m_used, l_sum);
+    named_barrier(9, kSmWarps * 32);
+    float l_tot = 0.f;
+    if (ok) {
+      const float2 o = l_part[(wg ^ 1) * kRows + r];
+      const float mf = fmaxf(m_used, o.x);  // O's scale: the maxima only grow
+      l_tot = (m_used == mf ? l_sum : l_sum * exp2f(m_used - mf)) + (o.x == mf ? o.y : o.y * exp2f(o.x - mf));
+      m_used = mf;
+    }
+    named_barrier(10, (kSmWarps + kPrWarps) * 32);  // gate rows are staged
     if (ok) {
       tc::fence_after_sync();
       const int hq = h * G + (r - ri * G);
@@ -721,16 +780,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       float* po = nullptr;
       if (sp.n > 1 && row_valid) {
         const int64_t row = ((int64_t)z * a.num_tokens + t) * a.num_q_heads + hq;
-        po = sp.o + row * D + half * kOHalf;
-        if (half == 0) *reinterpret_cast<float2*>(sp.ml + 2 * row) = make_float2(m_used, l_tot);
+        po = sp.o + row * D + wg * kOHalf;
+        if (wg == 0) *reinterpret_cast<float2*>(sp.ml + 2 * row) = make_float2(m_used, l_tot);
       }
-      T* orow = (T*)a.out + t * a.out_stride_tok + (int64_t)hq * a.out_stride_head + half * kOHalf;
-      const T* grow = (const T*)a.gate + t * a.gate_stride_tok + (int64_t)hq * a.gate_stride_head + half * kOHalf;
+      T* orow = (T*)a.out + t * a.out_stride_tok + (int64_t)hq * a.out_stride_head + wg * kOHalf;
+      const T* grow = (const T*)a.gate + t * a.gate_stride_tok + (int64_t)hq * a.gate_stride_head + wg * kOHalf;
       constexpr int kChunks = D / 8;
 #pragma unroll 1
       for (int cc = 0; cc < kOHalf / 32; ++cc) {
         float o[32];
-        tc::ld32(tmem + lane_base + C::kColO + half * kOHalf + cc * 32, o);
+        tc::ld32(tmem + lane_base + C::kColO + wg * kOHalf + cc * 32, o);
         tc::wait_ld();
         if (!row_valid) continue;
         if (sp.n > 1) {
@@ -742,7 +801,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           for (int c8 = 0; c8 < 4; ++c8) {
             uint32_t gw[4] = {0, 0, 0, 0}, ow[4];
             if (gated) {
-              const int chunk = (half * kOHalf + cc * 32) / 8 + c8;
+              const int chunk = (wg * kOHalf + cc * 32) / 8 + c8;
               asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
                            : "=r"(gw[0]), "=r"(gw[1]), "=r"(gw[2]), "=r"(gw[3])
                            : "r"(base + r * (D * 2) + ((chunk ^ (r & (kChunks - 1))) << 4)));
@@ -903,6 +962,8 @@ bool paged_fp8_extend_supported(const tf_paged_attn_args& a) {
   if (a.max_extend_len <= 0 || a.num_kv_heads > 65535) return false;
   if (!(a.scale > 0.f)) return false;  // the softmax takes its max before the scale
   auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  // row offsets are kept in 32 bits of 16-byte pieces: pools of up to 64 GiB a layer
+  if (a.num_slots * a.kv_stride_slot >= (int64_t)1 << 36) return false;
   return al(a.k_buffer) && al(a.v_buffer) && a.kv_stride_slot % 16 == 0 && a.kv_stride_head % 16 == 0;
 }
 

@@ -8,12 +8,18 @@
 // issues the products.  What the 8-bit pool changes:
 //   producers   load 16 codes a lane, convert them to f16 (exact) and store them into the swizzled
 //               tile.  Four warps make the K slots and four the V slots, each with the next slot of its
-//               kind on its way into registers while one is converted: a tile's slots are free too
-//               late for a load and a conversion in turn
-//   scales      are not multiplied into the tiles (a second rounding of every element): a key's logit
-//               is its product times ks_j in fp32, and its weight p_j = 2^(s_j - M) enters P as
-//               f16(p_j vs_j).  M follows s_j + ev_j, ev_j the exponent of the largest vs of the tile,
-//               so that P stays in f16's range whatever the scales are; l = sum p_j is fp32.
+//               kind on its way into registers while it waits for the slot to be free
+//   scales      enter as powers of two of groups of 32 keys (2^kx_g, 2^ev_g, the exponents of the
+//               group's largest ks and vs) in the softmax, where they cost nothing: a logit is
+//               S c2 2^kx_g, its weight for P 2^(logit + ev_g - M), and l sums the weights times 2^-ev_g.
+//               M follows logit + ev_g, so that P stays in f16's range whatever the scales are.
+//               The rest of each scale, in [0, 2):
+//               bfloat16: the producers multiply it into the codes (to f16: 11 bits, random, eight
+//               times finer than the output's rounding; two f16 operations a pair, with the scale's
+//               own low bits in the first, so that it is not rounded for a whole row at once);
+//               float16: the codes stay exact and the softmax multiplies logit and weight by it in
+//               fp32, which leaves the weight's f16 rounding alone before the output's.  It costs
+//               two reads and two products more per score: 2.5 us a key tile against MEASURED_FOLD.
 //   Q           is scaled by a power of two per row into f16's range (bfloat16 stays exact)
 // A scale that is not finite gives its key NaN logits and a V row of zeros, so that only the rows that
 // see it are NaN.  Every wait is bounded; one that gives up raises an abort flag in both CTAs and
@@ -47,19 +53,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-__device__ __forceinline__ float max_of_64(const float (&s)[2][32]) {
-  float t[22];
+__device__ __forceinline__ float max_of_32(const float (&s)[32]) {
+  float t[11];
 #pragma unroll
-  for (int i = 0; i < 21; ++i) {
-    const int k = 3 * i;
-    t[i] = max3(s[k >> 5][k & 31], s[(k + 1) >> 5][(k + 1) & 31], s[(k + 2) >> 5][(k + 2) & 31]);
-  }
-  t[21] = s[1][31];
-  float u[8];
-#pragma unroll
-  for (int i = 0; i < 7; ++i) u[i] = max3(t[3 * i], t[3 * i + 1], t[3 * i + 2]);
-  u[7] = t[21];
-  return fmaxf(max3(u[0], u[1], u[2]), max3(u[3], u[4], max3(u[5], u[6], u[7])));
+  for (int i = 0; i < 10; ++i) t[i] = max3(s[3 * i], s[3 * i + 1], s[3 * i + 2]);
+  t[10] = fmaxf(s[30], s[31]);
+  const float u0 = max3(t[0], t[1], t[2]), u1 = max3(t[3], t[4], t[5]), u2 = max3(t[6], t[7], t[8]);
+  return max3(max3(u0, u1, u2), t[9], t[10]);
 }
 __device__ __forceinline__ float ex2_ftz(float x) {
   float y;
@@ -92,26 +92,38 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
-// 64 raw products times their keys' scales; the ones from `vis` on are hidden
-__device__ __forceinline__ void scale_mask(float (&s)[2][32], const float* ks, int vis) {
-  const ulonglong2* kp = reinterpret_cast<const ulonglong2*>(ks);
+// the products of a group of 32 keys: times the keys' scales when those are not in the codes (ks), and
+// hidden from key `vis` on
+template <bool FOLD>
+__device__ __forceinline__ void scale_mask(float (&s)[32], const float* ks, int vis) {
+  if (!FOLD) {
+    const ulonglong2* kp = reinterpret_cast<const ulonglong2*>(ks);
 #pragma unroll
-  for (int k = 0; k < 16; ++k) {
-    const ulonglong2 v = kp[k];
-    float* x = &s[k >> 3][4 * (k & 7)];
-    up2(mul2(pk2(x[0], x[1]), v.x), x[0], x[1]);
-    up2(mul2(pk2(x[2], x[3]), v.y), x[2], x[3]);
+    for (int k = 0; k < 8; ++k) {
+      const ulonglong2 v = kp[k];
+      up2(mul2(pk2(s[4 * k], s[4 * k + 1]), v.x), s[4 * k], s[4 * k + 1]);
+      up2(mul2(pk2(s[4 * k + 2], s[4 * k + 3]), v.y), s[4 * k + 2], s[4 * k + 3]);
+    }
   }
-  if (vis < 64) {
+  if (vis < 32) {
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-      for (int k = 0; k < 32; ++k)
-        if (hh * 32 + k >= vis) s[hh][k] = -INFINITY;
+    for (int k = 0; k < 32; ++k)
+      if (k >= vis) s[k] = -INFINITY;
   }
 }
 __device__ __forceinline__ void bar_arrive(int id, int nthreads) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
+}
+
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
 }
 
 // ---- cluster pair helpers
@@ -238,15 +250,16 @@ struct Cfg {
   static_assert(kScaleTiles >= kSlots / 2 + 1, "scales in use are not overwritten");
   static constexpr int kOffRing = kQBytes;
   static constexpr int kOffBars = kOffRing + kSlots * kSlotBytes;
-  // full, empty [kSlots]; s_full[2], p_full[2], o_done, q_full, fin, q_dead, sc_full[kScaleTiles]
-  static constexpr int kNumBars = 2 * kSlots + 8 + kScaleTiles;
+  // full, empty [kSlots]; s_full[2], p_full[2][2], o_done, q_full, fin, q_dead, sc_full[kScaleTiles]
+  static constexpr int kNumBars = 2 * kSlots + 10 + kScaleTiles;
   static constexpr int kOffWords = kOffBars + 8 * kNumBars;      // tmem holder, abort, q0
   static constexpr int kOffM = (kOffWords + 16 + 15) & ~15;      // float [2][kRows]: running maxima
   static constexpr int kOffRow = kOffM + 2 * kRows * 4;          // float [kRows]: logit factor of a row
   static constexpr int kOffKs = kOffRow + kRows * 4;             // float [kScaleTiles][kKeys]
   static constexpr int kOffVs = kOffKs + kScaleTiles * kKeys * 4;
-  static constexpr int kOffEv = kOffVs + kScaleTiles * kKeys * 4;   // float [kScaleTiles][4]
-  static constexpr int kSmem = kOffEv + kScaleTiles * 4 * 4 + 1024;
+  static constexpr int kOffGrp = kOffVs + kScaleTiles * kKeys * 4;  // float4 [kScaleTiles][4]: a group's
+                                                                  // 2^kx, ev, 2^-ev
+  static constexpr int kSmem = kOffGrp + kScaleTiles * 4 * 16 + 1024;
   static constexpr int kColS = 0;                 // two S buffers of kKeys columns; P_j over S_j
   static constexpr int kColO = 2 * kKeys;
   static constexpr int kTmemCols = 512;
@@ -285,7 +298,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   uint64_t* empty = full + C::kSlots;
   uint64_t* s_full = empty + C::kSlots;
   uint64_t* p_full = s_full + 2;
-  uint64_t* o_done = p_full + 2;
+  uint64_t* o_done = p_full + 4;  // p_full[2 buffer + half]: 64 keys of P_j are in TMEM
   uint64_t* q_full = o_done + 1;
   uint64_t* fin = q_full + 1;
   uint64_t* q_dead = fin + 1;    // the last S product has completed: Q's shared memory is free
@@ -297,7 +310,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   float* rowf = reinterpret_cast<float*>(sbase + C::kOffRow);
   float* ks_s = reinterpret_cast<float*>(sbase + C::kOffKs);
   float* vs_s = reinterpret_cast<float*>(sbase + C::kOffVs);
-  float* ev_s = reinterpret_cast<float*>(sbase + C::kOffEv);
+  float4* grp_s = reinterpret_cast<float4*>(sbase + C::kOffGrp);
+  constexpr bool kFold = !std::is_same<T, __half>::value;  // scales multiplied into the codes
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_rank();
@@ -355,7 +369,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], rank == 0 ? kSmWarps / 2 + 1 : kSmWarps / 2);
+      for (int k = 0; k < 2; ++k) mbar_init(&p_full[2 * i + k], rank == 0 ? kSmWarps / 2 + 1 : kSmWarps / 2);
     }
     mbar_init(o_done, 1);
     mbar_init(q_full, in_count);
@@ -366,7 +380,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   // producers: the slot-id chain of the first key tiles is requested before the set-up barrier.  Lane
-  // l of K warp w takes key 64 rank + 16 w + l % 16 of a tile, lane l of V warp w key 32 w + l
+  // l takes key l of a group of 32: the one that holds K warp w's 16 rows (64 rank + 16 w), group w for
+  // V warp w
   constexpr int kPrefetch = 4;
   int64_t raw_q[kPrefetch] = {0, 0, 0, 0};
   const int64_t* r2t = a.req_to_token;
@@ -384,7 +399,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       row = 0;
     }
     r2t = a.req_to_token + row * a.r2t_stride;
-    my_key = pw < 4 ? 64 * (int)rank + 16 * pw + (lane & 15) : 32 * (pw - 4) + lane;
+    my_key = pw < 4 ? 64 * (int)rank + 32 * (pw >> 1) + lane : 32 * (pw - 4) + lane;
 #pragma unroll
     for (int i = 0; i < kPrefetch; ++i)
       if (i < ntiles) raw_q[i] = raw_of(i);
@@ -459,6 +474,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const char* src = kV ? (const char*)a.v_buffer + (int64_t)h * a.kv_stride_head + rank * (D / 2) + ch * 16
                            : (const char*)a.k_buffer + (int64_t)h * a.kv_stride_head + ch * 16;
       const int row0 = (kV ? 32 * (pw - 4) : 16 * pw) + sub;
+      const int lane0 = kV ? 0 : 16 * (pw & 1);        // the lane that knows the warp's first row
       // 16 codes are two 16-byte chunks of f16; lanes of odd 64-dim blocks store theirs in the other
       // order (a bank conflict otherwise)
       const int blk = ch >> 2;
@@ -473,27 +489,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const uint32_t off = (uint32_t)((sl * a.kv_stride_slot) >> 4);  // 16-byte pieces (the host checks)
         uint32_t o[kLoads];
 #pragma unroll
-        for (int k = 0; k < kLoads; ++k) o[k] = __shfl_sync(0xffffffffu, off, k * RPI + sub);
+        for (int k = 0; k < kLoads; ++k) o[k] = __shfl_sync(0xffffffffu, off, lane0 + k * RPI + sub);
 #pragma unroll
         for (int k = 0; k < kLoads; ++k) w[k] = ldg_nc(src + (uint64_t)o[k] * 16);
-        if (kV) s2 = __ldg(reinterpret_cast<const float2*>(scp + sl * sc.stride_slot));
+        s2 = __ldg(reinterpret_cast<const float2*>(scp + sl * sc.stride_slot));
       };
       int slot = kV ? 2 : 0;   // ring place: K0 K1 V0 K2 V1 K3 ... V_{n-2} V_{n-1}
       uint32_t phase = 0;
       auto put = [&](int tile, uint4 (&w)[kLoads], float2 s2) {
-        unsigned keep = 0xffffffffu;  // rows that are not zeroed
+        // A scale that is not finite: NaN logits (K), and a V row of zeros
+        const bool fin = kv8::abs_bits(s2.x) < 0x7f800000u && kv8::abs_bits(s2.y) < 0x7f800000u;
+        auto group_exp = [&](float x) {  // exponent of the group's largest |scale|
+          const uint32_t m = __reduce_max_sync(0xffffffffu, fin ? kv8::abs_bits(x) : 0u);
+          return min(max((int)(m >> 23) - 127, -100), 100);
+        };
+        const int kx = kFold || kV ? group_exp(s2.x) : 0, ev = kV ? group_exp(s2.y) : 0;
         if (kV) {
-          // scales of the tile.  One that is not finite: NaN logits, and a V row of zeros
-          const bool fin = kv8::abs_bits(s2.x) < 0x7f800000u && kv8::abs_bits(s2.y) < 0x7f800000u;
           const int st = tile & (C::kScaleTiles - 1);
-          ks_s[st * kKeys + my_key] = fin ? s2.x : NAN;
-          vs_s[st * kKeys + my_key] = fin ? s2.y : 0.f;
-          const float vm = warp_max(fin ? fabsf(s2.y) : 0.f);
-          if (lane == 0)
-            ev_s[st * 4 + pw - 4] = (float)min(max((int)(__float_as_uint(vm) >> 23) - 127, -100), 126);
-          keep = __ballot_sync(0xffffffffu, fin);
+          if (!kFold) {
+            ks_s[st * kKeys + my_key] = fin ? s2.x * pow2i(-kx) : NAN;
+            vs_s[st * kKeys + my_key] = fin ? s2.y : 0.f;
+          }
+          if (lane == 0) grp_s[st * 4 + pw - 4] = make_float4(pow2i(kx), (float)ev, pow2i(-ev), 0.f);
+          __syncwarp();
           if (lane == 0) mbar_arrive(&sc_full[st]);
         }
+        // what the codes of this lane's key are multiplied by, as two f16 terms; exact: 1, or 0
+        float mul = kV ? s2.y * pow2i(-ev) : s2.x * pow2i(-kx);
+        if (!kFold) mul = 1.f;
+        if (!fin) mul = kV ? 0.f : NAN;
+        const __half mh = __float2half_rn(mul);
+        const uint32_t mterms = (uint32_t)__half_as_ushort(mh) |
+                                ((uint32_t)__half_as_ushort(__float2half_rn(mul - __half2float(mh))) << 16);
         // the slot's place and round: position i = 2 tile - 1 (K), 2 tile + 2 (V), shifted at the ends
         const int i = kV ? (tile == ntiles - 1 ? 2 * ntiles - 1 : 2 * tile + 2) : (tile == 0 ? 0 : 2 * tile - 1);
         slot = i % C::kSlots;
@@ -505,26 +532,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         for (int k = 0; k < kLoads; ++k) {
           const int row = row0 + k * RPI;
           uint4 v = w[k];
-          if (kV && !((keep >> (k * RPI + sub)) & 1u)) v = make_uint4(0, 0, 0, 0);
           if (odd) v = make_uint4(v.z, v.w, v.x, v.y);
           const uint32_t dst = sb + row * 128;
-          sts128(dst + ((ca ^ (row & 7)) << 4), cvt_lo(v.x), cvt_hi(v.x), cvt_lo(v.y), cvt_hi(v.y));
-          sts128(dst + ((cb ^ (row & 7)) << 4), cvt_lo(v.z), cvt_hi(v.z), cvt_lo(v.w), cvt_hi(v.w));
+          uint32_t f[8] = {cvt_lo(v.x), cvt_hi(v.x), cvt_lo(v.y), cvt_hi(v.y),
+                           cvt_lo(v.z), cvt_hi(v.z), cvt_lo(v.w), cvt_hi(v.w)};
+          if (kFold || kV) {
+            const uint32_t t = __shfl_sync(0xffffffffu, mterms, lane0 + k * RPI + sub);
+            const uint32_t hi = __byte_perm(t, 0, 0x1010), lo = __byte_perm(t, 0, 0x3232);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) f[q] = kFold ? hfma2(f[q], hi, hmul2(f[q], lo)) : (hi == 0 ? 0u : f[q]);
+          }
+          sts128(dst + ((ca ^ (row & 7)) << 4), f[0], f[1], f[2], f[3]);
+          sts128(dst + ((cb ^ (row & 7)) << 4), f[4], f[5], f[6], f[7]);
         }
         tc::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&full[slot]);
       };
-      uint4 wa[kLoads], wb[kLoads];
-      float2 sa = make_float2(0.f, 0.f), sb2 = sa;
-      load(0, wa, sa);
+      // the next tile's rows are requested as soon as this one's registers are free; its slot is not
+      uint4 w[kLoads];
+      float2 s2;
+      load(0, w, s2);
 #pragma unroll 1
-      for (int j = 0; ok && j < ntiles; j += 2) {
-        if (j + 1 < ntiles) load(j + 1, wb, sb2);
-        put(j, wa, sa);
-        if (!ok || j + 1 >= ntiles) break;
-        if (j + 2 < ntiles) load(j + 2, wa, sa);
-        put(j + 1, wb, sb2);
+      for (int j = 0; ok && j < ntiles; ++j) {
+        put(j, w, s2);
+        if (j + 1 < ntiles) load(j + 1, w, s2);
       }
     };
     if (pw < 4) produce(std::false_type());
@@ -574,12 +606,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == kFwdWarp) {
     // =========== rank 1: "this CTA's P_j is in TMEM" -> rank 0's p_full, one arrive per tile ===========
     if (rank == 1 && lane == 0) {
-      const uint32_t pf0 = peer_addr(smem_u32(&p_full[0]), 0), pf1 = peer_addr(smem_u32(&p_full[1]), 0);
-      for (int j = 0; j < ntiles; ++j) {
-        if (!wait_bar<false>(&p_full[j & 1], (j >> 1) & 1, abort, peer_abort)) break;
+      const uint32_t pf = peer_addr(smem_u32(p_full), 0);
+      for (int j = 0; j < 2 * ntiles; ++j) {  // halves of tiles
+        const int k = j & 3;                  // 2 buffer + half
+        if (!wait_bar<false>(&p_full[k], (j >> 2) & 1, abort, peer_abort)) break;
         tc::fence_after_sync();
         tc::fence_before_sync();
-        remote_arrive((j & 1) ? pf1 : pf0);
+        remote_arrive(pf + 8 * k);
       }
     }
     __syncwarp();
@@ -615,12 +648,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         release();
       };
       auto issue_pv = [&](int t) {
-        ok = ok && wait_bar<true>(&p_full[t & 1], (t >> 1) & 1, abort, peer_abort);
-        tc::fence_after_sync();
         const uint32_t vb = take();
-        if (!ok) return;
+        // the first 64 keys' product starts while the others' weights are being made
 #pragma unroll
         for (int kk = 0; kk < kKeys / 16; ++kk) {
+          if ((kk & 3) == 0) {
+            ok = ok && wait_bar<true>(&p_full[2 * (t & 1) + (kk >> 2)], (t >> 1) & 1, abort, peer_abort);
+            if (!ok) return;
+            tc::fence_after_sync();
+          }
           // P_j: keys [64 hf, 64 hf + 64) packed in columns [64 hf, 64 hf + 32) of S buffer j & 1
           const uint64_t bd = tc::sw128_desc(vb + kk * 2048, C::kVBlk, 1024);
           mma2_ts(tmem + C::kColO, tmem + C::kColS + (t & 1) * kKeys + 64 * (kk >> 2) + (kk & 3) * 8, bd,
@@ -668,24 +704,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int vis = rem <= 0 ? 0 : (rem >= kKeys ? kKeys : (int)rem);
       if (ok) ok = __all_sync(0xffffffffu, wait_bar<false>(&sc_full[si], (j / C::kScaleTiles) & 1, abort, peer_abort));
       if (ok) ok = __all_sync(0xffffffffu, wait_bar<false>(&s_full[wg], (j >> 1) & 1, abort, peer_abort));
-      float s[2][32];
       float tmax = -INFINITY;
+      const float4* grp = grp_s + si * 4;
       if (ok) {
         tc::fence_after_sync();
 #pragma unroll 1
         for (int hf = 0; hf < 2; ++hf) {
+          float s[2][32];
           tc::ld32(sa + 64 * hf, s[0]);
           tc::ld32(sa + 64 * hf + 32, s[1]);
           tc::wait_ld();
-          scale_mask(s, ks + 64 * hf, vis - 64 * hf);
-          tc::st32(sa + 64 * hf, s[0]);  // scaled, for the second pass
-          tc::st32(sa + 64 * hf + 32, s[1]);
-          tmax = fmaxf(tmax, max_of_64(s));
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int g = 2 * hf + k;
+            scale_mask<kFold>(s[k], ks + 32 * g, vis - 32 * g);
+            const float2 e = *reinterpret_cast<const float2*>(grp + g);
+            tmax = fmaxf(tmax, fmaf(max_of_32(s[k]), c2 * e.x, e.y));  // c2 > 0
+          }
         }
-        tc::wait_st();
-        const float4 e0 = *reinterpret_cast<const float4*>(ev_s + si * 4);
-        const float ev = fmaxf(max3(e0.x, e0.y, e0.z), e0.w);
-        tmax = fmaf(tmax, c2, ev);  // c2 > 0
       }
       float m_prev = -INFINITY;
       if (j > 0) {
@@ -710,51 +746,61 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int cc = 0; cc < D / 32; ++cc) {
           const uint32_t ta = tmem + lane_base + C::kColO + cc * 32;
-          tc::ld32(ta, s[0]);
+          float s[32];
+          tc::ld32(ta, s);
           tc::wait_ld();
 #pragma unroll
-          for (int k = 0; k < 32; ++k) s[0][k] *= alpha;
-          tc::st32(ta, s[0]);
+          for (int k = 0; k < 32; ++k) s[k] *= alpha;
+          tc::st32(ta, s);
         }
       }
       const float nmu = m_new == -INFINITY ? 0.f : -m_new;
-      const uint64_t c22 = pk2(c2, c2), nmu2 = pk2(nmu, nmu);
-      uint64_t ls2[2] = {0, 0};
 #pragma unroll 1
-      for (int hf = 0; hf < 2; ++hf) {
-        tc::ld32(sa + 64 * hf, s[0]);
-        tc::ld32(sa + 64 * hf + 32, s[1]);
+      for (int g = 0; g < 4; ++g) {
+        float s[32];
+        tc::ld32(sa + 32 * g, s);
         tc::wait_ld();
-        const ulonglong2* vp = reinterpret_cast<const ulonglong2*>(vs + 64 * hf);
+        scale_mask<kFold>(s, ks + 32 * g, vis - 32 * g);
+        const float4 e = grp[g];
+        const float cg = c2 * e.x, ng = kFold ? nmu + e.y : nmu;
+        const uint64_t c22 = pk2(cg, cg), nmu2 = pk2(ng, ng);
+        uint64_t ls2[2] = {0, 0};
+        float pk[16];
+        const ulonglong2* vp = reinterpret_cast<const ulonglong2*>(vs + 32 * g);
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          float pk[16];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const ulonglong2 v = vp[8 * q + k];
-            const float* x = &s[q][4 * k];
-            float e0, e1, e2, e3;
-            up2(fma2(pk2(x[0], x[1]), c22, nmu2), e0, e1);
-            up2(fma2(pk2(x[2], x[3]), c22, nmu2), e2, e3);
-            const uint64_t p01 = pk2(ex2_ftz(e0), ex2_ftz(e1)), p23 = pk2(ex2_ftz(e2), ex2_ftz(e3));
-            ls2[0] = add2(ls2[0], p01);
-            ls2[1] = add2(ls2[1], p23);
+        for (int k = 0; k < 8; ++k) {
+          const float* x = &s[4 * k];
+          float e0, e1, e2, e3;
+          up2(fma2(pk2(x[0], x[1]), c22, nmu2), e0, e1);
+          up2(fma2(pk2(x[2], x[3]), c22, nmu2), e2, e3);
+          e0 = ex2_ftz(e0);
+          e1 = ex2_ftz(e1);
+          e2 = ex2_ftz(e2);
+          e3 = ex2_ftz(e3);
+          const uint64_t p01 = pk2(e0, e1), p23 = pk2(e2, e3);
+          ls2[0] = add2(ls2[0], p01);
+          ls2[1] = add2(ls2[1], p23);
+          if (!kFold) {
+            const ulonglong2 v = vp[k];
             up2(mul2(p01, v.x), e0, e1);
             up2(mul2(p23, v.y), e2, e3);
-            pk[2 * k] = __uint_as_float(pack2_rn<__half>(e0, e1));
-            pk[2 * k + 1] = __uint_as_float(pack2_rn<__half>(e2, e3));
           }
-          // P over the first 32 of these 64 S columns, which only this thread uses and has read
-          tc::st16(sa + 64 * hf + 16 * q, pk);
+          pk[2 * k] = __uint_as_float(pack2_rn<__half>(e0, e1));
+          pk[2 * k + 1] = __uint_as_float(pack2_rn<__half>(e2, e3));
+        }
+        float h0, h1;
+        up2(add2(ls2[0], ls2[1]), h0, h1);
+        l_sum = kFold ? fmaf(h0 + h1, e.z, l_sum) : l_sum + (h0 + h1);
+        // P over the first 32 columns of each 64 S columns: only this thread uses them, and it has read
+        // the ones written here
+        tc::st16(sa + 64 * (g >> 1) + 16 * (g & 1), pk);
+        if (g & 1) {
+          tc::wait_st();
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[2 * wg + (g >> 1)]);  // rank 1's are forwarded to rank 0
         }
       }
-      float q0s, q1s;
-      up2(add2(ls2[0], ls2[1]), q0s, q1s);
-      l_sum += q0s + q1s;
-      tc::wait_st();
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[wg]);  // rank 1's forward warp passes it on to rank 0
     }
     const bool gated = a.gate_mode != TF_GATE_NONE;
     const bool vec = rows_v16(a);

@@ -6,8 +6,8 @@
 // of an integer and an fp32 frequency in fp64, reduced by whole turns there: in fp32 its rounding
 // alone would reach 2^-9 of a radian at position 32768.
 //
-// A CTA takes kTPC tokens: their cos/sin and slots first, then its warps walk the tokens' rows,
-// kPF rows in flight per warp.  Lane l of the vector form holds the E = D/32 elements [E l, E l + E)
+// A CTA takes TPC tokens (4; 1 when there are too few tokens to fill the SMs otherwise): their cos/sin
+// and slots first, then its warps walk the tokens' rows, kPF rows in flight per warp.  Lane l of the vector form holds the E = D/32 elements [E l, E l + E)
 // of a row; the rotation partner d +- rotary_dim/2 sits in lane l ^ (rotary_dim/2/E) when that is a
 // power of two, and otherwise comes from a copy of the row in shared memory.
 #include "common.cuh"
@@ -20,28 +20,48 @@ namespace prologue8 {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxD = 256;
-constexpr int kTPC = 4;
 constexpr int kPF = 4;
+constexpr int kFewTokens = 592;  // four CTAs an SM
 
-template <typename T, int E, bool VEC>
-__device__ __forceinline__ void load_row(const T* p, float (&x)[E]) {
-  if constexpr (VEC && sizeof(T) == 2 && E == 8) {
-    const uint4 w = __ldcs(reinterpret_cast<const uint4*>(p));
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+// A lane's E elements of a row as loaded (unpacked only when they are used: an unpack next to the load
+// would wait for it), in E * sizeof(T) / 4 words.
+template <typename T, int E>
+struct RawRow {
+  static constexpr int kW = E * (int)sizeof(T) / 4;
+  uint32_t w[kW];
+  template <bool VEC>
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (VEC && kW % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { x[2 * i] = unpack_lo<T>(u[i]); x[2 * i + 1] = unpack_hi<T>(u[i]); }
-  } else if constexpr (VEC && sizeof(T) == 2 && E == 4) {
-    const uint2 w = __ldcs(reinterpret_cast<const uint2*>(p));
-    x[0] = unpack_lo<T>(w.x); x[1] = unpack_hi<T>(w.x);
-    x[2] = unpack_lo<T>(w.y); x[3] = unpack_hi<T>(w.y);
-  } else if constexpr (VEC && sizeof(T) == 2 && E == 2) {
-    const uint32_t w = __ldcs(reinterpret_cast<const unsigned int*>(p));
-    x[0] = unpack_lo<T>(w); x[1] = unpack_hi<T>(w);
-  } else {
+      for (int i = 0; i < kW / 4; ++i) {
+        const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+        w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+      }
+    } else if constexpr (VEC && kW == 2) {
+      const uint2 v = __ldcs(reinterpret_cast<const uint2*>(p));
+      w[0] = v.x; w[1] = v.y;
+    } else if constexpr (VEC && kW == 1) {
+      w[0] = __ldcs(reinterpret_cast<const unsigned int*>(p));
+    } else if constexpr (sizeof(T) == 2) {
+      const unsigned short* u = reinterpret_cast<const unsigned short*>(p);
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = to_f(p[e]);
+      for (int i = 0; i < kW; ++i) w[i] = u[2 * i] | ((uint32_t)u[2 * i + 1] << 16);
+    } else {
+      const uint32_t* u = reinterpret_cast<const uint32_t*>(p);
+#pragma unroll
+      for (int i = 0; i < kW; ++i) w[i] = u[i];
+    }
   }
-}
+  __device__ __forceinline__ void get(float (&x)[E]) const {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < kW; ++i) { x[2 * i] = unpack_lo<T>(w[i]); x[2 * i + 1] = unpack_hi<T>(w[i]); }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kW; ++i) x[i] = __uint_as_float(w[i]);
+    }
+  }
+};
 
 template <typename T, int E, bool VEC>
 __device__ __forceinline__ void store_row(T* p, const float (&x)[E]) {
@@ -85,22 +105,22 @@ __device__ __forceinline__ float store_codes(uint8_t* p, const float (&x)[E]) {
 }
 
 // VEC: rows aligned to the lane's E elements.  XOR: the partner lane is lane ^ pmask.
-template <typename T, int D, bool VEC, bool XOR>
+template <typename T, int D, int TPC, bool VEC, bool XOR>
 __global__ void __launch_bounds__(kThreads) prologue_kernel(tf_attn_prologue_args a,
                                                             tf_kv_scale sc) {
   constexpr int E = D / 32;
-  constexpr int kRowStep = kWarps / kTPC;
-  __shared__ float cs[kTPC][kMaxD / 2], sn[kTPC][kMaxD / 2];
-  __shared__ int64_t s_loc[kTPC];
+  constexpr int kRowStep = kWarps / TPC;
+  __shared__ float cs[TPC][kMaxD / 2], sn[TPC][kMaxD / 2];
+  __shared__ int64_t s_loc[TPC];
   __shared__ float s_row[XOR ? 1 : kWarps][XOR ? 1 : D];
-  const int64_t t0 = (int64_t)blockIdx.x * kTPC;
-  const int ntok = a.num_tokens - t0 < kTPC ? (int)(a.num_tokens - t0) : kTPC;
+  const int64_t t0 = (int64_t)blockIdx.x * TPC;
+  const int ntok = a.num_tokens - t0 < TPC ? (int)(a.num_tokens - t0) : TPC;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int Hq = a.num_q_heads, Hkv = a.num_kv_heads;
   const int half = a.rotary_dim / 2;
   const int d0 = lane * E;
-  // warp w serves token w % kTPC: its q rows, and its (k, v) row pairs as rows [Hq, Hq + Hkv)
-  const int tt = warp % kTPC, r0 = warp / kTPC;
+  // warp w serves token w % TPC: its q rows, and its (k, v) row pairs as rows [Hq, Hq + Hkv)
+  const int tt = warp % TPC, r0 = warp / TPC;
   const bool live = tt < ntok;
   const int64_t t = t0 + (live ? tt : 0);
   const int nrows = Hq + Hkv;
@@ -108,10 +128,10 @@ __global__ void __launch_bounds__(kThreads) prologue_kernel(tf_attn_prologue_arg
     return r < Hq ? (const T*)a.q + t * a.q_stride_tok + (int64_t)r * a.q_stride_head + d0
                   : (const T*)a.k + t * a.k_stride_tok + (int64_t)(r - Hq) * a.k_stride_head + d0;
   };
-  float ring[kPF][E];
+  RawRow<T, E> ring[kPF];
 #pragma unroll
   for (int u = 0; u < kPF; ++u)
-    if (live && r0 + u * kRowStep < nrows) load_row<T, E, VEC>(src_of(r0 + u * kRowStep), ring[u]);
+    if (live && r0 + u * kRowStep < nrows) ring[u].template load<VEC>(src_of(r0 + u * kRowStep));
 
   for (int j = tid; j < ntok * half; j += kThreads) {
     const int jt = j / half, jj = j - jt * half;
@@ -153,14 +173,13 @@ __global__ void __launch_bounds__(kThreads) prologue_kernel(tf_attn_prologue_arg
       const int r = r0 + (m0 + u) * kRowStep;
       if (r >= nrows) break;
       float y[E];
-#pragma unroll
-      for (int e = 0; e < E; ++e) y[e] = ring[u][e];
-      if (r + kPF * kRowStep < nrows) load_row<T, E, VEC>(src_of(r + kPF * kRowStep), ring[u]);
+      ring[u].get(y);
+      if (r + kPF * kRowStep < nrows) ring[u].template load<VEC>(src_of(r + kPF * kRowStep));
       const bool isq = r < Hq;
       if (!isq && loc < 0) continue;
-      float v[E];
+      RawRow<T, E> vraw;
       if (!isq)
-        load_row<T, E, VEC>((const T*)a.v + t * a.v_stride_tok + (int64_t)(r - Hq) * a.v_stride_head + d0, v);
+        vraw.template load<VEC>((const T*)a.v + t * a.v_stride_tok + (int64_t)(r - Hq) * a.v_stride_head + d0);
       float ss = 0.f;
 #pragma unroll
       for (int e = 0; e < E; ++e) ss = fmaf(y[e], y[e], ss);
@@ -199,6 +218,8 @@ __global__ void __launch_bounds__(kThreads) prologue_kernel(tf_attn_prologue_arg
       const int h = r - Hq;
       const int64_t off = loc * a.buf_stride_slot + (int64_t)h * a.buf_stride_head + d0;
       const float ks = store_codes<E, VEC>((uint8_t*)a.k_buffer + off, y);
+      float v[E];
+      vraw.get(v);
       const float vs = store_codes<E, VEC>((uint8_t*)a.v_buffer + off, v);
       if (lane == 0)
         *reinterpret_cast<float2*>(sc.data + loc * sc.stride_slot + h * sc.stride_head) =
@@ -207,11 +228,11 @@ __global__ void __launch_bounds__(kThreads) prologue_kernel(tf_attn_prologue_arg
   }
 }
 
-template <typename T, int D>
-static cudaError_t launch_d(const tf_attn_prologue_args& a, const tf_kv_scale& sc, cudaStream_t s) {
+template <typename T, int D, int TPC>
+static cudaError_t launch_dt(const tf_attn_prologue_args& a, const tf_kv_scale& sc, cudaStream_t s) {
   constexpr int E = D / 32;
   const int half = a.rotary_dim / 2;
-  const int vb = E * (int)sizeof(T);
+  const int vb = E * (int)sizeof(T) < 16 ? E * (int)sizeof(T) : 16;
   auto al = [](const void* p, int n) { return (reinterpret_cast<uintptr_t>(p) % n) == 0; };
   bool vec = al(a.q, vb) && al(a.k, vb) && al(a.v, vb) && al(a.q_out, vb) && al(a.k_buffer, E) &&
              al(a.v_buffer, E);
@@ -221,11 +242,16 @@ static cudaError_t launch_d(const tf_attn_prologue_args& a, const tf_kv_scale& s
     vec = vec && x % E == 0;
   const int pm = half / E;
   const bool xr = half % E == 0 && pm < 32 && (pm & (pm - 1)) == 0;
-  const unsigned g = (unsigned)((a.num_tokens + kTPC - 1) / kTPC);
-  if (vec && xr) prologue_kernel<T, D, true, true><<<g, kThreads, 0, s>>>(a, sc);
-  else if (vec) prologue_kernel<T, D, true, false><<<g, kThreads, 0, s>>>(a, sc);
-  else prologue_kernel<T, D, false, false><<<g, kThreads, 0, s>>>(a, sc);
+  const unsigned g = (unsigned)((a.num_tokens + TPC - 1) / TPC);
+  if (vec && xr) prologue_kernel<T, D, TPC, true, true><<<g, kThreads, 0, s>>>(a, sc);
+  else if (vec) prologue_kernel<T, D, TPC, true, false><<<g, kThreads, 0, s>>>(a, sc);
+  else prologue_kernel<T, D, TPC, false, false><<<g, kThreads, 0, s>>>(a, sc);
   return cudaGetLastError();
+}
+
+template <typename T, int D>
+static cudaError_t launch_d(const tf_attn_prologue_args& a, const tf_kv_scale& sc, cudaStream_t s) {
+  return a.num_tokens <= kFewTokens ? launch_dt<T, D, 1>(a, sc, s) : launch_dt<T, D, 4>(a, sc, s);
 }
 
 template <typename T>

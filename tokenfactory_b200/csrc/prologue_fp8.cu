@@ -104,10 +104,47 @@ __device__ __forceinline__ float store_codes(uint8_t* p, const float (&x)[E]) {
   return rs.scale;
 }
 
-// VEC: rows aligned to the lane's E elements.  XOR: the partner lane is lane ^ pmask.
+// RMSNorm of a row and rotation of its first 2 half values, in place.  c, sn: cos and sin of the lane's
+// values (VEC / XOR forms), or of the token (shared memory, partner values through `row`).
+template <int D, bool XOR>
+__device__ __forceinline__ void norm_rotate(float (&y)[D / 32], const float (&w)[D / 32], float eps,
+                                            const float (&c)[D / 32], const float (&sn)[D / 32], int half,
+                                            int lane, float* row) {
+  constexpr int E = D / 32;
+  const int d0 = lane * E;
+  float ss = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) ss = fmaf(y[e], y[e], ss);
+  ss = warp_sum(ss);
+  const float rs = rsqrtf(ss * (1.0f / D) + eps);  // D is a power of two
+#pragma unroll
+  for (int e = 0; e < E; ++e) y[e] = w[e] * (y[e] * rs);
+  if constexpr (XOR) {
+    // sn carries the sign of the lane's half; lanes that do not rotate keep their values
+    float p[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) p[e] = __shfl_xor_sync(0xffffffffu, y[e], half / E);
+    if (d0 < 2 * half) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[e] = fmaf(p[e], sn[e], y[e] * c[e]);
+    }
+  } else {
+    __syncwarp();
+#pragma unroll
+    for (int e = 0; e < E; ++e) row[d0 + e] = y[e];
+    __syncwarp();
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int d = d0 + e;
+      if (d < 2 * half) y[e] = fmaf(row[d < half ? d + half : d - half], sn[e], y[e] * c[e]);
+    }
+  }
+}
+
+// VEC: rows aligned to the lane's E elements.  XOR: the partner lane is lane ^ (half / E).
 template <typename T, int D, int TPC, bool VEC, bool XOR>
-__global__ void __launch_bounds__(kThreads) prologue_kernel(tf_attn_prologue_args a,
-                                                            tf_kv_scale sc) {
+__global__ void __launch_bounds__(kThreads) prologue_kernel(const __grid_constant__ tf_attn_prologue_args a,
+                                                            const __grid_constant__ tf_kv_scale sc) {
   constexpr int E = D / 32;
   constexpr int kRowStep = kWarps / TPC;
   __shared__ float cs[TPC][kMaxD / 2], sn[TPC][kMaxD / 2];
@@ -119,19 +156,31 @@ __global__ void __launch_bounds__(kThreads) prologue_kernel(tf_attn_prologue_arg
   const int Hq = a.num_q_heads, Hkv = a.num_kv_heads;
   const int half = a.rotary_dim / 2;
   const int d0 = lane * E;
-  // warp w serves token w % TPC: its q rows, and its (k, v) row pairs as rows [Hq, Hq + Hkv)
+  // warp w serves token w % TPC: its q rows r0, r0 + kRowStep, ..., then its (k, v) row pairs
   const int tt = warp % TPC, r0 = warp / TPC;
   const bool live = tt < ntok;
   const int64_t t = t0 + (live ? tt : 0);
-  const int nrows = Hq + Hkv;
-  auto src_of = [&](int r) -> const T* {
-    return r < Hq ? (const T*)a.q + t * a.q_stride_tok + (int64_t)r * a.q_stride_head + d0
-                  : (const T*)a.k + t * a.k_stride_tok + (int64_t)(r - Hq) * a.k_stride_head + d0;
-  };
+  const T* qp = (const T*)a.q + t * a.q_stride_tok + (int64_t)r0 * a.q_stride_head + d0;
+  const int64_t q_step = (int64_t)kRowStep * a.q_stride_head;
   RawRow<T, E> ring[kPF];
 #pragma unroll
   for (int u = 0; u < kPF; ++u)
-    if (live && r0 + u * kRowStep < nrows) ring[u].template load<VEC>(src_of(r0 + u * kRowStep));
+    if (live && r0 + u * kRowStep < Hq) ring[u].template load<VEC>(qp + u * q_step);
+  const T* kp = (const T*)a.k + t * a.k_stride_tok + d0;
+  const T* vp = (const T*)a.v + t * a.v_stride_tok + d0;
+  RawRow<T, E> kraw, vraw;  // of the warp's next kv head
+  if (live && r0 < Hkv) {
+    kraw.template load<VEC>(kp + (int64_t)r0 * a.k_stride_head);
+    vraw.template load<VEC>(vp + (int64_t)r0 * a.v_stride_head);
+  }
+  float w[E];
+  const bool wf32 = a.norm_weight_dtype == TF_DTYPE_F32;
+  auto load_w = [&](const void* p) {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      w[e] = wf32 ? reinterpret_cast<const float*>(p)[d0 + e] : to_f(reinterpret_cast<const T*>(p)[d0 + e]);
+  };
+  load_w(a.q_norm_weight);
 
   for (int j = tid; j < ntok * half; j += kThreads) {
     const int jt = j / half, jj = j - jt * half;
@@ -156,75 +205,47 @@ __global__ void __launch_bounds__(kThreads) prologue_kernel(tf_attn_prologue_arg
   if (tid < ntok) s_loc[tid] = kv8::store_slot(a.out_cache_loc[t0 + tid], a.num_slots, a.err);
   __syncthreads();
   if (!live) return;
-  float wq[E], wk[E];
-  const bool wf32 = a.norm_weight_dtype == TF_DTYPE_F32;
+  float c[E], s[E];  // of the lane's values, the sine with the sign of its half
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    wq[e] = wf32 ? reinterpret_cast<const float*>(a.q_norm_weight)[d0 + e]
-                 : to_f(reinterpret_cast<const T*>(a.q_norm_weight)[d0 + e]);
-    wk[e] = wf32 ? reinterpret_cast<const float*>(a.k_norm_weight)[d0 + e]
-                 : to_f(reinterpret_cast<const T*>(a.k_norm_weight)[d0 + e]);
+    const int d = d0 + e, j = d < half ? d : (d < 2 * half ? d - half : 0);
+    c[e] = cs[tt][j];
+    s[e] = d < half ? -sn[tt][j] : sn[tt][j];
   }
-  const int64_t loc = s_loc[tt];
-  const int pmask = half / E;
-  for (int m0 = 0; r0 + m0 * kRowStep < nrows; m0 += kPF) {
+  float* row = s_row[XOR ? 0 : warp];
+  T* op = (T*)a.q_out + t * a.q_out_stride_tok + (int64_t)r0 * a.q_out_stride_head + d0;
+  const int64_t o_step = (int64_t)kRowStep * a.q_out_stride_head;
+  qp += kPF * q_step;
+  for (int r = r0; r < Hq; r += kPF * kRowStep) {
 #pragma unroll
     for (int u = 0; u < kPF; ++u) {
-      const int r = r0 + (m0 + u) * kRowStep;
-      if (r >= nrows) break;
+      if (r + u * kRowStep >= Hq) break;
       float y[E];
       ring[u].get(y);
-      if (r + kPF * kRowStep < nrows) ring[u].template load<VEC>(src_of(r + kPF * kRowStep));
-      const bool isq = r < Hq;
-      if (!isq && loc < 0) continue;
-      RawRow<T, E> vraw;
-      if (!isq)
-        vraw.template load<VEC>((const T*)a.v + t * a.v_stride_tok + (int64_t)(r - Hq) * a.v_stride_head + d0);
-      float ss = 0.f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) ss = fmaf(y[e], y[e], ss);
-      ss = warp_sum(ss);
-      const float rs = 1.0f / sqrtf(ss / (float)D + a.eps);
-#pragma unroll
-      for (int e = 0; e < E; ++e) y[e] = (isq ? wq[e] : wk[e]) * (y[e] * rs);
-      if constexpr (XOR) {
-        const bool rotates = d0 < 2 * half, lower = d0 < half;
-        const int j0 = lower ? d0 : d0 - half;
-        float p[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) p[e] = __shfl_xor_sync(0xffffffffu, y[e], pmask);
-        if (rotates) {
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-            y[e] = y[e] * cs[tt][j0 + e] + (lower ? -p[e] : p[e]) * sn[tt][j0 + e];
-        }
-      } else {
-        __syncwarp();
-#pragma unroll
-        for (int e = 0; e < E; ++e) s_row[warp][d0 + e] = y[e];
-        __syncwarp();
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const int d = d0 + e;
-          if (d < half) y[e] = y[e] * cs[tt][d] - s_row[warp][d + half] * sn[tt][d];
-          else if (d < 2 * half)
-            y[e] = y[e] * cs[tt][d - half] + s_row[warp][d - half] * sn[tt][d - half];
-        }
-      }
-      if (isq) {
-        store_row<T, E, VEC>((T*)a.q_out + t * a.q_out_stride_tok + (int64_t)r * a.q_out_stride_head + d0, y);
-        continue;
-      }
-      const int h = r - Hq;
-      const int64_t off = loc * a.buf_stride_slot + (int64_t)h * a.buf_stride_head + d0;
-      const float ks = store_codes<E, VEC>((uint8_t*)a.k_buffer + off, y);
-      float v[E];
-      vraw.get(v);
-      const float vs = store_codes<E, VEC>((uint8_t*)a.v_buffer + off, v);
-      if (lane == 0)
-        *reinterpret_cast<float2*>(sc.data + loc * sc.stride_slot + h * sc.stride_head) =
-            make_float2(ks, vs);
+      if (r + (u + kPF) * kRowStep < Hq) ring[u].template load<VEC>(qp);
+      qp += q_step;
+      norm_rotate<D, XOR>(y, w, a.eps, c, s, half, lane, row);
+      store_row<T, E, VEC>(op, y);
+      op += o_step;
     }
+  }
+  const int64_t loc = s_loc[tt];
+  if (loc < 0 || r0 >= Hkv) return;
+  load_w(a.k_norm_weight);
+  for (int h = r0; h < Hkv; h += kRowStep) {
+    float y[E], v[E];
+    kraw.get(y);
+    vraw.get(v);
+    if (h + kRowStep < Hkv) {
+      kraw.template load<VEC>(kp + (int64_t)(h + kRowStep) * a.k_stride_head);
+      vraw.template load<VEC>(vp + (int64_t)(h + kRowStep) * a.v_stride_head);
+    }
+    norm_rotate<D, XOR>(y, w, a.eps, c, s, half, lane, row);
+    const int64_t off = loc * a.buf_stride_slot + (int64_t)h * a.buf_stride_head + d0;
+    const float ks = store_codes<E, VEC>((uint8_t*)a.k_buffer + off, y);
+    const float vs = store_codes<E, VEC>((uint8_t*)a.v_buffer + off, v);
+    if (lane == 0)
+      *reinterpret_cast<float2*>(sc.data + loc * sc.stride_slot + h * sc.stride_head) = make_float2(ks, vs);
   }
 }
 

@@ -1,6 +1,8 @@
 // KV-pool store with the rows quantized to e4m3 (formulas in tfattn.h): the 8-bit counterpart of
 // kv_store.cu.  HBM-bound: a row is read once, its largest magnitude found by shuffles among the
 // lanes that hold it, and the codes written from the same registers.
+#include <type_traits>
+
 #include "common.cuh"
 #include "kv_fp8.cuh"
 #include "launch.h"
@@ -10,20 +12,11 @@ namespace {
 
 constexpr int kThreads = 256;
 
-template <typename T> struct Vec8;  // eight elements of a row, loaded in 16-byte pieces
-template <> struct Vec8<float> {
-  float x[8];
-  __device__ __forceinline__ void load(const float* p) {
-    const float4 a = __ldcs(reinterpret_cast<const float4*>(p));
-    const float4 b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-  }
-};
+// eight elements of a row, loaded in 16-byte pieces and unpacked when used
 template <typename T> struct Vec8 {
-  float x[8];
-  __device__ __forceinline__ void load(const T* p) {
-    const uint4 w = __ldcs(reinterpret_cast<const uint4*>(p));
+  uint4 w;
+  __device__ __forceinline__ void load(const T* p) { w = __ldcs(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -32,49 +25,77 @@ template <typename T> struct Vec8 {
     }
   }
 };
+template <> struct Vec8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = __ldcs(reinterpret_cast<const float4*>(p));
+    b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  }
+};
 
-// LPR = D / 8 lanes hold a row, eight elements each; a group of LPR lanes takes the K and the V
-// row of one (token, kv head), so two rows are in flight per lane and the scale pair is one store.
-template <typename T, int LPR>
-__global__ void __launch_bounds__(kThreads) store_vec_kernel(tf_kv_store_args a, tf_kv_scale sc) {
-  const int64_t r = (blockIdx.x * (int64_t)kThreads + threadIdx.x) / LPR;
+// LPR = D / 8 lanes hold a row, eight elements each; a group of LPR lanes takes the K and the V rows
+// of N (token, kv head) pairs, so 2 N rows are in flight per lane and a scale pair is one store.
+template <typename T, int LPR, int N>
+__global__ void __launch_bounds__(kThreads) store_vec_kernel(const __grid_constant__ tf_kv_store_args a,
+                                                             const __grid_constant__ tf_kv_scale sc) {
+  const int64_t g = (blockIdx.x * (int64_t)kThreads + threadIdx.x) / LPR;
   const int l = threadIdx.x % LPR;
   const int64_t rows = a.num_tokens * (int64_t)a.num_kv_heads;
-  const bool live = r < rows;
-  const int64_t t = live ? r / a.num_kv_heads : 0;
-  const int h = live ? (int)(r - t * a.num_kv_heads) : 0;
-  Vec8<T> x[2];
-  x[0].load((const T*)a.k + t * a.k_stride_tok + h * a.k_stride_head + 8 * l);
-  x[1].load((const T*)a.v + t * a.v_stride_tok + h * a.v_stride_head + 8 * l);
-  const int64_t loc = a.out_cache_loc[t];
-  kv8::RowScale rs[2];
+  int h[N];
+  int64_t loc[N];
+  Vec8<T> x[N][2];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, kv8::abs_bits(x[j].x[i]));
-#pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    rs[j] = kv8::row_scale(m);
+  for (int n = 0; n < N; ++n) {
+    int64_t r = g * N + n;
+    if (r >= rows) r = rows - 1;  // in bounds; not stored
+    const int64_t t = a.num_kv_heads == 1 ? r : r / a.num_kv_heads;
+    h[n] = (int)(r - t * a.num_kv_heads);
+    loc[n] = a.out_cache_loc[t];
+    x[n][0].load((const T*)a.k + t * a.k_stride_tok + h[n] * a.k_stride_head + 8 * l);
+    x[n][1].load((const T*)a.v + t * a.v_stride_tok + h[n] * a.v_stride_head + 8 * l);
   }
-  if (!live) return;
-  const int64_t slot = kv8::store_slot(loc, a.num_slots, l == 0 ? a.err : nullptr);
-  if (slot < 0) return;
-  const int64_t off = slot * a.buf_stride_slot + h * a.buf_stride_head + 8 * l;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    uint2 c = make_uint2(0, 0);
-    if (rs[j].finite) {
-      const float m = rs[j].mul;
-      const float* v = x[j].x;
-      c.x = kv8::code4(v[0] * m, v[1] * m, v[2] * m, v[3] * m);
-      c.y = kv8::code4(v[4] * m, v[5] * m, v[6] * m, v[7] * m);
+  for (int n = 0; n < N; ++n) {
+    kv8::RowScale rs[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float v[8];
+      x[n][j].get(v);
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = max(m, kv8::abs_bits(v[i]));
+      if (LPR == 32) {
+        m = __reduce_max_sync(0xffffffffu, m);
+      } else {
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      }
+      rs[j] = kv8::row_scale(m);
     }
-    *reinterpret_cast<uint2*>((char*)(j ? a.v_buffer : a.k_buffer) + off) = c;
+    if (g * N + n >= rows) continue;
+    const int64_t slot = kv8::store_slot(loc[n], a.num_slots, l == 0 ? a.err : nullptr);
+    if (slot < 0) continue;
+    const int64_t off = slot * a.buf_stride_slot + h[n] * a.buf_stride_head + 8 * l;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float v[8];
+      x[n][j].get(v);
+      uint2 c = make_uint2(0, 0);
+      if (rs[j].finite) {
+        const float m = rs[j].mul;
+        c.x = kv8::code4(v[0] * m, v[1] * m, v[2] * m, v[3] * m);
+        c.y = kv8::code4(v[4] * m, v[5] * m, v[6] * m, v[7] * m);
+      }
+      *reinterpret_cast<uint2*>((char*)(j ? a.v_buffer : a.k_buffer) + off) = c;
+    }
+    if (l == 0)
+      *reinterpret_cast<float2*>(sc.data + slot * sc.stride_slot + h[n] * sc.stride_head) =
+          make_float2(rs[0].scale, rs[1].scale);
   }
-  if (l == 0)
-    *reinterpret_cast<float2*>(sc.data + slot * sc.stride_slot + h * sc.stride_head) =
-        make_float2(rs[0].scale, rs[1].scale);
 }
 
 // any head_dim, strides and alignment: a warp per (token, kv head), each row read twice
@@ -119,13 +140,20 @@ cudaError_t launch_t(const tf_kv_store_args& a, const tf_kv_scale& sc, cudaStrea
                    (a.k_stride_head * eb) % 16 == 0 && (a.v_stride_tok * eb) % 16 == 0 &&
                    (a.v_stride_head * eb) % 16 == 0 && a.buf_stride_slot % 8 == 0 &&
                    a.buf_stride_head % 8 == 0;
+  // two pairs a group once the groups of one pair each would fill the SMs
+  const int per = vec && rows * (d / 8) >= 148 * 2048 ? 2 : 1;
   const int lanes = vec ? d / 8 : 32;
-  const int64_t blocks = (rows * lanes + kThreads - 1) / kThreads;
+  const int64_t blocks = ((rows + per - 1) / per * lanes + kThreads - 1) / kThreads;
   if (vec && blocks <= 0x7fffffff) {
     const unsigned g = (unsigned)blocks;
-    if (d == 64) store_vec_kernel<T, 8><<<g, kThreads, 0, s>>>(a, sc);
-    else if (d == 128) store_vec_kernel<T, 16><<<g, kThreads, 0, s>>>(a, sc);
-    else store_vec_kernel<T, 32><<<g, kThreads, 0, s>>>(a, sc);
+    auto go = [&](auto lpr) {
+      constexpr int L = decltype(lpr)::value;
+      if (per == 2) store_vec_kernel<T, L, 2><<<g, kThreads, 0, s>>>(a, sc);
+      else store_vec_kernel<T, L, 1><<<g, kThreads, 0, s>>>(a, sc);
+    };
+    if (d == 64) go(std::integral_constant<int, 8>());
+    else if (d == 128) go(std::integral_constant<int, 16>());
+    else go(std::integral_constant<int, 32>());
   } else {
     const unsigned g = (unsigned)(blocks < 148 * 32 ? blocks : 148 * 32);
     store_any_kernel<T><<<g, kThreads, 0, s>>>(a, sc);

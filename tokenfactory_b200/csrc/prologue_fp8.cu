@@ -143,7 +143,7 @@ __device__ __forceinline__ void norm_rotate(float (&y)[D / 32], const float (&w)
 
 // VEC: rows aligned to the lane's E elements.  XOR: the partner lane is lane ^ (half / E).
 template <typename T, int D, int TPC, bool VEC, bool XOR>
-__global__ void __launch_bounds__(kThreads) prologue_kernel(const __grid_constant__ tf_attn_prologue_args a,
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) prologue_kernel(const __grid_constant__ tf_attn_prologue_args a,
                                                             const __grid_constant__ tf_kv_scale sc) {
   constexpr int E = D / 32;
   constexpr int kRowStep = kWarps / TPC;

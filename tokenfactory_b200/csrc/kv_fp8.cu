@@ -16,6 +16,17 @@ constexpr int kThreads = 256;
 template <typename T> struct Vec8 {
   uint4 w;
   __device__ __forceinline__ void load(const T* p) { w = __ldcs(reinterpret_cast<const uint4*>(p)); }
+  // abs_bits of the largest element: 16-bit magnitudes order like their bits, two to a word
+  __device__ __forceinline__ uint32_t amax() const {
+    uint32_t m = w.x & 0x7fff7fffu;
+    asm("max.u16x2 %0, %0, %1;" : "+r"(m) : "r"(w.y & 0x7fff7fffu));
+    asm("max.u16x2 %0, %0, %1;" : "+r"(m) : "r"(w.z & 0x7fff7fffu));
+    asm("max.u16x2 %0, %0, %1;" : "+r"(m) : "r"(w.w & 0x7fff7fffu));
+    return __float_as_uint(fmax_bits(m));
+  }
+  static __device__ __forceinline__ float fmax_bits(uint32_t m) {
+    return unpack_lo<T>(max(m & 0xffffu, m >> 16));
+  }
   __device__ __forceinline__ void get(float (&x)[8]) const {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -30,6 +41,14 @@ template <> struct Vec8<float> {
   __device__ __forceinline__ void load(const float* p) {
     a = __ldcs(reinterpret_cast<const float4*>(p));
     b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
+  }
+  __device__ __forceinline__ uint32_t amax() const {
+    float x[8];
+    get(x);
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, kv8::abs_bits(x[i]));
+    return m;
   }
   __device__ __forceinline__ void get(float (&x)[8]) const {
     x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
@@ -60,22 +79,18 @@ __global__ void __launch_bounds__(kThreads) store_vec_kernel(const __grid_consta
   }
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    kv8::RowScale rs[2];
+    uint32_t m[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      float v[8];
-      x[n][j].get(v);
-      uint32_t m = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) m = max(m, kv8::abs_bits(v[i]));
+      m[j] = x[n][j].amax();
       if (LPR == 32) {
-        m = __reduce_max_sync(0xffffffffu, m);
+        m[j] = __reduce_max_sync(0xffffffffu, m[j]);
       } else {
 #pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        for (int o = LPR / 2; o > 0; o >>= 1) m[j] = max(m[j], __shfl_xor_sync(0xffffffffu, m[j], o));
       }
-      rs[j] = kv8::row_scale(m);
     }
+    const kv8::PairScale ps = kv8::pair_scale<LPR>(m[0], m[1], l);
     if (g * N + n >= rows) continue;
     const int64_t slot = kv8::store_slot(loc[n], a.num_slots, l == 0 ? a.err : nullptr);
     if (slot < 0) continue;
@@ -85,16 +100,16 @@ __global__ void __launch_bounds__(kThreads) store_vec_kernel(const __grid_consta
       float v[8];
       x[n][j].get(v);
       uint2 c = make_uint2(0, 0);
-      if (rs[j].finite) {
-        const float m = rs[j].mul;
-        c.x = kv8::code4(v[0] * m, v[1] * m, v[2] * m, v[3] * m);
-        c.y = kv8::code4(v[4] * m, v[5] * m, v[6] * m, v[7] * m);
+      if (ps.finite[j]) {
+        const float f = ps.mul[j];
+        c.x = kv8::code4(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
+        c.y = kv8::code4(v[4] * f, v[5] * f, v[6] * f, v[7] * f);
       }
       *reinterpret_cast<uint2*>((char*)(j ? a.v_buffer : a.k_buffer) + off) = c;
     }
     if (l == 0)
       *reinterpret_cast<float2*>(sc.data + slot * sc.stride_slot + h[n] * sc.stride_head) =
-          make_float2(rs[0].scale, rs[1].scale);
+          make_float2(ps.scale[0], ps.scale[1]);
   }
 }
 

@@ -32,6 +32,28 @@ __device__ __forceinline__ RowScale row_scale(uint32_t amax) {
   return r;
 }
 
+// row_scale of a K row and a V row at once, for a group of W lanes (8, 16 or 32; lane l of the group):
+// the four quotients are one division, each in a lane of its own, instead of four.
+struct PairScale {
+  float mul[2], scale[2];
+  bool finite[2];
+};
+template <int W>
+__device__ __forceinline__ PairScale pair_scale(uint32_t amax_k, uint32_t amax_v, int l) {
+  const uint32_t bits = l & 2 ? amax_v : amax_k;
+  const float m = fmaxf(__uint_as_float(bits), kMinAmax);  // (fmaxf of a NaN: kMinAmax, not used)
+  const float q = __fdiv_rn(l & 1 ? m : kE4m3Max, l & 1 ? kE4m3Max : m);
+  PairScale r;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    r.finite[j] = (j ? amax_v : amax_k) < 0x7f800000u;
+    r.mul[j] = __shfl_sync(0xffffffffu, q, 2 * j, W);
+    const float sc = __shfl_sync(0xffffffffu, q, 2 * j + 1, W);
+    r.scale[j] = r.finite[j] ? sc : __uint_as_float(0x7fc00000u);
+  }
+  return r;
+}
+
 // two codes, round to nearest even, saturated at +-448, `a` in the low byte
 __device__ __forceinline__ uint32_t code2(float a, float b) {
   return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);

@@ -78,18 +78,21 @@ __device__ __forceinline__ void store_row(T* p, const float (&x)[E]) {
   }
 }
 
-// codes of the lane's E elements of a row (all lanes of the warp call it); returns the scale
-template <int E, bool VEC>
-__device__ __forceinline__ float store_codes(uint8_t* p, const float (&x)[E]) {
+// largest abs_bits of a row of which the warp's lanes hold E elements each
+template <int E>
+__device__ __forceinline__ uint32_t row_amax(const float (&x)[E]) {
   uint32_t m = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) m = max(m, kv8::abs_bits(x[e]));
-  m = __reduce_max_sync(0xffffffffu, m);
-  const kv8::RowScale rs = kv8::row_scale(m);
+  return __reduce_max_sync(0xffffffffu, m);
+}
+
+// codes of the lane's E elements of a row
+template <int E, bool VEC>
+__device__ __forceinline__ void store_codes(uint8_t* p, const float (&x)[E], float mul, bool finite) {
   uint32_t c[E / 2];
 #pragma unroll
-  for (int i = 0; i < E / 2; ++i)
-    c[i] = rs.finite ? kv8::code2(x[2 * i] * rs.mul, x[2 * i + 1] * rs.mul) : 0u;
+  for (int i = 0; i < E / 2; ++i) c[i] = finite ? kv8::code2(x[2 * i] * mul, x[2 * i + 1] * mul) : 0u;
   if constexpr (VEC && E == 8) {
     *reinterpret_cast<uint2*>(p) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
   } else if constexpr (VEC && E == 4) {
@@ -101,7 +104,6 @@ __device__ __forceinline__ float store_codes(uint8_t* p, const float (&x)[E]) {
       p[2 * i + 1] = (uint8_t)(c[i] >> 8);
     }
   }
-  return rs.scale;
 }
 
 // RMSNorm of a row and rotation of its first 2 half values, in place.  c, sn: cos and sin of the lane's
@@ -242,10 +244,12 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) prologue_ker
     }
     norm_rotate<D, XOR>(y, w, a.eps, c, s, half, lane, row);
     const int64_t off = loc * a.buf_stride_slot + (int64_t)h * a.buf_stride_head + d0;
-    const float ks = store_codes<E, VEC>((uint8_t*)a.k_buffer + off, y);
-    const float vs = store_codes<E, VEC>((uint8_t*)a.v_buffer + off, v);
+    const kv8::PairScale ps = kv8::pair_scale<32>(row_amax(y), row_amax(v), lane);
+    store_codes<E, VEC>((uint8_t*)a.k_buffer + off, y, ps.mul[0], ps.finite[0]);
+    store_codes<E, VEC>((uint8_t*)a.v_buffer + off, v, ps.mul[1], ps.finite[1]);
     if (lane == 0)
-      *reinterpret_cast<float2*>(sc.data + loc * sc.stride_slot + h * sc.stride_head) = make_float2(ks, vs);
+      *reinterpret_cast<float2*>(sc.data + loc * sc.stride_slot + h * sc.stride_head) =
+          make_float2(ps.scale[0], ps.scale[1]);
   }
 }
 

@@ -59,9 +59,10 @@ struct Cfg {
   static constexpr int kOffScale = kOffV + kTok * kVS;
   static constexpr int kStage = kOffScale + kTok * 8;
   static constexpr int kStages = D == 256 ? 12 : (D == 128 ? 20 : 40);  // at most
-  // epilogue: 64 dims of every warp's rows, then their (M, l) and what each is multiplied by
+  // epilogue: 64 dims of every warp's rows, then per row what it is multiplied by, (M, l), and its
+  // place in the output
   static constexpr int kEpiStride = 64 + 4;  // floats per row
-  static constexpr int kEpi = kWarps * kRows * (kEpiStride + 3) * 4;
+  static constexpr int kEpi = kWarps * kRows * (kEpiStride + 5) * 4;
   static constexpr int kFixed = kCache * (int)sizeof(ReqMeta) + 64;
   static_assert(kStage % 16 == 0 && kKS % 16 == 0 && kVS % 16 == 0, "bulk copy alignment");
 };
@@ -224,27 +225,23 @@ struct Walker {
   }
 };
 
-// 4 output values of a query row at dims d.. (times the gate's activation); v8: rows can be moved in
-// 8-byte pieces
+// 4 gate values of a query row at dims d..; v8: rows can be moved in 8-byte pieces
+template <typename T>
+__device__ __forceinline__ uint2 gate4(const tf_paged_attn_args& a, int64_t tok, int hq, int d, bool v8) {
+  const T* gp = (const T*)a.gate + tok * a.gate_stride_tok + (int64_t)hq * a.gate_stride_head + d;
+  if (v8) return __ldg(reinterpret_cast<const uint2*>(gp));
+  const unsigned short* u = reinterpret_cast<const unsigned short*>(gp);
+  return make_uint2(u[0] | ((uint32_t)u[1] << 16), u[2] | ((uint32_t)u[3] << 16));
+}
+// 4 output values, times the gate's activation
 template <typename T>
 __device__ __forceinline__ void put4(const tf_paged_attn_args& a, int64_t tok, int hq, int d, float4 x,
-                                     bool v8) {
+                                     uint2 gw, bool v8) {
   float o[4] = {x.x, x.y, x.z, x.w};
   if (a.gate_mode != TF_GATE_NONE) {
-    const T* gp = (const T*)a.gate + tok * a.gate_stride_tok + (int64_t)hq * a.gate_stride_head + d;
-    uint32_t w[2];
-    if (v8) {
-      const uint2 u = __ldg(reinterpret_cast<const uint2*>(gp));
-      w[0] = u.x;
-      w[1] = u.y;
-    } else {
-      const unsigned short* u = reinterpret_cast<const unsigned short*>(gp);
-      w[0] = u[0] | ((uint32_t)u[1] << 16);
-      w[1] = u[2] | ((uint32_t)u[3] << 16);
-    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float g = i & 1 ? unpack_hi<T>(w[i >> 1]) : unpack_lo<T>(w[i >> 1]);
+      const float g = i & 1 ? unpack_hi<T>(i < 2 ? gw.x : gw.y) : unpack_lo<T>(i < 2 ? gw.x : gw.y);
       const float sg = sigmoid_f(g);
       o[i] *= a.gate_mode == TF_GATE_SILU ? g * sg : sg;
     }
@@ -266,52 +263,57 @@ __device__ __forceinline__ bool rows_v8(const tf_paged_attn_args& a) {
          ((a.out_stride_tok | a.out_stride_head | a.gate_stride_tok | a.gate_stride_head) & 3) == 0;
 }
 
-// A finished piece, for the whole CTA.
-struct Piece {
-  int u, ext, start, slot;  // slot: partial place of this CTA (2 c or 2 c + 1)
-  bool whole;
-};
-
 // 64 dims (d0..) of every row of a piece from the epilogue buffer: the teams of a head are summed, and
 // the result is normalised and put out, or left as partials.  One copy of this code serves all
 // pieces and dims: unrolled into the kernel it ran once a piece from a cold instruction cache
 // (15-35 us a piece were measured).
 template <typename T, int D>
 __device__ __noinline__ void finish64(const tf_paged_attn_args& a, const Shape& sh, const Ws& ws,
-                                      const float* epi, const Piece& p, int d0) {
+                                      const float* epi, int slot, bool whole, int d0) {
   constexpr int kS = Cfg<D>::kEpiStride;
+  constexpr int kTwo = 2;  // items of a thread whose gate values are requested together
   const float* fac = epi + kWarps * kRows * kS;         // [warp][row] what the warp's row counts
   const float* ml = fac + kWarps * kRows;               // [warp][row][2]; the first team's: merged
+  const int2* to = reinterpret_cast<const int2*>(ml + 2 * kWarps * kRows);  // [place][row] token (or -1), head
   const int per = sh.hg * sh.team;
-  const int G = a.num_q_heads / a.num_kv_heads;
-  const bool v8 = rows_v8(a);
+  const bool v8 = rows_v8(a), gated = whole && a.gate_mode != TF_GATE_NONE;
 #pragma unroll 1
-  for (int e = threadIdx.x; e < per * kRows * 16; e += kThreads) {
-    const int v = e & 15, r = (e >> 4) & (kRows - 1), place = e >> 7;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-    for (int w = place; w < kWarps; w += per) {
-      const float f = fac[w * kRows + r];
-      const float4 x = *reinterpret_cast<const float4*>(epi + (w * kRows + r) * kS + 4 * v);
-      o.x = fmaf(f, x.x, o.x);
-      o.y = fmaf(f, x.y, o.y);
-      o.z = fmaf(f, x.z, o.z);
-      o.w = fmaf(f, x.w, o.w);
+  for (int e0 = threadIdx.x; e0 < per * kRows * 16; e0 += kTwo * kThreads) {
+    int2 th[kTwo];
+    uint2 gw[kTwo];
+#pragma unroll
+    for (int k = 0; k < kTwo; ++k) {
+      const int e = e0 + k * kThreads;
+      th[k] = make_int2(-1, 0);
+      gw[k] = make_uint2(0, 0);
+      if (e < per * kRows * 16) {
+        th[k] = to[e >> 4];
+        if (gated && th[k].x >= 0) gw[k] = gate4<T>(a, th[k].x, th[k].y, d0 + 4 * (e & 15), v8);
+      }
     }
-    if (p.whole) {
-      const int hsel = place / sh.team, member = place - hsel * sh.team;
-      const int row = ((p.u % sh.passes) * sh.team + member) * kRows + r;
-      const int64_t tok = p.start + row / G;
-      if (row >= p.ext * G || tok >= a.num_tokens) continue;
-      const int hq = ((p.u / sh.passes) * sh.hg + hsel) * G + row % G;
-      const float inv = (1.f / 128.f) / ml[(place * kRows + r) * 2 + 1];
-      put4<T>(a, tok, hq, d0 + 4 * v, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), v8);
-    } else {
-      const int64_t ps = (int64_t)(p.slot * kWarps + place) * kRows + r;
-      *reinterpret_cast<float4*>(ws.o + ps * D + d0 + 4 * v) = o;
-      if (d0 == 0 && v == 0)
-        *reinterpret_cast<float2*>(ws.ml + ps * 2) =
-            make_float2(ml[(place * kRows + r) * 2], ml[(place * kRows + r) * 2 + 1]);
+#pragma unroll
+    for (int k = 0; k < kTwo; ++k) {
+      const int e = e0 + k * kThreads;
+      if (th[k].x < 0) continue;
+      const int v = e & 15, pr = e >> 4;  // place * kRows + row
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+      for (int w = pr; w < kWarps * kRows; w += per * kRows) {
+        const float f = fac[w];
+        const float4 x = *reinterpret_cast<const float4*>(epi + w * kS + 4 * v);
+        o.x = fmaf(f, x.x, o.x);
+        o.y = fmaf(f, x.y, o.y);
+        o.z = fmaf(f, x.z, o.z);
+        o.w = fmaf(f, x.w, o.w);
+      }
+      if (whole) {
+        const float inv = (1.f / 128.f) / ml[2 * pr + 1];
+        put4<T>(a, th[k].x, th[k].y, d0 + 4 * v, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), gw[k], v8);
+      } else {
+        const int64_t ps = (int64_t)slot * kWarps * kRows + pr;
+        *reinterpret_cast<float4*>(ws.o + ps * D + d0 + 4 * v) = o;
+        if (d0 == 0 && v == 0) *reinterpret_cast<float2*>(ws.ml + ps * 2) = make_float2(ml[2 * pr], ml[2 * pr + 1]);
+      }
     }
   }
 }
@@ -496,6 +498,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kAhead = 2;
   int64_t raw[kAhead];
   int head[kAhead];           // their kv heads
+  int pf = 0, pf_unit = INT32_MIN;  // tiles of the unit whose entries have been asked for; its first tile
   int pq = wsel - kAhead * sh.wh;  // next tile to fetch (below 0: the entries' own head start)
   int p_st = first, p_round = 0;   // its stage and round
   bool ok = true;
@@ -554,6 +557,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int fq = pq + kAhead * sh.wh;
     if (fq < ntiles) {
       prod.seek(rq, fq);
+      // A load behind a saturated memory takes about the time that the ring lasts, more than the tile
+      // or two that this one is ahead: the entries of the next 16 to 32 tiles are asked into L2 (16
+      // tiles a warp instruction, 128 bytes a lane).
+      if (prod.unit_g != pf_unit) {
+        pf_unit = prod.unit_g;
+        pf = fq - prod.unit_g;
+      }
+      while (pf < min(fq - prod.unit_g + 17, prod.nt())) {
+        const int pos = pf * kTok + lane * 16;
+        if (pos < prod.m.len)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(a.req_to_token + (int64_t)prod.m.row * a.r2t_stride + pos));
+        pf += 16;
+      }
       const int pos = min((fq - prod.unit_g) * kTok + member * share + lane, prod.m.len - 1);
       raw[kAhead - 1] = a.req_to_token[(int64_t)prod.m.row * a.r2t_stride + pos];
       head[kAhead - 1] = (prod.u / sh.passes) * sh.hg + hsel;
@@ -564,7 +580,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Tile x of the ring may be fetched once x - stages has been consumed.  A team waits for that only
   // when x - stages is not behind its own current tile in the sequence: whoever has to consume it
   // is then not held up by this team (nor by the barriers at the end of a piece), and as a team's
-  // own tiles are at most a ring apart (step <= stages) its next tile is always on its way.
+  // own tiles are at most a ring apart (step <= stages) its next tile is always on its way.  `lag`
+  // tiles of slack keep a team from waiting for the slowest warp of the very tile it has just left.
+  const int lag = min(3, sh.stages - step);
   int x_lim = sh.stages - 1;  // the last tile that may be fetched now
   float* epi = reinterpret_cast<float*>(smem + sh.ring + C::kFixed + 16 * sh.stages);
   int cq = wsel, st = first;  // this team's next tile of the range and its stage
@@ -779,7 +797,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
       if (lane == 0) count_use(&used[st]);
-      x_lim = cq * sh.hg + hsel + sh.stages;
+      x_lim = max(x_lim, cq * sh.hg + hsel + sh.stages - lag);
       cq += sh.wh;
       st += step;
       if (st >= sh.stages) {
@@ -803,8 +821,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           *reinterpret_cast<float2*>(ml + (warp * kRows + 2 * tq + k) * 2) = make_float2(M[k], l[k]);
       }
       float* mine = epi + warp * kRows * C::kEpiStride;
-      const Piece pc = {u, E, cons.m.start, 2 * c + (p0 == 0 ? 0 : 1),
-                        p0 == cons.unit_g && p1 == cons.unit_g + cons.nt()};
+      const int slot = 2 * c + (p0 == 0 ? 0 : 1);  // partial place
+      const bool whole = p0 == cons.unit_g && p1 == cons.unit_g + cons.nt();
+      if (wsel == 0 && lane < kRows) {
+        const int row = row0 + lane;
+        const int64_t tok = qtok0 + row / G;
+        reinterpret_cast<int2*>(ml + 2 * kWarps * kRows)[warp * kRows + lane] =
+            make_int2(row < E * G && tok < a.num_tokens ? (int)tok : -1, kvh * G + row % G);
+      }
 #pragma unroll
       for (int m0 = 0; m0 < NM; m0 += 4) {
 #pragma unroll
@@ -829,7 +853,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           __syncthreads();
         }
-        finish64<T, D>(a, sh, ws, epi, pc, 16 * m0);
+        finish64<T, D>(a, sh, ws, epi, slot, whole, 16 * m0);
         __syncthreads();
       }
     }
@@ -839,39 +863,75 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ---------------------------------------------------------------------------------------------
-// combine: CTA (c, place, rows) merges RZ rows of one warp place of the unit that the boundary of range
-// c cuts, when it is the first boundary inside that unit.  A thread holds 4 values of one row; the
-// PG = 256 / (RZ D / 4) groups of threads take the pieces in turn (one row a CTA and many groups when
-// few units have many pieces each).
+// combine: merges the rows of one warp place of a cut unit.  A thread holds 4 values of one row; the PG
+// groups of threads take the unit's pieces in turn.
+//   wide (many units, few pieces each): CTA (c, place, z) looks at the boundary of range c, and merges RZ
+//     rows of the unit that it cuts when it is the first boundary inside that unit
+//   deep (few units, many pieces each): CTA (unit, place, row), 16 groups
 // ---------------------------------------------------------------------------------------------
-template <typename T, int D, int RZ>
-__global__ void __launch_bounds__(256)
+template <typename T, int D, int RZ, int THREADS, bool DEEP>
+__global__ void __launch_bounds__(THREADS)
     combine_kernel(const __grid_constant__ tf_paged_attn_args a, const __grid_constant__ Shape sh,
                    const __grid_constant__ Ws ws) {
   constexpr int kVec = D / 4;  // 4-value vectors of a row
-  constexpr int PG = 256 / (RZ * kVec);
-  static_assert(PG >= 1 && PG * RZ * kVec == 256, "threads of a CTA");
-  __shared__ float red[PG > 1 ? 256 : 1][PG > 1 ? 5 : 1];
+  constexpr int PG = THREADS / (RZ * kVec);
+  static_assert(PG >= 1 && PG * RZ * kVec == THREADS, "threads of a CTA");
+  __shared__ float red[PG > 1 ? THREADS : 1][PG > 1 ? 6 : 1];
   __shared__ int64_t s_g[kMaxCtas + 1];
   __shared__ int s_slot[kMaxCtas];
   __shared__ int s_np;
   const int tid = threadIdx.x, lane = tid & 31;
-  const int c = blockIdx.x + 1, w = blockIdx.y;
-  const int n = gridDim.x + 1;  // decode CTAs
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const CutInfo ci = ws.cut[c];
-  for (int i = tid; i <= n; i += 256) s_g[i] = ws.cta_g[i];
-  __syncthreads();
-  const int64_t g = s_g[c];
-  if (g >= s_g[n] || s_g[c + 1] == g || ci.t0 == 0) return;  // empty range, or nothing cut here
-  const int64_t su = g - ci.t0, eu = su + ci.nt;
-  int c0 = c - 1;
-  while (s_g[c0] == g) --c0;   // empty ranges before this one
-  if (s_g[c0] > su) return;    // not the first boundary inside the unit
+  const int w = blockIdx.y, n = sh.nctas;
   const int G = a.num_q_heads / a.num_kv_heads;
+  int u, start, ext, c0;
+  int64_t su, eu;
+  if (DEEP) {  // the unit's tiles from the lengths, while the main kernel still runs
+    const int b = blockIdx.x / sh.groups;
+    u = blockIdx.x - b * sh.groups;
+    int64_t before = 0, q = 0, e = 0;
+    int nt = 0;
+    for (int i = 0; i <= b; ++i) {
+      bool bad;
+      before += nt;
+      const int64_t L = checked_len(a, i, e, bad);
+      nt = tiles_of(L, e);
+      if (i < b) q += a.extend_lens ? max((int)a.extend_lens[i], 0) : 1;
+    }
+    if (nt == 0) return;
+    start = (int)q;
+    ext = (int)e;
+    su = before * sh.groups + (int64_t)u * nt;
+    eu = su + nt;
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!DEEP) {
+    const int c = blockIdx.x + 1;
+    const CutInfo ci = ws.cut[c];
+    const int64_t g = ws.cta_g[c], gn = ws.cta_g[c + 1];
+    if (gn == g || ci.t0 == 0) return;  // an empty range, or nothing cut here
+    su = g - ci.t0;
+    eu = su + ci.nt;
+    c0 = c - 1;
+    while (ws.cta_g[c0] == g) --c0;      // empty ranges before this one
+    if (ws.cta_g[c0] > su) return;       // not the first boundary inside the unit
+    u = ci.u;
+    start = ci.start;
+    ext = ci.ext;
+  }
   const int hsel = w / sh.team, member = w % sh.team;
-  const int row0 = ((ci.u % sh.passes) * sh.team + member) * kRows;
-  if (row0 >= ci.ext * G) return;
+  const int row0 = ((u % sh.passes) * sh.team + member) * kRows;
+  if (row0 >= ext * G) return;
+  for (int i = tid; i <= n; i += THREADS) s_g[i] = ws.cta_g[i];
+  __syncthreads();
+  if (DEEP) {  // the range that holds the unit's first tile
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (s_g[mid] <= su) lo = mid; else hi = mid - 1;
+    }
+    c0 = lo;
+    if (s_g[c0 + 1] >= eu) return;  // finished by that CTA
+  }
   // partial rows of the unit's pieces, one per range that is not empty: its first piece when the
   // range starts inside the unit (or with it), else its last
   if (tid < 32) {
@@ -892,7 +952,7 @@ __global__ void __launch_bounds__(256)
   // running merge of this group's pieces; a batch of pieces is requested before it is added
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   float M = -INFINITY, l = 0.f;
-  constexpr int kBatch = 4;
+  constexpr int kBatch = DEEP ? 8 : 4;
   for (int i0 = grp; i0 < np; i0 += kBatch * PG) {
     float2 ml[kBatch];
     float4 x[kBatch];
@@ -928,35 +988,38 @@ __global__ void __launch_bounds__(256)
       l = fmaf(f, ml[j].y, l);
     }
   }
-  if constexpr (PG > 1) {  // the groups meet: the maximum first
-    __shared__ float s_m[256];
-    s_m[tid] = M;
-    __syncthreads();
-    float mn = M;
-#pragma unroll
-    for (int p = 0; p < PG; ++p) mn = fmaxf(mn, s_m[p * RZ * kVec + tid % (RZ * kVec)]);
-    const float f = M == mn ? 1.f : ex2(M - mn);
-    red[tid][0] = o.x * f;
-    red[tid][1] = o.y * f;
-    red[tid][2] = o.z * f;
-    red[tid][3] = o.w * f;
-    red[tid][4] = l * f;
+  if constexpr (PG > 1) {  // the groups meet
+    red[tid][0] = o.x;
+    red[tid][1] = o.y;
+    red[tid][2] = o.z;
+    red[tid][3] = o.w;
+    red[tid][4] = l;
+    red[tid][5] = M;
     __syncthreads();
     if (grp > 0) return;
+    constexpr int kG = RZ * kVec;
+    float mn = M;
+#pragma unroll
+    for (int p = 1; p < PG; ++p) mn = fmaxf(mn, red[p * kG + tid][5]);
     float t[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int p = 0; p < PG; ++p)
+    for (int p = 0; p < PG; ++p) {
+      const float mp = red[p * kG + tid][5], f = mp == mn ? 1.f : ex2(mp - mn);
 #pragma unroll
-      for (int i = 0; i < 5; ++i) t[i] += red[p * RZ * kVec + tid][i];
+      for (int i = 0; i < 5; ++i) t[i] = fmaf(f, red[p * kG + tid][i], t[i]);
+    }
     o = make_float4(t[0], t[1], t[2], t[3]);
     l = t[4];
   }
   const int rr = row0 + r;
-  const int64_t tok = ci.start + rr / G;
-  if (rr < ci.ext * G && tok < a.num_tokens) {
-    const int hq = ((ci.u / sh.passes) * sh.hg + hsel) * G + rr % G;
+  const int64_t tok = start + rr / G;
+  if (rr < ext * G && tok < a.num_tokens) {
+    const int hq = ((u / sh.passes) * sh.hg + hsel) * G + rr % G;
     const float inv = (1.f / 128.f) / l;
-    put4<T>(a, tok, hq, 4 * v, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), rows_v8(a));
+    const bool v8 = rows_v8(a);
+    uint2 gw = make_uint2(0, 0);
+    if (a.gate_mode != TF_GATE_NONE) gw = gate4<T>(a, tok, hq, 4 * v, v8);
+    put4<T>(a, tok, hq, 4 * v, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), gw, v8);
   }
 }
 
@@ -999,20 +1062,21 @@ static cudaError_t launch_td(const tf_paged_attn_args& a, const tf_kv_scale& sc,
   rows_kernel<T, D><<<num_sms, kThreads, sh.smem, s>>>(a, sc, sh, ws);
   e = cudaGetLastError();
   if (e != cudaSuccess || num_sms == 1) return e;
-  // few units have many pieces each: a CTA per row, its groups of threads sharing the pieces
   constexpr int kWide = 256 / (D / 4) < kRows ? 256 / (D / 4) : kRows;
-  const bool deep = (int64_t)a.batch_size * sh.groups * 8 < num_sms;
+  const int64_t units = (int64_t)a.batch_size * sh.groups;
+  const bool deep = units * 8 < num_sms;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(num_sms - 1), (unsigned)(sh.hg * sh.team), (unsigned)(deep ? kRows : kRows / kWide));
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = deep ? dim3((unsigned)units, (unsigned)(sh.hg * sh.team), (unsigned)kRows)
+                     : dim3((unsigned)(num_sms - 1), (unsigned)(sh.hg * sh.team), (unsigned)(kRows / kWide));
+  cfg.blockDim = dim3(deep ? 4 * D : kWide * (D / 4));
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return deep ? cudaLaunchKernelEx(&cfg, combine_kernel<T, D, 1>, a, sh, ws)
-              : cudaLaunchKernelEx(&cfg, combine_kernel<T, D, kWide>, a, sh, ws);
+  return deep ? cudaLaunchKernelEx(&cfg, combine_kernel<T, D, 1, 4 * D, true>, a, sh, ws)
+              : cudaLaunchKernelEx(&cfg, combine_kernel<T, D, kWide, kWide * (D / 4), false>, a, sh, ws);
 }
 
 template <typename T>

@@ -1,10 +1,11 @@
 // Paged GQA extend over the 8-bit K/V pool on the 5th-generation tensor cores, for bf16 / fp16
-// activations at head_dim 128 and 256.  A dense contraction: 4 D flops per visible (query row, key).
+// activations at head_dim 64, 128 and 256.  A dense contraction: 4 D flops per visible (query row, key).
 //
 // Two CTAs of a cluster on an SM pair run one M=256 tile (128/G query tokens x G heads a CTA) with
 // tcgen05.mma.cta_group::2, as paged_extend_tc.cu does over 16-bit pools: CTA r holds query rows
 // [128 r, 128 r + 128) and of every 128-key tile keys [64 r, 64 r + 64) of K and dims [r D/2, (r+1) D/2)
-// of V; softmax warps own their CTA's rows, producer warps gather its halves, one thread of rank 0
+// of V (at D 64 both hold all 64 dims and the second copy's columns of O are ignored: a half of 32 dims
+// would need another tile layout, and the exponentials bound that size anyway); softmax warps own their CTA's rows, producer warps gather its halves, one thread of rank 0
 // issues the products.  What the 8-bit pool changes:
 //   producers   load 16 codes a lane, convert them to f16 (exact) and store them into the swizzled
 //               tile.  Four warps make the K slots and four the V slots, each with the next slot of its
@@ -241,7 +242,8 @@ struct Cfg {
   static constexpr int kQBytes = kKB * kQBlock;
   static constexpr int kKBlk = (kKeys / 2) * 128; // K half: 64 keys x 128 B per block
   static constexpr int kVBlk = kKeys * 128;       // V half: 128 keys x 128 B per block
-  static constexpr int kSlotBytes = kKB * kKBlk;  // == (kKB / 2) * kVBlk
+  static constexpr int kVD = D == 64 ? 64 : D / 2;  // dims of V that a CTA holds
+  static constexpr int kSlotBytes = D == 64 ? kVBlk : kKB * kKBlk;  // K halves and V halves alike
   static constexpr int kSlots = D == 256 ? 4 : 8;
   // Ring of the tiles' scales.  Those of tile t are written once V_{t-1} has been stored, for which
   // PV_{t-1-kSlots/2} had completed: the softmax of that tile is done with its scales, a later one's
@@ -263,7 +265,7 @@ struct Cfg {
   static constexpr int kColS = 0;                 // two S buffers of kKeys columns; P_j over S_j
   static constexpr int kColO = 2 * kKeys;
   static constexpr int kTmemCols = 512;
-  static_assert(kSlotBytes == (kKB / 2) * kVBlk, "K and V halves share the slot size");
+  static_assert(kSlotBytes >= kKB * kKBlk && kSlotBytes >= kVD / 64 * kVBlk, "K and V halves share the slot size");
   static_assert(kSmem <= 232448, "shared memory per CTA");
   static_assert(kColO + D <= kTmemCols, "TMEM columns");
   static_assert(4 * kRows * 4 <= kSlotBytes && kRows * D * 2 <= kQBytes, "epilogue staging");
@@ -467,11 +469,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     auto produce = [&](auto kind) {
       constexpr bool kV = decltype(kind)::value;
       constexpr int kRowsW = kV ? 32 : 16;             // rows of a tile that a warp makes
-      constexpr int CPR = kV ? D / 32 : D / 16;        // 16-byte pieces of a row of codes
+      constexpr int CPR = kV ? C::kVD / 16 : D / 16;        // 16-byte pieces of a row of codes
       constexpr int RPI = 32 / CPR, kLoads = kRowsW / RPI;
       constexpr int kBlkBytes = kV ? C::kVBlk : C::kKBlk;
       const int sub = lane / CPR, ch = lane - (lane / CPR) * CPR;
-      const char* src = kV ? (const char*)a.v_buffer + (int64_t)h * a.kv_stride_head + rank * (D / 2) + ch * 16
+      const char* src = kV ? (const char*)a.v_buffer + (int64_t)h * a.kv_stride_head + (D == 64 ? 0 : rank * (D / 2)) + ch * 16
                            : (const char*)a.k_buffer + (int64_t)h * a.kv_stride_head + ch * 16;
       const int row0 = (kV ? 32 * (pw - 4) : 16 * pw) + sub;
       const int lane0 = kV ? 0 : 16 * (pw & 1);        // the lane that knows the warp's first row
@@ -620,7 +622,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // ======================= MMA issue for the pair (rank 0, one thread) =======================
     if (lane == 0) {
       constexpr uint32_t kIdS = idesc_f16(2 * kRows, kKeys, false);
-      constexpr uint32_t kIdO = idesc_f16(2 * kRows, D, true);
+      constexpr uint32_t kIdO = idesc_f16(2 * kRows, 2 * C::kVD, true);
       bool ok = wait_bar<true>(q_full, 0, abort, peer_abort);
       tc::fence_proxy_async_smem();
       int slot = 0;
@@ -685,6 +687,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int wg = tid >> 7;
     const int ri = r / G;
     const bool row_valid = ri < n_tok;
+    const bool idle = (warp & 3) * 32 >= n_tok * G;  // no row of this warp is one of the request's
     const int64_t klim = P + cta_start + ri + 1;  // keys [0, klim) are visible to this row
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     constexpr int kOHalf = D / 2;  // O columns stored by this thread
@@ -704,6 +707,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int vis = rem <= 0 ? 0 : (rem >= kKeys ? kKeys : (int)rem);
       if (ok) ok = __all_sync(0xffffffffu, wait_bar<false>(&sc_full[si], (j / C::kScaleTiles) & 1, abort, peer_abort));
       if (ok) ok = __all_sync(0xffffffffu, wait_bar<false>(&s_full[wg], (j >> 1) & 1, abort, peer_abort));
+      if (idle) {  // P stays what S left there: it reaches only rows that are not stored
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0 && ok) {
+          mbar_arrive(&p_full[2 * wg]);
+          mbar_arrive(&p_full[2 * wg + 1]);
+        }
+        continue;
+      }
       float tmax = -INFINITY;
       const float4* grp = grp_s + si * 4;
       if (ok) {
@@ -928,51 +940,53 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ tf_p
   const int64_t step = a.num_tokens * (int64_t)a.num_q_heads;
   float M = -INFINITY;
   for (int z = 0; z < sp.n; ++z) M = fmaxf(M, mlp[2 * z * step]);
-  constexpr int V = D / 128;  // 16-byte pieces of a lane
-  float4 o[V];
+  constexpr int V = D / 32;  // values of a lane
+  float o[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < V; ++i) o[i] = 0.f;
   float l = 0.f;
   for (int z = 0; z < sp.n; ++z) {
     const float2 ml = *reinterpret_cast<const float2*>(mlp + 2 * z * step);
     if (ml.x == -INFINITY && ml.y == 0.f) continue;  // no keys there, and no O written
     const float f = ml.x == M ? 1.f : exp2f(ml.x - M);
     l = fmaf(f, ml.y, l);
+    const float2* x = reinterpret_cast<const float2*>(op + z * step * D + V * lane);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float4 x = *reinterpret_cast<const float4*>(op + z * step * D + 128 * i + 4 * lane);
-      o[i].x = fmaf(f, x.x, o[i].x);
-      o[i].y = fmaf(f, x.y, o[i].y);
-      o[i].z = fmaf(f, x.z, o[i].z);
-      o[i].w = fmaf(f, x.w, o[i].w);
+    for (int i = 0; i < V / 2; ++i) {
+      const float2 v = x[i];
+      o[2 * i] = fmaf(f, v.x, o[2 * i]);
+      o[2 * i + 1] = fmaf(f, v.y, o[2 * i + 1]);
     }
   }
   const float inv = 1.f / l;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const float x[4] = {o[i].x * inv, o[i].y * inv, o[i].z * inv, o[i].w * inv};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int d = 128 * i + 4 * lane + k;
-      float y = x[k];
-      if (a.gate_mode != TF_GATE_NONE)
-        y *= act(to_f(((const T*)a.gate)[t * a.gate_stride_tok + (int64_t)hq * a.gate_stride_head + d]), a.gate_mode);
-      ((T*)a.out)[t * a.out_stride_tok + (int64_t)hq * a.out_stride_head + d] = from_f<T>(y);
-    }
+    const int d = V * lane + i;
+    float y = o[i] * inv;
+    if (a.gate_mode != TF_GATE_NONE)
+      y *= act(to_f(((const T*)a.gate)[t * a.gate_stride_tok + (int64_t)hq * a.gate_stride_head + d]), a.gate_mode);
+    ((T*)a.out)[t * a.out_stride_tok + (int64_t)hq * a.out_stride_head + d] = from_f<T>(y);
   }
 }
 
-// Clusters that share a query tile's keys: enough to give every SM pair one, while each keeps at
-// least eight key tiles (a cluster's fixed cost, about 17 us, is that of eleven tiles).
+// Clusters that share a query tile's keys: the number with the shortest sequence of waves, a cluster
+// taking its share of the longest request's key tiles plus a fixed cost of about eight tiles (set-up,
+// first loads, epilogue).
 static int splits_of(const tf_paged_attn_args& a, int num_sms) {
-  const int G = a.num_q_heads / a.num_kv_heads;
-  const int64_t pairs = ((int64_t)a.max_extend_len * G + 2 * kRows - 1) / (2 * kRows);
-  const int64_t clusters = a.batch_size * pairs * a.num_kv_heads;
-  const int64_t slots = num_sms / 2;
-  int64_t n = clusters > 0 ? slots / clusters : 1;
-  const int64_t most = a.max_seq_len / (8 * kKeys);
-  n = n < most ? n : most;
-  return n < 1 ? 1 : (n > 32 ? 32 : (int)n);
+  const int TQ2 = 2 * (kRows / (a.num_q_heads / a.num_kv_heads));
+  const int64_t clusters = (int64_t)a.batch_size * ((a.max_extend_len + TQ2 - 1) / TQ2) * a.num_kv_heads;
+  const int64_t slots = num_sms / 2, tiles = (a.max_seq_len + kKeys - 1) / kKeys;
+  constexpr int64_t kFixed = 8;
+  int best = 1;
+  int64_t cost = INT64_MAX;
+  for (int n = 1; n <= 32 && (n == 1 || tiles / n >= 2); ++n) {
+    const int64_t c = (clusters * n + slots - 1) / slots * (kFixed + (tiles + n - 1) / n);
+    if (c < cost) {
+      cost = c;
+      best = n;
+    }
+  }
+  return best;
 }
 
 template <typename T, int D>
@@ -1002,7 +1016,7 @@ static cudaError_t launch_td(const tf_paged_attn_args& a, const tf_kv_scale& sc,
 
 bool paged_fp8_extend_supported(const tf_paged_attn_args& a) {
   if (a.dtype != TF_DTYPE_BF16 && a.dtype != TF_DTYPE_F16) return false;
-  if (a.head_dim != 128 && a.head_dim != 256) return false;
+  if (a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256) return false;
   const int G = a.num_q_heads / a.num_kv_heads;
   if (G < 1 || G > 16) return false;
   if (a.max_extend_len <= 0 || a.num_kv_heads > 65535) return false;
@@ -1023,6 +1037,9 @@ size_t paged_fp8_extend_workspace(const tf_paged_attn_args& a, int num_sms) {
 cudaError_t launch_paged_fp8_extend(const tf_paged_attn_args& a, const tf_kv_scale& sc, void* ws,
                                     int num_sms, cudaStream_t s) {
   const bool bf = a.dtype == TF_DTYPE_BF16;
+  if (a.head_dim == 64)
+    return bf ? ext8::launch_td<__nv_bfloat16, 64>(a, sc, ws, num_sms, s)
+              : ext8::launch_td<__half, 64>(a, sc, ws, num_sms, s);
   if (a.head_dim == 128)
     return bf ? ext8::launch_td<__nv_bfloat16, 128>(a, sc, ws, num_sms, s)
               : ext8::launch_td<__half, 128>(a, sc, ws, num_sms, s);

@@ -19,7 +19,8 @@
 //
 // Work.  A CTA has eight warps.  TEAM of them (a power of two) share stages of 32 tokens of one kv
 // head and take eight query rows each; HG kv heads of a group run side by side, so that a token's
-// rows of all heads, its scales and its slot id are read at about the same time; the
+// rows of all heads, its scales and its slot id are read at about the same time (the warps of a team fetch tiles in
+// turn); the
 // WH = 8 / (TEAM HG) teams of a head take its tiles in turn and merge in shared memory.  The sequence
 // of (request, head group) units, each of ceil(len / 32) tiles, is cut into one range per CTA,
 // balanced by tiles plus a fixed cost per unit; every CTA finds its own range from the lengths (a scan
@@ -460,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (tid == 0) {
     for (int i = 0; i < sh.stages; ++i) {
-      mbar_init(&bars[i], sh.team * 32);  // every lane's copies have landed
+      mbar_init(&bars[i], 32);  // the copies of every lane of the fetching warp have landed
       used[i] = 0;
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -483,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* full = bars;
   // tile q of head hsel of the group is number q hg + hsel of the ring
   const int step = sh.wh * sh.hg, first = wsel * sh.hg + hsel;
-  const int share = kTok / sh.team;  // tokens of a stage that this warp fetches
+  const int f_step = sh.wh * sh.team;  // tiles between the ones this warp fetches: a team's warps take turns
 
   const Requests rq{a, cache, bf, cn, NG};
   Walker prod;
@@ -499,16 +500,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   int64_t raw[kAhead];
   int head[kAhead];           // their kv heads
   int pf = 0, pf_unit = INT32_MIN;  // tiles of the unit whose entries have been asked for; its first tile
-  int pq = wsel - kAhead * sh.wh;  // next tile to fetch (below 0: the entries' own head start)
-  int p_st = first, p_round = 0;   // its stage and round
+  int pq = wsel + sh.wh * member - kAhead * f_step;  // next tile to fetch (before the first: the entries'
+  const int f_first = wsel + sh.wh * member;         // own head start)
+  int p_st = first + step * member, p_round = 0;     // its stage and round
   bool ok = true;
   auto issue = [&]() {
-    if (pq >= 0) {
+    if (pq >= f_first) {
       if (p_round > 0)
         ok = __all_sync(0xffffffffu, ok && wait_uses(&used[p_st], (uint32_t)(p_round * sh.team)));
       if (!ok) return;
       const uint32_t sp = ring + (uint32_t)(p_st * C::kStage);
-      const int64_t sl = resolve_slot(raw[0], a.num_slots, a.slot_mode, lane < share ? a.err : nullptr);
+      const int64_t sl = resolve_slot(raw[0], a.num_slots, a.slot_mode, a.err);
       // row offset of this lane's token in 16-byte pieces (32 bits: the host checks)
       const uint32_t off =
           (uint32_t)((sl * a.kv_stride_slot + (int64_t)head[0] * a.kv_stride_head) >> 4);
@@ -517,33 +519,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int sub = lane / CPR, ch = lane % CPR;
       const char* kg = (const char*)a.k_buffer + 16 * ch;
       const char* vg = (const char*)a.v_buffer + 16 * ch;
-      const uint32_t kd = sp + (member * share + sub) * C::kKS + 16 * ch;
-      const uint32_t vd = sp + C::kOffV + (member * share + sub) * C::kVS + 16 * ch;
-      auto rows = [&](int i0, auto n) {
-        constexpr int N = decltype(n)::value;
-        uint32_t o[N];
+      const uint32_t kd = sp + sub * C::kKS + 16 * ch;
+      const uint32_t vd = sp + C::kOffV + sub * C::kVS + 16 * ch;
 #pragma unroll
-        for (int i = 0; i < N; ++i) o[i] = __shfl_sync(0xffffffffu, off, i0 + i * RPI + sub);
+      for (int i0 = 0; i0 < kTok; i0 += 4 * RPI) {
+        uint32_t o[4];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
+        for (int i = 0; i < 4; ++i) o[i] = __shfl_sync(0xffffffffu, off, (i0 + i * RPI + sub) & 31);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (i0 + i * RPI >= kTok) break;
           cp_async16(kd + (i0 + i * RPI) * C::kKS, kg + (uint64_t)o[i] * 16);
           cp_async16(vd + (i0 + i * RPI) * C::kVS, vg + (uint64_t)o[i] * 16);
         }
-      };
-      if (sh.team == 1) {
-#pragma unroll
-        for (int i0 = 0; i0 < kTok; i0 += 4 * RPI) rows(i0, std::integral_constant<int, 4>());
-      } else {
-#pragma unroll 1
-        for (int i0 = 0; i0 < share; i0 += RPI) rows(i0, std::integral_constant<int, 1>());
       }
-      if (lane < share)
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(
-                         sp + C::kOffScale + (member * share + lane) * 8),
-                     "l"(sc.data + sl * sc.stride_slot + (int64_t)head[0] * sc.stride_head)
-                     : "memory");
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(sp + C::kOffScale + lane * 8),
+                   "l"(sc.data + sl * sc.stride_slot + (int64_t)head[0] * sc.stride_head)
+                   : "memory");
       cp_async_arrive_noinc(&full[p_st]);
-      p_st += step;
+      p_st += step * sh.team;
       if (p_st >= sh.stages) {
         p_st -= sh.stages;
         ++p_round;
@@ -554,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       raw[i] = raw[i + 1];
       head[i] = head[i + 1];
     }
-    const int fq = pq + kAhead * sh.wh;
+    const int fq = pq + kAhead * f_step;
     if (fq < ntiles) {
       prod.seek(rq, fq);
       // A load behind a saturated memory takes about the time that the ring lasts, more than the tile
@@ -570,11 +564,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           asm volatile("prefetch.global.L2 [%0];" ::"l"(a.req_to_token + (int64_t)prod.m.row * a.r2t_stride + pos));
         pf += 16;
       }
-      const int pos = min((fq - prod.unit_g) * kTok + member * share + lane, prod.m.len - 1);
+      const int pos = min((fq - prod.unit_g) * kTok + lane, prod.m.len - 1);
       raw[kAhead - 1] = a.req_to_token[(int64_t)prod.m.row * a.r2t_stride + pos];
       head[kAhead - 1] = (prod.u / sh.passes) * sh.hg + hsel;
     }
-    pq += sh.wh;
+    pq += f_step;
   };
 
   // Tile x of the ring may be fetched once x - stages has been consumed.  A team waits for that only
@@ -586,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int x_lim = sh.stages - 1;  // the last tile that may be fetched now
   float* epi = reinterpret_cast<float*>(smem + sh.ring + C::kFixed + 16 * sh.stages);
   int cq = wsel, st = first;  // this team's next tile of the range and its stage
-  uint32_t c_phase = 0;
+  int c_round = 0;
   for (int p0 = 0, p1; p0 < ntiles; p0 = p1) {  // pieces: tiles [p0, p1) of the range
     cons.seek(rq, p0);
     p1 = min(cons.unit_g + cons.nt(), ntiles);
@@ -680,7 +674,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (;;) {
       while (pq < ntiles && pq * sh.hg + hsel <= x_lim && ok) issue();
       if (cq >= p1) break;
-      ok = __all_sync(0xffffffffu, ok && mbar_wait(&full[st], c_phase));
+      // A warp that did not fetch this tile has not seen the stage's earlier round end: the parity below
+      // could be that of the round before it.
+      if (sh.team > 1 && c_round > 0)
+        ok = __all_sync(0xffffffffu, ok && wait_uses(&used[st], (uint32_t)(c_round * sh.team)));
+      ok = __all_sync(0xffffffffu, ok && mbar_wait(&full[st], c_round & 1));
       if (!ok) break;
       const uint32_t sp = ring + (uint32_t)(st * C::kStage);
       const unsigned char* stage = smem + st * C::kStage;
@@ -802,7 +800,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       st += step;
       if (st >= sh.stages) {
         st -= sh.stages;
-        c_phase ^= 1u;
+        ++c_round;
       }
     }
 

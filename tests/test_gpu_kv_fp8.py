@@ -424,6 +424,43 @@ def test_results_repeat():
     assert torch.equal(a, b)
 
 
+# many requests in one CTA's share, head groups above a tile's, batches above the plan's, and large
+# extends whose key blocks end at every place
+EDGES = {
+    # name: (dtype, hq, hkv, d, prefixes, new tokens, more)
+    "decode_many_tiny": ("bf16", 4, 2, 64, [i % 3 - 1 for i in range(20000)], [1] * 20000, {}),
+    "decode_beyond_the_plan": ("bf16", 2, 1, 64, [0] * 33000, [1] * 33000, {}),
+    "decode_gqa40": ("bf16", 40, 1, 128, [70, 3, 300], [1, 1, 1], dict(gate="sigmoid")),
+    "decode_gqa64": ("f16", 64, 1, 64, [70, 3, 300], [1, 1, 1], {}),
+    "decode_gqa1_h20": ("bf16", 20, 20, 128, [70, 3, 0], [1, 1, 1], {}),
+    "extend_many_tiny": ("bf16", 8, 2, 128, [i % 5 for i in range(6000)],
+                         [i % 4 for i in range(6000)], {}),
+    "extend_many_and_one_large": ("bf16", 8, 2, 64, [i % 5 for i in range(2000)],
+                                  [200 if i == 777 else i % 3 for i in range(2000)], {}),
+    "extend_gqa24": ("bf16", 24, 1, 128, [33], [40], {}),
+    "extend_gqa24_drafts": ("bf16", 24, 1, 128, [33, 250], [2, 1], dict(gate="silu")),
+    "extend_d64": ("bf16", 8, 2, 64, [500, 0], [301, 129], dict(gate="silu")),
+    "extend_d64_f16": ("f16", 16, 2, 64, [333, 1], [150, 257], {}),
+    "extend_split": ("bf16", 8, 1, 256, [3000, 0, 1], [70, 1, 200], dict(gate="sigmoid")),
+    "extend_split_f16": ("f16", 8, 1, 128, [2900, 0], [70, 1], {}),
+    "extend_gqa5": ("bf16", 10, 2, 256, [200, 14], [37, 90], {}),
+}
+
+
+@pytest.mark.parametrize("name", list(EDGES))
+def test_edges(name):
+    dtype, hq, hkv, d, pre, ext, more = EDGES[name]
+    c = Case(13, dtype, hq, hkv, d, pre, ext, **more)
+    check(c.run(), c.reference(), dtype, d, name)
+
+
+def test_more_than_64_query_heads_per_kv_head_are_refused():
+    from tokenfactory_b200 import _capi
+    for ext in (1, 2):
+        with pytest.raises(_capi.TFAttnError, match="64 query heads"):
+            Case(13, "bf16", 65, 1, 64, [70, 3], [ext, ext]).run()
+
+
 def test_refusals():
     from tokenfactory_b200 import _capi, ops
     c = Case(31, "bf16", 8, 2, 128, [30, 9], [1, 1])

@@ -138,3 +138,21 @@ def test_cpu_tensors_are_refused():
         ops.paged_extend_fp8(q, pool, pool, sc, i.view(1, 2), i, i, i, 0.125, 1, 1)
     with pytest.raises(ValueError, match="CUDA"):
         ops.attn_prologue_fp8(q, k, k, w, w, i, torch.ones(8), pool, pool, sc, i)
+
+
+def test_cache_pool_in_8_bits():
+    from tokenfactory_b200.hybrid_model import HybridCachePool, HybridConfig
+    cfg = HybridConfig(num_hidden_layers=8, num_key_value_heads=2, head_dim=64)
+    p = HybridCachePool(cfg, 10, 2, device="cpu", kv_dtype=torch.float8_e4m3fn)
+    k, v = p.get_full_kv_buffers(7)
+    sc = p.get_full_kv_scales(7)
+    assert k.shape == v.shape == (10, 2, 64) and k.dtype == v.dtype == torch.float8_e4m3fn
+    assert sc.shape == (10, 2, 2) and sc.dtype == torch.float32 and sc.is_contiguous()
+    assert v.data_ptr() - k.data_ptr() == 64 and k.stride() == v.stride() == (256, 128, 1)
+    assert sc.data_ptr() - p.get_full_kv_scales(3).data_ptr() == 10 * 2 * 2 * 4
+    plain = HybridCachePool(cfg, 10, 2, device="cpu")
+    assert plain.kv_scale is None and plain.get_full_kv_scales(3) is None
+    assert plain.k_buffer.dtype == plain.v_buffer.dtype == torch.bfloat16
+    assert plain.k_buffer.is_contiguous() and plain.v_buffer.is_contiguous()
+    with pytest.raises(TypeError):
+        HybridCachePool(cfg, 10, 2, device="cpu", kv_dtype=torch.float16)

@@ -30,8 +30,10 @@ from . import ops
 
 
 def _attend(q: torch.Tensor, k_buf: torch.Tensor, v_buf: torch.Tensor, batch, scaling: float,
-            gate: Optional[torch.Tensor], gate_mode: str) -> torch.Tensor:
-    """Dispatch of qwen3_8/full_attention.py:174-283 onto the kernels.
+            gate: Optional[torch.Tensor], gate_mode: str,
+            kv_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Dispatch of qwen3_8/full_attention.py:174-283 onto the kernels; with kv_scale given the buffers
+    are an 8-bit pool's codes and the calls are their _fp8 forms.
 
     bsz == 1   -> slots read with torch's wrap-around for negative entries (:188);
     all decode -> tf_paged_decode_attn (:232-242);
@@ -41,37 +43,49 @@ def _attend(q: torch.Tensor, k_buf: torch.Tensor, v_buf: torch.Tensor, batch, sc
     slot_mode = "wrap" if bsz == 1 else "clamp"
     max_seq = int(batch.max_seq_len) if batch.max_seq_len else int(batch.seq_lens.max().item())
     max_ext = int(batch.max_extend_len) if batch.max_extend_len else max(batch.extend_lens)
+    kw = dict(gate=gate, gate_mode=gate_mode if gate is not None else "none", slot_mode=slot_mode)
     if max_ext == 1:
+        if kv_scale is not None:
+            return ops.paged_decode_fp8(q, k_buf, v_buf, kv_scale, batch.req_to_token,
+                                        batch.req_pool_indices, batch.seq_lens, scaling, max_seq,
+                                        **kw)
         return ops.paged_decode(q, k_buf, v_buf, batch.req_to_token, batch.req_pool_indices,
-                                batch.seq_lens, scaling, max_seq, gate=gate,
-                                gate_mode=gate_mode if gate is not None else "none",
-                                slot_mode=slot_mode)
+                                batch.seq_lens, scaling, max_seq, **kw)
     ext = batch.extend_lens_tensor
     if ext is None:
         ext = torch.tensor(batch.extend_lens, dtype=torch.long, device=q.device)
+    if kv_scale is not None:
+        return ops.paged_extend_fp8(q, k_buf, v_buf, kv_scale, batch.req_to_token,
+                                    batch.req_pool_indices, batch.seq_lens, ext, scaling, max_seq,
+                                    max_ext, **kw)
     return ops.paged_extend(q, k_buf, v_buf, batch.req_to_token, batch.req_pool_indices,
-                            batch.seq_lens, ext, scaling, max_seq, max_ext, gate=gate,
-                            gate_mode=gate_mode if gate is not None else "none",
-                            slot_mode=slot_mode)
+                            batch.seq_lens, ext, scaling, max_seq, max_ext, **kw)
 
 
 def slot_based_attention(q: torch.Tensor, layer_k_buffer: torch.Tensor,
-                         layer_v_buffer: torch.Tensor, batch, scaling: float) -> torch.Tensor:
+                         layer_v_buffer: torch.Tensor, batch, scaling: float,
+                         kv_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Same inputs and output as Qwen3_8FullAttention._slot_based_attention
-    (qwen3_8/full_attention.py:163-283): q [T, Hq, D] -> attention output [T, Hq, D]."""
-    return _attend(q, layer_k_buffer, layer_v_buffer, batch, scaling, None, "none")
+    (qwen3_8/full_attention.py:163-283): q [T, Hq, D] -> attention output [T, Hq, D].  kv_scale: the
+    layer's scales when the buffers are those of an 8-bit pool."""
+    return _attend(q, layer_k_buffer, layer_v_buffer, batch, scaling, None, "none", kv_scale)
 
 
 def full_attention_core(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                         gate: Optional[torch.Tensor], layer_k_buffer: torch.Tensor,
                         layer_v_buffer: torch.Tensor, batch, scaling: float,
-                        gate_mode: str = "silu") -> torch.Tensor:
+                        gate_mode: str = "silu",
+                        kv_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Pool write + attention + output gate: qwen3_8/full_attention.py:146-158.
 
-    q [T, Hq, D] (normed, rotated), k/v [T, Hkv, D], gate [T, Hq, D] view or None.
-    Returns [T, Hq*D] ready for o_proj."""
-    ops.kv_store(layer_k_buffer, layer_v_buffer, batch.out_cache_loc, k, v)
-    out = _attend(q, layer_k_buffer, layer_v_buffer, batch, scaling, gate, gate_mode)
+    q [T, Hq, D] (normed, rotated), k/v [T, Hkv, D], gate [T, Hq, D] view or None; kv_scale: the
+    layer's scales when the buffers are those of an 8-bit pool.  Returns [T, Hq*D] ready for
+    o_proj."""
+    if kv_scale is not None:
+        ops.kv_store_fp8(layer_k_buffer, layer_v_buffer, kv_scale, batch.out_cache_loc, k, v)
+    else:
+        ops.kv_store(layer_k_buffer, layer_v_buffer, batch.out_cache_loc, k, v)
+    out = _attend(q, layer_k_buffer, layer_v_buffer, batch, scaling, gate, gate_mode, kv_scale)
     return out.reshape(q.shape[0], q.shape[1] * q.shape[2])
 
 
@@ -130,16 +144,24 @@ def _prologue_fusable(layer, q: torch.Tensor, positions: torch.Tensor) -> bool:
     return qn.weight.dtype in (q.dtype, torch.float32) and qn.weight.dtype == kn.weight.dtype
 
 
+def _pool_scales(cache_pool, layer_idx: int) -> Optional[torch.Tensor]:
+    """The layer's K/V scales when the pool is held in 8 bits (it has get_full_kv_scales), else None."""
+    get = getattr(cache_pool, "get_full_kv_scales", None)
+    return get(layer_idx) if get is not None else None
+
+
 class FullAttentionHotPath:
-    """Overrides Qwen3_8FullAttention.forward / _slot_based_attention.
+    """Overrides Qwen3_8FullAttention.forward / _slot_based_attention.  A cache pool whose
+    ``get_full_kv_scales(layer_idx)`` returns scales is one of float8_e4m3fn rows: k and v are
+    quantized as they are stored, and attention reads the codes.
 
     ``output_gate_mode`` selects the gate activation: "silu" is the reference line
     (qwen3_8/full_attention.py:157-158); "sigmoid" is the gate of the Qwen3-Next checkpoints."""
 
     output_gate_mode = "silu"
 
-    def _slot_based_attention(self, q, layer_k_buffer, layer_v_buffer, batch):
-        return slot_based_attention(q, layer_k_buffer, layer_v_buffer, batch, self.scaling)
+    def _slot_based_attention(self, q, layer_k_buffer, layer_v_buffer, batch, kv_scale=None):
+        return slot_based_attention(q, layer_k_buffer, layer_v_buffer, batch, self.scaling, kv_scale)
 
     def forward(self, hidden_states, positions, cache_pool, forward_batch):
         num_tokens = hidden_states.shape[0]
@@ -153,23 +175,27 @@ class FullAttentionHotPath:
         k = self.k_proj(hidden_states).view(num_tokens, self.num_kv_heads, d)
         v = self.v_proj(hidden_states).view(num_tokens, self.num_kv_heads, d)
         layer_k_buffer, layer_v_buffer = cache_pool.get_full_kv_buffers(self.layer_idx)
+        kv_scale = _pool_scales(cache_pool, self.layer_idx)
         if _prologue_fusable(self, q, positions):
             # q/k RMSNorm + partial RoPE + pool write in one pass (:142-149)
             rot = self.rotary_emb
-            q = ops.attn_prologue(q, k, v, self.q_norm.weight, self.k_norm.weight, positions,
-                                  rot.inv_freq, layer_k_buffer, layer_v_buffer,
-                                  forward_batch.out_cache_loc, eps=self.q_norm.eps,
-                                  mrope_section=tuple(rot.mrope_section),
-                                  mrope_interleaved=rot.mrope_interleaved)
+            kw = dict(eps=self.q_norm.eps, mrope_section=tuple(rot.mrope_section),
+                      mrope_interleaved=rot.mrope_interleaved)
+            rows = (q, k, v, self.q_norm.weight, self.k_norm.weight, positions, rot.inv_freq,
+                    layer_k_buffer, layer_v_buffer)
+            if kv_scale is not None:
+                q = ops.attn_prologue_fp8(*rows, kv_scale, forward_batch.out_cache_loc, **kw)
+            else:
+                q = ops.attn_prologue(*rows, forward_batch.out_cache_loc, **kw)
             out = _attend(q, layer_k_buffer, layer_v_buffer, forward_batch, self.scaling, gate,
-                          self.output_gate_mode).reshape(num_tokens, self.num_heads * d)
+                          self.output_gate_mode, kv_scale).reshape(num_tokens, self.num_heads * d)
             return self.o_proj(out)
         q = self.q_norm(q)
         k = self.k_norm(k)
         q, k = self.rotary_emb(q, k, positions)
         out = full_attention_core(q.contiguous(), k, v.contiguous(), gate, layer_k_buffer,
                                   layer_v_buffer, forward_batch, self.scaling,
-                                  self.output_gate_mode)
+                                  self.output_gate_mode, kv_scale)
         return self.o_proj(out)
 
 

@@ -14,7 +14,7 @@ same pieces so that whole decode/extend steps can run through the kernels:
 * ``HybridCachePool``: the K/V pool and the GDN state pool in the reference's layouts
   (k_buffer [n_full, slots, Hkv, D]; conv_state [n_lin, slots, conv_dim, K-1];
   ssm_state [n_lin, slots, Hv, dk, dv] fp32) with ``get_full_kv_buffers`` /
-  ``get_linear_states``.
+  ``get_linear_states``; K and V optionally in 8 bits (``kv_dtype``).
 
 Tensor parallelism follows the reference's Megatron split: attention heads as in ``layers``,
 gate/up projections by output rows, down projection by input columns, one all-reduce after each
@@ -184,10 +184,18 @@ class HybridForCausalLM(nn.Module):
 class HybridCachePool:
     """K/V and GDN state pools of one rank in the reference's layouts
     (qwen3_8/hybrid_cache_pool.py:14-113, req_to_state_pool.py:34-108).  GDN state slots
-    [0, max_reqs) are the working zone, [max_reqs, max_reqs + max_snapshots) the snapshots."""
+    [0, max_reqs) are the working zone, [max_reqs, max_reqs + max_snapshots) the snapshots.
+
+    kv_dtype=torch.float8_e4m3fn holds K and V in 8 bits: k_buffer / v_buffer are then code views of
+    one tensor in which a head's K and V rows of a slot are adjacent (attention reads both), and
+    kv_scale [n_full, slots, Hkv, 2] float32 their scales.  A slot costs Hkv * (2 D + 8) bytes a layer
+    instead of Hkv * 4 D in 16 bits."""
 
     def __init__(self, config: HybridConfig, max_total_tokens: int, max_reqs: int,
-                 max_snapshots: int = 0, dtype=torch.bfloat16, device="cuda"):
+                 max_snapshots: int = 0, dtype=torch.bfloat16, device="cuda",
+                 kv_dtype: Optional[torch.dtype] = None):
+        if kv_dtype not in (None, dtype, torch.float8_e4m3fn):
+            raise TypeError(f"kv_dtype must be {dtype} or float8_e4m3fn (got {kv_dtype})")
         types = config.layer_types
         self.full_layers = [i for i, t in enumerate(types) if t == "full_attention"]
         self.linear_layers = [i for i, t in enumerate(types) if t == "linear_attention"]
@@ -196,9 +204,15 @@ class HybridCachePool:
         tp = config.tp_size
         hkv = max(1, config.num_key_value_heads // tp)
         d = config.head_dim
-        self.k_buffer = torch.zeros((len(self.full_layers), max_total_tokens, hkv, d), dtype=dtype,
-                                    device=device)
-        self.v_buffer = torch.zeros_like(self.k_buffer)
+        shape = (len(self.full_layers), max_total_tokens, hkv)
+        self.kv_scale = None
+        if kv_dtype == torch.float8_e4m3fn:
+            codes = torch.zeros((*shape, 2, d), dtype=torch.uint8, device=device).view(kv_dtype)
+            self.k_buffer, self.v_buffer = codes[..., 0, :], codes[..., 1, :]
+            self.kv_scale = torch.zeros((*shape, 2), dtype=torch.float32, device=device)
+        else:
+            self.k_buffer = torch.zeros((*shape, d), dtype=dtype, device=device)
+            self.v_buffer = torch.zeros_like(self.k_buffer)
         nk = config.linear_num_key_heads // tp
         nv = config.linear_num_value_heads // tp
         dk, dv = config.linear_key_head_dim, config.linear_value_head_dim
@@ -213,6 +227,10 @@ class HybridCachePool:
     def get_full_kv_buffers(self, layer_idx: int):
         j = self.full_map[layer_idx]
         return self.k_buffer[j], self.v_buffer[j]
+
+    def get_full_kv_scales(self, layer_idx: int) -> Optional[torch.Tensor]:
+        """The layer's (K, V) scales [slots, Hkv, 2] of an 8-bit pool, else None."""
+        return None if self.kv_scale is None else self.kv_scale[self.full_map[layer_idx]]
 
     def get_linear_states(self, layer_idx: int):
         j = self.linear_map[layer_idx]

@@ -40,18 +40,21 @@ namespace rows8 {
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kTok = 32;  // tokens of a tile
-constexpr int kRows = 8;  // query rows of a warp (n of the mma tiles)
 constexpr int kCache = 96;  // requests whose metadata a CTA keeps in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxCtas = 256;
-constexpr int kMaxBatch = 32768;  // the batch scan lives in the ring's shared memory
+constexpr int kMaxBatch = 32768;  // passes of all requests: their scan lives in the ring's shared memory
 
+// One pass over a request's tokens for the query rows that a team holds; a request has as many passes
+// as the longest one needs, those behind its own rows without tiles.
 struct ReqMeta {
-  int32_t len, ext, row, start;  // tokens, new tokens, req_to_token row, first query token
+  int32_t len, ext, row, start, nt;  // tokens, new tokens, req_to_token row, first query token, tiles
 };
 
-template <int D>
+// NT: 8-row tiles of a warp
+template <int D, int NT>
 struct Cfg {
+  static constexpr int kRows = 8 * NT;  // query rows of a warp
   // row strides in shared memory: 64 mod 128 bytes for the 16-byte fragment reads of K (two rows a
   // phase), an odd multiple of 16 for the 8-row matrices of V
   static constexpr int kKS = D % 128 == 0 ? D + 64 : D;
@@ -60,10 +63,12 @@ struct Cfg {
   static constexpr int kOffScale = kOffV + kTok * kVS;
   static constexpr int kStage = kOffScale + kTok * 8;
   static constexpr int kStages = D == 256 ? 12 : (D == 128 ? 20 : 40);  // at most
-  // epilogue: 64 dims of every warp's rows, then per row what it is multiplied by, (M, l), and its
-  // place in the output
+  // epilogue: 64 dims of each warp's rows (the place of its Q fragments, with two row tiles), then per
+  // row what it is multiplied by, (M, l), and its place in the output
   static constexpr int kEpiStride = 64 + 4;  // floats per row
-  static constexpr int kEpi = kWarps * kRows * (kEpiStride + 5) * 4;
+  static constexpr int kEpiRows = kRows * kEpiStride * 4, kQ = NT > 1 ? kRows * D * 2 : 0;
+  static constexpr int kEpiWarp = kEpiRows > kQ ? kEpiRows : kQ;  // bytes of a warp
+  static constexpr int kEpi = kWarps * (kEpiWarp + kRows * 5 * 4);
   static constexpr int kFixed = kCache * (int)sizeof(ReqMeta) + 64;
   static_assert(kStage % 16 == 0 && kKS % 16 == 0 && kVS % 16 == 0, "bulk copy alignment");
 };
@@ -71,8 +76,9 @@ struct Cfg {
 // What a launch is divided by; computed on the host.
 struct Shape {
   int team, hg, wh;   // warps sharing a ring, kv heads side by side, teams taking a head's tiles in turn
-  int groups;         // units per request
-  int passes;         // row passes of a kv head (more than 8 * team query rows)
+  int groups;         // units of a pass: head groups
+  int passes;         // passes of a request (more query rows than a team holds)
+  int row_tiles;      // 8-row tiles of a warp
   int stages;         // ring stages
   int nctas;
   int min_tiles;      // tiles worth a CTA of their own
@@ -82,18 +88,18 @@ struct Shape {
 
 // The unit that a CTA's range starts in, for the combine kernel.
 struct CutInfo {
-  int b, u, start, ext, nt, t0;
+  int pass, u, start, ext, nt, t0;
 };
 
 struct Ws {
   int64_t* cta_g;  // [nctas + 1] first tile of each CTA's range
   CutInfo* cut;    // [nctas]
-  float* ml;       // [2 nctas][8 warps][8 rows][2]
-  float* o;        // [2 nctas][8 warps][8 rows][D]
+  float* ml;       // [2 nctas][8 warps][rows][2]
+  float* o;        // [2 nctas][8 warps][rows][D]
 };
 
 __host__ __device__ inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
-__host__ __device__ inline Ws carve(void* base, int nctas, int D) {
+__host__ __device__ inline Ws carve(void* base, int nctas, int rows) {
   char* p = (char*)base;
   Ws w;
   w.cta_g = (int64_t*)p;
@@ -101,14 +107,14 @@ __host__ __device__ inline Ws carve(void* base, int nctas, int D) {
   w.cut = (CutInfo*)p;
   p += align256((size_t)nctas * sizeof(CutInfo));
   w.ml = (float*)p;
-  p += align256((size_t)2 * nctas * kWarps * kRows * 2 * 4);
+  p += align256((size_t)2 * nctas * kWarps * rows * 2 * 4);
   w.o = (float*)p;
   return w;
 }
-inline size_t ws_bytes(int nctas, int D) {
+inline size_t ws_bytes(int nctas, int rows, int D) {
   return align256((size_t)(nctas + 1) * 8) + align256((size_t)nctas * sizeof(CutInfo)) +
-         align256((size_t)2 * nctas * kWarps * kRows * 2 * 4) +
-         (size_t)2 * nctas * kWarps * kRows * D * 4;
+         align256((size_t)2 * nctas * kWarps * rows * 2 * 4) +
+         (size_t)2 * nctas * kWarps * rows * D * 4;
 }
 
 __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -181,24 +187,28 @@ __device__ __forceinline__ int64_t checked_len(const tf_paged_attn_args& a, int 
   }
   return L;
 }
-__device__ __forceinline__ int tiles_of(int64_t L, int64_t ext) {
-  return ext > 0 ? (int)((L + kTok - 1) / kTok) : 0;
+// tiles of pass p: those of the request when it has rows there
+__device__ __forceinline__ int tiles_of(int64_t L, int64_t ext, int p, const Shape& sh, int G) {
+  return ext * G > (int64_t)p * sh.team * sh.row_tiles * 8 ? (int)((L + kTok - 1) / kTok) : 0;
 }
 
-// The requests a walk can be at: the first kCache of the range from shared memory, further ones from
-// global memory as the walk reaches them.
+// The passes a walk can be at (pass b % passes of request b / passes): the first kCache of the range
+// from shared memory, further ones from global memory as the walk reaches them.
 struct Requests {
   const tf_paged_attn_args& a;
+  const Shape& sh;
   const ReqMeta* cache;
-  int b0, n, groups;
+  int b0, n, G;
   __device__ __forceinline__ ReqMeta at(int b, int start) const {
     if (b - b0 < n) return cache[b - b0];
+    const int i = b / sh.passes;
     int64_t ext;
     bool bad;
     ReqMeta m;
-    m.len = (int32_t)checked_len(a, b, ext, bad);
+    m.len = (int32_t)checked_len(a, i, ext, bad);
     m.ext = (int32_t)ext;
-    const int64_t r = a.req_pool_indices[b];
+    m.nt = tiles_of(m.len, ext, b - i * sh.passes, sh, G);
+    const int64_t r = a.req_pool_indices[i];
     if (r < 0 || r >= a.r2t_rows) record_err(a.err, TF_KERR_REQ_RANGE);
     m.row = r < 0 || r >= a.r2t_rows ? 0 : (int32_t)r;
     m.start = start;
@@ -208,17 +218,19 @@ struct Requests {
 
 // The units of a CTA's range in order; tiles are counted from the range's first.
 struct Walker {
-  int b, u;     // request and group
+  int b, u;     // pass and group
   int unit_g;   // first tile of unit (b, u)
   ReqMeta m;
-  __device__ __forceinline__ int nt() const { return tiles_of(m.len, m.ext); }
+  __device__ __forceinline__ int nt() const { return m.nt; }
   // the unit that holds tile q (of the current unit or a later one)
   __device__ __forceinline__ void seek(const Requests& rq, int q) {
     while (q >= unit_g + nt()) {
       unit_g += nt();
-      if (++u == rq.groups) {
+      if (++u == rq.sh.groups) {
         u = 0;
-        const int before = rq.a.extend_lens && b + 1 - rq.b0 >= rq.n ? max((int)rq.a.extend_lens[b], 0) : 1;
+        int before = 0;  // query tokens between the two passes (the cache knows them)
+        if (b + 1 - rq.b0 >= rq.n && (b + 1) % rq.sh.passes == 0)
+          before = rq.a.extend_lens ? max((int)rq.a.extend_lens[b / rq.sh.passes], 0) : 1;
         ++b;
         m = rq.at(b, m.start + before);
       }
@@ -268,12 +280,13 @@ __device__ __forceinline__ bool rows_v8(const tf_paged_attn_args& a) {
 // the result is normalised and put out, or left as partials.  One copy of this code serves all
 // pieces and dims: unrolled into the kernel it ran once a piece from a cold instruction cache
 // (15-35 us a piece were measured).
-template <typename T, int D>
+template <typename T, int D, int NT>
 __device__ __noinline__ void finish64(const tf_paged_attn_args& a, const Shape& sh, const Ws& ws,
                                       const float* epi, int slot, bool whole, int d0) {
-  constexpr int kS = Cfg<D>::kEpiStride;
+  using C = Cfg<D, NT>;
+  constexpr int kRows = C::kRows, kS = C::kEpiStride;
   constexpr int kTwo = 2;  // items of a thread whose gate values are requested together
-  const float* fac = epi + kWarps * kRows * kS;         // [warp][row] what the warp's row counts
+  const float* fac = epi + kWarps * C::kEpiWarp / 4;    // [warp][row] what the warp's row counts
   const float* ml = fac + kWarps * kRows;               // [warp][row][2]; the first team's: merged
   const int2* to = reinterpret_cast<const int2*>(ml + 2 * kWarps * kRows);  // [place][row] token (or -1), head
   const int per = sh.hg * sh.team;
@@ -301,7 +314,8 @@ __device__ __noinline__ void finish64(const tf_paged_attn_args& a, const Shape& 
 #pragma unroll 1
       for (int w = pr; w < kWarps * kRows; w += per * kRows) {
         const float f = fac[w];
-        const float4 x = *reinterpret_cast<const float4*>(epi + w * kS + 4 * v);
+        const float4 x = *reinterpret_cast<const float4*>(epi + (w / kRows) * (C::kEpiWarp / 4) +
+                                                          (w % kRows) * kS + 4 * v);
         o.x = fmaf(f, x.x, o.x);
         o.y = fmaf(f, x.y, o.y);
         o.z = fmaf(f, x.z, o.z);
@@ -319,17 +333,18 @@ __device__ __noinline__ void finish64(const tf_paged_attn_args& a, const Shape& 
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kThreads, 1)
     rows_kernel(const __grid_constant__ tf_paged_attn_args a, const __grid_constant__ tf_kv_scale sc,
                 const __grid_constant__ Shape sh, const __grid_constant__ Ws ws) {
-  using C = Cfg<D>;
+  using C = Cfg<D, NT>;
+  constexpr int kRows = C::kRows;
   constexpr int NJ = D / 64;   // 16-byte reads of a K row per thread
   constexpr int NM = D / 16;   // dim tiles of O
   extern __shared__ __align__(128) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gq = lane >> 2, tq = lane & 3;
-  const int B = a.batch_size;
+  const int P = sh.passes, B = a.batch_size * P;  // passes over all requests
   const int G = a.num_q_heads / a.num_kv_heads;
   const int c = blockIdx.x;
 
@@ -341,13 +356,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   // the combine kernel's CTAs may take their places now; they wait for this grid
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // ---- this CTA's range: ts[b] = first tile of request b (all groups of a request are adjacent)
+  // ---- this CTA's range: ts[b] = first tile of pass b (all groups of a pass are adjacent)
   int* ts = reinterpret_cast<int*>(smem);  // in the ring's space, before its first copy
   const int plan_per = (B + kThreads - 1) / kThreads;
   const int plan_lo = min(tid * plan_per, B), plan_hi = min(plan_lo + plan_per, B);
-  ReqMeta mine_m = {0, 0, 0, 0};  // of request plan_lo when every thread has at most one
+  ReqMeta mine_m = {0, 0, 0, 0, 0};  // of pass plan_lo when every thread has at most one
   if (plan_per == 1 && plan_lo < B) {
-    const int64_t r = a.req_pool_indices[plan_lo];
+    const int64_t r = a.req_pool_indices[plan_lo / P];
     mine_m.row = r < 0 || r >= a.r2t_rows ? -1 : (int32_t)r;
   }
   {
@@ -356,12 +371,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int b = lo; b < hi; ++b) {
       int64_t ext;
       bool bad;
-      const int64_t L = checked_len(a, b, ext, bad);
+      const int64_t L = checked_len(a, b / P, ext, bad);
       if (bad && c == 0) record_err(a.err, TF_KERR_SLOT_RANGE);
       mine_m.len = (int32_t)L;
       mine_m.ext = (int32_t)ext;
+      mine_m.nt = tiles_of(L, ext, b % P, sh, G);
       ts[b] = sum;
-      sum += tiles_of(L, ext);
+      sum += mine_m.nt;
     }
     int incl = sum;
 #pragma unroll
@@ -383,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int nctas = want < gridDim.x ? (int)want : (int)gridDim.x;
   const int64_t beta = sh.piece_cost;
   // A range begins at cost position x = cc (total + beta units) / nctas: a unit's first beta of cost is
-  // fixed.  The request holding x lies with one thread; the range's first request with another.
+  // fixed.  The pass holding x lies with one thread; the range's first pass with another.
   const int64_t U = (int64_t)B * NG;
   int64_t* sh_g = reinterpret_cast<int64_t*>(sh_i + 8);  // g0, g1
   int* sh_b = sh_i + 12;
@@ -410,8 +426,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   // requests without keys: softmax over nothing is NaN
   if (a.extend_lens == nullptr) {
-    for (int b = c; b < B; b += gridDim.x) {
-      if (ts[b + 1] != ts[b]) continue;
+    for (int b = c; b < a.batch_size; b += gridDim.x) {
+      if (ts[b * P + 1] != ts[b * P]) continue;
       for (int e = tid; e < a.num_q_heads * D; e += kThreads)
         ((T*)a.out)[(int64_t)b * a.out_stride_tok + (int64_t)(e / D) * a.out_stride_head + e % D] =
             from_f<T>(NAN);
@@ -419,17 +435,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (g0 >= g1) return;
 #pragma unroll 1
-  for (int b = plan_lo; b < plan_hi; ++b)  // the range's first request: ts[b] NG <= g0 < ts[b + 1] NG
+  for (int b = plan_lo; b < plan_hi; ++b)  // the range's first pass: ts[b] NG <= g0 < ts[b + 1] NG
     if ((int64_t)ts[b] * NG <= g0 && g0 < (int64_t)ts[b + 1] * NG) *sh_b = b;
   __syncthreads();
   const int bf = *sh_b;
   const int cn = min(kCache, B - bf);
   const int64_t bf_g = (int64_t)ts[bf] * NG;
   const int bf_nt = ts[bf + 1] - ts[bf];
-  int q_before = bf;  // query tokens before request bf
+  int q_before = bf / P;  // query tokens before that request
   if (a.extend_lens != nullptr) {
     int s = 0;
-    for (int b = tid; b < bf; b += kThreads) s += max((int)a.extend_lens[b], 0);
+    for (int b = tid; b < bf / P; b += kThreads) s += max((int)a.extend_lens[b], 0);
     s = __reduce_add_sync(0xffffffffu, s);
     __syncthreads();
     if (lane == 0) sh_i[warp] = s;
@@ -443,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         record_err(a.err, TF_KERR_REQ_RANGE);
         mine_m.row = 0;
       }
-      mine_m.start = plan_lo;
+      mine_m.start = plan_lo / P;
       cache[plan_lo - bf] = mine_m;
     }
   } else for (int i = tid; i < cn; i += kThreads) {
@@ -451,12 +467,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     int64_t ext;
     bool bad;
     ReqMeta m;
-    m.len = (int32_t)checked_len(a, b, ext, bad);
+    m.len = (int32_t)checked_len(a, b / P, ext, bad);
     m.ext = (int32_t)ext;
-    const int64_t r = a.req_pool_indices[b];
+    m.nt = tiles_of(m.len, ext, b % P, sh, G);
+    const int64_t r = a.req_pool_indices[b / P];
     if (r < 0 || r >= a.r2t_rows) record_err(a.err, TF_KERR_REQ_RANGE);
     m.row = r < 0 || r >= a.r2t_rows ? 0 : (int32_t)r;
-    m.start = b;
+    m.start = b / P;
     cache[i] = m;
   }
   if (tid == 0) {
@@ -471,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int s = q_before;
     for (int i = 0; i < cn; ++i) {
       cache[i].start = s;
-      s += max((int)a.extend_lens[bf + i], 0);
+      if ((bf + i + 1) % P == 0) s += max((int)a.extend_lens[(bf + i) / P], 0);
     }
   }
   __syncthreads();
@@ -486,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int step = sh.wh * sh.hg, first = wsel * sh.hg + hsel;
   const int f_step = sh.wh * sh.team;  // tiles between the ones this warp fetches: a team's warps take turns
 
-  const Requests rq{a, cache, bf, cn, NG};
+  const Requests rq{a, sh, cache, bf, cn, G};
   Walker prod;
   prod.b = bf;
   prod.u = (int)((g0 - bf_g) / bf_nt);
@@ -566,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const int pos = min((fq - prod.unit_g) * kTok + lane, prod.m.len - 1);
       raw[kAhead - 1] = a.req_to_token[(int64_t)prod.m.row * a.r2t_stride + pos];
-      head[kAhead - 1] = (prod.u / sh.passes) * sh.hg + hsel;
+      head[kAhead - 1] = prod.u * sh.hg + hsel;
     }
     pq += f_step;
   };
@@ -575,8 +592,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   // when x - stages is not behind its own current tile in the sequence: whoever has to consume it
   // is then not held up by this team (nor by the barriers at the end of a piece), and as a team's
   // own tiles are at most a ring apart (step <= stages) its next tile is always on its way.  `lag`
-  // tiles of slack keep a team from waiting for the slowest warp of the very tile it has just left.
-  const int lag = min(3, sh.stages - step);
+  // tiles of slack keep a team from waiting for the slowest warp of the very tile it has just left,
+  // where the ring has them beside a tile to work on and one on its way for each team.
+  const int lag = min(3, sh.stages >= 2 * step ? sh.stages - 2 * step : sh.stages - step);
   int x_lim = sh.stages - 1;  // the last tile that may be fetched now
   float* epi = reinterpret_cast<float*>(smem + sh.ring + C::kFixed + 16 * sh.stages);
   int cq = wsel, st = first;  // this team's next tile of the range and its stage
@@ -585,11 +603,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     cons.seek(rq, p0);
     p1 = min(cons.unit_g + cons.nt(), ntiles);
     if (p0 == 0 && tid == 0)
-      ws.cut[c] = CutInfo{cons.b, cons.u, cons.m.start, cons.m.ext, cons.nt(), -cons.unit_g};
-    const int u = cons.u, L = cons.m.len, E = cons.m.ext;
-    const int kvh = (u / sh.passes) * sh.hg + hsel;
-    const int row0 = ((u % sh.passes) * sh.team + member) * kRows;  // first of this warp's rows
-    const int nrows = E * G - row0;                                 // valid ones (may be <= 0)
+      ws.cut[c] = CutInfo{cons.b % P, cons.u, cons.m.start, cons.m.ext, cons.nt(), -cons.unit_g};
+    const int u = cons.u, L = cons.m.len, E = cons.m.ext, pass = cons.b % P;
+    const int kvh = u * sh.hg + hsel;
+    const int row0 = (pass * sh.team + member) * kRows;  // first of this warp's rows
+    const int nrows = E * G - row0;                      // valid ones (may be <= 0)
     const int64_t qtok0 = cons.m.start;
 
     // the gate rows of the piece are wanted at its end: into L2 now, 128 bytes a thread (a load under
@@ -599,21 +617,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int per = sh.hg * sh.team;
       for (int e = tid; e < per * kRows * kLines; e += kThreads) {
         const int r = (e / kLines) % kRows, place = e / kLines / kRows;
-        const int row = ((u % sh.passes) * sh.team + place % sh.team) * kRows + r;
+        const int row = (pass * sh.team + place % sh.team) * kRows + r;
         const int64_t tok = qtok0 + row / G;
         if (row < E * G && tok < a.num_tokens)
           asm volatile("prefetch.global.L2 [%0];" ::"l"(
               (const T*)a.gate + tok * a.gate_stride_tok +
-              (int64_t)(((u / sh.passes) * sh.hg + place / sh.team) * G + row % G) * a.gate_stride_head +
+              (int64_t)((u * sh.hg + place / sh.team) * G + row % G) * a.gate_stride_head +
               (e % kLines) * 64));
       }
     }
-    // ---- Q: row gq of this warp, dims 64 j + 16 tq + [0, 16), scaled into f16's range
-    uint32_t qf[NJ][8];
-    float c2[2];
-    {
-      const int r = row0 + gq;
-      const bool valid = gq < nrows && qtok0 + r / G < a.num_tokens;
+    // ---- Q: rows gq + 8 n of this warp, dims 64 j + 16 tq + [0, 16), scaled into f16's range
+    uint32_t qf[NJ][8];  // of the one row tile; two are kept in shared memory
+    uint4* q_frag = reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(epi) + warp * C::kEpiWarp) + lane;
+    float c2[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = row0 + 8 * n + gq;
+      const bool valid = gq + 8 * n < nrows && qtok0 + r / G < a.num_tokens;
       const T* qp = (const T*)a.q + (qtok0 + r / G) * a.q_stride_tok +
                     (int64_t)(kvh * G + r % G) * a.q_stride_head + 16 * tq;
       const bool vec = ((reinterpret_cast<uintptr_t>(a.q) & 15) |
@@ -653,21 +673,36 @@ __global__ void __launch_bounds__(kThreads, 1)
           qf[j][i] = pack2_rn<__half>(unpack_lo<T>(qf[j][i]) * mul, unpack_hi<T>(qf[j][i]) * mul);
       // logit factor of row gq; a row that is not finite gives NaN logits
       const float cr = am < 0x7f800000u ? a.scale * kLog2e * pow2i(max(ex - 14, -126)) : NAN;
-      c2[0] = __shfl_sync(0xffffffffu, cr, (2 * tq) * 4);
-      c2[1] = __shfl_sync(0xffffffffu, cr, (2 * tq + 1) * 4);
-    }
-    int lim[2];  // tokens visible to rows 2 tq and 2 tq + 1
+      c2[n][0] = __shfl_sync(0xffffffffu, cr, (2 * tq) * 4);
+      c2[n][1] = __shfl_sync(0xffffffffu, cr, (2 * tq + 1) * 4);
+      if (NT > 1) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int i = (row0 + 2 * tq + k) / G;
-      lim[k] = i < E ? L - E + i + 1 : L;
+        for (int j = 0; j < NJ; ++j) {
+          q_frag[((j * NT + n) * 2) * 32] = make_uint4(qf[j][0], qf[j][1], qf[j][2], qf[j][3]);
+          q_frag[((j * NT + n) * 2 + 1) * 32] = make_uint4(qf[j][4], qf[j][5], qf[j][6], qf[j][7]);
+        }
+      }
     }
+    int lim[NT][2];  // tokens visible to rows 8 n + 2 tq and + 1
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int i = (row0 + 8 * n + 2 * tq + k) / G;
+        lim[n][k] = i < E ? L - E + i + 1 : L;
+      }
     const int lim_min = L - E + row0 / G + 1;  // tokens visible to every row of the warp
 
-    float acc[NM][4];
+    float acc[NT][NM][4];
+    float M[NT][2], l[NT][2];
 #pragma unroll
-    for (int m = 0; m < NM; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
-    float M[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int m = 0; m < NM; ++m) acc[n][m][0] = acc[n][m][1] = acc[n][m][2] = acc[n][m][3] = 0.f;
+      M[n][0] = M[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+    }
+    const bool second = nrows > 8;  // the second row tile has rows
 
     // this team's tiles of the piece: those with cq % wh == wsel
 #pragma unroll 1
@@ -684,26 +719,45 @@ __global__ void __launch_bounds__(kThreads, 1)
       const unsigned char* stage = smem + st * C::kStage;
       const int tok0 = (cq - cons.unit_g) * kTok;
       if (nrows > 0) {
-        // ---- S^T = K8.Q^T: tokens 16 mt + gq (+8), rows 2 tq, 2 tq + 1; two chains per token tile
-        float s[2][2][4];
+        // ---- S^T = K8.Q^T: tokens 16 mt + gq (+8), rows 8 n + 2 tq, + 1; four chains
+        constexpr int CH = NT == 1 ? 2 : 1;  // chains of a token and row tile
+        float s[2][NT][CH][4];
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-          for (int k = 0; k < 2; ++k) s[mt][k][0] = s[mt][k][1] = s[mt][k][2] = s[mt][k][3] = 0.f;
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int k = 0; k < CH; ++k) s[mt][n][k][0] = s[mt][n][k][1] = s[mt][n][k][2] = s[mt][n][k][3] = 0.f;
         const unsigned char* kp = stage + gq * C::kKS + 16 * tq;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-          uint4 kf[4];
+          uint4 kf[4], qa[NT], qb[NT];
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             kf[i] = *reinterpret_cast<const uint4*>(kp + 8 * i * C::kKS + 64 * j);
 #pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            if (NT == 1) {
+              qa[n] = make_uint4(qf[j][0], qf[j][1], qf[j][2], qf[j][3]);
+              qb[n] = make_uint4(qf[j][4], qf[j][5], qf[j][6], qf[j][7]);
+            } else {
+              qa[n] = q_frag[((j * NT + n) * 2) * 32];
+              qb[n] = q_frag[((j * NT + n) * 2 + 1) * 32];
+            }
+          }
+#pragma unroll
           for (int mt = 0; mt < 2; ++mt) {
             const uint4 k0 = kf[2 * mt], k1 = kf[2 * mt + 1];
-            mma16(s[mt][0], cvt_lo(k0.x), cvt_lo(k1.x), cvt_hi(k0.x), cvt_hi(k1.x), qf[j][0], qf[j][1]);
-            mma16(s[mt][1], cvt_lo(k0.y), cvt_lo(k1.y), cvt_hi(k0.y), cvt_hi(k1.y), qf[j][2], qf[j][3]);
-            mma16(s[mt][0], cvt_lo(k0.z), cvt_lo(k1.z), cvt_hi(k0.z), cvt_hi(k1.z), qf[j][4], qf[j][5]);
-            mma16(s[mt][1], cvt_lo(k0.w), cvt_lo(k1.w), cvt_hi(k0.w), cvt_hi(k1.w), qf[j][6], qf[j][7]);
+            auto four = [&](uint32_t w0, uint32_t w1, int chain, auto q0, auto q1) {
+              const uint32_t a0 = cvt_lo(w0), a1 = cvt_lo(w1), a2 = cvt_hi(w0), a3 = cvt_hi(w1);
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+                if (n == 0 || second) mma16(s[mt][n][chain % CH], a0, a1, a2, a3, q0(n), q1(n));
+            };
+            four(k0.x, k1.x, 0, [&](int n) { return qa[n].x; }, [&](int n) { return qa[n].y; });
+            four(k0.y, k1.y, 1, [&](int n) { return qa[n].z; }, [&](int n) { return qa[n].w; });
+            four(k0.z, k1.z, 0, [&](int n) { return qb[n].x; }, [&](int n) { return qb[n].y; });
+            four(k0.w, k1.w, 1, [&](int n) { return qb[n].z; }, [&](int n) { return qb[n].w; });
           }
         }
         // ---- scales of tokens gq + 8 i.  One that is not finite: NaN logits for the rows that see
@@ -717,65 +771,74 @@ __global__ void __launch_bounds__(kThreads, 1)
           vsc[i] = fin ? p.y : 0.f;
           vmax = fmaxf(vmax, fabsf(vsc[i]));
         }
-        float sv[4][2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int o = 4; o < 32; o <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+        const int ev = min(max((int)(__float_as_uint(vmax) >> 23) - 127, -100), 126);
+        const float vmul = pow2i(max(7 - ev, -126)), lmul = pow2i(max(-ev, -126));
+        uint32_t wb[NT][4];
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int e = 2 * (i & 1) + k;
-            sv[i][k] = (s[i >> 1][0][e] + s[i >> 1][1][e]) * ksc[i] * c2[k];
+        for (int n = 0; n < NT; ++n) {
+          if (n > 0 && !second) {
+            wb[n][0] = wb[n][1] = wb[n][2] = wb[n][3] = 0u;
+            continue;
           }
-        if (tok0 + kTok > lim_min) {  // some token is hidden from some row
+          float sv[4][2];
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
-              if (tok0 + gq + 8 * i >= lim[k]) sv[i][k] = -INFINITY;
-        }
-        float mx[2];
+            for (int k = 0; k < 2; ++k) {
+              const int e = 2 * (i & 1) + k;
+              const float x = CH == 1 ? s[i >> 1][n][0][e] : s[i >> 1][n][0][e] + s[i >> 1][n][CH - 1][e];
+              sv[i][k] = x * ksc[i] * c2[n][k];
+            }
+          if (tok0 + kTok > lim_min) {  // some token is hidden from some row
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-          mx[k] = fmaxf(fmaxf(sv[0][k], sv[1][k]), fmaxf(sv[2][k], sv[3][k]));
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-          mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], o));
-          mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], o));
-          vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
-        }
-        const int ev = min(max((int)(__float_as_uint(vmax) >> 23) - 127, -100), 126);
-        const float vmul = pow2i(max(7 - ev, -126)), lmul = pow2i(max(-ev, -126));
-        float al[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          // a tile hidden from the row as a whole keeps M (and -inf - -inf out of the exponent)
-          const float mn = fmaxf(M[k], mx[k] + (float)ev);
-          al[k] = M[k] == mn ? 1.f : ex2(M[k] - mn);
-          M[k] = mn;
-          const float sub = mn == -INFINITY && tok0 >= lim[k] ? 0.f : (float)ev - mn;
-          float ls = 0.f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            sv[i][k] = ex2(sv[i][k] + sub);
-            ls += sv[i][k];
+              for (int k = 0; k < 2; ++k)
+                if (tok0 + gq + 8 * i >= lim[n][k]) sv[i][k] = -INFINITY;
           }
-          l[k] = fmaf(ls, lmul, l[k] * al[k]);
+          float mx[2];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sv[i][k] *= vsc[i] * vmul;
-        }
-        if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {
+          for (int k = 0; k < 2; ++k)
+            mx[k] = fmaxf(fmaxf(sv[0][k], sv[1][k]), fmaxf(sv[2][k], sv[3][k]));
 #pragma unroll
-          for (int m = 0; m < NM; ++m) {
-            acc[m][0] *= al[0];
-            acc[m][1] *= al[1];
-            acc[m][2] *= al[0];
-            acc[m][3] *= al[1];
+          for (int o = 4; o < 32; o <<= 1) {
+            mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], o));
+            mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], o));
           }
-        }
-        // ---- W^T as B fragments: (token gq + 8 i; rows 2 tq, 2 tq + 1) transposed to (row gq; tokens
-        // 8 i + 2 tq, + 1)
-        uint32_t wb[4];
+          float al[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) wb[i] = movmatrix_t(pack2_rn<__half>(sv[i][0], sv[i][1]));
+          for (int k = 0; k < 2; ++k) {
+            // a tile hidden from the row as a whole keeps M (and -inf - -inf out of the exponent)
+            const float mn = fmaxf(M[n][k], mx[k] + (float)ev);
+            al[k] = M[n][k] == mn ? 1.f : ex2(M[n][k] - mn);
+            M[n][k] = mn;
+            const float sub = mn == -INFINITY && tok0 >= lim[n][k] ? 0.f : (float)ev - mn;
+            float ls = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              sv[i][k] = ex2(sv[i][k] + sub);
+              ls += sv[i][k];
+            }
+            l[n][k] = fmaf(ls, lmul, l[n][k] * al[k]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sv[i][k] *= vsc[i] * vmul;
+          }
+          if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {
+#pragma unroll
+            for (int m = 0; m < NM; ++m) {
+              acc[n][m][0] *= al[0];
+              acc[n][m][1] *= al[1];
+              acc[n][m][2] *= al[0];
+              acc[n][m][3] *= al[1];
+            }
+          }
+          // W^T as B fragments: (token gq + 8 i; rows 2 tq, 2 tq + 1) transposed to (row gq; tokens
+          // 8 i + 2 tq, + 1)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) wb[n][i] = movmatrix_t(pack2_rn<__half>(sv[i][0], sv[i][1]));
+        }
         // ---- O^T += V8^T.W^T
         const uint32_t vp = sp + C::kOffV + lane * C::kVS;
 #pragma unroll
@@ -787,9 +850,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 4; ++i) {
             // codes (2 g, 2 g + 1) of tokens 2 t, 2 t + 1 -> dim 2 g of both, dim 2 g + 1 of both
 #pragma unroll
-            for (int k = 0; k < 4; ++k) r[i][k] = __byte_perm(r[i][k], 0, 0x3120);
-            mma16(acc[m0 + i], cvt_lo(r[i][0]), cvt_hi(r[i][0]), cvt_lo(r[i][1]), cvt_hi(r[i][1]), wb[0], wb[1]);
-            mma16(acc[m0 + i], cvt_lo(r[i][2]), cvt_hi(r[i][2]), cvt_lo(r[i][3]), cvt_hi(r[i][3]), wb[2], wb[3]);
+            for (int k = 0; k < 4; k += 2) {
+              const uint32_t x = __byte_perm(r[i][k], 0, 0x3120), y = __byte_perm(r[i][k + 1], 0, 0x3120);
+              const uint32_t a0 = cvt_lo(x), a1 = cvt_hi(x), a2 = cvt_lo(y), a3 = cvt_hi(y);
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+                if (n == 0 || second) mma16(acc[n][m0 + i], a0, a1, a2, a3, wb[n][k], wb[n][k + 1]);
+            }
           }
         }
       }
@@ -806,19 +873,24 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     // ---- the piece is done: O / l, or partials when the unit goes on in another CTA
 #pragma unroll
-    for (int o = 4; o < 32; o <<= 1) {
-      l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
-      l[1] += __shfl_xor_sync(0xffffffffu, l[1], o);
-    }
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        l[n][0] += __shfl_xor_sync(0xffffffffu, l[n][0], o);
+        l[n][1] += __shfl_xor_sync(0xffffffffu, l[n][1], o);
+      }
     {
-      float* fac = epi + kWarps * kRows * C::kEpiStride;
+      float* fac = epi + kWarps * C::kEpiWarp / 4;
       float* ml = fac + kWarps * kRows;
       if (gq == 0) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-          *reinterpret_cast<float2*>(ml + (warp * kRows + 2 * tq + k) * 2) = make_float2(M[k], l[k]);
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            *reinterpret_cast<float2*>(ml + (warp * kRows + 8 * n + 2 * tq + k) * 2) =
+                make_float2(M[n][k], l[n][k]);
       }
-      float* mine = epi + warp * kRows * C::kEpiStride;
+      float* mine = epi + warp * (C::kEpiWarp / 4);
       const int slot = 2 * c + (p0 == 0 ? 0 : 1);  // partial place
       const bool whole = p0 == cons.unit_g && p1 == cons.unit_g + cons.nt();
       if (wsel == 0 && lane < kRows) {
@@ -827,14 +899,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         reinterpret_cast<int2*>(ml + 2 * kWarps * kRows)[warp * kRows + lane] =
             make_int2(row < E * G && tok < a.num_tokens ? (int)tok : -1, kvh * G + row % G);
       }
+      __syncwarp();  // every lane is done with the Q fragments
 #pragma unroll
       for (int m0 = 0; m0 < NM; m0 += 4) {
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int k = 0; k < 2; ++k)
-            *reinterpret_cast<float2*>(mine + (2 * tq + k) * C::kEpiStride + 16 * m + 2 * gq) =
-                make_float2(acc[m0 + m][k], acc[m0 + m][2 + k]);
+          for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              *reinterpret_cast<float2*>(mine + (8 * n + 2 * tq + k) * C::kEpiStride + 16 * m + 2 * gq) =
+                  make_float2(acc[n][m0 + m][k], acc[n][m0 + m][2 + k]);
         __syncthreads();
         if (m0 == 0) {  // factors of the teams of a head, and its (M, l) in the first team's place
           const int per = sh.hg * sh.team;
@@ -851,7 +926,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           __syncthreads();
         }
-        finish64<T, D>(a, sh, ws, epi, slot, whole, 16 * m0);
+        finish64<T, D, NT>(a, sh, ws, epi, slot, whole, 16 * m0);
         __syncthreads();
       }
     }
@@ -867,10 +942,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 //     rows of the unit that it cuts when it is the first boundary inside that unit
 //   deep (few units, many pieces each): CTA (unit, place, row), 16 groups
 // ---------------------------------------------------------------------------------------------
-template <typename T, int D, int RZ, int THREADS, bool DEEP>
+template <typename T, int D, int NT, int RZ, int THREADS, bool DEEP>
 __global__ void __launch_bounds__(THREADS)
     combine_kernel(const __grid_constant__ tf_paged_attn_args a, const __grid_constant__ Shape sh,
                    const __grid_constant__ Ws ws) {
+  constexpr int kRows = 8 * NT;
   constexpr int kVec = D / 4;  // 4-value vectors of a row
   constexpr int PG = THREADS / (RZ * kVec);
   static_assert(PG >= 1 && PG * RZ * kVec == THREADS, "threads of a CTA");
@@ -881,19 +957,21 @@ __global__ void __launch_bounds__(THREADS)
   const int tid = threadIdx.x, lane = tid & 31;
   const int w = blockIdx.y, n = sh.nctas;
   const int G = a.num_q_heads / a.num_kv_heads;
-  int u, start, ext, c0;
+  int pass, u, start, ext, c0;
   int64_t su, eu;
   if (DEEP) {  // the unit's tiles from the lengths, while the main kernel still runs
     const int b = blockIdx.x / sh.groups;
     u = blockIdx.x - b * sh.groups;
+    pass = b % sh.passes;
     int64_t before = 0, q = 0, e = 0;
     int nt = 0;
     for (int i = 0; i <= b; ++i) {
       bool bad;
       before += nt;
-      const int64_t L = checked_len(a, i, e, bad);
-      nt = tiles_of(L, e);
-      if (i < b) q += a.extend_lens ? max((int)a.extend_lens[i], 0) : 1;
+      const int64_t L = checked_len(a, i / sh.passes, e, bad);
+      nt = tiles_of(L, e, i % sh.passes, sh, G);
+      if (i < b && (i + 1) % sh.passes == 0)
+        q += a.extend_lens ? max((int)a.extend_lens[i / sh.passes], 0) : 1;
     }
     if (nt == 0) return;
     start = (int)q;
@@ -912,12 +990,13 @@ __global__ void __launch_bounds__(THREADS)
     c0 = c - 1;
     while (ws.cta_g[c0] == g) --c0;      // empty ranges before this one
     if (ws.cta_g[c0] > su) return;       // not the first boundary inside the unit
+    pass = ci.pass;
     u = ci.u;
     start = ci.start;
     ext = ci.ext;
   }
   const int hsel = w / sh.team, member = w % sh.team;
-  const int row0 = ((u % sh.passes) * sh.team + member) * kRows;
+  const int row0 = (pass * sh.team + member) * kRows;
   if (row0 >= ext * G) return;
   for (int i = tid; i <= n; i += THREADS) s_g[i] = ws.cta_g[i];
   __syncthreads();
@@ -1012,7 +1091,7 @@ __global__ void __launch_bounds__(THREADS)
   const int rr = row0 + r;
   const int64_t tok = start + rr / G;
   if (rr < ext * G && tok < a.num_tokens) {
-    const int hq = ((u / sh.passes) * sh.hg + hsel) * G + rr % G;
+    const int hq = (u * sh.hg + hsel) * G + rr % G;
     const float inv = (1.f / 128.f) / l;
     const bool v8 = rows_v8(a);
     uint2 gw = make_uint2(0, 0);
@@ -1023,19 +1102,30 @@ __global__ void __launch_bounds__(THREADS)
 
 inline int gcd(int a, int b) { return b == 0 ? a : gcd(b, a % b); }
 
-// how a call is divided (max_rows: query rows of one kv head of the longest request)
-template <int D>
+// rows of one kv head of the longest request
+inline int64_t max_rows(const tf_paged_attn_args& a) {
+  return (int64_t)(a.num_q_heads / a.num_kv_heads) * (a.extend_lens ? a.max_extend_len : 1);
+}
+// 8-row tiles of a warp, warps of a team, passes of a request
+inline int row_tiles_of(int64_t rows) { return rows > 16 ? 2 : 1; }
+inline int team_of(int64_t rows) { return rows > 8 ? 2 : 1; }
+inline int passes_of(int64_t rows) {
+  const int held = 8 * row_tiles_of(rows) * team_of(rows);
+  return rows > held ? (int)((rows + held - 1) / held) : 1;
+}
+
+// how a call is divided
+template <int D, int NT>
 static Shape shape_of(const tf_paged_attn_args& a, int num_sms) {
-  using C = Cfg<D>;
-  const int G = a.num_q_heads / a.num_kv_heads;
-  const int64_t rows = (int64_t)G * (a.extend_lens ? a.max_extend_len : 1);
-  const int need = rows > kRows ? (int)((rows + kRows - 1) / kRows) : 1;
+  using C = Cfg<D, NT>;
+  const int64_t rows = max_rows(a);
   Shape s;
-  s.team = need <= 1 ? 1 : (need <= 2 ? 2 : (need <= 4 ? 4 : 8));
-  s.passes = (need + s.team - 1) / s.team;
+  s.row_tiles = NT;
+  s.team = team_of(rows);
+  s.passes = passes_of(rows);
   s.hg = gcd(a.num_kv_heads, kWarps / s.team);
   s.wh = kWarps / (s.team * s.hg);
-  s.groups = a.num_kv_heads / s.hg * s.passes;
+  s.groups = a.num_kv_heads / s.hg;
   s.stages = C::kStages;
   auto bytes = [&](int n) { return n * C::kStage + C::kFixed + 16 * n + C::kEpi; };
   while (bytes(s.stages) > 232448) --s.stages;
@@ -1047,21 +1137,22 @@ static Shape shape_of(const tf_paged_attn_args& a, int num_sms) {
   return s;
 }
 
-template <typename T, int D>
-static cudaError_t launch_td(const tf_paged_attn_args& a, const tf_kv_scale& sc, void* wsp,
-                             int num_sms, cudaStream_t s) {
+template <typename T, int D, int NT>
+static cudaError_t launch_tdn(const tf_paged_attn_args& a, const tf_kv_scale& sc, void* wsp,
+                              int num_sms, cudaStream_t s) {
+  constexpr int kRows = 8 * NT;
   if (num_sms > kMaxCtas) num_sms = kMaxCtas;
-  const Shape sh = shape_of<D>(a, num_sms);
-  if ((int64_t)(a.batch_size + 1) * 4 > sh.ring) return cudaErrorInvalidValue;
-  const Ws ws = carve(wsp, num_sms, D);
-  cudaError_t e = cudaFuncSetAttribute(rows_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       sh.smem);
+  const Shape sh = shape_of<D, NT>(a, num_sms);
+  if (((int64_t)a.batch_size * sh.passes + 1) * 4 > sh.ring) return cudaErrorInvalidValue;
+  const Ws ws = carve(wsp, num_sms, kRows);
+  cudaError_t e = cudaFuncSetAttribute(rows_kernel<T, D, NT>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, sh.smem);
   if (e != cudaSuccess) return e;
-  rows_kernel<T, D><<<num_sms, kThreads, sh.smem, s>>>(a, sc, sh, ws);
+  rows_kernel<T, D, NT><<<num_sms, kThreads, sh.smem, s>>>(a, sc, sh, ws);
   e = cudaGetLastError();
   if (e != cudaSuccess || num_sms == 1) return e;
   constexpr int kWide = 256 / (D / 4) < kRows ? 256 / (D / 4) : kRows;
-  const int64_t units = (int64_t)a.batch_size * sh.groups;
+  const int64_t units = (int64_t)a.batch_size * sh.passes * sh.groups;
   const bool deep = units * 8 < num_sms;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = deep ? dim3((unsigned)units, (unsigned)(sh.hg * sh.team), (unsigned)kRows)
@@ -1073,8 +1164,15 @@ static cudaError_t launch_td(const tf_paged_attn_args& a, const tf_kv_scale& sc,
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return deep ? cudaLaunchKernelEx(&cfg, combine_kernel<T, D, 1, 4 * D, true>, a, sh, ws)
-              : cudaLaunchKernelEx(&cfg, combine_kernel<T, D, kWide, kWide * (D / 4), false>, a, sh, ws);
+  return deep ? cudaLaunchKernelEx(&cfg, combine_kernel<T, D, NT, 1, 4 * D, true>, a, sh, ws)
+              : cudaLaunchKernelEx(&cfg, combine_kernel<T, D, NT, kWide, kWide * (D / 4), false>, a, sh, ws);
+}
+
+template <typename T, int D>
+static cudaError_t launch_td(const tf_paged_attn_args& a, const tf_kv_scale& sc, void* ws,
+                             int num_sms, cudaStream_t s) {
+  return row_tiles_of(max_rows(a)) == 2 ? launch_tdn<T, D, 2>(a, sc, ws, num_sms, s)
+                                        : launch_tdn<T, D, 1>(a, sc, ws, num_sms, s);
 }
 
 template <typename T>
@@ -1092,7 +1190,7 @@ static cudaError_t launch_t(const tf_paged_attn_args& a, const tf_kv_scale& sc, 
 bool paged_fp8_rows_supported(const tf_paged_attn_args& a) {
   if (a.dtype != TF_DTYPE_BF16 && a.dtype != TF_DTYPE_F16) return false;
   if (a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256) return false;
-  if (a.batch_size > rows8::kMaxBatch || a.r2t_rows > 0x7fffffff || a.r2t_cols > 0x7fffffff)
+  if ((int64_t)a.batch_size * rows8::passes_of(rows8::max_rows(a)) > rows8::kMaxBatch || a.r2t_rows > 0x7fffffff || a.r2t_cols > 0x7fffffff)
     return false;
   auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   // row offsets are kept in 32 bits of 16-byte pieces: pools of up to 64 GiB a layer
@@ -1101,7 +1199,8 @@ bool paged_fp8_rows_supported(const tf_paged_attn_args& a) {
 }
 
 size_t paged_fp8_rows_workspace(const tf_paged_attn_args& a, int num_sms) {
-  return rows8::ws_bytes(num_sms < rows8::kMaxCtas ? num_sms : rows8::kMaxCtas, a.head_dim);
+  return rows8::ws_bytes(num_sms < rows8::kMaxCtas ? num_sms : rows8::kMaxCtas,
+                         8 * rows8::row_tiles_of(rows8::max_rows(a)), a.head_dim);
 }
 
 cudaError_t launch_paged_fp8_rows(const tf_paged_attn_args& a, const tf_kv_scale& sc, void* ws,

@@ -1123,7 +1123,14 @@ static Shape shape_of(const tf_paged_attn_args& a, int num_sms) {
   s.row_tiles = NT;
   s.team = team_of(rows);
   s.passes = passes_of(rows);
+  // Heads side by side read whole tokens (128 decode requests of 512 to 8192 tokens: 233 us, 250 us with
+  // two heads, 285 us with one).  One head a CTA leaves a quarter of the partial rows and its teams
+  // meet in shared memory, which counts when a CTA has few tiles: 4 requests of 300 to 6000 tokens and
+  // 2..5 drafts 41 us against 78 us with four heads, 8 decode requests of 1000 to 6000 43 us against
+  // 47 us; the two meet at about 48 tiles of a head per CTA.
   s.hg = gcd(a.num_kv_heads, kWarps / s.team);
+  const int64_t tiles = (int64_t)a.batch_size * s.passes * a.num_kv_heads * ((a.max_seq_len + kTok - 1) / kTok);
+  if (tiles < (int64_t)48 * num_sms) s.hg = 1;
   s.wh = kWarps / (s.team * s.hg);
   s.groups = a.num_kv_heads / s.hg;
   s.stages = C::kStages;
@@ -1132,7 +1139,7 @@ static Shape shape_of(const tf_paged_attn_args& a, int num_sms) {
   s.ring = s.stages * C::kStage;
   s.smem = bytes(s.stages);
   s.nctas = num_sms;
-  s.min_tiles = 2 * s.wh;
+  s.min_tiles = s.wh;  // one for each team (1000 tokens: 24.6 us, 28.7 us with two)
   s.piece_cost = 8;
   return s;
 }

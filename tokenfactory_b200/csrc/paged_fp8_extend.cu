@@ -27,7 +27,7 @@
 // TF_KERR_TIMEOUT.
 //
 // Few query tiles over a long prefix leave SM pairs idle: the key tiles are then split over
-// grid.z clusters, which leave (M, l, O) partials for a combine kernel.
+// grid.y clusters, which leave (M, l, O) partials for a combine kernel.
 #include <type_traits>
 
 #include "common.cuh"
@@ -321,14 +321,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const uint32_t peer_abort = peer_addr(smem_u32((const void*)abort), peer);
   const int Hkv = a.num_kv_heads, G = a.num_q_heads / Hkv;
   const int TQ = kRows / G;  // query tokens per CTA
-  const int pidx = blockIdx.x >> 1;
-  const int b = pidx / pairs_per_req;
-  const int qp = pairs_per_req - 1 - (pidx - b * pairs_per_req);  // longest tiles first
-  const int h = blockIdx.y, z = blockIdx.z;
-  const int64_t E = a.extend_lens ? a.extend_lens[b] : 1;
+  // Longest query tiles first, so that the last ones to finish are short: the longest request before
+  // the others (of up to 32, which a warp ranks; of more, each is a small part of the whole), and a
+  // head's later tiles before its earlier ones.  3 requests of 64 to 1009 new tokens on up to 2904: 122 us,
+  // 129 us in the batch's order, head by head; 4 of 512 to 2048 on up to 4096: 664 us against 672 us
+  // (695 us with the kv heads of a query tile side by side).
+  const int z = blockIdx.y, rank_h = (blockIdx.x >> 1) / pairs_per_req;
+  const int qp = pairs_per_req - 1 - ((blockIdx.x >> 1) - rank_h * pairs_per_req);
+  const int h = rank_h % Hkv;
+  int b = rank_h / Hkv;
+  int64_t E, L;
+  if (a.batch_size <= 32) {
+    const bool in = lane < a.batch_size;
+    const int64_t Li = in ? a.seq_lens[lane] : INT64_MIN;
+    const int64_t Ei = in && a.extend_lens ? a.extend_lens[lane] : 1;
+    int place = 0;
+    for (int j = 0; j < a.batch_size; ++j) {
+      const int64_t Lj = __shfl_sync(0xffffffffu, Li, j);
+      place += Lj > Li || (Lj == Li && j < lane);
+    }
+    b = __ffs(__ballot_sync(0xffffffffu, in && place == b)) - 1;
+    E = __shfl_sync(0xffffffffu, Ei, b);
+    L = __shfl_sync(0xffffffffu, Li, b);
+  } else {
+    E = a.extend_lens ? a.extend_lens[b] : 1;
+    L = a.seq_lens[b];
+  }
   const int64_t pair_start = (int64_t)qp * 2 * TQ;
   if (pair_start >= E) return;  // both CTAs of the pair leave here, before any cluster barrier
-  const int64_t L = a.seq_lens[b];
   if (L > a.r2t_cols || L < E) {
     if (tid == 0 && rank == 0) record_err(a.err, TF_KERR_SLOT_RANGE);
     return;
@@ -1004,7 +1024,7 @@ static cudaError_t launch_td(const tf_paged_attn_args& a, const tf_kv_scale& sc,
   cudaError_t e = cudaFuncSetAttribute(extend_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        Cfg<D>::kSmem);
   if (e != cudaSuccess) return e;
-  dim3 grid((unsigned)(2 * a.batch_size * pairs), (unsigned)a.num_kv_heads, (unsigned)sp.n);
+  dim3 grid((unsigned)(2 * (int64_t)a.batch_size * pairs * a.num_kv_heads), (unsigned)sp.n);
   extend_kernel<T, D><<<grid, kThreads, Cfg<D>::kSmem, s>>>(a, sc, pairs, sp);
   e = cudaGetLastError();
   if (e != cudaSuccess || sp.n == 1) return e;
@@ -1019,7 +1039,9 @@ bool paged_fp8_extend_supported(const tf_paged_attn_args& a) {
   if (a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256) return false;
   const int G = a.num_q_heads / a.num_kv_heads;
   if (G < 1 || G > 16) return false;
-  if (a.max_extend_len <= 0 || a.num_kv_heads > 65535) return false;
+  if (a.max_extend_len <= 0) return false;
+  const int64_t TQ2 = 2 * (ext8::kRows / G);
+  if ((int64_t)a.batch_size * ((a.max_extend_len + TQ2 - 1) / TQ2) * a.num_kv_heads > 0x3fffffff) return false;
   if (!(a.scale > 0.f)) return false;  // the softmax takes its max before the scale
   auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   // row offsets are kept in 32 bits of 16-byte pieces: pools of up to 64 GiB a layer

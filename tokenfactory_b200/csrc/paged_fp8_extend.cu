@@ -254,7 +254,7 @@ struct Cfg {
   static constexpr int kOffBars = kOffRing + kSlots * kSlotBytes;
   // full, empty [kSlots]; s_full[2], p_full[2][2], o_done, q_full, fin, q_dead, sc_full[kScaleTiles]
   static constexpr int kNumBars = 2 * kSlots + 10 + kScaleTiles;
-  static constexpr int kOffWords = kOffBars + 8 * kNumBars;      // tmem holder, abort, q0
+  static constexpr int kOffWords = kOffBars + 8 * kNumBars;      // tmem holder, abort
   static constexpr int kOffM = (kOffWords + 16 + 15) & ~15;      // float [2][kRows]: running maxima
   static constexpr int kOffRow = kOffM + 2 * kRows * 4;          // float [kRows]: logit factor of a row
   static constexpr int kOffKs = kOffRow + kRows * 4;             // float [kScaleTiles][kKeys]
@@ -277,13 +277,27 @@ struct Split {
   float* o;     // [n][T][Hq][D]
 };
 
+// 16 columns of this lane's TMEM row
+__device__ __forceinline__ void ld16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
 // 16-byte pieces of the gate and output rows can be moved whole
 __device__ __forceinline__ bool rows_v16(const tf_paged_attn_args& a) {
   return ((reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.gate)) & 15) == 0 &&
          ((a.out_stride_tok | a.out_stride_head | a.gate_stride_tok | a.gate_stride_head) & 7) == 0;
 }
+// the gate's activation; __fdividef is off by at most two units of 2^-23
 __device__ __forceinline__ float act(float x, int mode) {
-  const float s = sigmoid_f(x);
+  const float s = __fdividef(1.f, 1.f + __expf(-x));
   return mode == TF_GATE_SILU ? x * s : s;
 }
 
@@ -307,7 +321,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   uint64_t* sc_full = q_dead + 1;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(sbase + C::kOffWords);
   volatile int* abort = reinterpret_cast<volatile int*>(sbase + C::kOffWords + 4);
-  int64_t* s_q0 = reinterpret_cast<int64_t*>(sbase + C::kOffWords + 8);
   float* m_s = reinterpret_cast<float*>(sbase + C::kOffM);
   float* rowf = reinterpret_cast<float*>(sbase + C::kOffRow);
   float* ks_s = reinterpret_cast<float*>(sbase + C::kOffKs);
@@ -330,7 +343,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int qp = pairs_per_req - 1 - ((blockIdx.x >> 1) - rank_h * pairs_per_req);
   const int h = rank_h % Hkv;
   int b = rank_h / Hkv;
-  int64_t E, L;
+  int64_t E, L, before = 0;  // before: query tokens of the requests before this one
   if (a.batch_size <= 32) {
     const bool in = lane < a.batch_size;
     const int64_t Li = in ? a.seq_lens[lane] : INT64_MIN;
@@ -343,10 +356,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     b = __ffs(__ballot_sync(0xffffffffu, in && place == b)) - 1;
     E = __shfl_sync(0xffffffffu, Ei, b);
     L = __shfl_sync(0xffffffffu, Li, b);
+    if (in && lane < b && Ei > 0) before = Ei;
   } else {
     E = a.extend_lens ? a.extend_lens[b] : 1;
     L = a.seq_lens[b];
+    for (int i = lane; i < b; i += 32) {
+      const int64_t e = a.extend_lens ? a.extend_lens[i] : 1;
+      before += e > 0 ? e : 0;
+    }
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
   const int64_t pair_start = (int64_t)qp * 2 * TQ;
   if (pair_start >= E) return;  // both CTAs of the pair leave here, before any cluster barrier
   if (L > a.r2t_cols || L < E) {
@@ -363,19 +383,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int jb = z * per;
   const int ntiles = all_tiles - jb < per ? all_tiles - jb : per;
 
-  if (warp == 0) {
-    int64_t acc = 0;
-    for (int i = lane; i < b; i += 32) {
-      const int64_t e = a.extend_lens ? a.extend_lens[i] : 1;
-      acc += e > 0 ? e : 0;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-    if (lane == 0) *s_q0 = acc;
-  }
+  const int64_t q0 = before + cta_start;
+  int64_t left = E - cta_start < TQ ? E - cta_start : TQ;
+  if (left > a.num_tokens - q0) left = a.num_tokens - q0;
+  const int n_tok = left > 0 ? (int)left : 0;  // query tokens of this CTA
+
   if (ntiles <= 0) {  // nothing left for this cluster: an empty partial (both CTAs come here)
-    __syncthreads();
-    const int64_t q0 = *s_q0 + cta_start;
     const int ri = tid / G;
     if (tid < kRows && ri < TQ && cta_start + ri < E && q0 + ri < a.num_tokens) {
       const int64_t row = ((int64_t)z * a.num_tokens + q0 + ri) * a.num_q_heads + h * G + tid % G;
@@ -384,7 +397,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     return;
   }
   if (tid == 0) {
-    const uint32_t in_count = rank == 0 ? kPrWarps + 1 : kPrWarps;  // one arrive a warp
     for (int i = 0; i < C::kSlots; ++i) {
       mbar_init(&full[i], rank == 0 ? kPrWarps / 2 + 1 : kPrWarps / 2);
       mbar_init(&empty[i], 1);
@@ -394,7 +406,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       for (int k = 0; k < 2; ++k) mbar_init(&p_full[2 * i + k], rank == 0 ? kSmWarps / 2 + 1 : kSmWarps / 2);
     }
     mbar_init(o_done, 1);
-    mbar_init(q_full, in_count);
+    mbar_init(q_full, rank == 0 ? kSmWarps + 1 : kSmWarps);  // one arrive a warp
     mbar_init(fin, 1);
     mbar_init(q_dead, 1);
     for (int i = 0; i < C::kScaleTiles; ++i) mbar_init(&sc_full[i], kPrWarps / 2);
@@ -426,6 +438,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (int i = 0; i < kPrefetch; ++i)
       if (i < ntiles) raw_q[i] = raw_of(i);
   }
+  // Q: the softmax warps request this CTA's 128 rows before the set-up barrier, all at once (16 rows a
+  // warp, four at a time behind the barrier, took 13 us); a row sits with D / 8 lanes
+  constexpr int kQLanes = D / 8, kQRpi = 32 / kQLanes, kQLoads = kRows / kSmWarps / kQRpi;
+  uint4 qw[kQLoads];
+  if (warp < kSmWarps) {
+    const int sub = lane / kQLanes, ch = lane - sub * kQLanes;
+    const T* q = reinterpret_cast<const T*>(a.q);
+    const bool vec = ((reinterpret_cast<uintptr_t>(a.q) & 15) | ((a.q_stride_tok | a.q_stride_head) & 7)) == 0;
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < kQLoads; ++i) {
+        const int r = warp * (kRows / kSmWarps) + i * kQRpi + sub;
+        const int ti = r / G, g = r - (r / G) * G;
+        qw[i] = make_uint4(0, 0, 0, 0);
+        if (ti < n_tok)
+          qw[i] = ldg_nc(q + (q0 + ti) * a.q_stride_tok + (int64_t)(h * G + g) * a.q_stride_head + ch * 8);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kQLoads; ++i) {
+        const int r = warp * (kRows / kSmWarps) + i * kQRpi + sub;
+        const int ti = r / G, g = r - (r / G) * G;
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (ti < n_tok) {
+          const unsigned short* u = reinterpret_cast<const unsigned short*>(
+              q + (q0 + ti) * a.q_stride_tok + (int64_t)(h * G + g) * a.q_stride_head + ch * 8);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = u[2 * k] | ((uint32_t)u[2 * k + 1] << 16);
+        }
+        qw[i] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
   if (warp == kIssueWarp) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(tmem_holder)), "r"(C::kTmemCols)
@@ -436,53 +481,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   cluster_sync();  // barriers of both CTAs initialised, TMEM allocated in both
   tc::fence_after_sync();
   const uint32_t tmem = *tmem_holder;
-  const int64_t q0 = *s_q0 + cta_start;
-  int64_t left = E - cta_start < TQ ? E - cta_start : TQ;
-  if (left > a.num_tokens - q0) left = a.num_tokens - q0;
-  const int n_tok = left > 0 ? (int)left : 0;  // query tokens of this CTA
 
   if (warp >= kPrWarp0 && warp < kIssueWarp) {
     // ======================= producers: this CTA's halves =======================
-    {  // Q: this CTA's 128 rows, scaled into f16's range; a row sits with D / 8 lanes
-      constexpr int CPR = D / 8, RPI = 32 / CPR;
-      const int sub = lane / CPR, ch = lane - (lane / CPR) * CPR;
-      const T* q = reinterpret_cast<const T*>(a.q);
-      const bool vec = ((reinterpret_cast<uintptr_t>(a.q) & 15) |
-                        ((a.q_stride_tok | a.q_stride_head) & 7)) == 0;
-#pragma unroll 4
-      for (int i = 0; i < kRows / kPrWarps; i += RPI) {
-        const int r = pw * (kRows / kPrWarps) + i + sub;
-        const int ti = r / G, g = r - (r / G) * G;
-        uint32_t w[4] = {0, 0, 0, 0};
-        if (ti < n_tok) {
-          const T* src = q + (q0 + ti) * a.q_stride_tok + (int64_t)(h * G + g) * a.q_stride_head + ch * 8;
-          if (vec) {
-            const uint4 v = *reinterpret_cast<const uint4*>(src);
-            w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-          } else {
-            const unsigned short* u = reinterpret_cast<const unsigned short*>(src);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = u[2 * k] | ((uint32_t)u[2 * k + 1] << 16);
-          }
-        }
-        uint32_t am = 0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          am = max(am, max(kv8::abs_bits(unpack_lo<T>(w[k])), kv8::abs_bits(unpack_hi<T>(w[k]))));
-#pragma unroll
-        for (int o = CPR / 2; o > 0; o >>= 1) am = max(am, __shfl_xor_sync(0xffffffffu, am, o));
-        const int ex = max((int)(am >> 23) - 127, -100);  // row maximum in [2^ex, 2^(ex+1))
-        const float mul = pow2i(14 - ex);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = pack2_rn<__half>(unpack_lo<T>(w[k]) * mul, unpack_hi<T>(w[k]) * mul);
-        sts128(base + (ch >> 3) * C::kQBlock + r * 128 + (((ch & 7) ^ (r & 7)) << 4), w[0], w[1], w[2], w[3]);
-        // a row that is not finite gives NaN logits
-        if (ch == 0) rowf[r] = am < 0x7f800000u ? a.scale * kLog2e * pow2i(max(ex - 14, -126)) : NAN;
-      }
-      tc::fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
-    }
     const float* scp = sc.data + (int64_t)h * sc.stride_head;
     bool ok = true;
     // the slots of one kind
@@ -713,6 +714,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     constexpr int kOHalf = D / 2;  // O columns stored by this thread
     const int bar_in = 1 + 2 * (warp & 3) + wg, bar_out = 1 + 2 * (warp & 3) + (wg ^ 1);
     float m_used = -INFINITY, l_sum = 0.f;
+    {  // Q, scaled into f16's range
+      const int sub = lane / kQLanes, ch = lane - sub * kQLanes;
+#pragma unroll
+      for (int i = 0; i < kQLoads; ++i) {
+        const int qr = warp * (kRows / kSmWarps) + i * kQRpi + sub;
+        uint32_t w[4] = {qw[i].x, qw[i].y, qw[i].z, qw[i].w}, am = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          am = max(am, max(kv8::abs_bits(unpack_lo<T>(w[k])), kv8::abs_bits(unpack_hi<T>(w[k]))));
+#pragma unroll
+        for (int o = kQLanes / 2; o > 0; o >>= 1) am = max(am, __shfl_xor_sync(0xffffffffu, am, o));
+        const int ex = max((int)(am >> 23) - 127, -100);  // row maximum in [2^ex, 2^(ex+1))
+        const float mul = pow2i(14 - ex);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = pack2_rn<__half>(unpack_lo<T>(w[k]) * mul, unpack_hi<T>(w[k]) * mul);
+        sts128(base + (ch >> 3) * C::kQBlock + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4), w[0], w[1], w[2], w[3]);
+        // a row that is not finite gives NaN logits
+        if (ch == 0) rowf[qr] = am < 0x7f800000u ? a.scale * kLog2e * pow2i(max(ex - 14, -126)) : NAN;
+      }
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    }
     bool ok = __all_sync(0xffffffffu, wait_bar<false>(q_full, 0, abort, peer_abort));
     const float c2 = rowf[r];
     // No early exit from this loop: the warps of a pair meet at a barrier every tile, so a failed
@@ -864,43 +888,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       T* orow = (T*)a.out + t * a.out_stride_tok + (int64_t)hq * a.out_stride_head + wg * kOHalf;
       const T* grow = (const T*)a.gate + t * a.gate_stride_tok + (int64_t)hq * a.gate_stride_head + wg * kOHalf;
       constexpr int kChunks = D / 8;
+      // 16 columns a pass in one copy of this code: it runs once a query tile from a cold instruction
+      // cache (12 us with 32 columns unrolled and the gate's divisions in full precision)
 #pragma unroll 1
-      for (int cc = 0; cc < kOHalf / 32; ++cc) {
-        float o[32];
-        tc::ld32(tmem + lane_base + C::kColO + wg * kOHalf + cc * 32, o);
+      for (int cc = 0; cc < kOHalf / 16; ++cc) {
+        float o[16];
+        ld16(tmem + lane_base + C::kColO + wg * kOHalf + cc * 16, o);
         tc::wait_ld();
         if (!row_valid) continue;
         if (sp.n > 1) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            *reinterpret_cast<float4*>(po + cc * 32 + 4 * k) = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-        } else if (vec) {
+          for (int k = 0; k < 4; ++k)
+            *reinterpret_cast<float4*>(po + cc * 16 + 4 * k) = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          continue;
+        }
+        uint32_t gw[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (gated && vec) {
 #pragma unroll
-          for (int c8 = 0; c8 < 4; ++c8) {
-            uint32_t gw[4] = {0, 0, 0, 0}, ow[4];
-            if (gated) {
-              const int chunk = (wg * kOHalf + cc * 32) / 8 + c8;
-              asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                           : "=r"(gw[0]), "=r"(gw[1]), "=r"(gw[2]), "=r"(gw[3])
-                           : "r"(base + r * (D * 2) + ((chunk ^ (r & (kChunks - 1))) << 4)));
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              float x0 = o[c8 * 8 + 2 * k] * inv, x1 = o[c8 * 8 + 2 * k + 1] * inv;
-              if (gated) {
-                x0 *= act(unpack_lo<T>(gw[k]), a.gate_mode);
-                x1 *= act(unpack_hi<T>(gw[k]), a.gate_mode);
-              }
-              ow[k] = pack2_rn<T>(x0, x1);
-            }
-            *reinterpret_cast<uint4*>(orow + cc * 32 + c8 * 8) = make_uint4(ow[0], ow[1], ow[2], ow[3]);
+          for (int c8 = 0; c8 < 2; ++c8) {
+            const int chunk = (wg * kOHalf + cc * 16) / 8 + c8;
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(gw[4 * c8]), "=r"(gw[4 * c8 + 1]), "=r"(gw[4 * c8 + 2]), "=r"(gw[4 * c8 + 3])
+                         : "r"(base + r * (D * 2) + ((chunk ^ (r & (kChunks - 1))) << 4)));
           }
-        } else {
+        } else if (gated) {
+          const unsigned short* u = reinterpret_cast<const unsigned short*>(grow + cc * 16);
 #pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            float x = o[k] * inv;
-            if (gated) x *= act(to_f(grow[cc * 32 + k]), a.gate_mode);
-            orow[cc * 32 + k] = from_f<T>(x);
+          for (int k = 0; k < 8; ++k) gw[k] = u[2 * k] | ((uint32_t)u[2 * k + 1] << 16);
+        }
+        uint32_t ow[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          float x0 = o[2 * k] * inv, x1 = o[2 * k + 1] * inv;
+          if (gated) {
+            x0 *= act(unpack_lo<T>(gw[k]), a.gate_mode);
+            x1 *= act(unpack_hi<T>(gw[k]), a.gate_mode);
+          }
+          ow[k] = pack2_rn<T>(x0, x1);
+        }
+        if (vec) {
+          *reinterpret_cast<uint4*>(orow + cc * 16) = make_uint4(ow[0], ow[1], ow[2], ow[3]);
+          *reinterpret_cast<uint4*>(orow + cc * 16 + 8) = make_uint4(ow[4], ow[5], ow[6], ow[7]);
+        } else {
+          unsigned short* u = reinterpret_cast<unsigned short*>(orow + cc * 16);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            u[2 * k] = (unsigned short)ow[k];
+            u[2 * k + 1] = (unsigned short)(ow[k] >> 16);
           }
         }
       }

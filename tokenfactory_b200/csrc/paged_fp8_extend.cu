@@ -439,35 +439,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (i < ntiles) raw_q[i] = raw_of(i);
   }
   // Q: the softmax warps request this CTA's 128 rows before the set-up barrier, all at once (16 rows a
-  // warp, four at a time behind the barrier, took 13 us); a row sits with D / 8 lanes
+  // warp, four at a time behind the barrier, took 13 us); a row sits with D / 8 lanes, 16 bytes each
   constexpr int kQLanes = D / 8, kQRpi = 32 / kQLanes, kQLoads = kRows / kSmWarps / kQRpi;
-  uint4 qw[kQLoads];
+  const int q_sub = lane / kQLanes, q_ch = lane - q_sub * kQLanes;
+  auto q_row = [&](int i) { return warp * (kRows / kSmWarps) + i * kQRpi + q_sub; };
+  auto q_dst = [&](int qr) {
+    return base + (q_ch >> 3) * C::kQBlock + qr * 128 + (((q_ch & 7) ^ (qr & 7)) << 4);
+  };
   if (warp < kSmWarps) {
-    const int sub = lane / kQLanes, ch = lane - sub * kQLanes;
-    const T* q = reinterpret_cast<const T*>(a.q);
+    const T* q = reinterpret_cast<const T*>(a.q) + q0 * a.q_stride_tok + (int64_t)h * G * a.q_stride_head + q_ch * 8;
     const bool vec = ((reinterpret_cast<uintptr_t>(a.q) & 15) | ((a.q_stride_tok | a.q_stride_head) & 7)) == 0;
-    if (vec) {
-#pragma unroll
-      for (int i = 0; i < kQLoads; ++i) {
-        const int r = warp * (kRows / kSmWarps) + i * kQRpi + sub;
-        const int ti = r / G, g = r - (r / G) * G;
-        qw[i] = make_uint4(0, 0, 0, 0);
-        if (ti < n_tok)
-          qw[i] = ldg_nc(q + (q0 + ti) * a.q_stride_tok + (int64_t)(h * G + g) * a.q_stride_head + ch * 8);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kQLoads; ++i) {
-        const int r = warp * (kRows / kSmWarps) + i * kQRpi + sub;
-        const int ti = r / G, g = r - (r / G) * G;
-        uint32_t w[4] = {0, 0, 0, 0};
-        if (ti < n_tok) {
-          const unsigned short* u = reinterpret_cast<const unsigned short*>(
-              q + (q0 + ti) * a.q_stride_tok + (int64_t)(h * G + g) * a.q_stride_head + ch * 8);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) w[k] = u[2 * k] | ((uint32_t)u[2 * k + 1] << 16);
-        }
-        qw[i] = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll 4
+    for (int i = 0; i < kQLoads; ++i) {
+      const int qr = q_row(i), ti = qr / G;
+      const T* src = q + ti * a.q_stride_tok + (int64_t)(qr - ti * G) * a.q_stride_head;
+      if (ti >= n_tok) {
+        sts128(q_dst(qr), 0, 0, 0, 0);
+      } else if (vec) {
+        cp_async16(q_dst(qr), src);
+      } else {
+        const unsigned short* u = reinterpret_cast<const unsigned short*>(src);
+        sts128(q_dst(qr), u[0] | ((uint32_t)u[1] << 16), u[2] | ((uint32_t)u[3] << 16),
+               u[4] | ((uint32_t)u[5] << 16), u[6] | ((uint32_t)u[7] << 16));
       }
     }
   }
@@ -714,12 +707,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     constexpr int kOHalf = D / 2;  // O columns stored by this thread
     const int bar_in = 1 + 2 * (warp & 3) + wg, bar_out = 1 + 2 * (warp & 3) + (wg ^ 1);
     float m_used = -INFINITY, l_sum = 0.f;
-    {  // Q, scaled into f16's range
-      const int sub = lane / kQLanes, ch = lane - sub * kQLanes;
-#pragma unroll
+    {  // Q, scaled into f16's range in place (a lane's own pieces; a short loop, as the epilogue)
+      cp_async_wait_all();
+#pragma unroll 4
       for (int i = 0; i < kQLoads; ++i) {
-        const int qr = warp * (kRows / kSmWarps) + i * kQRpi + sub;
-        uint32_t w[4] = {qw[i].x, qw[i].y, qw[i].z, qw[i].w}, am = 0;
+        const int qr = q_row(i);
+        uint32_t w[4], am = 0;
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                     : "r"(q_dst(qr))
+                     : "memory");
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           am = max(am, max(kv8::abs_bits(unpack_lo<T>(w[k])), kv8::abs_bits(unpack_hi<T>(w[k]))));
@@ -729,9 +726,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const float mul = pow2i(14 - ex);
 #pragma unroll
         for (int k = 0; k < 4; ++k) w[k] = pack2_rn<__half>(unpack_lo<T>(w[k]) * mul, unpack_hi<T>(w[k]) * mul);
-        sts128(base + (ch >> 3) * C::kQBlock + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4), w[0], w[1], w[2], w[3]);
+        sts128(q_dst(qr), w[0], w[1], w[2], w[3]);
         // a row that is not finite gives NaN logits
-        if (ch == 0) rowf[qr] = am < 0x7f800000u ? a.scale * kLog2e * pow2i(max(ex - 14, -126)) : NAN;
+        if (q_ch == 0) rowf[qr] = am < 0x7f800000u ? a.scale * kLog2e * pow2i(max(ex - 14, -126)) : NAN;
       }
       tc::fence_proxy_async_smem();
       __syncwarp();

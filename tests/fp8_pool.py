@@ -7,8 +7,8 @@ from oracle import kv_fp8 as O
 
 DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 # relative error of an attention weight before the fp32 sums: the tensor-core kernels hold weights
-# in 16 significant-bit halves or in sums of e4m3 terms, of at least 8 bits for bfloat16 activations
-# (half a step is 2^-9, and a sum of two terms can be off by twice that) and 11 for float16; the
+# in f16 (11 bits; half a step is 2^-12 of the value), with bfloat16 activations the large-tile kernel
+# also rounds scaled codes to f16; 2^-8 and 2^-11 also admit weights in sums of e4m3 terms; the
 # fp32 path's exponentials are good to a few units of 2^-24
 WEIGHT_ERR = {"f32": 2.0 ** -20, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}
 

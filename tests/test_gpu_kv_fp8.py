@@ -439,6 +439,8 @@ EDGES = {
                                   [200 if i == 777 else i % 3 for i in range(2000)], {}),
     "extend_gqa24": ("bf16", 24, 1, 128, [33], [40], {}),
     "extend_gqa24_drafts": ("bf16", 24, 1, 128, [33, 250], [2, 1], dict(gate="silu")),
+    "extend_two_passes": ("bf16", 32, 4, 256, [900, 30, 513, 2000], [6, 1, 3, 5], dict(gate="sigmoid")),
+    "extend_two_passes_f16": ("f16", 12, 2, 64, [300, 7, 0], [8, 2, 1], {}),
     "extend_d64": ("bf16", 8, 2, 64, [500, 0], [301, 129], dict(gate="silu")),
     "extend_d64_f16": ("f16", 16, 2, 64, [333, 1], [150, 257], {}),
     "extend_split": ("bf16", 8, 1, 256, [3000, 0, 1], [70, 1, 200], dict(gate="sigmoid")),

@@ -11,18 +11,25 @@
 // mma.m16n8k32 on the codes themselves was measured at 36 clocks a warp instruction, against 8 for
 // the f16 form with half its depth plus its conversions.
 //
+// Measured (bf16, 32 heads over 4, head_dim 256).  128 decode requests of 512 to 8192 tokens: 226 to 239 us, 4.9 to
+// 5.2 TB/s (0.75 to 0.79 of the copy rate; 6.8 TB/s between the first tile and the last piece, the rest
+// is the plan, 4 us, the epilogues and the combine kernel, 9 us).  One request of 8191: 22.5 us, of which
+// the combine kernel 8 us.  24 requests with 2 to 5 new tokens: 102 us, bound by instruction latency
+// with two warps a scheduler (33% of issue slots; the registers hold no third).
+//
 // Fragments.  S^T = K8.Q^T: A = 16 tokens x 16 dims.  A thread's 16-byte read of a token's row is its A
 // fragment of four k-steps for the dim order 64 j + 16 t + 4 i + {0,1 | 2,3} (t = lane % 4), and Q^T is
 // held in the same order.  O^T = V8^T.W^T: A = 16 dims x 16 tokens, from ldmatrix.trans on pairs of
 // codes and a byte permute; row r of the fragment is dim 2 r, row r + 8 dim 2 r + 1.  W^T comes from
 // the logits' layout through movmatrix.
 //
-// Work.  A CTA has eight warps.  TEAM of them (a power of two) share stages of 32 tokens of one kv
-// head and take eight query rows each; HG kv heads of a group run side by side, so that a token's
-// rows of all heads, its scales and its slot id are read at about the same time (the warps of a team fetch tiles in
-// turn); the
+// Work.  A CTA has eight warps.  TEAM of them (one, or two above eight query rows) share stages of 32
+// tokens of one kv head, fetch them in turn and take eight query rows each, sixteen of them above 16 rows (two
+// row tiles on the same converted codes: 64 rows of a kv head 169 us, 192 us with eight rows a warp and
+// teams of eight); more rows than a team holds take further passes.  HG kv heads of a group run side by
+// side, so that a token's rows of all heads, its scales and its slot id are read at about the same time; the
 // WH = 8 / (TEAM HG) teams of a head take its tiles in turn and merge in shared memory.  The sequence
-// of (request, head group) units, each of ceil(len / 32) tiles, is cut into one range per CTA,
+// of (request, pass, head group) units, each of ceil(len / 32) tiles, is cut into one range per CTA,
 // balanced by tiles plus a fixed cost per unit; every CTA finds its own range from the lengths (a scan
 // of the batch in shared memory: no plan launch).  Units cut by a boundary leave (M, l, O) partials
 // for a combine kernel.  Rows are fetched by 16-byte cp.async (a bulk copy per row was measured at
@@ -1140,7 +1147,7 @@ static Shape shape_of(const tf_paged_attn_args& a, int num_sms) {
   s.smem = bytes(s.stages);
   s.nctas = num_sms;
   s.min_tiles = s.wh;  // one for each team (1000 tokens: 24.6 us, 28.7 us with two)
-  s.piece_cost = 8;
+  s.piece_cost = 8;  // a unit's epilogue and first loads, in tiles
   return s;
 }
 

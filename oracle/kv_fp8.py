@@ -1,6 +1,6 @@
 """The K/V pool held in 8 bits, in float64 numpy: quantization of rows to e4m3 codes and a scale, the
 prologue over it and attention over it (formulas in include/tfattn.h; the reference has no such
-pool).  The checker of the tf_*_fp8 entry points; the product path never touches it."""
+pool).  The oracle of the tf_*_fp8 entry points; the product path never touches it."""
 
 import numpy as np
 

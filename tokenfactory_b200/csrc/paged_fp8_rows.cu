@@ -1206,6 +1206,9 @@ bool paged_fp8_rows_supported(const tf_paged_attn_args& a) {
   if (a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256) return false;
   if ((int64_t)a.batch_size * rows8::passes_of(rows8::max_rows(a)) > rows8::kMaxBatch || a.r2t_rows > 0x7fffffff || a.r2t_cols > 0x7fffffff)
     return false;
+  // the scan of the tiles is kept in 32 bits
+  if (a.batch_size * (int64_t)rows8::passes_of(rows8::max_rows(a)) * (a.r2t_cols / rows8::kTok + 1) > 0x7fffffff)
+    return false;
   auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   // row offsets are kept in 32 bits of 16-byte pieces: pools of up to 64 GiB a layer
   if (a.num_slots * a.kv_stride_slot + a.num_kv_heads * a.kv_stride_head >= (int64_t)1 << 36) return false;

@@ -456,6 +456,19 @@ def test_edges(name):
     check(c.run(), c.reference(), dtype, d, name)
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("ext", [[1] * 9, [80, 1, 90]])
+def test_a_row_of_one_key_is_that_key(d, ext):
+    """float16: the only key's value, off by the output's rounding (half a step, 2^-11 of the value) and
+    a few fp32 operations (2^-20), whatever the weight's rounding was."""
+    c = Case(17, "f16", 8, 2, d, [0] * len(ext), ext, scale_spread=2.0)
+    got = c.run().double().cpu().numpy()
+    ref = c.reference()[0]
+    first = np.cumsum([0] + ext[:-1])
+    tol = (2.0 ** -11 + 2.0 ** -20) * np.abs(ref[first]) + 2.0 ** -25
+    assert (np.abs(got[first] - ref[first]) <= tol).all()
+
+
 def test_more_than_64_query_heads_per_kv_head_are_refused():
     from tokenfactory_b200 import _capi
     for ext in (1, 2):

@@ -118,6 +118,18 @@ __device__ __forceinline__ void scale_mask(float (&s)[32], const float* ks, int 
       if (k >= vis) s[k] = -INFINITY;
   }
 }
+// two exponentials p from their weights w = f16(p v): w / v, or p where w is below f16's normal range (a
+// small scale)
+__device__ __forceinline__ uint64_t as_rounded(uint32_t w, uint64_t v, uint64_t p) {
+  constexpr float kNormal = 1.f / 16384.f;
+  const float w0 = unpack_lo<__half>(w), w1 = unpack_hi<__half>(w);
+  float v0, v1, p0, p1;
+  up2(v, v0, v1);
+  up2(p, p0, p1);
+  if (fabsf(w0) >= kNormal) p0 = w0 * __fdividef(1.f, v0);
+  if (fabsf(w1) >= kNormal) p1 = w1 * __fdividef(1.f, v1);
+  return pk2(p0, p1);
+}
 __device__ __forceinline__ void bar_arrive(int id, int nthreads) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }
@@ -814,6 +826,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
       }
       const float nmu = m_new == -INFINITY ? 0.f : -m_new;
+      // float16 outputs carry as many bits as the weights.  In a request's first tile l sums the weights as
+      // rounded, so that a rounding moves weight between keys and leaves their sum one (a row of one key
+      // is exact); over more keys the roundings average out, and the reciprocals would cost 128 a row.
+      const bool sum_rounded = !kFold && jb + j == 0;
 #pragma unroll 1
       for (int g = 0; g < 4; ++g) {
         float s[32];
@@ -836,16 +852,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           e1 = ex2_ftz(e1);
           e2 = ex2_ftz(e2);
           e3 = ex2_ftz(e3);
-          const uint64_t p01 = pk2(e0, e1), p23 = pk2(e2, e3);
-          ls2[0] = add2(ls2[0], p01);
-          ls2[1] = add2(ls2[1], p23);
+          uint64_t p01 = pk2(e0, e1), p23 = pk2(e2, e3);
           if (!kFold) {
             const ulonglong2 v = vp[k];
             up2(mul2(p01, v.x), e0, e1);
             up2(mul2(p23, v.y), e2, e3);
+            pk[2 * k] = __uint_as_float(pack2_rn<__half>(e0, e1));
+            pk[2 * k + 1] = __uint_as_float(pack2_rn<__half>(e2, e3));
+            if (sum_rounded) {
+              p01 = as_rounded(__float_as_uint(pk[2 * k]), v.x, p01);
+              p23 = as_rounded(__float_as_uint(pk[2 * k + 1]), v.y, p23);
+            }
+          } else {
+            pk[2 * k] = __uint_as_float(pack2_rn<__half>(e0, e1));
+            pk[2 * k + 1] = __uint_as_float(pack2_rn<__half>(e2, e3));
           }
-          pk[2 * k] = __uint_as_float(pack2_rn<__half>(e0, e1));
-          pk[2 * k + 1] = __uint_as_float(pack2_rn<__half>(e2, e3));
+          ls2[0] = add2(ls2[0], p01);
+          ls2[1] = add2(ls2[1], p23);
         }
         float h0, h1;
         up2(add2(ls2[0], ls2[1]), h0, h1);

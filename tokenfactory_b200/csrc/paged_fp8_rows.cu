@@ -7,7 +7,8 @@
 // a power of two per row into f16's range (exact for bfloat16 too); the only rounding before the
 // output is that of the weights w_j = 2^(s_j + ev - M) vs_j 2^(7 - ev) to f16 (11 bits).  ev is the
 // exponent of the largest vs of a tile and M the running maximum of s_j + ev, so that w stays in
-// f16's range whatever the scales are; the sum of weights l = sum 2^(s_j - M) is fp32.
+// f16's range whatever the scales are; the sum of weights l = sum 2^(s_j - M) is fp32 (for float16, of
+// the weights as rounded).
 // mma.m16n8k32 on the codes themselves was measured at 36 clocks a warp instruction, against 8 for
 // the f16 form with half its depth plus its conversions.
 //
@@ -521,8 +522,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   // ---- producer: this team's tiles in sequence, their req_to_token entries kAhead tiles ahead
   const int ntiles = (int)(g1 - g0);
   constexpr int kAhead = 2;
-  int64_t raw[kAhead];
-  int head[kAhead];           // their kv heads
+  int64_t raw[kAhead] = {};
+  int head[kAhead] = {};           // their kv heads
   int pf = 0, pf_unit = INT32_MIN;  // tiles of the unit whose entries have been asked for; its first tile
   int pq = wsel + sh.wh * member - kAhead * f_step;  // next tile to fetch (before the first: the entries'
   const int f_first = wsel + sh.wh * member;         // own head start)
@@ -782,6 +783,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int o = 4; o < 32; o <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
         const int ev = min(max((int)(__float_as_uint(vmax) >> 23) - 127, -100), 126);
         const float vmul = pow2i(max(7 - ev, -126)), lmul = pow2i(max(-ev, -126));
+        // float16 outputs carry as many bits as the weights: l then sums the weights as rounded, so that a
+        // rounding moves weight between tokens and leaves their sum one (a row of one token is exact).  Weights
+        // below f16's normal range (a small scale beside the tile's largest) count as they are.
+        constexpr bool kSumRounded = std::is_same<T, __half>::value;
+        float rv[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rv[i] = kSumRounded ? __fdividef(1.f, vsc[i] * vmul) : 0.f;
         uint32_t wb[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -826,11 +834,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               sv[i][k] = ex2(sv[i][k] + sub);
-              ls += sv[i][k];
+              const float w = sv[i][k] * (vsc[i] * vmul);
+              if (kSumRounded) {
+                const float wr = __half2float(__float2half_rn(w));
+                ls += fabsf(wr) >= 1.f / 16384.f ? wr * rv[i] : sv[i][k];
+              } else {
+                ls += sv[i][k];
+              }
+              sv[i][k] = w;
             }
             l[n][k] = fmaf(ls, lmul, l[n][k] * al[k]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sv[i][k] *= vsc[i] * vmul;
           }
           if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {
 #pragma unroll

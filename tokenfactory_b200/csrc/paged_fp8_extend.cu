@@ -75,6 +75,15 @@ __device__ __forceinline__ float ex2_ftz(float x) {
 }
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126..127
 
+// What a group's products are multiplied by to be logits: the row's factor times the group's 2^kx, kept in
+// fp32's normal range.  Both are small for a row of zeros over keys of zeros, and a product of 0 would
+// turn the -inf of a hidden key into a NaN; products are at most 2^32, so that with 2^-126 their logits
+// are 0 to 2^-94.  A factor that is NaN (a query row that is not finite) stays NaN.
+__device__ __forceinline__ float logit_factor(float c2, float kx) {
+  const float f = c2 * kx;
+  return f < 0x1p-126f ? 0x1p-126f : f;
+}
+
 // two fp32 operations in one instruction (each rounded as its scalar form)
 __device__ __forceinline__ uint64_t pk2(float a, float b) {
   uint64_t r;
@@ -790,7 +799,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const int g = 2 * hf + k;
             scale_mask<kFold>(s[k], ks + 32 * g, vis - 32 * g);
             const float2 e = *reinterpret_cast<const float2*>(grp + g);
-            tmax = fmaxf(tmax, fmaf(max_of_32(s[k]), c2 * e.x, e.y));  // c2 > 0
+            tmax = fmaxf(tmax, fmaf(max_of_32(s[k]), logit_factor(c2, e.x), e.y));  // factor > 0
           }
         }
       }
@@ -837,7 +846,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         tc::wait_ld();
         scale_mask<kFold>(s, ks + 32 * g, vis - 32 * g);
         const float4 e = grp[g];
-        const float cg = c2 * e.x, ng = kFold ? nmu + e.y : nmu;
+        const float cg = logit_factor(c2, e.x), ng = kFold ? nmu + e.y : nmu;
         const uint64_t c22 = pk2(cg, cg), nmu2 = pk2(ng, ng);
         uint64_t ls2[2] = {0, 0};
         float pk[16];

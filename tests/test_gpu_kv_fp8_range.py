@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 from oracle import kv_fp8 as O
+from tests import kv_fp8_bounds as B
 from tests.fp8_pool import DTYPES, Case, check
 
 torch = pytest.importorskip("torch")
@@ -70,3 +71,69 @@ def test_extend_over_a_pool_of_zero_scales(name):
     c.q[::3] = 0
     c.scale.zero_()
     check(c.run(), c.reference(), "bf16", d, name)
+
+
+# rows of very different size beside each other: what is hidden from a query, or seen with next to no
+# weight, must not cost the others their bits.  dtype, (hq, hkv, d, prefixes, new tokens), and whether
+# single tokens go through decode
+MIXED = {
+    "decode": ("bf16", 8, 2, 128, [399, 0, 70], [1, 1, 1]),
+    "decode_f16": ("f16", 8, 1, 256, [399, 0, 70], [1, 1, 1]),
+    "drafts": ("bf16", 8, 2, 256, [300, 0, 61], [5, 1, 8]),
+    "drafts_f16": ("f16", 8, 2, 64, [300, 0, 61], [5, 1, 8]),
+    "simt": ("bf16", 8, 2, 80, [0, 40], [5, 49]),
+}
+
+
+def _check_bound(c, what):
+    ext = any(e != 1 for e in c.ext)
+    B.check(c.run(force_extend=ext), B.reference(c, B.kernel_of(c, ext)), what)
+
+
+@pytest.mark.parametrize("name", [n for n in MIXED if "decode" not in n])
+@pytest.mark.parametrize("which", [0, 1])
+def test_large_rows_hidden_from_earlier_queries(name, which):
+    """K or V rows of the type's largest size (bf16: 3e38, a scale of 2^119) at the last new token of each
+    request, which only the last query sees; its queries are zeros, so that no logit overflows."""
+    dtype, hq, hkv, d, pre, ext = MIXED[name]
+    c = Case(44, dtype, hq, hkv, d, pre, ext)
+    big = 0.9 * torch.finfo(DTYPES[dtype]).max
+    g = torch.Generator().manual_seed(1)
+    at = np.cumsum(ext) - 1
+    for r, n in enumerate(c.seq):
+        x = torch.rand(d, generator=g) * 2 - 1
+        x[0] = 1
+        _put(c, r, n - 1, which, big * x)
+        c.q[at[r]] = 0
+    _check_bound(c, name)
+
+
+@pytest.mark.parametrize("name", list(MIXED))
+def test_large_values_beside_small_ones(name):
+    """Every seventh V row is 2^20 (fp16: 2^12) larger and meets logits far below the others' (its K row
+    points away from the queries): weights of about 2^-45 beside ordinary ones."""
+    dtype, hq, hkv, d, pre, ext = MIXED[name]
+    c = Case(45, dtype, hq, hkv, d, pre, ext, scale_spread=0.0)
+    u = torch.zeros(d)
+    u[::2] = 1
+    c.q = (c.q.float() * 0.5 + u).to(DTYPES[dtype])
+    v = torch.randn(d, generator=torch.Generator().manual_seed(2))
+    for r, n in enumerate(c.seq):
+        for j in range(3, n, 7):
+            _put(c, r, j, 0, -(64.0 / d ** 0.5) * u)
+            _put(c, r, j, 1, (2.0 ** 20 if dtype == "bf16" else 2.0 ** 12) * v)
+    _check_bound(c, name)
+
+
+@pytest.mark.parametrize("name", list(MIXED))
+def test_rows_of_every_size(name):
+    """K and V scales spread over 2^+-40 (fp16 outputs: V over 2^-30 to 2^6), query sizes to match, so that
+    logits stay ordinary."""
+    dtype, hq, hkv, d, pre, ext = MIXED[name]
+    c = Case(46, dtype, hq, hkv, d, pre, ext, scale_spread=0.0)
+    g = torch.Generator().manual_seed(3)
+    n = len(c.scale)
+    lo, hi = (-40, 40) if dtype == "bf16" else (-30, 6)
+    c.scale[..., 1] *= torch.exp2(torch.randint(lo, hi, (n, hkv), generator=g).float())
+    c.scale[..., 0] *= torch.exp2(torch.randint(-40, 1, (n, hkv), generator=g).float())
+    _check_bound(c, name)

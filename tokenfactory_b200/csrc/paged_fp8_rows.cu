@@ -5,10 +5,12 @@
 //   s_j = (q . K8_j) ks_j scale log2(e)      out = sum_j 2^(s_j) vs_j V8_j / sum_j 2^(s_j).
 // Both products run as mma.m16n8k16 f16 with fp32 sums.  e4m3 codes are exact in f16; q is scaled by
 // a power of two per row into f16's range (exact for bfloat16 too); the only rounding before the
-// output is that of the weights w_j = 2^(s_j + ev - M) vs_j 2^(7 - ev) to f16 (11 bits).  ev is the
-// exponent of the largest vs of a tile and M the running maximum of s_j + ev, so that w stays in
-// f16's range whatever the scales are; the sum of weights l = sum 2^(s_j - M) is fp32 (for float16, of
-// the weights as rounded).
+// output is that of the weights w_j = 2^(s_j - M) vs_j 2^7 to f16 (11 bits).  With ev_j the exponent of
+// vs_j, M is the running maximum of s_j + ev_j over the tokens that the row sees: its largest w is in
+// [2^7, 2^8) whatever the scales are, and only weights 2^21 below it are subnormal in f16.  (With one
+// exponent for a tile, a token of a large scale took the bits of its neighbours' weights, also for rows
+// that do not see it.)  The sum of weights l = sum 2^(s_j - M) is fp32 (for float16, of the weights as
+// rounded), kept times 2^40 so that no scale takes it out of range.
 // mma.m16n8k32 on the codes themselves was measured at 36 clocks a warp instruction, against 8 for
 // the f16 form with half its depth plus its conversions.
 //
@@ -50,6 +52,9 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kTok = 32;  // tokens of a tile
 constexpr int kCache = 96;  // requests whose metadata a CTA keeps in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
+// Exponentials 2^(s - M) and their sum are kept times 2^40: as M is the maximum of s + ev, the largest of
+// them is between 2^-119 (the store's largest scale) and 2^50 (its smallest), and fp32 has room around both.
+constexpr float kBiasLog2 = 40.f, kBias = 0x1p40f;
 constexpr int kMaxCtas = 256;
 constexpr int kMaxBatch = 32768;  // passes of all requests: their scan lives in the ring's shared memory
 
@@ -178,6 +183,12 @@ __device__ __forceinline__ bool wait_uses(const uint32_t* c, uint32_t n) {  // b
   }
 }
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126..127
+// 2^((from - to) / 2), from <= to: sums relative to `from` times its square are relative to `to`.  A sum of
+// weights is multiplied by it twice: maxima of s + ev can be more than fp32's 2^126 apart where the sums
+// of 2^s are not.
+__device__ __forceinline__ float fade(float from, float to) {
+  return from == to ? 1.f : ex2(0.5f * (from - to));
+}
 
 // tiles of a request: none when it has no query rows or a length its table cannot hold
 __device__ __forceinline__ int64_t checked_len(const tf_paged_attn_args& a, int b, int64_t& ext,
@@ -330,7 +341,7 @@ __device__ __noinline__ void finish64(const tf_paged_attn_args& a, const Shape& 
         o.w = fmaf(f, x.w, o.w);
       }
       if (whole) {
-        const float inv = (1.f / 128.f) / ml[2 * pr + 1];
+        const float inv = (kBias / 128.f) / ml[2 * pr + 1];
         put4<T>(a, th[k].x, th[k].y, d0 + 4 * v, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), gw[k], v8);
       } else {
         const int64_t ps = (int64_t)slot * kWarps * kRows + pr;
@@ -770,26 +781,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // ---- scales of tokens gq + 8 i.  One that is not finite: NaN logits for the rows that see
         // the token, weight 0 for the others
-        float ksc[4], vsc[4], vmax = 0.f;
+        float ksc[4], ev[4], vn[4];  // K scale, exponent of the V scale, V scale 2^7 / kBias
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float2 p = *reinterpret_cast<const float2*>(stage + C::kOffScale + (gq + 8 * i) * 8);
           const bool fin = kv8::abs_bits(p.x) < 0x7f800000u && kv8::abs_bits(p.y) < 0x7f800000u;
           ksc[i] = fin ? p.x : NAN;
-          vsc[i] = fin ? p.y : 0.f;
-          vmax = fmaxf(vmax, fabsf(vsc[i]));
+          const float vs = fin ? p.y : 0.f;
+          // (the store's smallest scale is 1e-12 / 448, its exponent -49)
+          ev[i] = (float)max((int)(kv8::abs_bits(vs) >> 23) - 127, -50);
+          vn[i] = vs * (128.f / kBias);
         }
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
-        const int ev = min(max((int)(__float_as_uint(vmax) >> 23) - 127, -100), 126);
-        const float vmul = pow2i(max(7 - ev, -126)), lmul = pow2i(max(-ev, -126));
         // float16 outputs carry as many bits as the weights: l then sums the weights as rounded, so that a
         // rounding moves weight between tokens and leaves their sum one (a row of one token is exact).  Weights
-        // below f16's normal range (a small scale beside the tile's largest) count as they are.
+        // below f16's normal range count as they are.
         constexpr bool kSumRounded = std::is_same<T, __half>::value;
         float rv[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) rv[i] = kSumRounded ? __fdividef(1.f, vsc[i] * vmul) : 0.f;
+        for (int i = 0; i < 4; ++i) rv[i] = kSumRounded ? __fdividef(1.f, vn[i]) : 0.f;
         uint32_t wb[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -804,7 +813,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int k = 0; k < 2; ++k) {
               const int e = 2 * (i & 1) + k;
               const float x = CH == 1 ? s[i >> 1][n][0][e] : s[i >> 1][n][0][e] + s[i >> 1][n][CH - 1][e];
-              sv[i][k] = x * ksc[i] * c2[n][k];
+              sv[i][k] = x * (ksc[i] * c2[n][k]);
             }
           if (tok0 + kTok > lim_min) {  // some token is hidden from some row
 #pragma unroll
@@ -816,7 +825,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           float mx[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k)
-            mx[k] = fmaxf(fmaxf(sv[0][k], sv[1][k]), fmaxf(sv[2][k], sv[3][k]));
+            mx[k] = fmaxf(fmaxf(sv[0][k] + ev[0], sv[1][k] + ev[1]), fmaxf(sv[2][k] + ev[2], sv[3][k] + ev[3]));
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) {
             mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], o));
@@ -826,15 +835,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             // a tile hidden from the row as a whole keeps M (and -inf - -inf out of the exponent)
-            const float mn = fmaxf(M[n][k], mx[k] + (float)ev);
-            al[k] = M[n][k] == mn ? 1.f : ex2(M[n][k] - mn);
+            const float mn = fmaxf(M[n][k], mx[k]);
+            const float ah = fade(M[n][k], mn);
+            al[k] = ah * ah;
             M[n][k] = mn;
-            const float sub = mn == -INFINITY && tok0 >= lim[n][k] ? 0.f : (float)ev - mn;
-            float ls = 0.f;
+            const float sub = mn == -INFINITY && tok0 >= lim[n][k] ? 0.f : kBiasLog2 - mn;
+            float ls = l[n][k] * ah * ah;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               sv[i][k] = ex2(sv[i][k] + sub);
-              const float w = sv[i][k] * (vsc[i] * vmul);
+              const float w = sv[i][k] * vn[i];
               if (kSumRounded) {
                 const float wr = __half2float(__float2half_rn(w));
                 ls += fabsf(wr) >= 1.f / 16384.f ? wr * rv[i] : sv[i][k];
@@ -843,7 +853,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               sv[i][k] = w;
             }
-            l[n][k] = fmaf(ls, lmul, l[n][k] * al[k]);
+            l[n][k] = ls;
           }
           if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {
 #pragma unroll
@@ -937,9 +947,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             float mx = -INFINITY, ls = 0.f;
             for (int w = tid; w < kWarps * kRows; w += per * kRows) mx = fmaxf(mx, ml[2 * w]);
             for (int w = tid; w < kWarps * kRows; w += per * kRows) {
-              const float mw = ml[2 * w], f = mw == mx ? 1.f : ex2(mw - mx);
-              fac[w] = f;
-              ls = fmaf(f, ml[2 * w + 1], ls);
+              const float h = fade(ml[2 * w], mx);
+              fac[w] = h * h;
+              ls = fmaf(h, h * ml[2 * w + 1], ls);
             }
             ml[2 * tid] = mx;
             ml[2 * tid + 1] = ls;
@@ -1068,21 +1078,22 @@ __global__ void __launch_bounds__(THREADS)
     float mn = M;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) mn = fmaxf(mn, ml[j].x);
-    const float f0 = M == mn ? 1.f : ex2(M - mn);
+    const float h0 = fade(M, mn), f0 = h0 * h0;
     o.x *= f0;
     o.y *= f0;
     o.z *= f0;
     o.w *= f0;
-    l *= f0;
+    l *= h0;
+    l *= h0;
     M = mn;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      const float f = ml[j].x == mn ? 1.f : ex2(ml[j].x - mn);
+      const float h = fade(ml[j].x, mn), f = h * h;
       o.x = fmaf(f, x[j].x, o.x);
       o.y = fmaf(f, x[j].y, o.y);
       o.z = fmaf(f, x[j].z, o.z);
       o.w = fmaf(f, x[j].w, o.w);
-      l = fmaf(f, ml[j].y, l);
+      l = fmaf(h, h * ml[j].y, l);
     }
   }
   if constexpr (PG > 1) {  // the groups meet
@@ -1101,9 +1112,10 @@ __global__ void __launch_bounds__(THREADS)
     float t[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int p = 0; p < PG; ++p) {
-      const float mp = red[p * kG + tid][5], f = mp == mn ? 1.f : ex2(mp - mn);
+      const float h = fade(red[p * kG + tid][5], mn), f = h * h;
 #pragma unroll
-      for (int i = 0; i < 5; ++i) t[i] = fmaf(f, red[p * kG + tid][i], t[i]);
+      for (int i = 0; i < 4; ++i) t[i] = fmaf(f, red[p * kG + tid][i], t[i]);
+      t[4] = fmaf(h, h * red[p * kG + tid][4], t[4]);
     }
     o = make_float4(t[0], t[1], t[2], t[3]);
     l = t[4];
@@ -1112,7 +1124,7 @@ __global__ void __launch_bounds__(THREADS)
   const int64_t tok = start + rr / G;
   if (rr < ext * G && tok < a.num_tokens) {
     const int hq = (u * sh.hg + hsel) * G + rr % G;
-    const float inv = (1.f / 128.f) / l;
+    const float inv = (kBias / 128.f) / l;
     const bool v8 = rows_v8(a);
     uint2 gw = make_uint2(0, 0);
     if (a.gate_mode != TF_GATE_NONE) gw = gate4<T>(a, tok, hq, 4 * v, v8);

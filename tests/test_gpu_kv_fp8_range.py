@@ -81,6 +81,11 @@ MIXED = {
     "decode_f16": ("f16", 8, 1, 256, [399, 0, 70], [1, 1, 1]),
     "drafts": ("bf16", 8, 2, 256, [300, 0, 61], [5, 1, 8]),
     "drafts_f16": ("f16", 8, 2, 64, [300, 0, 61], [5, 1, 8]),
+    "tile": ("bf16", 8, 2, 256, [0, 40], [150, 77]),
+    "tile_f16": ("f16", 8, 2, 128, [0, 40], [150, 77]),
+    "tile_d64": ("bf16", 8, 2, 64, [0, 40], [150, 77]),
+    "tile_split": ("bf16", 8, 1, 256, [3000, 0, 1], [70, 1, 200]),
+    "tile_split_f16": ("f16", 8, 1, 256, [3000, 0, 1], [70, 1, 200]),
     "simt": ("bf16", 8, 2, 80, [0, 40], [5, 49]),
 }
 
@@ -136,4 +141,21 @@ def test_rows_of_every_size(name):
     lo, hi = (-40, 40) if dtype == "bf16" else (-30, 6)
     c.scale[..., 1] *= torch.exp2(torch.randint(lo, hi, (n, hkv), generator=g).float())
     c.scale[..., 0] *= torch.exp2(torch.randint(-40, 1, (n, hkv), generator=g).float())
+    _check_bound(c, name)
+
+
+@pytest.mark.parametrize("name", [n for n in MIXED if MIXED[n][0] == "bf16"])
+def test_groups_of_large_values_far_above_the_others(name):
+    """V rows 2^110 larger in whole groups of keys, with logits 14 below the others': they make the output, the
+    others its sum of weights."""
+    dtype, hq, hkv, d, pre, ext = MIXED[name]
+    c = Case(47, dtype, hq, hkv, d, pre, ext, scale_spread=0.0)
+    u = torch.zeros(d)
+    u[::2] = 1
+    c.q = (c.q.float() * 0.5 + u).to(DTYPES[dtype])
+    g = torch.Generator().manual_seed(4)
+    for r, n in enumerate(c.seq):
+        for j in range(128, 256) if n > 256 else range(32, min(n, 64)):
+            _put(c, r, j, 0, -(28.0 / d ** 0.5) * u)
+            _put(c, r, j, 1, 2.0 ** 110 * torch.randn(d, generator=g))
     _check_bound(c, name)

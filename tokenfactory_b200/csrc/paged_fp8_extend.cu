@@ -13,14 +13,20 @@
 //   scales      enter as powers of two of groups of 32 keys (2^kx_g, 2^ev_g, the exponents of the
 //               group's largest ks and vs) in the softmax, where they cost nothing: a logit is
 //               S c2 2^kx_g, its weight for P 2^(logit + ev_g - M), and l sums the weights times 2^-ev_g.
-//               M follows logit + ev_g, so that P stays in f16's range whatever the scales are.
-//               The rest of each scale, in [0, 2):
+//               M follows logit + ev_g, so that P stays in f16's range.
+//               The rest of each scale, in [2^-6, 2):
 //               bfloat16: the producers multiply it into the codes (to f16: 11 bits, random, eight
 //               times finer than the output's rounding; two f16 operations a pair, with the scale's
 //               own low bits in the first, so that it is not rounded for a whole row at once);
 //               float16: the codes stay exact and the softmax multiplies logit and weight by it in
 //               fp32, which leaves the weight's f16 rounding alone before the output's.  It costs
 //               two reads and two products more per score: 2.5 us a key tile against 2.3 us.
+//               A group whose scales are further than 2^6 apart (rows of zeros among others, outliers) is
+//               "wide": one key must not take the bits of the others, least of all a key that a row does
+//               not see.  Its keys have exponents of their own, which the softmax reads from shared
+//               memory; the codes carry what is left of a scale, in [1, 2).
+//               l and its exponentials are kept times 2^40: M is between s_max - 50 and s_max + 119 (the
+//               store's smallest and largest scale), and both ends then lie inside fp32's range.
 //   Q           is scaled by a power of two per row into f16's range (bfloat16 stays exact)
 // A scale that is not finite gives its key NaN logits and a V row of zeros, so that only the rows that
 // see it are NaN.  Every wait is bounded; one that gives up raises an abort flag in both CTAs and
@@ -54,6 +60,10 @@ constexpr int kFwdWarp = kIssueWarp + 1;         // rank 1: forwards "P written"
 constexpr int kThreads = (kFwdWarp + 1) * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleLog2 = 8.f;
+constexpr float kBiasLog2 = 40.f, kBias = 0x1p40f;  // of l and its exponentials
+constexpr int kSpread = 6;           // exponents that a group's scales may be apart
+constexpr float kWide = -1000.f;     // in the place of a wide group's ev
+constexpr float kFarLog2 = 80.f;     // M this far above a group's ev: P may be 0 where l's terms are not
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
@@ -75,13 +85,25 @@ __device__ __forceinline__ float ex2_ftz(float x) {
 }
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126..127
 
-// What a group's products are multiplied by to be logits: the row's factor times the group's 2^kx, kept in
-// fp32's normal range.  Both are small for a row of zeros over keys of zeros, and a product of 0 would
-// turn the -inf of a hidden key into a NaN; products are at most 2^32, so that with 2^-126 their logits
-// are 0 to 2^-94.  A factor that is NaN (a query row that is not finite) stays NaN.
+// 2^((from - to) / 2), from <= to; a sum of weights goes from one maximum to another by its square, taken
+// in two steps: maxima can be more than fp32's 2^126 apart where the sums of weights are not
+__device__ __forceinline__ float fade(float from, float to) {
+  return from == to ? 1.f : ex2_ftz(0.5f * (from - to));
+}
+__device__ __forceinline__ float lg2_ftz(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// What a group's products are multiplied by to be logits: the row's factor times the group's 2^kx, at least
+// kFloor.  Both are small for a row of zeros over keys of zeros, and a product of 0 would turn the -inf of a
+// hidden key into a NaN; products are at most 2^32, so that with 2^-90 their logits are 0 to 2^-58.  A factor
+// that is NaN (a query row that is not finite) stays NaN.
+constexpr float kFloor = 0x1p-90f;
 __device__ __forceinline__ float logit_factor(float c2, float kx) {
   const float f = c2 * kx;
-  return f < 0x1p-126f ? 0x1p-126f : f;
+  return f < kFloor ? kFloor : f;
 }
 
 // two fp32 operations in one instruction (each rounded as its scalar form)
@@ -287,8 +309,9 @@ struct Cfg {
   static constexpr int kOffKs = kOffRow + kRows * 4;             // float [kScaleTiles][kKeys]
   static constexpr int kOffVs = kOffKs + kScaleTiles * kKeys * 4;
   static constexpr int kOffGrp = kOffVs + kScaleTiles * kKeys * 4;  // float4 [kScaleTiles][4]: a group's
-                                                                  // 2^kx, ev, 2^-ev
-  static constexpr int kSmem = kOffGrp + kScaleTiles * 4 * 16 + 1024;
+                                                                  // 2^kx, ev, 2^-ev kBias
+  static constexpr int kOffEv = kOffGrp + kScaleTiles * 4 * 16;  // float [kScaleTiles][4]: ev, or kWide
+  static constexpr int kSmem = kOffEv + kScaleTiles * 4 * 4 + 1024;
   static constexpr int kColS = 0;                 // two S buffers of kKeys columns; P_j over S_j
   static constexpr int kColO = 2 * kKeys;
   static constexpr int kTmemCols = 512;
@@ -315,6 +338,65 @@ __device__ __forceinline__ void ld16(uint32_t taddr, float (&v)[16]) {
       : "memory");
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// What a tile of wide groups needs beside the common path.  Out of line: it is rare, and the tile loop's
+// instructions are fetched once a tile.  A row's products S of the tile's 128 keys sit in the lane's TMEM
+// columns sa..; keys [0, vis) are visible.
+//
+// exact codes: the largest logit + log2 of the V scale (ks times 2^kx of the group times c2 is what the
+// products are multiplied by, vs the V scales over kBias)
+__device__ __noinline__ float wide_max(uint32_t sa, const float* ks, const float* vs, const float4* grp, float c2,
+                                       int vis) {
+  float m = -INFINITY;
+#pragma unroll 1
+  for (int g = 0; g < 8; ++g) {
+    const float factor = logit_factor(c2, grp[g >> 1].x);
+    float s[16];
+    ld16(sa + 16 * g, s);
+    tc::wait_ld();
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      // (a V row of zeros counts as one of the store's smallest scale)
+      const float x = fmaf(s[k], ks[16 * g + k] * factor, fmaxf(lg2_ftz(fabsf(vs[16 * g + k])) + kBiasLog2, -50.f));
+      if (16 * g + k < vis) m = fmaxf(m, x);
+    }
+  }
+  return m;
+}
+// folded codes: the products of wide groups (2^kx of 0) become (logit + ev) / kFloor with their keys' own
+// exponents, ks = 2^kx and vs = 2^ev / kBias; logit_factor of such a group is kFloor
+__device__ __noinline__ void wide_logits(uint32_t sa, const float* ks, const float* vs, const float4* grp, float c2) {
+#pragma unroll 1
+  for (int g = 0; g < 8; ++g) {
+    if (grp[g >> 1].x != 0.f) continue;
+    float s[16];
+    ld16(sa + 16 * g, s);
+    tc::wait_ld();
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      s[k] = fmaf(s[k], ks[16 * g + k] * c2, lg2_ftz(vs[16 * g + k]) + kBiasLog2) * (1.f / kFloor);
+    tc::st16(sa + 16 * g, s);
+  }
+  tc::wait_st();
+}
+// the sum of 2^(logit - M) kBias, bias_m = kBiasLog2 - M, where a sum of weights over 2^ev would not do
+__device__ __noinline__ float wide_sum(uint32_t sa, const float* ks, const float* vs, const float4* grp, float c2,
+                                       int vis, float bias_m) {
+  float sum = 0.f;
+#pragma unroll 1
+  for (int g = 0; g < 8; ++g) {
+    const bool own = grp[g >> 1].x == 0.f;
+    float s[16];
+    ld16(sa + 16 * g, s);
+    tc::wait_ld();
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const float x = own ? s[k] * kFloor - (lg2_ftz(vs[16 * g + k]) + kBiasLog2) : s[k] * (ks[16 * g + k] * c2);
+      if (16 * g + k < vis) sum += ex2_ftz(x + bias_m);
+    }
+  }
+  return sum;
 }
 
 // 16-byte pieces of the gate and output rows can be moved whole
@@ -353,6 +435,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   float* ks_s = reinterpret_cast<float*>(sbase + C::kOffKs);
   float* vs_s = reinterpret_cast<float*>(sbase + C::kOffVs);
   float4* grp_s = reinterpret_cast<float4*>(sbase + C::kOffGrp);
+  float* ev_s = reinterpret_cast<float*>(sbase + C::kOffEv);
   constexpr bool kFold = !std::is_same<T, __half>::value;  // scales multiplied into the codes
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -542,18 +625,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       auto put = [&](int tile, uint4 (&w)[kLoads], float2 s2) {
         // A scale that is not finite: NaN logits (K), and a V row of zeros
         const bool fin = kv8::abs_bits(s2.x) < 0x7f800000u && kv8::abs_bits(s2.y) < 0x7f800000u;
-        auto group_exp = [&](float x) {  // exponent of the group's largest |scale|
-          const uint32_t m = __reduce_max_sync(0xffffffffu, fin ? kv8::abs_bits(x) : 0u);
-          return min(max((int)(m >> 23) - 127, -100), 100);
-        };
-        const int kx = kFold || kV ? group_exp(s2.x) : 0, ev = kV ? group_exp(s2.y) : 0;
+        const int gk = (int)(__reduce_max_sync(0xffffffffu, fin ? kv8::abs_bits(s2.x) : 0u) >> 23);
+        const int gv = (int)(__reduce_max_sync(0xffffffffu, fin ? kv8::abs_bits(s2.y) : 0u) >> 23);
+        const int own_k = (int)(kv8::abs_bits(s2.x) >> 23), own_v = (int)(kv8::abs_bits(s2.y) >> 23);
+        const bool wide = __any_sync(0xffffffffu, fin && (gk - own_k > kSpread || gv - own_v > kSpread));
+        // exponents of the key, its own or its group's (fp16 keeps the rest of a scale in fp32: its group's)
+        const int kx = min(max((kFold && wide && fin ? own_k : gk) - 127, -100), 126);
+        const int ev = min(max((kFold && wide && fin ? own_v : gv) - 127, -50), 126);
         if (kV) {
           const int st = tile & (C::kScaleTiles - 1);
-          if (!kFold) {
-            ks_s[st * kKeys + my_key] = fin ? s2.x * pow2i(-kx) : NAN;
-            vs_s[st * kKeys + my_key] = fin ? s2.y : 0.f;
+          ks_s[st * kKeys + my_key] = fin ? (kFold ? pow2i(kx) : s2.x * pow2i(-kx)) : NAN;
+          vs_s[st * kKeys + my_key] = kFold ? pow2i(ev) * (1.f / kBias) : fin ? s2.y * (1.f / kBias) : 0.f;
+          if (lane == 0) {
+            const bool own = kFold && wide;  // (logit_factor, wide_logits)
+            grp_s[st * 4 + pw - 4] = own ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                         : make_float4(pow2i(kx), (float)ev, pow2i(-ev) * kBias, 0.f);
+            ev_s[st * 4 + pw - 4] = wide ? kWide : (float)ev;
           }
-          if (lane == 0) grp_s[st * 4 + pw - 4] = make_float4(pow2i(kx), (float)ev, pow2i(-ev), 0.f);
           __syncwarp();
           if (lane == 0) mbar_arrive(&sc_full[st]);
         }
@@ -774,6 +862,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int64_t rem = row_valid ? klim - (int64_t)(jb + j) * kKeys : 0;
       const int vis = rem <= 0 ? 0 : (rem >= kKeys ? kKeys : (int)rem);
       if (ok) ok = __all_sync(0xffffffffu, wait_bar<false>(&sc_full[si], (j / C::kScaleTiles) & 1, abort, peer_abort));
+      const float4 evs = *reinterpret_cast<const float4*>(ev_s + si * 4);
+      const float ev_min = fminf(fminf(evs.x, evs.y), fminf(evs.z, evs.w));
+      const bool wide = ev_min == kWide;  // some group of the tile
       if (ok) ok = __all_sync(0xffffffffu, wait_bar<false>(&s_full[wg], (j >> 1) & 1, abort, peer_abort));
       if (idle) {  // P stays what S left there: it reaches only rows that are not stored
         tc::fence_before_sync();
@@ -786,8 +877,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       float tmax = -INFINITY;
       const float4* grp = grp_s + si * 4;
-      if (ok) {
-        tc::fence_after_sync();
+      if (ok) tc::fence_after_sync();
+      if (ok && wide && kFold) wide_logits(sa, ks, vs, grp, c2);
+      if (ok && wide && !kFold) {
+        tmax = wide_max(sa, ks, vs, grp, c2, vis);
+      } else if (ok) {
 #pragma unroll 1
         for (int hf = 0; hf < 2; ++hf) {
           float s[2][32];
@@ -816,25 +910,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         bar_arrive(bar_out, 64);
       }
       if (!ok) continue;
-      l_sum *= m_used == m_new ? 1.f : ex2_ftz(m_used - m_new);  // from this warpgroup's last tile
-      m_used = m_new;
-      if (j > 0 && __any_sync(0xffffffffu, need)) {  // rescale the O rows (after PV_{j-1})
-        const float alpha = m_prev == m_new ? 1.f : ex2_ftz(m_prev - m_new);
-        ok = __all_sync(0xffffffffu, wait_bar<false>(o_done, (j - 1) & 1, abort, peer_abort));
-        if (!ok) continue;
-        tc::fence_after_sync();
-#pragma unroll 1
-        for (int cc = 0; cc < D / 32; ++cc) {
-          const uint32_t ta = tmem + lane_base + C::kColO + cc * 32;
-          float s[32];
-          tc::ld32(ta, s);
-          tc::wait_ld();
-#pragma unroll
-          for (int k = 0; k < 32; ++k) s[k] *= alpha;
-          tc::st32(ta, s);
-        }
+      {  // from this warpgroup's last tile
+        const float h = fade(m_used, m_new);
+        l_sum = l_sum * h * h;
       }
+      m_used = m_new;
       const float nmu = m_new == -INFINITY ? 0.f : -m_new;
+      // a wide tile, or one that a key of a far larger scale leaves behind
+      const bool apart = kFold && (wide || m_new - ev_min > kFarLog2);
+      const bool moved = j > 0 && need;
+      float l_apart = -1.f;  // l with this tile's share where the weights do not give it
+      if (__any_sync(0xffffffffu, moved || apart)) {  // the rare steps of a tile behind one branch
+        if (__any_sync(0xffffffffu, moved)) {  // rescale the O rows (after PV_{j-1})
+          const float alpha = m_prev == m_new ? 1.f : ex2_ftz(m_prev - m_new);
+          ok = __all_sync(0xffffffffu, wait_bar<false>(o_done, (j - 1) & 1, abort, peer_abort));
+          if (!ok) continue;
+          tc::fence_after_sync();
+#pragma unroll 1
+          for (int cc = 0; cc < D / 32; ++cc) {
+            const uint32_t ta = tmem + lane_base + C::kColO + cc * 32;
+            float s[32];
+            tc::ld32(ta, s);
+            tc::wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) s[k] *= alpha;
+            tc::st32(ta, s);
+          }
+        }
+        if (__any_sync(0xffffffffu, apart)) l_apart = l_sum + wide_sum(sa, ks, vs, grp, c2, vis, nmu + kBiasLog2);
+      }
       // float16 outputs carry as many bits as the weights.  In a request's first tile l sums the weights as
       // rounded, so that a rounding moves weight between keys and leaves their sum one (a row of one key
       // is exact); over more keys the roundings average out, and the reciprocals would cost 128 a row.
@@ -846,7 +950,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         tc::wait_ld();
         scale_mask<kFold>(s, ks + 32 * g, vis - 32 * g);
         const float4 e = grp[g];
-        const float cg = logit_factor(c2, e.x), ng = kFold ? nmu + e.y : nmu;
+        const float cg = logit_factor(c2, e.x), ng = kFold ? nmu + e.y : nmu + kBiasLog2;
         const uint64_t c22 = pk2(cg, cg), nmu2 = pk2(ng, ng);
         uint64_t ls2[2] = {0, 0};
         float pk[16];
@@ -892,6 +996,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (lane == 0) mbar_arrive(&p_full[2 * wg + (g >> 1)]);  // rank 1's are forwarded to rank 0
         }
       }
+      if (kFold) l_sum = l_apart < 0.f ? l_sum : l_apart;
     }
     const bool gated = a.gate_mode != TF_GATE_NONE;
     const bool vec = rows_v16(a);
@@ -905,7 +1010,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (ok) {
       const float2 o = l_part[(wg ^ 1) * kRows + r];
       const float mf = fmaxf(m_used, o.x);  // O's scale: the maxima only grow
-      l_tot = (m_used == mf ? l_sum : l_sum * exp2f(m_used - mf)) + (o.x == mf ? o.y : o.y * exp2f(o.x - mf));
+      const float h0 = fade(m_used, mf), h1 = fade(o.x, mf);
+      l_tot = l_sum * h0 * h0 + o.y * h1 * h1;
       m_used = mf;
     }
     named_barrier(10, (kSmWarps + kPrWarps) * 32);  // gate rows are staged
@@ -913,7 +1019,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       tc::fence_after_sync();
       const int hq = h * G + (r - ri * G);
       const int64_t t = q0 + ri;
-      const float inv = 1.f / l_tot;
+      const float inv = kBias / l_tot;
       float* po = nullptr;
       if (sp.n > 1 && row_valid) {
         const int64_t row = ((int64_t)z * a.num_tokens + t) * a.num_q_heads + hq;
@@ -1037,8 +1143,8 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ tf_p
   for (int z = 0; z < sp.n; ++z) {
     const float2 ml = *reinterpret_cast<const float2*>(mlp + 2 * z * step);
     if (ml.x == -INFINITY && ml.y == 0.f) continue;  // no keys there, and no O written
-    const float f = ml.x == M ? 1.f : exp2f(ml.x - M);
-    l = fmaf(f, ml.y, l);
+    const float h = fade(ml.x, M), f = h * h;
+    l = fmaf(h, h * ml.y, l);
     const float2* x = reinterpret_cast<const float2*>(op + z * step * D + V * lane);
 #pragma unroll
     for (int i = 0; i < V / 2; ++i) {
@@ -1047,7 +1153,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ tf_p
       o[2 * i + 1] = fmaf(f, v.y, o[2 * i + 1]);
     }
   }
-  const float inv = 1.f / l;
+  const float inv = kBias / l;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int d = V * lane + i;

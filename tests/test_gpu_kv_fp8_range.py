@@ -159,3 +159,29 @@ def test_groups_of_large_values_far_above_the_others(name):
             _put(c, r, j, 0, -(28.0 / d ** 0.5) * u)
             _put(c, r, j, 1, 2.0 ** 110 * torch.randn(d, generator=g))
     _check_bound(c, name)
+
+
+@pytest.mark.parametrize("extend", [False, True])
+def test_empty_requests_before_a_dependent_launch(extend):
+    """A call in which no request has tokens or queries, a read of its output right behind it, and another
+    call whose scratch may be the first one's."""
+    from tokenfactory_b200 import ops
+    c = Case(48, "bf16", 8, 2, 128, [0, 0], [1, 1])
+    busy = Case(49, "bf16", 8, 2, 128, [700, 90], [1, 1])
+    zero = torch.zeros(2, dtype=torch.int64, device="cuda")
+    q, pool, (r2t, rows, _) = c.q.cuda(), c.pool(), c.args()
+    qb, poolb, argsb = busy.q.cuda(), busy.pool(), busy.args()
+    out = torch.empty_like(q)
+    seen, kept = [], []
+    for _ in range(50):
+        out.fill_(3)
+        if extend:
+            ops.paged_extend_fp8(q, *pool, r2t, rows, zero, zero, 128 ** -0.5, 1, 1, out=out)
+        else:
+            ops.paged_decode_fp8(q, *pool, r2t, rows, zero, 128 ** -0.5, 1, out=out)
+        seen.append(out.clone())
+        kept.append(ops.paged_decode_fp8(qb, *poolb, *argsb, 128 ** -0.5, max(busy.seq)))
+    seen, want = torch.stack(seen), B.reference(busy, B.ROWS)
+    assert (seen == 3).all() if extend else torch.isnan(seen).all()
+    for k in kept:
+        B.check(k, want)

@@ -1003,13 +1003,15 @@ __global__ void __launch_bounds__(THREADS)
       if (i < b && (i + 1) % sh.passes == 0)
         q += a.extend_lens ? max((int)a.extend_lens[i / sh.passes], 0) : 1;
     }
-    if (nt == 0) return;
     start = (int)q;
     ext = (int)e;
     su = before * sh.groups + (int64_t)u * nt;
     eu = su + nt;
   }
+  // on every path: a grid whose CTAs all left without it would complete beside the main kernel, and what
+  // follows in the stream would read rows and reuse scratch that the main kernel still writes
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (DEEP && su == eu) return;
   if (!DEEP) {
     const int c = blockIdx.x + 1;
     const CutInfo ci = ws.cut[c];

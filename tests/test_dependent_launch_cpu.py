@@ -25,7 +25,7 @@ def _bodies(path):
         yield m.group(1), text[at:end]
 
 
-@pytest.mark.parametrize("name", ["paged_fp8_rows.cu"])
+@pytest.mark.parametrize("name", ["paged_fp8_rows.cu", "paged_decode_mma.cu"])
 def test_dependent_grids_wait_before_any_exit(name):
     waits = 0
     for kernel, body in _bodies(os.path.join(CSRC, name)):

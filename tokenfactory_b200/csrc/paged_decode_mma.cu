@@ -644,23 +644,29 @@ __global__ void __launch_bounds__(256) combine_kernel(tf_paged_attn_args a, Ws w
   for (int i = tid; i <= nctas; i += blockDim.x) cgs[i] = ws.cta_g[i];
   __syncthreads();
   const int c = blockIdx.x;
-  if (c == 0 || c >= nctas) return;
-  const int64_t g = cgs[c];  // this CTA's boundary: the unit cut there, merged if this is its first cut
-  const int b = first_req_after(ts, B, Hkv, g);
-  const int nt = ts[b + 1] - ts[b];
-  const int h = (int)((g - (int64_t)ts[b] * Hkv) / nt);
-  const int64_t su = (int64_t)ts[b] * Hkv + (int64_t)h * nt, eu = su + nt;
-  const int c0 = cta_of(cgs, nctas, su), c1 = cta_of(cgs, nctas, eu - 1);
-  if (c0 == c1 || c != c0 + 1) return;  // finished inside one CTA, or merged at its first boundary
-  const int np = c1 - c0 + 1;
-  for (int i = tid; i < np; i += blockDim.x) {
-    const int cc = c0 + i;
-    const int64_t rc = cgs[cc];
-    sl[i] = 2 * cc + ((su > rc ? su : rc) == rc ? 0 : 1);
+  int b = 0, h = 0, np = 0;
+  if (c > 0 && c < nctas) {
+    const int64_t g = cgs[c];  // this CTA's boundary: the unit cut there, merged if this is its first cut
+    b = first_req_after(ts, B, Hkv, g);
+    const int nt = ts[b + 1] - ts[b];
+    h = (int)((g - (int64_t)ts[b] * Hkv) / nt);
+    const int64_t su = (int64_t)ts[b] * Hkv + (int64_t)h * nt, eu = su + nt;
+    const int c0 = cta_of(cgs, nctas, su), c1 = cta_of(cgs, nctas, eu - 1);
+    if (c0 != c1 && c == c0 + 1) {  // else finished inside one CTA, or merged at its first boundary
+      np = c1 - c0 + 1;
+      for (int i = tid; i < np; i += blockDim.x) {
+        const int cc = c0 + i;
+        const int64_t rc = cgs[cc];
+        sl[i] = 2 * cc + ((su > rc ? su : rc) == rc ? 0 : 1);
+      }
+    }
   }
   // everything above reads only the plan; the decode grid's partials are complete and visible
-  // after this wait (a no-op when the launch has no programmatic dependency)
+  // after this wait (a no-op when the launch has no programmatic dependency).  Every CTA waits, also those
+  // with nothing to merge: where no unit is cut this grid would otherwise complete beside the decode
+  // grid, and the next launch would read rows that are still being written.
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (np == 0) return;
   __syncthreads();
   for (int e = tid; e < np * G; e += blockDim.x) {  // every piece's (max, sum) at once
     const int i = e / G, hd = e - (e / G) * G;

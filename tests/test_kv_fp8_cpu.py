@@ -156,3 +156,17 @@ def test_cache_pool_in_8_bits():
     assert plain.k_buffer.is_contiguous() and plain.v_buffer.is_contiguous()
     with pytest.raises(TypeError):
         HybridCachePool(cfg, 10, 2, device="cpu", kv_dtype=torch.float16)
+
+
+@pytest.mark.parametrize("hq,max_ext", [(64, 0), (64, 9), (8, 4000), (2, 1 << 20)])
+def test_decode_workspace_does_not_follow_the_extend_fields(hq, max_ext):
+    """A caller that shares one argument structure between extend and decode calls: the decode's size
+    is that of one query row per head, whatever the extend fields say."""
+    from tokenfactory_b200 import _capi
+    lib = _capi.load()
+    kw = dict(num_q_heads=hq, num_kv_heads=2, head_dim=128)
+    want = lib.tf_paged_decode_fp8_workspace_size(
+        ctypes.byref(_paged(extend_lens=None, max_extend_len=1, **kw)))
+    got = lib.tf_paged_decode_fp8_workspace_size(
+        ctypes.byref(_paged(extend_lens=FAKE, max_extend_len=max_ext, **kw)))
+    assert want > 0 and got == want

@@ -522,9 +522,20 @@ static size_t fp8_path_workspace(const tf_paged_attn_args& a, Fp8Path path) {
   }
 }
 
+// the problem that a call computes: a decode has no extend fields, whatever the caller's structure holds
+static tf_paged_attn_args fp8_args(const tf_paged_attn_args& a, bool decode) {
+  tf_paged_attn_args d = a;
+  if (decode) {
+    d.extend_lens = nullptr;
+    d.max_extend_len = 1;
+  }
+  return d;
+}
+
 static size_t fp8_workspace(const tf_paged_attn_args* a, bool decode) {
   if (check_paged(a, decode) != TF_OK || a->batch_size == 0 || a->num_tokens == 0) return 0;
-  return fp8_path_workspace(*a, fp8_path(*a, decode));
+  const tf_paged_attn_args d = fp8_args(*a, decode);
+  return fp8_path_workspace(d, fp8_path(d, decode));
 }
 
 static tf_status paged_fp8(const tf_paged_attn_args* a, const tf_kv_scale* sc, void* ws,
@@ -533,8 +544,7 @@ static tf_status paged_fp8(const tf_paged_attn_args* a, const tf_kv_scale* sc, v
   if (st != TF_OK || a->batch_size == 0 || a->num_tokens == 0) return st;
   st = check_kv_scale(sc);
   if (st != TF_OK) return st;
-  tf_paged_attn_args d = *a;
-  if (decode) d.extend_lens = nullptr;
+  const tf_paged_attn_args d = fp8_args(*a, decode);
   const Fp8Path path = fp8_path(d, decode);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   DeviceGuard g(s);

@@ -185,3 +185,25 @@ def test_empty_requests_before_a_dependent_launch(extend):
     assert (seen == 3).all() if extend else torch.isnan(seen).all()
     for k in kept:
         B.check(k, want)
+
+
+@pytest.mark.parametrize("dtype,d", [("f32", 64), ("bf16", 48), ("f16", 80), ("bf16", 128)])
+@pytest.mark.parametrize("extend", [False, True])
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+def test_scales_that_are_not_finite_make_the_rows_that_see_them_nan(dtype, d, extend, which, value):
+    """A K or V scale that is not finite, its codes all 1 and the queries negative (logits of -inf): NaN in
+    every element of the rows of its head that see the token, and nothing in the others."""
+    ext = [9, 4] if extend else [1, 1]
+    c = Case(50, dtype, 8, 2, d, [40, 20], ext)
+    c.q = -c.q.abs()
+    slot = int(c.r2t[c.rows[0], 42 if extend else 10])
+    c.codes.view(torch.uint8)[slot, 1] = 0x38  # 1.0
+    c.scale[slot, 1, which] = value
+    got = c.run(force_extend=extend).double().cpu().numpy()
+    nan = np.zeros(got.shape, bool)
+    nan[2 if extend else 0:ext[0], 4:] = True
+    assert np.array_equal(np.isnan(got), nan)
+    c.scale[slot, 1, which] = 1e-3
+    ref, tol = B.reference(c, B.kernel_of(c, extend))
+    assert (np.abs(got - ref)[~nan] <= tol[~nan]).all()

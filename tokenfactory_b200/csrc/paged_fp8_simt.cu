@@ -143,16 +143,19 @@ __global__ void __launch_bounds__(kThreads) paged_fp8_simt_kernel(tf_paged_attn_
     for (int i = 0; i < kRowsPerThread; ++i) {
       const int r = ty + i * (kThreads / kRowThreads);
       float* dst = (r >= kBK ? v_s : k_s) + (r % kBK) * KP;
+      // NaN for a scale of infinity too: a K row of infinities could make a logit of -inf, and its token
+      // would vanish
+      const float mul = rs[i] + (rs[i] - rs[i]);
 #pragma unroll
       for (int c = 0; c < kWords; ++c) {
         const int d = 4 * (tx + c * kRowThreads);
         if (d >= DP) break;
         const uint32_t w = code[i][c];
         float4 x;
-        x.x = kv8::decode1(w & 0xff) * rs[i];
-        x.y = kv8::decode1((w >> 8) & 0xff) * rs[i];
-        x.z = kv8::decode1((w >> 16) & 0xff) * rs[i];
-        x.w = kv8::decode1(w >> 24) * rs[i];
+        x.x = kv8::decode1(w & 0xff) * mul;
+        x.y = kv8::decode1((w >> 8) & 0xff) * mul;
+        x.z = kv8::decode1((w >> 16) & 0xff) * mul;
+        x.w = kv8::decode1(w >> 24) * mul;
         if (!VEC) {  // a scale that is not finite must not reach the padding
           if (d + 1 >= D) x.y = 0.f;
           if (d + 2 >= D) x.z = 0.f;

@@ -431,9 +431,16 @@ TF_API tf_status tf_kv_store_fp8(const tf_kv_store_args* args, const tf_kv_scale
 TF_API tf_status tf_attn_prologue_fp8(const tf_attn_prologue_args* args, const tf_kv_scale* scale,
                                       void* stream);
 
-/* tf_paged_decode_attn and tf_paged_extend_attn over such a pool; the attention output and its gate
- * are computed in fp32 and rounded once.  A request without tokens gets NaN rows in a decode call.
- * A scale that is not finite makes the rows that see its token NaN and leaves the others alone. */
+/* tf_paged_decode_attn and tf_paged_extend_attn over such a pool.  Logits, softmax statistics, sums,
+ * the output and its gate are fp32, and the output is rounded once.  Calls with 16-bit activations at
+ * head_dim 64, 128 and 256 run on tensor cores with f16 operands: each weight (times its V scale)
+ * is rounded to f16, and in a bfloat16 extend of more than 48 query rows a kv head the K and V codes
+ * times their scales too; each is off by at most 2^-11 of itself, whatever the scales of other tokens
+ * are (weights below 2^-21 of a row's largest, in the larger extends 2^-8 at worst, by a fixed step
+ * instead).  fp32 activations and other head dims have no such rounding.  Exponentials and the
+ * gate's division are approximations good to about 2^-20 of their result.
+ * A request without tokens gets NaN rows in a decode call.  A scale that is not finite makes the
+ * rows that see its token NaN and leaves the others alone. */
 TF_API size_t tf_paged_decode_fp8_workspace_size(const tf_paged_attn_args* args);
 TF_API tf_status tf_paged_decode_fp8(const tf_paged_attn_args* args, const tf_kv_scale* scale,
                                      void* workspace, size_t workspace_bytes, void* stream);

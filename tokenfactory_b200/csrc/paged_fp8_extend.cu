@@ -941,7 +941,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       // float16 outputs carry as many bits as the weights.  In a request's first tile l sums the weights as
       // rounded, so that a rounding moves weight between keys and leaves their sum one (a row of one key
-      // is exact); over more keys the roundings average out, and the reciprocals would cost 128 a row.
+      // is exact).  Over more keys the error of l is the average of the weights' roundings, small beside
+      // what those do to P V themselves, and the reciprocals would cost 128 a row and tile.
       const bool sum_rounded = !kFold && jb + j == 0;
 #pragma unroll 1
       for (int g = 0; g < 4; ++g) {

@@ -340,8 +340,10 @@ def paged_decode_fp8(q: torch.Tensor, k_buffer: torch.Tensor, v_buffer: torch.Te
                      max_seq_len: int, gate: Optional[torch.Tensor] = None,
                      gate_mode: str = "none", out: Optional[torch.Tensor] = None,
                      slot_mode: str = "clamp", err: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """paged_decode over an 8-bit pool: softmax(q K^T scale) V, times act(gate), in fp32 and rounded
-    once to q's dtype.  A request of length 0 gets NaN rows.  Returns out [B, Hq, D]."""
+    """paged_decode over an 8-bit pool: softmax(q K^T scale) V, times act(gate), with fp32 sums and
+    softmax statistics, rounded once to q's dtype.  With 16-bit q at head_dim 64, 128 and 256 the softmax
+    weights enter their product as f16 (2^-11 of each).  A request of length 0 gets NaN rows.
+    Returns out [B, Hq, D]."""
     return _C.paged_decode_fp8(q, k_buffer, v_buffer, kv_scale, req_to_token, req_pool_indices,
                                seq_lens, float(scale), int(max_seq_len), gate,
                                GATE_MODES[gate_mode], out, SLOT_MODES[slot_mode], err)
@@ -356,7 +358,8 @@ def paged_extend_fp8(q: torch.Tensor, k_buffer: torch.Tensor, v_buffer: torch.Te
                      slot_mode: str = "clamp", err: Optional[torch.Tensor] = None) -> torch.Tensor:
     """paged_extend over an 8-bit pool (the new tokens' rows already stored): query i of request b
     sees positions <= seq_len_b - extend_len_b + i; rows of q behind the last request are left as
-    they were in ``out``.  Returns out [T, Hq, D]."""
+    they were in ``out``.  Roundings as in paged_decode_fp8; with bfloat16 q and more than 48 query rows a
+    kv head the K and V codes times their scales are rounded to f16 too.  Returns out [T, Hq, D]."""
     return _C.paged_extend_fp8(q, k_buffer, v_buffer, kv_scale, req_to_token, req_pool_indices,
                                seq_lens, extend_lens, float(scale), int(max_seq_len),
                                int(max_extend_len), gate, GATE_MODES[gate_mode], out,

@@ -207,3 +207,60 @@ def test_scales_that_are_not_finite_make_the_rows_that_see_them_nan(dtype, d, ex
     c.scale[slot, 1, which] = 1e-3
     ref, tol = B.reference(c, B.kernel_of(c, extend))
     assert (np.abs(got - ref)[~nan] <= tol[~nan]).all()
+
+
+@pytest.mark.parametrize("name", list(MIXED))
+@pytest.mark.parametrize("what", ["q", "gate"])
+def test_queries_and_gates_that_are_not_finite(name, what):
+    """Infinities and NaNs in one query row (or one element of its gate) make that row (element) NaN and leave
+    every other one alone."""
+    dtype, hq, hkv, d, pre, ext = MIXED[name]
+    c = Case(51, dtype, hq, hkv, d, pre, ext, gate="sigmoid")
+    extend = any(e != 1 for e in ext)
+    t = len(c.q)
+    ref, tol = B.reference(c, B.kernel_of(c, extend))
+    nan = np.zeros(ref.shape, bool)
+    for i, x in enumerate((float("inf"), -float("inf"), float("nan"))):
+        row, head = min(i * 2, t - 1), (3 * i) % hq
+        if what == "q":
+            c.q[row, head, 5 * i + 1] = x
+            nan[row, head] = True
+        elif i == 2:
+            c.gate = c.gate.clone()
+            c.gate[row, head, 7] = x
+            nan[row, head, 7] = True
+    got = c.run(force_extend=extend).double().cpu().numpy()
+    assert np.array_equal(np.isnan(got), nan)
+    assert (np.abs(got - ref)[~nan] <= tol[~nan]).all()
+
+
+@pytest.mark.parametrize("name", list(MIXED))
+def test_results_repeat_whatever_the_scales(name):
+    dtype, hq, hkv, d, pre, ext = MIXED[name]
+    c = Case(52, dtype, hq, hkv, d, pre, ext)
+    c.scale *= torch.exp2(torch.randint(-12, 13, c.scale.shape).float())
+    extend = any(e != 1 for e in ext)
+    a = c.run(force_extend=extend)
+    for _ in range(3):
+        assert torch.equal(a, c.run(force_extend=extend))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_a_model_on_a_prompt_of_zeros(dtype):
+    """Hidden states of zero through the full-attention layers and their 8-bit pool: zeros, as from a 16-bit
+    pool, and later tokens are finite."""
+    from tests.test_gpu_kv_fp8_model import _model, _step
+    from tokenfactory_b200.hybrid_model import HybridCachePool
+    dt = DTYPES[dtype]
+    cfg, model = _model(128, 8, 1, dt)
+    with torch.no_grad():
+        model.model.language_model.embed_tokens.weight[0] = 0
+    r2t = torch.arange(300, device="cuda").view(1, 300)
+    outs = []
+    for kv in (torch.float8_e4m3fn, None):
+        pool = HybridCachePool(cfg, 300, 2, dtype=dt, kv_dtype=kv)
+        first = _step(model, pool, r2t, [0], [0], [150], torch.zeros(150, dtype=torch.int64))
+        later = _step(model, pool, r2t, [0], [150], [1], torch.tensor([7]))
+        outs.append(first)
+        assert torch.isfinite(first).all() and torch.isfinite(later).all()
+    assert (outs[0] == 0).all() and (outs[1] == 0).all()

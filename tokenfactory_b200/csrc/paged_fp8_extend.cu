@@ -32,11 +32,14 @@
 // see it are NaN.  Every wait is bounded; one that gives up raises an abort flag in both CTAs and
 // TF_KERR_TIMEOUT.
 //
-// Measured (bf16, 32 heads over 4, head_dim 256).  A chunk of 512 tokens behind 28000: 511 us, 928 TFLOP/s;
-// 2.0 us a key tile, bound by the softmax warps (two exponentials' worth of issue slots a score) with the
-// products' 1.1 us beside them.  4 requests of 512 to 2048 tokens on up to 4096: 587 us, 765 TFLOP/s; a
-// query tile's first product starts 10 us after its CTAs do (lengths, table, rows: dependent reads) and
-// its epilogue takes 5 us, with nothing beside them as O and the two S buffers fill TMEM.
+// Measured (bf16, 32 heads over 4, head_dim 256; ranges are boxes).  A chunk of 512 tokens behind 28000:
+// 514 to 550 us, 862 to 922 TFLOP/s; about 2.1 us a key tile, held by the latency of the softmax warps'
+// reads of TMEM (each is waited for where it is issued, and S is read twice; 45% of the issue slots used)
+// with the products' 1.1 us beside them.  4 requests of 512 to 2048 tokens on up to 4096: 576 to 614 us, 733
+// to 781 TFLOP/s; a query tile's first product starts 10 us after its CTAs do (lengths, table, rows:
+// dependent reads) and its epilogue takes 5 us, with nothing beside them as O and the two S buffers fill
+// TMEM.  Where every tile is wide (scales 2^+-9 apart) the two take 1150 and 1170 us.  The same chunk over a
+// 16-bit pool (paged_extend_tc.cu) takes 381 us, the prompts 468.
 //
 // Few query tiles over a long prefix leave SM pairs idle: the key tiles are then split over
 // grid.y clusters, which leave (M, l, O) partials for a combine kernel.
@@ -446,7 +449,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int TQ = kRows / G;  // query tokens per CTA
   // Longest query tiles first, so that the last ones to finish are short: the longest request before
   // the others (of up to 32, which a warp ranks; of more, each is a small part of the whole), and a
-  // head's later tiles before its earlier ones.  3 requests of 64 to 1009 new tokens on up to 2904: 122 us,
+  // head's later tiles before its earlier ones.  When they were introduced, 3 requests of 64 to 1009 new tokens on up to 2904: 122 us,
   // 129 us in the batch's order, head by head; 4 of 512 to 2048 on up to 4096: 664 us against 672 us
   // (695 us with the kv heads of a query tile side by side).
   const int z = blockIdx.y, rank_h = (blockIdx.x >> 1) / pairs_per_req;

@@ -9,7 +9,7 @@
 // -> scores -> sum of each block of 32 keys.  The table's entries run two blocks ahead and the rows
 // one, in registers, 16 threads to a row, and the lanes of the warp that holds a head's 32 scores
 // take their softmax without another exchange.  4 requests of 17 to 96 tokens, 8 heads over 2,
-// head_dim 64, fp32: 11.2 us, 30.7 us with rows loaded byte by byte when they were needed.
+// head_dim 64, fp32: 11.7 to 12.3 us, 30.7 us with rows loaded byte by byte when they were needed.
 #include "common.cuh"
 #include "kv_fp8.cuh"
 #include "launch.h"

@@ -11,7 +11,8 @@
 // vector form holds the E = D/32 elements [E l, E l + E) of a row; the rotation partner d +- rotary_dim/2 sits in lane l ^ (rotary_dim/2/E) when that is a
 // power of two, and otherwise comes from a copy of the row in shared memory.
 // 7001 tokens, 24 heads over 4 of 256 float16 values: 51 us, 4.2 TB/s (0.64 of the copy rate; 57 us with
-// fewer rows in flight a lane); 128 tokens: 7.2 us (23 us with four tokens a CTA throughout), a launch
+// fewer rows in flight a lane): 62% of the issue slots used, stalls on rows in flight and on shared memory;
+// at the 80 registers of three CTAs an SM the head_dim 256 forms spill 24 to 140 bytes a thread; 128 tokens: 7.2 us (23 us with four tokens a CTA throughout), a launch
 // and two dependent reads.
 #include "common.cuh"
 #include "kv_fp8.cuh"

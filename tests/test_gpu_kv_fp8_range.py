@@ -264,3 +264,57 @@ def test_a_model_on_a_prompt_of_zeros(dtype):
         outs.append(first)
         assert torch.isfinite(first).all() and torch.isfinite(later).all()
     assert (outs[0] == 0).all() and (outs[1] == 0).all()
+
+
+@pytest.mark.parametrize("name,size", [(n, 2.0 ** s) for n in MIXED
+                                       for s in (8, 15, 24, 29, 33, 60, 100)
+                                       if s < 16 or MIXED[n][0] == "bf16"])
+def test_logits_of_every_size(name, size):
+    """One K row of a given size in the middle of each request, and one twice that size a little behind it:
+    where a query's logit is positive it takes all the weight, where it is negative it takes none."""
+    dtype, hq, hkv, d, pre, ext = MIXED[name]
+    extend = any(e != 1 for e in ext)
+    c = Case(53, dtype, hq, hkv, d, pre, ext)
+    g = torch.Generator().manual_seed(5)
+    for r, n in enumerate(c.seq):
+        for at, f in ((n // 2, 0.5), (min(n // 2 + 5, n - 1), 1.0)):
+            x = torch.rand(d, generator=g) * 2 - 1
+            x[0] = 1
+            _put(c, r, at, 0, f * size * x)
+    got = c.run(force_extend=extend).double().cpu().numpy()
+    kernel, t = B.kernel_of(c, extend), 0
+    q, sure, rows = c.q.double().numpy(), 0, 0
+    for r, (n, e) in enumerate(zip(c.seq, c.ext)):
+        s = c.r2t[c.rows[r], :n].numpy()
+        for h in range(hkv):
+            k, v, ks, vs = B._group(c, s, h)
+            for i in range(e):
+                m = n - e + i + 1
+                for hh in range(h * (hq // hkv), (h + 1) * (hq // hkv)):
+                    rows += 1
+                    x = k[:m] @ q[t + i, hh] * d ** -0.5
+                    # fp32 logits are off by 2^-18 of their terms' sum (bfloat16's large extends 2^-10); a lead of more than
+                    # that and 40 (2^-57 of weight) leaves the leader alone
+                    err = (np.abs(k[:m]) @ np.abs(q[t + i, hh]) * d ** -0.5).max() * 2.0 ** -10
+                    top = np.argsort(x)[::-1]
+                    if m > 1 and x[top[0]] - x[top[1]] > 2 * err + 40:
+                        want, tol = v[top[0]], 2.0 ** -9 * np.abs(v[top[0]])
+                    elif np.abs(x).max() < 40:
+                        want, tol = B.row_terms(c, kernel, q[t + i, hh][None], k[:m], v[:m], ks[:m],
+                                                vs[:m], d ** -0.5)
+                        want, tol = want[0], tol[0]
+                    elif x.max() < 40 and x[x > -60].size:  # the large rows take nothing: the others' average
+                        keep = np.flatnonzero(x > -60 - 2 * err * (np.abs(x) > 60))
+                        keep = keep[np.abs(x[keep]) < 60]
+                        if (np.abs(np.delete(x, keep)) < 60 + 4 * err).any():
+                            continue
+                        want, tol = B.row_terms(c, kernel, q[t + i, hh][None], k[keep], v[keep],
+                                                ks[keep], vs[keep], d ** -0.5)
+                        want, tol = want[0], tol[0]
+                    else:
+                        continue
+                    sure += 1
+                    assert (np.abs(got[t + i, hh] - want) <= B.rounded(dtype, want, tol)).all(), (
+                        r, i, hh, np.abs(got[t + i, hh] - want).max(), x[top[:2]])
+        t += e
+    assert sure > rows // 4

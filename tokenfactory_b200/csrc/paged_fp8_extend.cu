@@ -25,7 +25,7 @@
 //               "wide": one key must not take the bits of the others, least of all a key that a row does
 //               not see.  Its keys have exponents of their own, which the softmax reads from shared
 //               memory; the codes carry what is left of a scale, in [1, 2).
-//               l and its exponentials are kept times 2^40: M is between s_max - 50 and s_max + 119 (the
+//               bfloat16's l and its exponentials are kept times 2^40: M is between s_max - 50 and s_max + 119 (the
 //               store's smallest and largest scale), and both ends then lie inside fp32's range.
 //   Q           is scaled by a power of two per row into f16's range (bfloat16 stays exact)
 // A scale that is not finite gives its key NaN logits and a V row of zeros, so that only the rows that
@@ -63,10 +63,11 @@ constexpr int kFwdWarp = kIssueWarp + 1;         // rank 1: forwards "P written"
 constexpr int kThreads = (kFwdWarp + 1) * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleLog2 = 8.f;
-constexpr float kBiasLog2 = 40.f, kBias = 0x1p40f;  // of l and its exponentials
+// what bfloat16's l and its exponentials are kept times (fp16's scales reach neither end)
+template <typename T> constexpr float kBiasLog2 = std::is_same<T, __half>::value ? 0.f : 40.f;
+template <typename T> constexpr float kBias = std::is_same<T, __half>::value ? 1.f : 0x1p40f;
 constexpr int kSpread = 6;           // exponents that a group's scales may be apart
-constexpr float kWide = -1000.f;     // in the place of a wide group's ev
-constexpr float kFarLog2 = 80.f;     // M this far above a group's ev: P may be 0 where l's terms are not
+constexpr int kTopExp = 30;          // V scales from 2^31 on: beside them P may be 0 where l's terms are not
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
@@ -99,14 +100,15 @@ __device__ __forceinline__ float lg2_ftz(float x) {
   return y;
 }
 
-// What a group's products are multiplied by to be logits: the row's factor times the group's 2^kx, at least
-// kFloor.  Both are small for a row of zeros over keys of zeros, and a product of 0 would turn the -inf of a
-// hidden key into a NaN; products are at most 2^32, so that with 2^-90 their logits are 0 to 2^-58.  A factor
-// that is NaN (a query row that is not finite) stays NaN.
-constexpr float kFloor = 0x1p-90f;
-__device__ __forceinline__ float logit_factor(float c2, float kx) {
-  const float f = c2 * kx;
-  return f < kFloor ? kFloor : f;
+// What a group's products are multiplied by to be logits: the row's factor times the group's 2^kx, kept in
+// fp32's normal range (floor 2^-126).  Both are small for a row of zeros over keys of zeros, and a product of
+// 0 would turn the -inf of a hidden key into a NaN; products are at most 2^33, so that with 2^-126 their
+// logits are 0 to 2^-93.  A factor that is NaN (a query row that is not finite) stays NaN.  kx 0 with floor
+// 1: a group that wide_logits has already multiplied.
+__device__ __forceinline__ float logit_factor(float c2, float kx, float floor) {
+  float f;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(f) : "f"(c2 * kx), "f"(floor));
+  return f;
 }
 
 // two fp32 operations in one instruction (each rounded as its scalar form)
@@ -312,9 +314,10 @@ struct Cfg {
   static constexpr int kOffKs = kOffRow + kRows * 4;             // float [kScaleTiles][kKeys]
   static constexpr int kOffVs = kOffKs + kScaleTiles * kKeys * 4;
   static constexpr int kOffGrp = kOffVs + kScaleTiles * kKeys * 4;  // float4 [kScaleTiles][4]: a group's
-                                                                  // 2^kx, ev, 2^-ev kBias
-  static constexpr int kOffEv = kOffGrp + kScaleTiles * 4 * 16;  // float [kScaleTiles][4]: ev, or kWide
-  static constexpr int kSmem = kOffEv + kScaleTiles * 4 * 4 + 1024;
+                                                                  // 2^kx, ev, 2^-ev kBias, floor
+  static constexpr int kOffApart = kOffGrp + kScaleTiles * 4 * 16;  // float [kScaleTiles][4]: not 0 where a tile
+                                                                    // needs the steps of a wide one
+  static constexpr int kSmem = kOffApart + kScaleTiles * 4 * 4 + 1024;
   static constexpr int kColS = 0;                 // two S buffers of kKeys columns; P_j over S_j
   static constexpr int kColO = 2 * kKeys;
   static constexpr int kTmemCols = 512;
@@ -345,30 +348,30 @@ __device__ __forceinline__ void ld16(uint32_t taddr, float (&v)[16]) {
 
 // What a tile of wide groups needs beside the common path.  Out of line: it is rare, and the tile loop's
 // instructions are fetched once a tile.  A row's products S of the tile's 128 keys sit in the lane's TMEM
-// columns sa..; keys [0, vis) are visible.
+// columns sa..
 //
-// exact codes: the largest logit + log2 of the V scale (ks times 2^kx of the group times c2 is what the
-// products are multiplied by, vs the V scales over kBias)
+// exact codes: the largest logit + log2 of the V scale among keys [0, vis) (ks times 2^kx of the group times
+// c2 is what the products are multiplied by)
 __device__ __noinline__ float wide_max(uint32_t sa, const float* ks, const float* vs, const float4* grp, float c2,
                                        int vis) {
   float m = -INFINITY;
 #pragma unroll 1
   for (int g = 0; g < 8; ++g) {
-    const float factor = logit_factor(c2, grp[g >> 1].x);
+    const float factor = logit_factor(c2, grp[g >> 1].x, grp[g >> 1].w);
     float s[16];
     ld16(sa + 16 * g, s);
     tc::wait_ld();
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
       // (a V row of zeros counts as one of the store's smallest scale)
-      const float x = fmaf(s[k], ks[16 * g + k] * factor, fmaxf(lg2_ftz(fabsf(vs[16 * g + k])) + kBiasLog2, -50.f));
+      const float x = fmaf(s[k], ks[16 * g + k] * factor, fmaxf(lg2_ftz(fabsf(vs[16 * g + k])), -50.f));
       if (16 * g + k < vis) m = fmaxf(m, x);
     }
   }
   return m;
 }
-// folded codes: the products of wide groups (2^kx of 0) become (logit + ev) / kFloor with their keys' own
-// exponents, ks = 2^kx and vs = 2^ev / kBias; logit_factor of such a group is kFloor
+// folded codes: the products of wide groups (2^kx of 0) become logit + ev with their keys' own exponents,
+// ks = 2^kx and vs = 2^ev
 __device__ __noinline__ void wide_logits(uint32_t sa, const float* ks, const float* vs, const float4* grp, float c2) {
 #pragma unroll 1
   for (int g = 0; g < 8; ++g) {
@@ -377,26 +380,28 @@ __device__ __noinline__ void wide_logits(uint32_t sa, const float* ks, const flo
     ld16(sa + 16 * g, s);
     tc::wait_ld();
 #pragma unroll
-    for (int k = 0; k < 16; ++k)
-      s[k] = fmaf(s[k], ks[16 * g + k] * c2, lg2_ftz(vs[16 * g + k]) + kBiasLog2) * (1.f / kFloor);
+    for (int k = 0; k < 16; ++k) s[k] = fmaf(s[k], ks[16 * g + k] * c2, lg2_ftz(vs[16 * g + k]));
     tc::st16(sa + 16 * g, s);
   }
   tc::wait_st();
 }
-// the sum of 2^(logit - M) kBias, bias_m = kBiasLog2 - M, where a sum of weights over 2^ev would not do
-__device__ __noinline__ float wide_sum(uint32_t sa, const float* ks, const float* vs, const float4* grp, float c2,
-                                       int vis, float bias_m) {
+// the sum of 2^(logit - M) 2^bias over keys [0, vis), where a sum of weights over 2^ev would not do; the
+// exponents of the weights are formed as the common path does and ev comes off them, so that a rounding of M
+// or of logit + ev (logits above 2^24) is the same in both
+__device__ __noinline__ float wide_sum(uint32_t sa, const float* vs, const float4* grp, float c2, int vis, float nmu,
+                                       float bias) {
   float sum = 0.f;
 #pragma unroll 1
   for (int g = 0; g < 8; ++g) {
-    const bool own = grp[g >> 1].x == 0.f;
+    const float4 e = grp[g >> 1];
+    const float factor = logit_factor(c2, e.x, e.w), ng = nmu + e.y;
     float s[16];
     ld16(sa + 16 * g, s);
     tc::wait_ld();
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
-      const float x = own ? s[k] * kFloor - (lg2_ftz(vs[16 * g + k]) + kBiasLog2) : s[k] * (ks[16 * g + k] * c2);
-      if (16 * g + k < vis) sum += ex2_ftz(x + bias_m);
+      const float ev = e.x == 0.f ? lg2_ftz(vs[16 * g + k]) : e.y;
+      if (16 * g + k < vis) sum += ex2_ftz(fmaf(s[k], factor, ng) + (bias - ev));
     }
   }
   return sum;
@@ -438,7 +443,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   float* ks_s = reinterpret_cast<float*>(sbase + C::kOffKs);
   float* vs_s = reinterpret_cast<float*>(sbase + C::kOffVs);
   float4* grp_s = reinterpret_cast<float4*>(sbase + C::kOffGrp);
-  float* ev_s = reinterpret_cast<float*>(sbase + C::kOffEv);
+  float* apart_s = reinterpret_cast<float*>(sbase + C::kOffApart);
   constexpr bool kFold = !std::is_same<T, __half>::value;  // scales multiplied into the codes
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -625,25 +630,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       };
       int slot = kV ? 2 : 0;   // ring place: K0 K1 V0 K2 V1 K3 ... V_{n-2} V_{n-1}
       uint32_t phase = 0;
+      bool large = false;      // a group so far had a V scale above kTopExp
       auto put = [&](int tile, uint4 (&w)[kLoads], float2 s2) {
         // A scale that is not finite: NaN logits (K), and a V row of zeros
         const bool fin = kv8::abs_bits(s2.x) < 0x7f800000u && kv8::abs_bits(s2.y) < 0x7f800000u;
-        const int gk = (int)(__reduce_max_sync(0xffffffffu, fin ? kv8::abs_bits(s2.x) : 0u) >> 23);
-        const int gv = (int)(__reduce_max_sync(0xffffffffu, fin ? kv8::abs_bits(s2.y) : 0u) >> 23);
+        // Exponents of the key: its group's, or its own where the group's are further apart than kSpread (K
+        // and V each for itself; fp16 keeps the rest of a scale in fp32 and its group's).
         const int own_k = (int)(kv8::abs_bits(s2.x) >> 23), own_v = (int)(kv8::abs_bits(s2.y) >> 23);
-        const bool wide = __any_sync(0xffffffffu, fin && (gk - own_k > kSpread || gv - own_v > kSpread));
-        // exponents of the key, its own or its group's (fp16 keeps the rest of a scale in fp32: its group's)
-        const int kx = min(max((kFold && wide && fin ? own_k : gk) - 127, -100), 126);
-        const int ev = min(max((kFold && wide && fin ? own_v : gv) - 127, -50), 126);
+        int gk = 0, gv = 0;
+        bool wide_k = false, wide_v = false;
+        if (kFold || kV) gk = (int)(__reduce_max_sync(0xffffffffu, fin ? kv8::abs_bits(s2.x) : 0u) >> 23);
+        if (kFold) wide_k = __any_sync(0xffffffffu, fin && gk - own_k > kSpread);
+        if (kV) {
+          gv = (int)(__reduce_max_sync(0xffffffffu, fin ? kv8::abs_bits(s2.y) : 0u) >> 23);
+          wide_v = __any_sync(0xffffffffu, fin && gv - own_v > kSpread);
+        }
+        const int kx = min(max((wide_k && fin ? own_k : gk) - 127, -100), 126);
+        const int ev = min(max((kFold && wide_v && fin ? own_v : gv) - 127, -50), 126);
         if (kV) {
           const int st = tile & (C::kScaleTiles - 1);
           ks_s[st * kKeys + my_key] = fin ? (kFold ? pow2i(kx) : s2.x * pow2i(-kx)) : NAN;
-          vs_s[st * kKeys + my_key] = kFold ? pow2i(ev) * (1.f / kBias) : fin ? s2.y * (1.f / kBias) : 0.f;
+          vs_s[st * kKeys + my_key] = kFold ? pow2i(ev) : fin ? s2.y : 0.f;
+          const bool wide = wide_k || wide_v;
           if (lane == 0) {
-            const bool own = kFold && wide;  // (logit_factor, wide_logits)
-            grp_s[st * 4 + pw - 4] = own ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                         : make_float4(pow2i(kx), (float)ev, pow2i(-ev) * kBias, 0.f);
-            ev_s[st * 4 + pw - 4] = wide ? kWide : (float)ev;
+            grp_s[st * 4 + pw - 4] = kFold && wide
+                                         ? make_float4(0.f, 0.f, 0.f, 1.f)  // (logit_factor, wide_logits)
+                                         : make_float4(pow2i(kx), (float)ev, pow2i(-ev) * kBias<T>, 0x1p-126f);
+            large = large || (kFold && gv - 127 > kTopExp);
+            apart_s[st * 4 + pw - 4] = wide || large ? 1.f : 0.f;
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(&sc_full[st]);
@@ -865,9 +879,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int64_t rem = row_valid ? klim - (int64_t)(jb + j) * kKeys : 0;
       const int vis = rem <= 0 ? 0 : (rem >= kKeys ? kKeys : (int)rem);
       if (ok) ok = __all_sync(0xffffffffu, wait_bar<false>(&sc_full[si], (j / C::kScaleTiles) & 1, abort, peer_abort));
-      const float4 evs = *reinterpret_cast<const float4*>(ev_s + si * 4);
-      const float ev_min = fminf(fminf(evs.x, evs.y), fminf(evs.z, evs.w));
-      const bool wide = ev_min == kWide;  // some group of the tile
       if (ok) ok = __all_sync(0xffffffffu, wait_bar<false>(&s_full[wg], (j >> 1) & 1, abort, peer_abort));
       if (idle) {  // P stays what S left there: it reaches only rows that are not stored
         tc::fence_before_sync();
@@ -878,11 +889,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         continue;
       }
+      const float4 ap = *reinterpret_cast<const float4*>(apart_s + si * 4);
+      const bool apart = ap.x + ap.y + ap.z + ap.w != 0.f;
       float tmax = -INFINITY;
       const float4* grp = grp_s + si * 4;
       if (ok) tc::fence_after_sync();
-      if (ok && wide && kFold) wide_logits(sa, ks, vs, grp, c2);
-      if (ok && wide && !kFold) {
+      if (ok && apart && kFold) wide_logits(sa, ks, vs, grp, c2);
+      if (ok && apart && !kFold) {
         tmax = wide_max(sa, ks, vs, grp, c2, vis);
       } else if (ok) {
 #pragma unroll 1
@@ -895,8 +908,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           for (int k = 0; k < 2; ++k) {
             const int g = 2 * hf + k;
             scale_mask<kFold>(s[k], ks + 32 * g, vis - 32 * g);
-            const float2 e = *reinterpret_cast<const float2*>(grp + g);
-            tmax = fmaxf(tmax, fmaf(max_of_32(s[k]), logit_factor(c2, e.x), e.y));  // factor > 0
+            const float4 e = grp[g];
+            tmax = fmaxf(tmax, fmaf(max_of_32(s[k]), logit_factor(c2, e.x, e.w), e.y));  // factor > 0
           }
         }
       }
@@ -919,11 +932,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       m_used = m_new;
       const float nmu = m_new == -INFINITY ? 0.f : -m_new;
-      // a wide tile, or one that a key of a far larger scale leaves behind
-      const bool apart = kFold && (wide || m_new - ev_min > kFarLog2);
       const bool moved = j > 0 && need;
       float l_apart = -1.f;  // l with this tile's share where the weights do not give it
-      if (__any_sync(0xffffffffu, moved || apart)) {  // the rare steps of a tile behind one branch
+      if (__any_sync(0xffffffffu, moved || (kFold && apart))) {  // the rare steps of a tile behind one branch
         if (__any_sync(0xffffffffu, moved)) {  // rescale the O rows (after PV_{j-1})
           const float alpha = m_prev == m_new ? 1.f : ex2_ftz(m_prev - m_new);
           ok = __all_sync(0xffffffffu, wait_bar<false>(o_done, (j - 1) & 1, abort, peer_abort));
@@ -940,7 +951,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             tc::st32(ta, s);
           }
         }
-        if (__any_sync(0xffffffffu, apart)) l_apart = l_sum + wide_sum(sa, ks, vs, grp, c2, vis, nmu + kBiasLog2);
+        if (kFold && apart) l_apart = l_sum + wide_sum(sa, vs, grp, c2, vis, nmu, kBiasLog2<T>);
       }
       // float16 outputs carry as many bits as the weights.  In a request's first tile l sums the weights as
       // rounded, so that a rounding moves weight between keys and leaves their sum one (a row of one key
@@ -954,7 +965,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         tc::wait_ld();
         scale_mask<kFold>(s, ks + 32 * g, vis - 32 * g);
         const float4 e = grp[g];
-        const float cg = logit_factor(c2, e.x), ng = kFold ? nmu + e.y : nmu + kBiasLog2;
+        const float cg = logit_factor(c2, e.x, e.w), ng = kFold ? nmu + e.y : nmu;
         const uint64_t c22 = pk2(cg, cg), nmu2 = pk2(ng, ng);
         uint64_t ls2[2] = {0, 0};
         float pk[16];
@@ -1000,7 +1011,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (lane == 0) mbar_arrive(&p_full[2 * wg + (g >> 1)]);  // rank 1's are forwarded to rank 0
         }
       }
-      if (kFold) l_sum = l_apart < 0.f ? l_sum : l_apart;
+      if (kFold && apart) l_sum = l_apart;
     }
     const bool gated = a.gate_mode != TF_GATE_NONE;
     const bool vec = rows_v16(a);
@@ -1023,7 +1034,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       tc::fence_after_sync();
       const int hq = h * G + (r - ri * G);
       const int64_t t = q0 + ri;
-      const float inv = kBias / l_tot;
+      const float inv = kBias<T> / l_tot;
       float* po = nullptr;
       if (sp.n > 1 && row_valid) {
         const int64_t row = ((int64_t)z * a.num_tokens + t) * a.num_q_heads + hq;
@@ -1157,7 +1168,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ tf_p
       o[2 * i + 1] = fmaf(f, v.y, o[2 * i + 1]);
     }
   }
-  const float inv = kBias / l;
+  const float inv = kBias<T> / l;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int d = V * lane + i;

@@ -839,11 +839,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float ah = fade(M[n][k], mn);
             al[k] = ah * ah;
             M[n][k] = mn;
-            const float sub = mn == -INFINITY && tok0 >= lim[n][k] ? 0.f : kBiasLog2 - mn;
+            const float sub = mn == -INFINITY && tok0 >= lim[n][k] ? 0.f : mn;
             float ls = l[n][k] * ah * ah;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              sv[i][k] = ex2(sv[i][k] + sub);
+              sv[i][k] = ex2((sv[i][k] - sub) + kBiasLog2);  // (in this order: M may be above 2^24)
               const float w = sv[i][k] * vn[i];
               if (kSumRounded) {
                 const float wr = __half2float(__float2half_rn(w));

@@ -33,12 +33,12 @@
 // TF_KERR_TIMEOUT.
 //
 // Measured (bf16, 32 heads over 4, head_dim 256; ranges are boxes).  A chunk of 512 tokens behind 28000:
-// 514 to 550 us, 862 to 922 TFLOP/s; about 2.1 us a key tile, held by the latency of the softmax warps'
+// 528 to 560 us, 847 to 897 TFLOP/s; about 2.1 us a key tile, held by the latency of the softmax warps'
 // reads of TMEM (each is waited for where it is issued, and S is read twice; 45% of the issue slots used)
-// with the products' 1.1 us beside them.  4 requests of 512 to 2048 tokens on up to 4096: 576 to 614 us, 733
-// to 781 TFLOP/s; a query tile's first product starts 10 us after its CTAs do (lengths, table, rows:
+// with the products' 1.1 us beside them.  4 requests of 512 to 2048 tokens on up to 4096: 578 to 616 us, 730
+// to 778 TFLOP/s; a query tile's first product starts 10 us after its CTAs do (lengths, table, rows:
 // dependent reads) and its epilogue takes 5 us, with nothing beside them as O and the two S buffers fill
-// TMEM.  Where every tile is wide (scales 2^+-9 apart) the two take 1150 and 1170 us.  The same chunk over a
+// TMEM.  Where every tile is wide (scales 2^+-9 apart) the two take 1130 and 1155 us.  The same chunk over a
 // 16-bit pool (paged_extend_tc.cu) takes 381 us, the prompts 468.
 //
 // Few query tiles over a long prefix leave SM pairs idle: the key tiles are then split over

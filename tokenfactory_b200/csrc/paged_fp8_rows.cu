@@ -17,7 +17,7 @@
 // Measured (bf16, 32 heads over 4, head_dim 256).  128 decode requests of 512 to 8192 tokens: 225 to 239 us, 4.9 to
 // 5.2 TB/s (0.75 to 0.79 of the copy rate; 6.8 TB/s between the first tile and the last piece, the rest
 // is the plan, 4 us, the epilogues and the combine kernel, 9 us).  One request of 8191: 22.5 us, of which
-// the combine kernel 8 us.  24 requests with 2 to 5 new tokens: 103 us, bound by instruction latency
+// the combine kernel 8 us.  24 requests with 2 to 5 new tokens: 104 us, bound by instruction latency
 // with two warps a scheduler (33% of issue slots; the registers hold no third).
 //
 // Fragments.  S^T = K8.Q^T: A = 16 tokens x 16 dims.  A thread's 16-byte read of a token's row is its A

@@ -203,10 +203,14 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) prologue_ker
     // whole turns are removed in fp64 (2 pi to 53 bits: an error of 2^-53 per radian turned)
     const double f = (double)a.positions[prow * a.pos_stride + t0 + jt] * (double)a.inv_freq[jj];
     constexpr double k2Pi = 6.283185307179586;
+    const double turn = f - rint(f * (1.0 / k2Pi)) * k2Pi;
+    // the angle in two floats: sine and cosine of the first, turned on by the second (first order: it is below
+    // 2^-22).  Rounded to one float its error, up to 2^-23, would be all that is left of a sine near 0.
+    const float hi = (float)turn, lo = (float)(turn - (double)hi);
     float sf, cf;
-    sincosf((float)(f - rint(f * (1.0 / k2Pi)) * k2Pi), &sf, &cf);
-    cs[jt][jj] = cf;
-    sn[jt][jj] = sf;
+    sincosf(hi, &sf, &cf);
+    cs[jt][jj] = fmaf(-sf, lo, cf);
+    sn[jt][jj] = fmaf(cf, lo, sf);
   }
   if (tid < ntok) s_loc[tid] = kv8::store_slot(a.out_cache_loc[t0 + tid], a.num_slots, a.err);
   __syncthreads();
